@@ -377,6 +377,150 @@ int qs_dec_attention_rope(const void *q, const void *k, const void *v, const voi
 int qs_dec_silu_mul(const void *gate, const void *up, void *out, int64_t rows, int64_t m, int64_t ldg, int64_t ldu,
                     int64_t ldo, qs_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Paged key-value cache: attention over it, and the work on its pages.  No
+ * counterpart in the reference, which keeps no cache (its evaluation runs
+ * whole windows, scripts/eval_ppl.py:41-65); for decode loops around
+ * QuantizedLinear that serve several sequences, search with beams or stream
+ * under a window.
+ *
+ * A pool holds `pages` pages of `page` positions for every kv head.  Row r of
+ * a batch keeps its position p on page table[r][p / page] at place p % page;
+ * -1 stands for no page.  refs[i] is the number of table entries that hold
+ * page i; a page with none is free.  All of it is device memory, read and
+ * written by kernels alone, so that a captured step replays.
+ * --------------------------------------------------------------------------- */
+
+/* One layer's keys and values.  Strides in elements, multiples of 8; the
+ * head_dim elements of a position lie together.  page: a power of two from 16
+ * to 4096.  A table entry that names no page of the pool, and a position
+ * beyond the table, is left out of an attention and not written. */
+typedef struct qs_page_pool {
+  void *k, *v;
+  int64_t k_page, k_head, k_pos;
+  int64_t v_page, v_head, v_pos;
+  int64_t pages;
+  int page;
+  const int32_t *table; /* [rows][cols], row stride table_ld */
+  int64_t table_ld, cols;
+  const int32_t *lengths; /* [rows]: positions that the row holds, the new tokens included */
+} qs_page_pool;
+
+/* Stores the keys and values of new tokens (bf16 or fp16, [tokens][kv_heads]
+ * [head_dim] with the strides given, head_dim a multiple of 8): token t of
+ * row r, starts[r] <= t < starts[r + 1], at position lengths[r] - starts[r +
+ * 1] + t.  starts NULL: one token per row. */
+int qs_page_append(const void *k, const void *v, int64_t tokens, int64_t rows, int kv_heads, int head_dim,
+                   int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t *starts,
+                   const qs_page_pool *pool, qs_stream_t stream);
+
+/* qs_dec_qk_norm_rope for a paged cache, one token per row, each at its own
+ * position lengths[r] - 1 (the row of the cos / sin tables, of table_rows
+ * rows, too): q and k heads get their norm and the rotary embedding, q into
+ * q_out, k and v into the pages.  bf16, head_dim 128; the same bits. */
+int qs_page_append_rope(const void *q, const void *k, const void *v, const void *q_norm_w, const void *k_norm_w,
+                        const void *cos_table, const void *sin_table, int64_t table_rows, void *q_out, int64_t rows,
+                        int nh, int nkv, int head_dim, const qs_page_pool *pool, float eps, qs_stream_t stream);
+
+/* Attention of one new token per row, at position lengths[r] - 1, over the
+ * row's pages: out[r][h * head_dim + d] = sum_p softmax_p(scale q_h . k_p)
+ * v_p with kv head h / (heads / kv_heads), over the positions p <= lengths[r]
+ * - 1 that are within the last `window` (0: all) or among the first `sinks`.
+ * A row that sees nothing gets zeros.  scale: finite, not 0.  bf16 or fp16, head_dim 64, 128 or 256;
+ * scores, softmax and sums in fp32, weights in the cache's type.  q: strides
+ * q_row, q_head; 16-byte aligned like out, whose rows are out_row apart. */
+size_t qs_attend_token_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim, int64_t cols, int page,
+                                       int window, int sinks);
+int qs_attend_token(const void *q, int dtype, int64_t rows, int heads, int kv_heads, int head_dim, int64_t q_row,
+                    int64_t q_head, const qs_page_pool *pool, float scale, int window, int sinks, void *out,
+                    int64_t out_row, void *workspace, size_t workspace_bytes, qs_stream_t stream);
+
+/* The same for several new tokens per row, each seeing the positions up to
+ * its own: the tokens of row r are starts[r] .. starts[r + 1] - 1 of q and
+ * out, the last of them at position lengths[r] - 1, their keys and values in
+ * the pages already.  starts: [rows + 1], not decreasing, starts[rows] =
+ * tokens.  Values at the row's positions have to be finite where another
+ * query of the call sees them. */
+int qs_attend_chunk(const void *q, int dtype, int64_t tokens, int64_t rows, int heads, int kv_heads, int head_dim,
+                    int64_t q_token, int64_t q_head, const int32_t *starts, const qs_page_pool *pool, float scale,
+                    int window, int sinks, void *out, int64_t out_token, qs_stream_t stream);
+
+/* The whole cache of a model, for the calls that move pages: `planes` (keys
+ * and values of every layer) of [pages][kv_heads][page][row_bytes], one after
+ * the other.  row_bytes a multiple of 16. */
+typedef struct qs_page_store {
+  void *data;
+  int64_t planes, pages;
+  int kv_heads, page;
+  int64_t row_bytes;
+} qs_page_store;
+
+/* A step of every row (at most 1024): row i takes the pages and the length of
+ * row parents[i] (its own where parents is NULL; none where parents[i] names
+ * no row), gives back pages beyond that length, and gets room for `tokens`
+ * more, by which its length grows.  The partly filled page that is written
+ * next is copied (its filled positions, all planes) where several rows hold
+ * it, for each of them but the longest, or the first of the longest.  New
+ * pages are the free ones in ascending order, given out by row, then by
+ * column.  short_pages[0] gets the number of pages that were asked for and
+ * could not be given (none free, or the table full): those entries are -1.
+ * Outputs may be the inputs.  workspace: qs_page_advance_workspace_bytes. */
+size_t qs_page_advance_workspace_bytes(int64_t rows);
+int qs_page_advance(const qs_page_store *store, const int32_t *table, const int32_t *lengths, const int32_t *refs,
+                    const int32_t *parents, int64_t rows, int64_t cols, int tokens, int32_t *table_out,
+                    int32_t *lengths_out, int32_t *refs_out, int32_t *short_pages, void *workspace,
+                    size_t workspace_bytes, qs_stream_t stream);
+
+/* Gives pages back: all of the rows with keep[i] == 0 (their length becomes
+ * 0; keep may be NULL), and with a window the pages that no token at position
+ * lengths[i] or later sees, being neither in its window nor among the sinks.
+ * Outputs may be the inputs. */
+int qs_page_free(const int32_t *table, const int32_t *lengths, const int32_t *refs, const uint8_t *keep, int64_t rows,
+                 int64_t cols, int64_t pages, int page, int window, int sinks, int32_t *table_out,
+                 int32_t *lengths_out, int32_t *refs_out, qs_stream_t stream);
+
+/* Moves the n pages in use to places 0 .. n - 1 of the pool: those beyond, in
+ * ascending order, to the free places in ascending order.  Outputs may be the
+ * inputs.  workspace: qs_page_compact_workspace_bytes. */
+size_t qs_page_compact_workspace_bytes(int64_t pages);
+int qs_page_compact(const qs_page_store *store, const int32_t *table, const int32_t *refs, int64_t rows, int64_t cols,
+                    int32_t *table_out, int32_t *refs_out, void *workspace, size_t workspace_bytes,
+                    qs_stream_t stream);
+
+/* Copies page src[i] to page dst[i] in every plane, i < count.  Pairs that
+ * name a page outside the store are left out; no dst may be a src or dst of
+ * another pair. */
+int qs_page_copy(const qs_page_store *store, const int32_t *src, const int32_t *dst, int64_t count,
+                 qs_stream_t stream);
+
+/* ---------------------------------------------------------------------------
+ * Beam search
+ * --------------------------------------------------------------------------- */
+
+/* For each of `batch` requests the `keep` best of its beams' continuations:
+ * beam j with token t scores scores[b][j] + log softmax(logits[b * beams +
+ * j])[t], in fp64; a finished beam has the one continuation eos at its own
+ * score.  In descending order, ties to the lower beam, then the lower token.
+ * A logit that is NaN counts as -inf; so does every continuation of a beam
+ * whose score is not finite or whose largest logit is not.  Outputs [batch]
+ * [keep]: the score (fp32), the parent as a row of logits (b * beams + j),
+ * the token.  logits: fp32, fp16 or bf16, row stride ld; finished may be
+ * NULL.  keep <= 128, keep <= beams * vocab, beams <= 1024. */
+size_t qs_beam_select_workspace_bytes(int64_t batch, int beams, int64_t vocab, int keep);
+int qs_beam_select(const void *logits, int dtype, int64_t ld, int64_t batch, int beams, int64_t vocab,
+                   const float *scores, const uint8_t *finished, int64_t eos, int keep, float *scores_out,
+                   int32_t *parents_out, int32_t *tokens_out, void *workspace, size_t workspace_bytes,
+                   qs_stream_t stream);
+
+/* Row i of dst[s] becomes row parents[i] of src[s] (zeros where that names no
+ * row of the source), for `count` states at once; row s is row_bytes[s] long,
+ * rows of a source src_stride[s] bytes apart, of a destination
+ * row_bytes[s].  No source may overlap a destination. */
+enum { QS_MAX_STATES = 8 };
+int qs_reorder_states(int count, const void *const *src, void *const *dst, const int64_t *row_bytes,
+                      const int64_t *src_stride, const int32_t *parents, int64_t rows_out, int64_t rows_in,
+                      qs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -23,6 +23,7 @@ QS_MAX_KRON = 64
 QS_MAX_GROUP = 4
 QS_NOALLOC_SCRATCH_BYTES = 32 << 20
 QS_PREOP_RMSNORM, QS_PREOP_SILU_MUL = 1, 2
+QS_MAX_STATES = 8
 
 _vp = ctypes.c_void_p
 
@@ -43,11 +44,29 @@ class PreOp(ctypes.Structure):
                 ("weight", ctypes.c_void_p), ("h_out", ctypes.c_void_p), ("ldo", ctypes.c_int64),
                 ("eps", ctypes.c_float)]
 
+
+class PagePool(ctypes.Structure):
+    """qs_page_pool (include/quipsharp_hip.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_page", ctypes.c_int64),
+                ("k_head", ctypes.c_int64), ("k_pos", ctypes.c_int64), ("v_page", ctypes.c_int64),
+                ("v_head", ctypes.c_int64), ("v_pos", ctypes.c_int64), ("pages", ctypes.c_int64),
+                ("page", ctypes.c_int), ("table", ctypes.c_void_p), ("table_ld", ctypes.c_int64),
+                ("cols", ctypes.c_int64), ("lengths", ctypes.c_void_p)]
+
+
+class PageStore(ctypes.Structure):
+    """qs_page_store (include/quipsharp_hip.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("planes", ctypes.c_int64), ("pages", ctypes.c_int64),
+                ("kv_heads", ctypes.c_int), ("page", ctypes.c_int), ("row_bytes", ctypes.c_int64)]
+
+
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
 _f32 = ctypes.c_float
 _int_p = ctypes.POINTER(ctypes.c_int)
 _f32_p = ctypes.POINTER(ctypes.c_float)
+_pool_p = ctypes.POINTER(PagePool)
+_store_p = ctypes.POINTER(PageStore)
 
 _SIGNATURES = {
     "qs_last_error": ([], ctypes.c_char_p),
@@ -86,6 +105,26 @@ _SIGNATURES = {
     "qs_dec_attention_rope": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _i64, _int,
                                _int, _int, _i64, _f32, _f32, _vp], _int),
     "qs_dec_silu_mul": ([_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp], _int),
+    "qs_page_append": ([_vp, _vp, _i64, _i64, _int, _int, _i64, _i64, _i64, _i64, _vp, _pool_p, _vp], _int),
+    "qs_page_append_rope": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _int, _int, _int, _pool_p, _f32,
+                             _vp], _int),
+    "qs_attend_token_workspace_bytes": ([_i64, _int, _int, _int, _i64, _int, _int, _int], ctypes.c_size_t),
+    "qs_attend_token": ([_vp, _int, _i64, _int, _int, _int, _i64, _i64, _pool_p, _f32, _int, _int, _vp, _i64, _vp,
+                         ctypes.c_size_t, _vp], _int),
+    "qs_attend_chunk": ([_vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _vp, _pool_p, _f32, _int, _int, _vp,
+                         _i64, _vp], _int),
+    "qs_page_advance_workspace_bytes": ([_i64], ctypes.c_size_t),
+    "qs_page_advance": ([_store_p, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
+                         _vp], _int),
+    "qs_page_free": ([_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp], _int),
+    "qs_page_compact_workspace_bytes": ([_i64], ctypes.c_size_t),
+    "qs_page_compact": ([_store_p, _vp, _vp, _i64, _i64, _vp, _vp, _vp, ctypes.c_size_t, _vp], _int),
+    "qs_page_copy": ([_store_p, _vp, _vp, _i64, _vp], _int),
+    "qs_beam_select_workspace_bytes": ([_i64, _int, _i64, _int], ctypes.c_size_t),
+    "qs_beam_select": ([_vp, _int, _i64, _i64, _int, _i64, _vp, _vp, _i64, _int, _vp, _vp, _vp, _vp,
+                        ctypes.c_size_t, _vp], _int),
+    "qs_reorder_states": ([_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_i64),
+                           ctypes.POINTER(_i64), _vp, _i64, _i64, _vp], _int),
 }
 
 EXPORTED = tuple(_SIGNATURES)

@@ -1,0 +1,92 @@
+"""Beam search over a quantized decoder's logits: the best continuations over
+beams and vocabulary, and the states that follow them.  No counterpart in the
+reference.  The computation runs in libquipsharp_hip.so (csrc/qs_beam.hip)."""
+import ctypes
+
+import torch
+from torch import Tensor
+
+from . import _lib
+from .pages import _int32, _rows_flag, _workspace
+
+
+def beam_select(logits: Tensor, scores: Tensor, keep: int = None, finished: Tensor = None, eos: int = -1, *,
+                workspace: Tensor = None):
+    """The ``keep`` (default: as many as beams) best continuations of each
+    request's beams.
+
+    logits: (batch * beams, vocab) or (batch, beams, vocab), float32, float16
+    or bfloat16; scores: (batch, beams) float32.  Beam j with token t scores
+    ``scores[b, j] + log_softmax(logits[b, j])[t]``, taken in 64 bits; a beam
+    whose ``finished`` (bool) is set goes on with ``eos`` alone, at its own
+    score.  Ties go to the lower beam, then the lower token.  A NaN logit
+    counts as -inf, and so does every continuation of a beam whose score or
+    largest logit is not finite.
+
+    Returns ``(scores, parents, tokens)``, (batch, keep) each and in descending
+    order: float32, the parent's row ``b * beams + j`` and the token (int32)."""
+    if scores.dim() != 2 or scores.dtype != torch.float32 or not scores.is_contiguous():
+        raise ValueError(f"scores must be a contiguous float32 (batch, beams), got {tuple(scores.shape)} x {scores.dtype}")
+    batch, beams = scores.shape
+    vocab = logits.shape[-1]
+    if tuple(logits.shape) not in ((batch * beams, vocab), (batch, beams, vocab)):
+        raise ValueError(f"logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
+    if logits.dim() == 3:
+        if batch > 1 and beams > 1 and logits.stride(0) != beams * logits.stride(1):
+            raise ValueError("the rows of logits must lie one stride apart")
+        ld = logits.stride(1) if beams > 1 else logits.stride(0)
+    else:
+        ld = logits.stride(0)
+    if batch * beams == 1:
+        ld = vocab
+    if logits.stride(-1) != 1 and vocab > 1:
+        raise ValueError("the logits of a row must lie together (stride 1)")
+    dev = logits.device
+    if scores.device != dev:
+        raise ValueError(f"scores is on {scores.device}, logits on {dev}")
+    if finished is not None:
+        _rows_flag("finished", finished, scores.shape, dev)
+    keep = beams if keep is None else keep
+    if keep < 1:
+        raise ValueError(f"keep {keep} must be 1 or more")
+    code = _lib.dtype_code(logits.dtype)
+    _lib.require_gpu(logits, what="beam_select")
+    out = torch.empty(3, batch, keep, dtype=torch.int32, device=dev)
+    best, parents, tokens = out.unbind()
+    best = best.view(torch.float32)
+    L = _lib.lib()
+    workspace = _workspace(workspace, L.qs_beam_select_workspace_bytes(batch, beams, vocab, keep), dev)
+    _lib.check(L.qs_beam_select(logits.data_ptr(), code, ld, batch, beams, vocab,
+                                scores.data_ptr(), _lib.ptr(finished), -1 if eos is None else eos, keep,
+                                best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _lib.ptr(workspace),
+                                0 if workspace is None else workspace.numel(), _lib.stream_of(logits)))
+    return best, parents, tokens
+
+
+def reorder_states(states, parents: Tensor):
+    """New states whose row i is row ``parents[i]`` (int32, any shape, taken
+    flat) of the given ones, up to 8 tensors at once whose first dimension
+    counts rows; zeros where a parent names no row."""
+    states = list(states)
+    if not 1 <= len(states) <= _lib.QS_MAX_STATES:
+        raise ValueError(f"{len(states)} states (1 to {_lib.QS_MAX_STATES})")
+    dev, n = states[0].device, parents.numel()
+    _int32("parents", parents, parents.shape, dev)
+    rows = states[0].shape[0]
+    size, stride = [], []
+    for s in states:
+        if s.device != dev or s.dim() < 1 or s.shape[0] != rows:
+            raise ValueError(f"every state must have {rows} rows on {dev}, got {tuple(s.shape)} on {s.device}")
+        row = s[0].numel() if rows else 0
+        if rows and not s[0].is_contiguous():
+            raise ValueError("the elements of a state's row must lie together")
+        size.append(row * s.element_size())
+        stride.append(s.stride(0) * s.element_size() if rows > 1 else size[-1])
+    _lib.require_gpu(*states, what="reorder_states")
+    out = [torch.empty((n,) + tuple(s.shape[1:]), dtype=s.dtype, device=dev) for s in states]
+    k = len(states)
+    _lib.check(_lib.lib().qs_reorder_states(k, (ctypes.c_void_p * k)(*[s.data_ptr() for s in states]),
+                                            (ctypes.c_void_p * k)(*[o.data_ptr() for o in out]),
+                                            (ctypes.c_int64 * k)(*size), (ctypes.c_int64 * k)(*stride),
+                                            parents.data_ptr(), n, rows, _lib.stream_of(states[0])))
+    return out

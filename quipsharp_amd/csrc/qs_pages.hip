@@ -1,0 +1,564 @@
+// The work on a paged key-value cache's pages: storing new tokens, copying,
+// forking rows (beams), giving pages out and back, and moving the pages in
+// use together.  The tables are small and their work is a chain of short
+// steps, so one work-group does all of it (no step waits for another
+// work-group); it leaves a list of copies, and a second launch, as wide as
+// the chip, moves the bytes.
+#include "qs_rope_dev.h"
+
+namespace qs {
+namespace {
+
+constexpr int kMaxRows = 1024;
+constexpr int kThreads = 1024;
+
+struct Store {
+  char* data;
+  int64_t planes, pages, row_bytes;
+  int kv_heads, page;
+};
+
+// A copy of the first `used` positions of every head of a page.
+struct Copy {
+  int32_t src, dst, used;
+};
+
+// plan[0]: the number of copies; the copies from plan + 4.
+__device__ __host__ __forceinline__ int32_t* plan_copies(int32_t* plan) { return plan + 4; }
+
+// Reference counts are changed with atomics, which act in the L2: they are
+// read with atomic loads too, which do not take a line that the L1 still has.
+__device__ __forceinline__ int ref_load(const int32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void ref_add(int32_t* p, int v) {
+  __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void ref_store(int32_t* p, int v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+// Every global access of the work-group before the barrier is done when a
+// thread goes on after it (loads and atomics of another wave see it in the L2).
+__device__ __forceinline__ void group_sync() {
+  __threadfence();
+  __syncthreads();
+}
+
+// Exclusive prefix sum over the 1024 threads; *total gets the sum.  `part` is
+// 16 ints of LDS; a barrier stands before and after.
+__device__ __forceinline__ int scan1024(int v, int* part, int* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int x = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int y = __shfl_up(x, d, 64);
+    if (lane >= d) x += y;
+  }
+  __syncthreads();
+  if (lane == 63) part[w] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kThreads / 64; ++i) {
+    const int y = part[i];
+    before += i < w ? y : 0;
+    all += y;
+  }
+  *total = all;
+  return before + x - v;
+}
+
+// ---------------------------------------------------------------------------
+// copies
+// ---------------------------------------------------------------------------
+
+// Pieces of 4 KB of (copy, plane, head), dealt over the grid.
+__global__ __launch_bounds__(256) void page_copy_kernel(Store st, const int32_t* plan) {
+  const int count = plan[0];
+  const Copy* copies = reinterpret_cast<const Copy*>(plan + 4);
+  const int64_t head_bytes = st.page * st.row_bytes, page_bytes = head_bytes * st.kv_heads;
+  const int pieces = (int)((head_bytes + 4095) / 4096);
+  const int64_t per = st.planes * st.kv_heads * pieces, all = per * count;
+  for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
+    const Copy c = copies[i / per];
+    int64_t rest = i % per;
+    const int piece = (int)(rest % pieces);
+    rest /= pieces;
+    const int head = (int)(rest % st.kv_heads);
+    const int64_t plane = rest / st.kv_heads;
+    const int64_t at = (int64_t)piece * 4096 + threadIdx.x * 16;
+    if (at >= c.used * st.row_bytes) continue;
+    char* base = st.data + plane * st.pages * page_bytes + head * head_bytes + at;
+    *reinterpret_cast<uint4*>(base + c.dst * page_bytes) = *reinterpret_cast<const uint4*>(base + c.src * page_bytes);
+  }
+}
+
+// The plan of qs_page_copy: the caller's pairs, those outside the pool with
+// nothing to copy.
+__global__ __launch_bounds__(256) void page_list_kernel(Store st, const int32_t* src, const int32_t* dst, int64_t count) {
+  const int64_t head_bytes = st.page * st.row_bytes, page_bytes = head_bytes * st.kv_heads;
+  const int pieces = (int)((head_bytes + 4095) / 4096);
+  const int64_t per = st.planes * st.kv_heads * pieces, all = per * count;
+  for (int64_t i = blockIdx.x; i < all; i += gridDim.x) {
+    const int64_t s = src[i / per], d = dst[i / per];
+    if (s < 0 || d < 0 || s >= st.pages || d >= st.pages) continue;
+    int64_t rest = i % per;
+    const int piece = (int)(rest % pieces);
+    rest /= pieces;
+    const int64_t at = (int64_t)piece * 4096 + threadIdx.x * 16;
+    if (at >= head_bytes) continue;
+    char* base = st.data + (rest / st.kv_heads) * st.pages * page_bytes + (rest % st.kv_heads) * head_bytes + at;
+    *reinterpret_cast<uint4*>(base + d * page_bytes) = *reinterpret_cast<const uint4*>(base + s * page_bytes);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// advance: fork, give back, give out
+// ---------------------------------------------------------------------------
+
+struct AdvanceArgs {
+  const int32_t *table, *lengths, *refs, *parents;
+  int32_t *table_out, *lengths_out, *refs_out, *short_pages, *plan;
+  int rows, cols, pages, page, tokens;
+};
+
+constexpr int kTileInts = 8192;  // table entries staged at a time
+
+__global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
+  __shared__ int32_t tile[kTileInts];
+  __shared__ int32_t len[kMaxRows], from[kMaxRows], need[kMaxRows + 1], mine[kMaxRows];
+  __shared__ uint8_t shared_page[kMaxRows];
+  __shared__ int part[kThreads / 64];
+  __shared__ int copies, lost;
+  const int tid = threadIdx.x;
+  const int64_t room = (int64_t)a.cols * a.page;
+  if (a.refs_out != a.refs)
+    for (int p = tid; p < a.pages; p += kThreads) ref_store(a.refs_out + p, a.refs[p]);
+  int old_len = 0;
+  if (tid < a.rows) {
+    int par = a.parents ? a.parents[tid] : tid;
+    par = par >= 0 && par < a.rows ? par : -1;
+    from[tid] = par;
+    int n = par >= 0 ? a.lengths[par] : 0;
+    old_len = n < 0 ? 0 : n > room ? (int)room : n;
+    len[tid] = old_len;
+    shared_page[tid] = 0;
+  }
+  if (tid == 0) copies = 0, lost = 0;
+  group_sync();
+  // rows take their parents' pages up to the parents' lengths, a block of
+  // columns of every row at a time (outputs may be the inputs)
+  const int width = kTileInts / a.rows < a.cols ? kTileInts / a.rows : a.cols;
+  for (int c0 = 0; c0 < a.cols; c0 += width) {
+    const int n = a.cols - c0 < width ? a.cols - c0 : width, all = a.rows * n;
+    for (int e = tid; e < all; e += kThreads) tile[e] = a.table[(int64_t)(e / n) * a.cols + c0 + e % n];
+    __syncthreads();
+    for (int e = tid; e < all; e += kThreads) {
+      const int i = e / n, c = e % n, par = from[i];
+      int old = tile[e], now = par >= 0 && (int64_t)(c0 + c) * a.page < len[i] ? tile[par * n + c] : -1;
+      old = old >= 0 && old < a.pages ? old : -1;
+      now = now >= 0 && now < a.pages ? now : -1;
+      if (now != old) {
+        if (now >= 0) ref_add(a.refs_out + now, 1);
+        if (old >= 0) ref_add(a.refs_out + old, -1);
+      }
+      a.table_out[(int64_t)i * a.cols + c0 + c] = now;
+    }
+    __syncthreads();
+  }
+  group_sync();
+  // the page that a row writes next, where it is partly filled and another row holds it too
+  int c0 = 0, used = 0;
+  if (tid < a.rows) {
+    c0 = old_len / a.page, used = old_len % a.page;
+    int p = -1;
+    if (a.tokens > 0 && used > 0) p = a.table_out[(int64_t)tid * a.cols + c0];
+    mine[tid] = p >= 0 && ref_load(a.refs_out + p) > 1 ? p : -1;
+  }
+  __syncthreads();
+  for (int e = tid; e < a.rows * a.rows; e += kThreads) {
+    const int i = e / a.rows, j = e % a.rows;
+    if (mine[i] < 0 || i == j) continue;
+    if (len[j] > len[i] || (len[j] == len[i] && j < i))
+      if (a.table_out[(int64_t)j * a.cols + len[i] / a.page] == mine[i]) shared_page[i] = 1;
+  }
+  __syncthreads();
+  // pages that a row needs: a copy's, then those of columns first .. last
+  int wants = 0, first = 0;
+  bool copy = false;
+  if (tid < a.rows) {
+    copy = shared_page[tid];
+    first = c0 + (used > 0);
+    int64_t last = a.tokens > 0 ? ((int64_t)old_len + a.tokens - 1) / a.page : -1;
+    if (last >= a.cols) atomicAdd(&lost, (int)(last - a.cols + 1)), last = a.cols - 1;
+    wants = copy + (last >= first ? (int)(last - first + 1) : 0);
+    const int64_t end = (int64_t)old_len + a.tokens;
+    a.lengths_out[tid] = (int)(end < room ? end : room);
+  }
+  int total;
+  const int mark = scan1024(wants, part, &total);
+  if (tid < a.rows) need[tid] = mark, from[tid] = copy;
+  if (tid == 0) need[a.rows] = total;
+  __syncthreads();
+  // free pages in ascending order; the page of rank k goes to the row whose
+  // share of the ranks holds k
+  int found = 0;
+  for (int p0 = 0; p0 < a.pages && found < total; p0 += kThreads) {
+    const int p = p0 + tid;
+    const bool is_free = p < a.pages && ref_load(a.refs_out + p) <= 0;
+    int n;
+    const int k = found + scan1024(is_free, part, &n);
+    found += n;
+    if (!is_free || k >= total) continue;
+    int lo = 0, hi = a.rows;  // need[lo] <= k < need[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (need[mid] <= k) lo = mid; else hi = mid;
+    }
+    const int n0 = len[lo] / a.page, u = len[lo] % a.page;
+    int nth = k - need[lo], col;
+    if (from[lo] && nth == 0) {
+      col = n0;
+      const int at = atomicAdd(&copies, 1);
+      Copy* c = reinterpret_cast<Copy*>(plan_copies(a.plan)) + at;
+      c->src = mine[lo], c->dst = p, c->used = u;
+      ref_add(a.refs_out + mine[lo], -1);
+    } else {
+      col = n0 + (u > 0) + nth - from[lo];
+    }
+    a.table_out[(int64_t)lo * a.cols + col] = p;
+    ref_store(a.refs_out + p, 1);
+  }
+  // a copy that got no page: the row loses its hold
+  if (tid < a.rows && copy && mark >= found) {
+    a.table_out[(int64_t)tid * a.cols + c0] = -1;
+    ref_add(a.refs_out + mine[tid], -1);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    a.plan[0] = copies;
+    a.short_pages[0] = lost + (total > found ? total - found : 0);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// give back
+// ---------------------------------------------------------------------------
+
+struct FreeArgs {
+  const int32_t *table, *lengths, *refs;
+  const uint8_t* keep;
+  int32_t *table_out, *lengths_out, *refs_out;
+  int rows, cols, pages, page, window, sinks;
+};
+
+__global__ __launch_bounds__(kThreads) void page_free_kernel(FreeArgs a) {
+  const int tid = threadIdx.x;
+  if (a.refs_out != a.refs)
+    for (int p = tid; p < a.pages; p += kThreads) ref_store(a.refs_out + p, a.refs[p]);
+  group_sync();
+  const int64_t all = (int64_t)a.rows * a.cols;
+  for (int64_t e = tid; e < all; e += kThreads) {
+    const int i = (int)(e / a.cols), c = (int)(e % a.cols);
+    const int old = a.table[e];
+    const bool valid = old >= 0 && old < a.pages;
+    bool drop = a.keep && !a.keep[i];
+    if (!drop && a.window > 0)
+      drop = (int64_t)c * a.page >= a.sinks && (int64_t)(c + 1) * a.page <= (int64_t)a.lengths[i] - a.window + 1;
+    if (drop && valid) ref_add(a.refs_out + old, -1);
+    a.table_out[e] = valid && !drop ? old : -1;
+  }
+  __syncthreads();  // lengths_out may be lengths, which all of a row's threads read above
+  for (int i = tid; i < a.rows; i += kThreads) {
+    const int n = a.lengths[i];
+    a.lengths_out[i] = a.keep && !a.keep[i] ? 0 : n;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// move together
+// ---------------------------------------------------------------------------
+
+struct CompactArgs {
+  const int32_t* refs;
+  int32_t *refs_out, *plan, *map;
+  int pages, page;
+};
+
+__global__ __launch_bounds__(kThreads) void page_compact_kernel(CompactArgs a) {
+  __shared__ int part[kThreads / 64];
+  const int tid = threadIdx.x;
+  int mine = 0, live;
+  for (int p = tid; p < a.pages; p += kThreads) mine += a.refs[p] > 0;
+  scan1024(mine, part, &live);
+  // the k-th free place below `live` takes the k-th page in use beyond it
+  Copy* copies = reinterpret_cast<Copy*>(plan_copies(a.plan));
+  int free_before = 0, high_before = 0;
+  for (int p0 = 0; p0 < a.pages; p0 += kThreads) {
+    const int p = p0 + tid;
+    const bool used = p < a.pages && a.refs[p] > 0;
+    const bool hole = p < live && !used, high = used && p >= live;
+    int n;
+    const int k = scan1024(hole ? 1 : high ? 1 << 16 : 0, part, &n);
+    if (hole) copies[free_before + (k & 0xFFFF)].dst = p;
+    if (high) copies[high_before + (k >> 16)].src = p;
+    if (p < a.pages) a.map[p] = p;
+    free_before += n & 0xFFFF, high_before += n >> 16;
+  }
+  group_sync();
+  if (a.refs_out != a.refs)
+    for (int p = tid; p < a.pages; p += kThreads) a.refs_out[p] = a.refs[p];
+  group_sync();
+  for (int k = tid; k < high_before; k += kThreads) {
+    const int s = copies[k].src, d = copies[k].dst;
+    copies[k].used = a.page;
+    a.map[s] = d;
+    const int n = a.refs[s];
+    a.refs_out[d] = n;
+    a.refs_out[s] = 0;
+  }
+  if (tid == 0) a.plan[0] = high_before;
+}
+
+__global__ __launch_bounds__(256) void page_remap_kernel(const int32_t* table, int32_t* table_out, const int32_t* map,
+                                                         int64_t entries, int pages) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= entries) return;
+  const int p = table[e];
+  table_out[e] = p >= 0 && p < pages ? map[p] : -1;
+}
+
+// ---------------------------------------------------------------------------
+// new tokens
+// ---------------------------------------------------------------------------
+
+struct AppendArgs {
+  const uint16_t *k, *v;
+  int64_t k_token, k_head, v_token, v_head, tokens;
+  const int32_t* starts;
+  int rows, kv_heads, head_dim;
+};
+
+// Element address of position p of a row's page, or null.
+__device__ __forceinline__ uint16_t* place(void* base, int64_t s_page, int64_t s_head, int64_t s_pos, const qs_page_pool& pool,
+                                           int row, int64_t p, int head) {
+  if (p < 0 || p >= pool.cols * pool.page) return nullptr;
+  const int id = pool.table[row * pool.table_ld + p / pool.page];
+  if (id < 0 || id >= pool.pages) return nullptr;
+  return static_cast<uint16_t*>(base) + id * s_page + head * s_head + (p % pool.page) * s_pos;
+}
+
+// One thread per 8 elements of a head.
+__global__ __launch_bounds__(256) void page_append_kernel(qs_page_pool pool, AppendArgs a) {
+  const int per = a.head_dim / 8;
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t t = i / (per * a.kv_heads);
+  if (t >= a.tokens) return;
+  const int rest = (int)(i % (per * a.kv_heads)), head = rest / per, d = rest % per * 8;
+  int row = (int)t;
+  int64_t back = 1;
+  if (a.starts) {
+    int lo = 0, hi = a.rows;  // the last row that starts at t or before
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (a.starts[mid] <= t) lo = mid; else hi = mid;
+    }
+    row = lo;
+    back = a.starts[row + 1] - t;
+    if (a.starts[row] > t || back <= 0) return;
+  }
+  const int64_t p = pool.lengths[row] - back;
+  if (uint16_t* to = place(pool.k, pool.k_page, pool.k_head, pool.k_pos, pool, row, p, head))
+    *reinterpret_cast<uint4*>(to + d) = *reinterpret_cast<const uint4*>(a.k + t * a.k_token + head * a.k_head + d);
+  if (uint16_t* to = place(pool.v, pool.v_page, pool.v_head, pool.v_pos, pool, row, p, head))
+    *reinterpret_cast<uint4*>(to + d) = *reinterpret_cast<const uint4*>(a.v + t * a.v_token + head * a.v_head + d);
+}
+
+// One wave per head of one row, as qk_norm_rope_kernel.
+__global__ __launch_bounds__(256) void page_append_rope_kernel(const uint16_t* q, const uint16_t* k, const uint16_t* v,
+                                                               const uint16_t* qw, const uint16_t* kw,
+                                                               const uint16_t* cos_t, const uint16_t* sin_t,
+                                                               int64_t table_rows, uint16_t* q_out, qs_page_pool pool,
+                                                               int nh, int nkv, float eps) {
+  const LaneX lx = lane_x_init();
+  const int b = blockIdx.x, hh = blockIdx.y * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
+  if (hh >= nh + 2 * nkv) return;
+  const int64_t pos = (int64_t)pool.lengths[b] - 1;
+  if (hh >= nh + nkv) {
+    const int g = hh - nh - nkv;
+    const uint16_t* src = v + ((int64_t)b * nkv + g) * 128;
+    if (uint16_t* to = place(pool.v, pool.v_page, pool.v_head, pool.v_pos, pool, b, pos, g)) to[l] = src[l], to[l + 64] = src[l + 64];
+    return;
+  }
+  // a row without tokens, or a position beyond the tables, has no rotation: its queries are zeros and nothing is stored
+  const bool inside = pos >= 0 && pos < table_rows, isq = hh < nh;
+  const int g = isq ? hh : hh - nh;
+  uint16_t o0 = 0, o1 = 0;
+  if (inside) {
+    const uint16_t* src = isq ? q + ((int64_t)b * nh + g) * 128 : k + ((int64_t)b * nkv + g) * 128;
+    const uint16_t* w = isq ? qw : kw;
+    norm_rope(bf(src[l]), bf(src[l + 64]), bf(w[l]), bf(w[l + 64]), load_rot(cos_t + pos * 128, sin_t + pos * 128, l), eps, lx, o0, o1);
+  }
+  uint16_t* to = isq ? q_out + ((int64_t)b * nh + g) * 128
+                     : inside ? place(pool.k, pool.k_page, pool.k_head, pool.k_pos, pool, b, pos, g) : nullptr;
+  if (to) to[l] = o0, to[l + 64] = o1;
+}
+
+int store_checks(const char* fn, const qs_page_store* s, Store& out) {
+  QS_REQUIRE(s && s->data, "%s: null pointer", fn);
+  QS_REQUIRE(s->planes >= 1 && s->pages >= 1 && s->pages <= INT32_MAX && s->kv_heads >= 1 && s->page >= 1 &&
+                 s->page <= 4096 && s->row_bytes >= 16 && s->row_bytes % 16 == 0 && s->row_bytes <= 65536,
+             "%s: %lld planes of %lld pages, %d heads, %d positions of %lld bytes (a multiple of 16)", fn,
+             (long long)s->planes, (long long)s->pages, s->kv_heads, s->page, (long long)s->row_bytes);
+  QS_REQUIRE((reinterpret_cast<uintptr_t>(s->data) & 15) == 0, "%s: the store must be 16-byte aligned", fn);
+  out = Store{static_cast<char*>(s->data), s->planes, s->pages, s->row_bytes, s->kv_heads, s->page};
+  return QS_OK;
+}
+
+int table_checks(const char* fn, int64_t rows, int64_t cols, int64_t pages, int page) {
+  QS_REQUIRE(rows >= 1 && cols >= 1 && cols <= (1 << 24) && pages >= 1 && pages <= INT32_MAX - kThreads && page >= 1 &&
+                 cols * page <= INT32_MAX - 65536,
+             "%s: table of %lld x %lld, %lld pages of %d", fn, (long long)rows, (long long)cols, (long long)pages, page);
+  return QS_OK;
+}
+
+constexpr int kCopyGroups = 2048;
+
+int launch_copies(const Store& st, const int32_t* plan, hipStream_t stream) {
+  hipLaunchKernelGGL(page_copy_kernel, dim3(kCopyGroups), dim3(256), 0, stream, st, plan);
+  QS_LAUNCHED("page_copy_kernel");
+  return QS_OK;
+}
+
+int pool_checks(const char* fn, const qs_page_pool* p, int64_t rows, int kv_heads, int head_dim) {
+  QS_REQUIRE(p && p->k && p->v && p->table && p->lengths, "%s: null pointer", fn);
+  QS_REQUIRE(rows >= 1 && rows <= (1 << 20) && kv_heads >= 1 && kv_heads <= 65535 && head_dim >= 8 && head_dim % 8 == 0 &&
+                 head_dim <= 4096 && p->pages >= 1 && p->pages <= INT32_MAX && p->page >= 1 && p->cols >= 1 &&
+                 p->table_ld >= p->cols && p->cols * p->page <= INT32_MAX,
+             "%s: rows %lld, %d heads of %d, %lld pages of %d, table of %lld columns", fn, (long long)rows, kv_heads,
+             head_dim, (long long)p->pages, p->page, (long long)p->cols);
+  const int64_t st[6] = {p->k_page, p->k_head, p->k_pos, p->v_page, p->v_head, p->v_pos};
+  for (int64_t x : st) QS_REQUIRE(x >= 0 && x % 8 == 0, "%s: pool strides must be multiples of 8 elements, got %lld", fn, (long long)x);
+  QS_REQUIRE(((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) & 15) == 0,
+             "%s: the pools must be 16-byte aligned", fn);
+  return QS_OK;
+}
+
+}  // namespace
+}  // namespace qs
+
+using namespace qs;
+
+extern "C" int qs_page_append(const void* k, const void* v, int64_t tokens, int64_t rows, int kv_heads, int head_dim,
+                              int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* starts,
+                              const qs_page_pool* pool, qs_stream_t stream) {
+  if (tokens == 0 || rows == 0) return QS_OK;
+  if (const int rc = pool_checks("qs_page_append", pool, rows, kv_heads, head_dim)) return rc;
+  QS_REQUIRE(k && v && tokens >= 1 && (starts || tokens == rows), "qs_page_append: %lld tokens of %lld rows",
+             (long long)tokens, (long long)rows);
+  const int64_t st[4] = {k_token, k_head, v_token, v_head};
+  for (int64_t x : st) QS_REQUIRE(x >= 0 && x % 8 == 0, "qs_page_append: strides must be multiples of 8 elements, got %lld", (long long)x);
+  QS_REQUIRE(((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0,
+             "qs_page_append: keys and values must be 16-byte aligned");
+  const int64_t threads = tokens * kv_heads * (head_dim / 8);
+  QS_REQUIRE(threads <= ((int64_t)INT32_MAX << 8), "qs_page_append: %lld tokens", (long long)tokens);
+  const AppendArgs a{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_token, k_head, v_token, v_head,
+                     tokens, starts, (int)rows, kv_heads, head_dim};
+  hipLaunchKernelGGL(page_append_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, as_stream(stream), *pool, a);
+  QS_LAUNCHED("page_append_kernel");
+  return QS_OK;
+}
+
+extern "C" int qs_page_append_rope(const void* q, const void* k, const void* v, const void* q_norm_w,
+                                   const void* k_norm_w, const void* cos_table, const void* sin_table,
+                                   int64_t table_rows, void* q_out, int64_t rows, int nh, int nkv, int head_dim,
+                                   const qs_page_pool* pool, float eps, qs_stream_t stream) {
+  if (rows == 0) return QS_OK;
+  QS_REQUIRE(q && k && v && q_norm_w && k_norm_w && cos_table && sin_table && q_out, "qs_page_append_rope: null pointer");
+  QS_SUPPORTED(head_dim == 128, "qs_page_append_rope: head_dim %d (128 only)", head_dim);
+  if (const int rc = pool_checks("qs_page_append_rope", pool, rows, nkv, head_dim)) return rc;
+  QS_REQUIRE(nh >= 1 && nh % nkv == 0 && nh <= 65535 && rows <= INT32_MAX && table_rows >= 1,
+             "qs_page_append_rope: heads %d / %d, tables of %lld rows", nh, nkv, (long long)table_rows);
+  hipLaunchKernelGGL(page_append_rope_kernel, dim3((unsigned)rows, (unsigned)((nh + 2 * nkv + 3) / 4)), dim3(256), 0,
+                     as_stream(stream), static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
+                     static_cast<const uint16_t*>(v), static_cast<const uint16_t*>(q_norm_w),
+                     static_cast<const uint16_t*>(k_norm_w), static_cast<const uint16_t*>(cos_table),
+                     static_cast<const uint16_t*>(sin_table), table_rows, static_cast<uint16_t*>(q_out), *pool, nh, nkv, eps);
+  QS_LAUNCHED("page_append_rope_kernel");
+  return QS_OK;
+}
+
+extern "C" size_t qs_page_advance_workspace_bytes(int64_t rows) {
+  return rows < 1 ? 0 : 16 + (size_t)rows * sizeof(Copy);
+}
+
+extern "C" int qs_page_advance(const qs_page_store* store, const int32_t* table, const int32_t* lengths,
+                               const int32_t* refs, const int32_t* parents, int64_t rows, int64_t cols, int tokens,
+                               int32_t* table_out, int32_t* lengths_out, int32_t* refs_out, int32_t* short_pages,
+                               void* workspace, size_t workspace_bytes, qs_stream_t stream) {
+  Store st;
+  if (const int rc = store_checks("qs_page_advance", store, st)) return rc;
+  if (const int rc = table_checks("qs_page_advance", rows, cols, st.pages, st.page)) return rc;
+  QS_SUPPORTED(rows <= kMaxRows, "qs_page_advance: %lld rows (at most %d)", (long long)rows, kMaxRows);
+  QS_REQUIRE(table && lengths && refs && table_out && lengths_out && refs_out && short_pages, "qs_page_advance: null pointer");
+  QS_REQUIRE(tokens >= 0 && tokens <= (1 << 30), "qs_page_advance: %d tokens", tokens);
+  QS_REQUIRE(workspace && workspace_bytes >= qs_page_advance_workspace_bytes(rows) && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+             "qs_page_advance: workspace of %zu bytes (16-byte aligned), %zu needed", workspace_bytes,
+             qs_page_advance_workspace_bytes(rows));
+  int32_t* plan = static_cast<int32_t*>(workspace);
+  const AdvanceArgs a{table, lengths, refs, parents, table_out, lengths_out, refs_out, short_pages, plan,
+                      (int)rows, (int)cols, (int)st.pages, st.page, tokens};
+  hipLaunchKernelGGL(page_advance_kernel, dim3(1), dim3(kThreads), 0, as_stream(stream), a);
+  QS_LAUNCHED("page_advance_kernel");
+  return launch_copies(st, plan, as_stream(stream));
+}
+
+extern "C" int qs_page_free(const int32_t* table, const int32_t* lengths, const int32_t* refs, const uint8_t* keep,
+                            int64_t rows, int64_t cols, int64_t pages, int page, int window, int sinks,
+                            int32_t* table_out, int32_t* lengths_out, int32_t* refs_out, qs_stream_t stream) {
+  if (const int rc = table_checks("qs_page_free", rows, cols, pages, page)) return rc;
+  QS_REQUIRE(rows <= (1 << 20) && table && lengths && refs && table_out && lengths_out && refs_out, "qs_page_free: null pointer or %lld rows", (long long)rows);
+  QS_REQUIRE(window >= 0 && sinks >= 0 && (sinks == 0 || window > 0), "qs_page_free: window %d, sinks %d", window, sinks);
+  const FreeArgs a{table, lengths, refs, keep, table_out, lengths_out, refs_out, (int)rows, (int)cols, (int)pages, page, window, sinks};
+  hipLaunchKernelGGL(page_free_kernel, dim3(1), dim3(kThreads), 0, as_stream(stream), a);
+  QS_LAUNCHED("page_free_kernel");
+  return QS_OK;
+}
+
+extern "C" size_t qs_page_compact_workspace_bytes(int64_t pages) {
+  return pages < 1 ? 0 : 16 + (size_t)pages * (sizeof(Copy) + sizeof(int32_t));
+}
+
+extern "C" int qs_page_compact(const qs_page_store* store, const int32_t* table, const int32_t* refs, int64_t rows,
+                               int64_t cols, int32_t* table_out, int32_t* refs_out, void* workspace,
+                               size_t workspace_bytes, qs_stream_t stream) {
+  Store st;
+  if (const int rc = store_checks("qs_page_compact", store, st)) return rc;
+  if (const int rc = table_checks("qs_page_compact", rows, cols, st.pages, st.page)) return rc;
+  QS_REQUIRE(rows <= (1 << 20) && table && refs && table_out && refs_out, "qs_page_compact: null pointer or %lld rows", (long long)rows);
+  const size_t need = qs_page_compact_workspace_bytes(st.pages);
+  QS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
+             "qs_page_compact: workspace of %zu bytes (16-byte aligned), %zu needed", workspace_bytes, need);
+  int32_t* plan = static_cast<int32_t*>(workspace);
+  int32_t* map = plan + 4 + 3 * st.pages;
+  const CompactArgs a{refs, refs_out, plan, map, (int)st.pages, st.page};
+  hipLaunchKernelGGL(page_compact_kernel, dim3(1), dim3(kThreads), 0, as_stream(stream), a);
+  QS_LAUNCHED("page_compact_kernel");
+  const int64_t entries = rows * cols;
+  hipLaunchKernelGGL(page_remap_kernel, dim3((unsigned)((entries + 255) / 256)), dim3(256), 0, as_stream(stream), table,
+                     table_out, map, entries, (int)st.pages);
+  QS_LAUNCHED("page_remap_kernel");
+  return launch_copies(st, plan, as_stream(stream));
+}
+
+extern "C" int qs_page_copy(const qs_page_store* store, const int32_t* src, const int32_t* dst, int64_t count,
+                            qs_stream_t stream) {
+  if (count == 0) return QS_OK;
+  Store st;
+  if (const int rc = store_checks("qs_page_copy", store, st)) return rc;
+  QS_REQUIRE(src && dst && count >= 1 && count <= INT32_MAX, "qs_page_copy: null pointer or %lld pairs", (long long)count);
+  hipLaunchKernelGGL(page_list_kernel, dim3(kCopyGroups), dim3(256), 0, as_stream(stream), st, src, dst, count);
+  QS_LAUNCHED("page_list_kernel");
+  return QS_OK;
+}

@@ -1,0 +1,168 @@
+"""Beam search's selection and its states (csrc/qs_beam.hip) against the
+definition in 64 bits on the CPU.  Parents and tokens are exact; a score is
+one rounding to fp32 (2^-24 relative) of a number whose log-sum is taken from
+fp32 exponentials and slice sums: each term is off by 4 units relative (2^-22)
+at most and the sums of up to 16 terms and 256 partial sums by 24 units more,
+so the logarithm by 28 2^-24 absolutely."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def select(logits, scores, keep, finished, eos):
+    B, K = scores.shape
+    V = logits.shape[-1]
+    x = logits.reshape(B, K, V).double()
+    x = torch.where(torch.isnan(x), -math.inf, x)
+    out = []
+    for b in range(B):
+        total = torch.full((K, V), -math.inf, dtype=torch.float64)
+        for j in range(K):
+            s, top = scores[b, j].double(), x[b, j].max()
+            if not torch.isfinite(s):
+                continue
+            if finished is not None and finished[b, j]:
+                if 0 <= eos < V:
+                    total[j, eos] = s
+            elif torch.isfinite(top):
+                total[j] = s + (x[b, j] - (top + (x[b, j] - top).exp().sum().log()))
+        value, at = torch.sort(total.view(-1), descending=True, stable=True)
+        out.append((value[:keep], at[:keep] // V + b * K, at[:keep] % V))
+    return [torch.stack(t) for t in zip(*out)]
+
+
+def check(dev, logits, scores, keep, finished=None, eos=-1):
+    from quipsharp_amd.beam import beam_select
+    want = select(logits, scores, keep, finished, eos)
+    got = beam_select(logits.to(dev), scores.to(dev), keep, None if finished is None else finished.to(dev), eos)
+    s, p, t = (x.cpu() for x in got)
+    assert torch.equal(p.long(), want[1]) and torch.equal(t.long(), want[2])
+    infinite = torch.isinf(want[0])
+    assert torch.equal(torch.isinf(s), infinite) and (s[infinite] < 0).all()
+    bound = want[0].abs() * 2.0 ** -24 + 28 * 2.0 ** -24
+    assert ((s.double() - want[0]).abs()[~infinite] <= bound[~infinite]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("batch,beams,vocab,keep", [
+    (1, 1, 1, 1), (1, 1, 50, 50), (2, 3, 7, 20), (1, 4, 1000, 4), (3, 5, 4096, 10), (2, 4, 4097, 8), (1, 2, 32000, 128),
+    (5, 8, 12289, 16), (2, 16, 50257, 16), (1, 4, 151936, 8)])
+def test_select(dev, batch, beams, vocab, keep, dtype):
+    g = torch.Generator().manual_seed(vocab + keep)
+    logits = (torch.randn(batch * beams, vocab, generator=g) * 3).to(dtype)
+    scores = -20 * torch.rand(batch, beams, generator=g)
+    check(dev, logits, scores, keep)
+
+
+@pytest.mark.parametrize("order", ["ascending", "descending", "equal", "two values"])
+def test_ties_and_orders(dev, order):
+    """Everything equal, long runs of equal logits, and logits that lie in order (the best in few threads)."""
+    V = 9000
+    x = {"ascending": torch.arange(V) / 512.0, "descending": -torch.arange(V) / 512.0, "equal": torch.zeros(V),
+         "two values": (torch.arange(V) % 3 == 0).float()}[order]
+    logits = x.repeat(6, 1)
+    check(dev, logits, torch.tensor([[-1.0, -1.0, -1.0], [-2.0, -1.0, -2.0]]), 64)
+    check(dev, logits.half(), torch.zeros(2, 3), 7)
+
+
+def test_zeros_of_both_signs_tie(dev):
+    logits = torch.zeros(2, 100)
+    logits[0, ::2] = -0.0
+    check(dev, logits, torch.zeros(1, 2), 30)
+
+
+def test_finished_and_dead_beams(dev):
+    g = torch.Generator().manual_seed(1)
+    logits = torch.randn(12, 300, generator=g)
+    scores = -torch.rand(3, 4, generator=g) * 5
+    finished = torch.tensor([[0, 1, 0, 1], [1, 1, 1, 1], [0, 0, 0, 1]], dtype=torch.bool)
+    scores[2, 1] = -math.inf
+    scores[2, 2] = math.nan
+    for eos in (0, 2, 299, -1):
+        check(dev, logits, scores, 6, finished, eos)
+    first = torch.full((3, 4), -math.inf)
+    first[:, 0] = 0  # the first step: one beam alive
+    check(dev, logits, first, 4)
+    check(dev, logits, torch.full((3, 4), -math.inf), 5)
+
+
+def test_banned_tokens_nan_and_infinities(dev):
+    logits = torch.full((4, 500), -math.inf)
+    logits[0, 3] = 1.0  # one token allowed
+    logits[1, 7], logits[1, 9] = math.nan, 0.5
+    logits[2] = math.nan
+    logits[3, :2] = torch.tensor([math.inf, 1.0])
+    check(dev, logits, torch.tensor([[-1.0, -2.0], [-0.5, -0.1]]), 5)
+    low = torch.full((2, 500), torch.finfo(torch.bfloat16).min).bfloat16()
+    low[0, 77] = 0
+    check(dev, low, torch.zeros(1, 2), 4)
+
+
+def test_strided_logits(dev):
+    from quipsharp_amd.beam import beam_select
+    g = torch.Generator().manual_seed(2)
+    wide = torch.randn(8, 1003, generator=g).bfloat16()
+    logits = wide[:, 3:1000]  # rows that no vector access fits
+    check(dev, logits, -torch.rand(2, 4, generator=g), 4)
+    # the last position of a prompt's logits
+    seq = torch.randn(2, 4, 997, generator=g)
+    s = -torch.rand(2, 4, generator=g)
+    a = beam_select(seq.to(dev), s.to(dev))
+    b = beam_select(seq.view(8, 997).to(dev), s.to(dev))
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    check(dev, wide.to(dev)[:, :1000].cpu(), s, 4)
+
+
+def test_reorder_states(dev):
+    from quipsharp_amd.beam import reorder_states
+    g = torch.Generator().manual_seed(3)
+    states = [torch.randint(0, 1 << 40, (6, 37), generator=g), torch.randn(6, 3, 5, generator=g).half(),
+              torch.randint(0, 255, (6, 7), generator=g, dtype=torch.uint8), torch.randn(6, generator=g),
+              torch.randn(6, 4096, generator=g), torch.randn(6, 20, generator=g)[:, 4:12], torch.zeros(6, 0)]
+    parents = torch.tensor([[5, 5, 0, 2], [1, -1, 6, 3]], dtype=torch.int32)
+    got = reorder_states([s.to(dev) for s in states[:5]] + [torch.cat([states[5], states[5]], 1).to(dev)[:, :8], states[6].to(dev)],
+                         parents.to(dev))
+    flat = parents.view(-1).long()
+    inside = (flat >= 0) & (flat < 6)
+    for s, o in zip(states, got):
+        want = s[flat.clamp(0, 5)].clone()
+        want[~inside] = 0
+        assert o.shape == want.shape and torch.equal(o.cpu(), want)
+
+
+def test_captured_select(dev):
+    """A captured selection with its states: every replay equals the eager call."""
+    from quipsharp_amd.beam import beam_select, reorder_states
+    g = torch.Generator().manual_seed(4)
+    logits = torch.zeros(8, 20000, dtype=torch.bfloat16, device=dev)
+    scores = torch.zeros(2, 4, device=dev)
+    history = torch.zeros(8, 50, dtype=torch.int64, device=dev)
+
+    def step():
+        s, p, t = beam_select(logits, scores)
+        return [s, p, t] + reorder_states([history], p)
+
+    def fill():
+        logits.copy_(torch.randn(8, 20000, generator=g))
+        scores.copy_(-torch.rand(2, 4, generator=g))
+        history.copy_(torch.randint(0, 99, (8, 50), generator=g))
+
+    fill()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(8):
+        fill()
+        graph.replay()
+        if i % 2:
+            torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step())), i
