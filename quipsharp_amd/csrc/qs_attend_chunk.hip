@@ -8,9 +8,8 @@
 namespace qs {
 namespace {
 
-constexpr int kTile = 32;
-constexpr int kWavesC = 4;
-constexpr int kCols = 16 * kWavesC;  // query columns (a head of a token each) of a work-group
+constexpr int kWaves = 4;
+constexpr int kCols = 32 * kWaves;  // query columns (a head of a token each) of a work-group
 
 struct ChunkArgs {
   const uint16_t* q;
@@ -24,69 +23,294 @@ struct ChunkArgs {
   uint32_t flip;  // its sign, for a pair of elements
 };
 
-// One work-group per kv head and 64 columns of a row, column c being head c %
-// group of the row's token c / group; one wave per 16 of them.
-template <bool BF, int HD>
-__global__ __launch_bounds__(64 * kWavesC) void attend_chunk_kernel(PagePool pp, ChunkArgs a) {
-  typedef WaveAttend<BF, HD, false> W;
-  const int group = a.heads / a.kv_heads, g = blockIdx.y;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r16 = lane & 15, qd = lane >> 4;
-  const LaneX lx = lane_x_init();
-  // the row and its block of columns
-  int64_t b = blockIdx.x, first = 0, count = 0;
-  int row = 0;
-  for (; row < a.rows; ++row) {
-    first = a.starts[row];
-    first = first < 0 ? 0 : first > a.tokens ? a.tokens : first;
-    const int64_t end = a.starts[row + 1] > a.tokens ? a.tokens : a.starts[row + 1];
-    count = end > first ? end - first : 0;
-    const int64_t n = (count * group + kCols - 1) / kCols;
-    if (b < n) break;
-    b -= n;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <bool BF>
+__device__ __forceinline__ f32x16 mma_32x32x16(const uint4& a, const uint4& b, f32x16 c) {
+  if constexpr (BF)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// 4 rows of 16 elements from LDS, transposed: lane i of 16 gives the address
+// of elements 4 (i % 4) .. + 3 of row i / 4 and gets element i of the rows.
+__device__ __forceinline__ uint2 read_transposed(const char* at) {
+  typedef __attribute__((address_space(3))) s16x4* lds_t;
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(at)));
+}
+
+// The query columns of a work-group: columns 128 b .. of row `row`, whose
+// tokens are first .. first + count - 1.  False where there are none.
+struct Block {
+  int row;
+  int64_t b, first, count;
+};
+
+__device__ __forceinline__ bool find_block(const ChunkArgs& a, int64_t b, int group, Block& out) {
+  const int lane = __lane_id();
+  for (int r0 = 0; r0 < a.rows; r0 += 64) {
+    const int r = r0 + lane;
+    int64_t first = 0, end = 0;
+    if (r < a.rows) {
+      first = a.starts[r], end = a.starts[r + 1];
+      first = first < 0 ? 0 : first > a.tokens ? a.tokens : first;
+      end = end > a.tokens ? a.tokens : end;
+    }
+    const int count = end > first ? (int)(end - first) : 0;
+    const int n = (int)(((int64_t)count * group + kCols - 1) / kCols);
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(upto, d, 64);
+      if (lane >= d) upto += y;
+    }
+    const uint64_t over = __ballot(b < upto);
+    if (over) {
+      const int l = __ffsll((unsigned long long)over) - 1;
+      out.row = r0 + l;
+      out.b = b - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
+      out.first = __builtin_amdgcn_readlane((int)first, l);
+      out.count = __builtin_amdgcn_readlane(count, l);
+      return true;
+    }
+    b -= __builtin_amdgcn_readlane(upto, 63);
   }
-  if (row == a.rows) return;
+  return false;
+}
+
+// out[t][h] = sum_p w_p v_p, w = softmax(scale q_t,h . k_p) over the positions
+// that token t sees, in one pass with the running maximum and sum.
+//
+// One work-group per kv head and 128 columns of a row, column c being head c %
+// group of the row's token c / group; one wave per 32 of them.  Tiles of kT
+// positions go through LDS, which all four waves read (straight from the L1
+// every wave loads every tile, 4 times the bytes that its rate allows beside
+// the products); the next tile is on its way in registers while one is worked
+// on.  As in WaveAttend both products are transposed, so that a column stays
+// the lane's own (lane & 31): a 32x32 result of K Q^T leaves lane (hf = lane /
+// 32) with positions 8 a + 4 hf + {0 .. 3}, and the second product takes 8 of
+// them at a step, with the values read through LDS's transposing load.
+//
+// The weights refer to a base that follows the running maximum only where it
+// has fallen 2^8 behind, so that most tiles rescale nothing; in fp16 they
+// carry a factor of 2^7 too, which keeps 2^-21 of the largest from being
+// subnormal and the largest below 2^15.
+template <bool BF, int HD>
+__global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_kernel(PagePool pp, ChunkArgs a) {
+  constexpr int kT = HD == 256 ? 32 : 64;   // positions of a tile
+  constexpr int RT = kT / 32, G = kT / 16;  // matrix rows of 32 positions; groups of 16, which lie on one page
+  constexpr int KS = HD / 16, DT = HD / 32;
+  constexpr int CPR = HD / 8;               // 16-byte pieces of a position
+  constexpr int NJ = kT * CPR / (64 * kWaves);
+  constexpr int kRow = HD * 2;
+  __shared__ __align__(16) char Ks[2][kT * kRow];
+  __shared__ __align__(16) char Vs[2][kT * kRow];
+  const int group = a.heads / a.kv_heads, g = blockIdx.x % a.kv_heads;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r32 = lane & 31, hf = lane >> 5;
+  const LaneX lx = lane_x_init();
+  Block blk;
+  if (!find_block(a, gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads, group, blk)) return;
+  const int row = blk.row;
+  const int64_t count = blk.count, columns = count * group;
   int len = pp.lengths[row];
   const int64_t most = (int64_t)pp.cols << pp.shift;
-  len = len > most ? (int)most : len;
-  const int64_t c = b * kCols + 16 * w + r16;
-  if (b * kCols + 16 * w >= count * group) return;  // a whole wave without columns
-  const bool live = c < count * group;
+  len = __builtin_amdgcn_readfirstlane(len > most ? (int)most : len);
+  const int64_t cw = blk.b * kCols + 32 * w, c = cw + r32;
+  const bool live = c < columns;
   const int64_t t = live ? c / group : count - 1;
   const int h = g * group + (int)(live ? c % group : 0);
-  const int last = len - (int)(count - t);  // may be negative: sees nothing
-  const Span s = span_of(last, a.window, a.sinks);
-  // the wave's columns together: the first and the last token's spans
-  const int64_t c0 = b * kCols + 16 * w, c1 = c0 + 15 < count * group ? c0 + 15 : count * group - 1;
-  const Span s0 = span_of(len - (int)(count - c0 / group), a.window, a.sinks);
-  const Span s1 = span_of(len - (int)(count - c1 / group), a.window, a.sinks);
-  const Span both{s0.low, s1.last, a.window > 0 ? (a.sinks < s0.low ? a.sinks : s0.low) : 0};
-  const TileList<kTile> tiles(both);
-  W wv;
-  wv.init();
-  wv.filled = len;
-  const uint16_t* qp = a.q + (first + t) * a.q_token + h * a.q_head;
+  const Span s = span_of(len - (int)(count - t), a.window, a.sinks);  // last may be negative: sees nothing
+  // the spans of the first and the last token of the wave and of the work-group
+  auto span_at = [&](int64_t col) {
+    const int64_t cc = col < columns ? col : columns - 1;
+    return span_of(len - (int)(count - cc / group), a.window, a.sinks);
+  };
+  const Span s0 = span_at(cw), s1 = span_at(cw + 31);
+  const Span g0 = span_at(blk.b * kCols), g1 = span_at(blk.b * kCols + kCols - 1);
+  const TileList<kT> tiles(Span{g0.low, g1.last, a.window > 0 ? (a.sinks < g0.low ? a.sinks : g0.low) : 0});
+  const int last_w = s1.last, low_w = s0.low, sinks_w = a.window > 0 ? (a.sinks < s0.low ? a.sinks : s0.low) : 0;
+  const bool any = cw < columns;
+  uint4 q[KS];
+  const uint16_t* qp = a.q + (blk.first + t) * a.q_token + h * a.q_head;
 #pragma unroll
-  for (int ks = 0; ks < W::KS; ++ks) wv.q[ks] = flipped(*reinterpret_cast<const uint4*>(qp + 32 * ks + 8 * qd), a.flip);
+  for (int ks = 0; ks < KS; ++ks) q[ks] = flipped(*reinterpret_cast<const uint4*>(qp + 16 * ks + 8 * hf), a.flip);
   const int32_t* trow = pp.table + row * pp.table_ld;
-  for (int u = 0; u < tiles.count; ++u) {
-    const int p0 = kTile * tiles.at(u);
-    const bool all = p0 + kTile - 1 <= s0.last && (p0 >= s1.low || p0 + kTile - 1 < s0.sinks);
-    wv.step(pp, trow, g, p0, s, all, a.scale, lx);
+
+  // a tile's entries: the page of each 16 positions, -1 for none
+  auto entries = [&](int u, int (&e)[G]) {
+    const int p0 = kT * tiles.at(u);
+#pragma unroll
+    for (int i = 0; i < G; ++i) {
+      const int col = (p0 + 16 * i) >> pp.shift;
+      const int x = col < pp.cols ? __builtin_amdgcn_readfirstlane(trow[col]) : -1;
+      e[i] = x >= 0 && x < pp.pages ? x : -1;
+    }
+  };
+  uint4 kr[NJ], vr[NJ];
+  const int mask = (1 << pp.shift) - 1;
+  auto fetch = [&](int u, const int (&e)[G]) {
+    const int p0 = kT * tiles.at(u);
+    bool whole = p0 + kT <= len;
+#pragma unroll
+    for (int i = 0; i < G; ++i) whole = whole && e[i] >= 0;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int flat = (j * kWaves + w) * 64, gi = flat / CPR / 16;
+      const int r = (flat + lane) / CPR, piece = (flat + lane) % CPR;
+      int id = e[0];
+#pragma unroll
+      for (int i = 1; i < G; ++i) id = gi == i ? e[i] : id;
+      const bool ok = id >= 0;
+      id = ok ? id : 0;
+      const int at = (p0 + r) & mask;
+      kr[j] = *reinterpret_cast<const uint4*>(pp.k + (int64_t)id * pp.k_page + g * pp.k_head + (int64_t)at * pp.k_pos + 8 * piece);
+      uint4 v = *reinterpret_cast<const uint4*>(pp.v + (int64_t)id * pp.v_page + g * pp.v_head + (int64_t)at * pp.v_pos + 8 * piece);
+      // what lies in a place that the row has not filled may be no number, and 0 times it would be none either
+      if (!whole) {
+        const bool filled = ok && p0 + r < len;
+        v.x = filled ? v.x : 0u, v.y = filled ? v.y : 0u, v.z = filled ? v.z : 0u, v.w = filled ? v.w : 0u;
+      }
+      vr[j] = v;
+    }
+  };
+  auto store = [&](int buf) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int flat = (j * kWaves + w) * 64 + lane, r = flat / CPR, piece = flat % CPR;
+      *reinterpret_cast<uint4*>(Ks[buf] + r * kRow + 16 * (piece ^ (r & (CPR < 16 ? 7 : 15)))) = kr[j];
+      *reinterpret_cast<uint4*>(Vs[buf] + r * kRow + 16 * (piece ^ (2 * (r & 3)))) = vr[j];
+    }
+  };
+
+  f32x16 o[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+  float top = -INFINITY, sum = 0.f;
+  int now[G], next[G];
+  if (tiles.count > 0) {
+    entries(0, now);
+    fetch(0, now);
+    if (tiles.count > 1) entries(1, next);
+    store(0);
   }
-  const float l = wv.total(lx), r = l == 0.f ? 0.f : 1.f / l;
+  __syncthreads();
+  for (int u = 0; u < tiles.count; ++u) {
+    const int p0 = kT * tiles.at(u), buf = u & 1;
+    const bool more = u + 1 < tiles.count;
+    int cur[G];
+#pragma unroll
+    for (int i = 0; i < G; ++i) cur[i] = now[i];
+    if (more) {
+      fetch(u + 1, next);
+#pragma unroll
+      for (int i = 0; i < G; ++i) now[i] = next[i];
+      if (u + 2 < tiles.count) entries(u + 2, next);
+    }
+    if (any && p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
+      f32x16 st[RT];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) st[r][i] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const uint4 kf = *reinterpret_cast<const uint4*>(Ks[buf] + (32 * r + r32) * kRow + 16 * ((2 * ks + hf) ^ (r32 & (CPR < 16 ? 7 : 15))));
+          st[r] = mma_32x32x16<BF>(kf, q[ks], st[r]);
+        }
+      bool all = p0 + kT - 1 <= s0.last && (p0 >= s1.low || p0 + kT - 1 < s0.sinks);
+#pragma unroll
+      for (int i = 0; i < G; ++i) all = all && cur[i] >= 0;
+      if (!all) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int p = p0 + 32 * r + 8 * (i / 4) + 4 * hf + i % 4;
+            const bool see = cur[2 * r + i / 8] >= 0 && p <= s.last && (p >= s.low || p < s.sinks);
+            st[r][i] = see ? st[r][i] : -INFINITY;
+          }
+      }
+      float mx = st[0][0];
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[r][i]);
+      mx = fmaxf(mx, lane_xor<32>(mx, lx));
+      // the base of the weights follows the maximum only where it has fallen 2^8 behind
+      if (__any((mx - top) * a.scale > 8.f)) {
+        const float up = fmaxf(mx, top), f = up == -INFINITY ? 1.f : weight(top - up, a.scale);
+        top = up;
+        sum *= f;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[d][i] *= f;
+      }
+      const float base = top == -INFINITY ? 0.f : top;
+      float back = BF ? -base * a.scale : __builtin_fmaf(-base, a.scale, 7.f);
+      if (__any(fabsf(base) > 1e36f)) {
+        // the product with scale could leave the range of fp32: the difference first
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st[r][i] -= base;
+        back = BF ? 0.f : 7.f;
+      }
+      uint4 pb[RT][2];
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float part = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          st[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r][i], a.scale, back));
+          part += st[r][i];
+        }
+        sum += part;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          pb[r][x] = make_uint4(pack16<BF>(st[r][8 * x], st[r][8 * x + 1]), pack16<BF>(st[r][8 * x + 2], st[r][8 * x + 3]),
+                                pack16<BF>(st[r][8 * x + 4], st[r][8 * x + 5]), pack16<BF>(st[r][8 * x + 6], st[r][8 * x + 7]));
+      }
+      // positions 32 r + 16 x + 4 hf + {0 .. 3, 8 .. 11} are this lane's operand of a step
+      const int i16 = lane & 15, vrow = 4 * hf + (i16 >> 2), flipv = 2 * (i16 >> 2);
+      const char* vbase = Vs[buf] + vrow * kRow + 8 * (i16 & 1);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+            const char* at = vbase + (32 * r + 16 * x) * kRow + 16 * (piece ^ flipv);
+            const uint2 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
+            o[d] = mma_32x32x16<BF>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[r][x], o[d]);
+          }
+    }
+    if (more) store(buf ^ 1);
+    __syncthreads();
+  }
+  float l = sum + lane_xor<32>(sum, lx);
+  const float rcp = l == 0.f ? 0.f : 1.f / l;
   if (!live) return;
-  uint16_t* to = a.out + (first + t) * a.out_token + (int64_t)h * HD + 4 * W::DPL * qd;
+  uint16_t* to = a.out + (blk.first + t) * a.out_token + (int64_t)h * HD;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int j = 0; j < W::DPL; j += 2)
-      *reinterpret_cast<uint32_t*>(to + W::DPL * i + j) = pack16<BF>(wv.o[j][i] * r, wv.o[j + 1][i] * r);
+    for (int i = 0; i < 16; i += 4)
+      *reinterpret_cast<uint2*>(to + 32 * d + 2 * i + 4 * hf) =
+          make_uint2(pack16<BF>(o[d][i] * rcp, o[d][i + 1] * rcp), pack16<BF>(o[d][i + 2] * rcp, o[d][i + 3] * rcp));
 }
 
 template <bool BF, int HD>
 int launch_chunk(const PagePool& pp, const ChunkArgs& a, hipStream_t stream) {
   const int64_t blocks = (a.tokens * (a.heads / a.kv_heads) + kCols - 1) / kCols + a.rows;
-  hipLaunchKernelGGL((attend_chunk_kernel<BF, HD>), dim3((unsigned)blocks, (unsigned)a.kv_heads), dim3(64 * kWavesC), 0, stream, pp, a);
+  hipLaunchKernelGGL((attend_chunk_kernel<BF, HD>), dim3((unsigned)(blocks * a.kv_heads)), dim3(64 * kWaves), 0, stream, pp, a);
   QS_LAUNCHED("attend_chunk_kernel");
   return QS_OK;
 }

@@ -1,6 +1,6 @@
-// Attention over a paged key-value cache: the page lookup and the step of one
-// wave that both attention kernels share (qs_attend_token.hip,
-// qs_attend_chunk.hip).
+// Attention over a paged key-value cache: what the kernels for single tokens
+// (qs_attend_token.hip) and for several (qs_attend_chunk.hip) share, and the
+// step of one wave for a single token.
 //
 // A cache page holds `page` positions (a power of two, 16 or more) of every
 // kv head: element (id, head, position, d) of the key pool is
@@ -95,7 +95,7 @@ __device__ __forceinline__ uint4 flipped(uint4 x, uint32_t flip) {
   return make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
 }
 
-// One wave's attention of 16 query columns (a head of a token each) over
+// One wave's attention of 16 query columns (the heads of a token) over
 // tiles of 32 positions, with the running maximum and sum of the softmax.
 //
 // Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T, so that
@@ -109,14 +109,13 @@ __device__ __forceinline__ uint4 flipped(uint4 x, uint32_t flip) {
 // j and puts halves together, and the dimension of operand row m of tile j is
 // DPL m + j.  Nothing goes through LDS.
 //
-// ONE: all columns are heads of one token and see the same positions.
-template <bool BF, int HD, bool ONE>
+// All columns are heads of one token and see the same positions.
+template <bool BF, int HD>
 struct WaveAttend {
   static constexpr int DPL = HD / 16;  // dimensions per lane of a value row
   static constexpr int KS = HD / 32;   // steps of the score product
   uint4 q[KS];
   f32x4 o[DPL];
-  int filled;      // positions that the row has filled
   float top, sum;  // of the products q k; the sum is over this lane's positions
 
   __device__ __forceinline__ void init() {
@@ -183,10 +182,9 @@ struct WaveAttend {
           const int p = p0 + 16 * t + 4 * qd + j;
           const bool see = ok[t] && p <= s.last && (p >= s.low || p < s.sinks);
           st[t][j] = see ? st[t][j] : -INFINITY;
-          // what lies in a place that the row has not filled may be no number, and 0 times it would be none either
-          const bool take = ONE ? see : ok[t] && p < filled;
+          // what lies in a place that is not seen may be no number, and 0 times it would be none either
 #pragma unroll
-          for (int i = 0; i < DPL / 2; ++i) vr[4 * t + j][i] = take ? vr[4 * t + j][i] : 0u;
+          for (int i = 0; i < DPL / 2; ++i) vr[4 * t + j][i] = see ? vr[4 * t + j][i] : 0u;
         }
     }
     float mx = fmaxf(fmaxf(fmaxf(st[0][0], st[0][1]), fmaxf(st[0][2], st[0][3])),

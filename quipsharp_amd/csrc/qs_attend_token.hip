@@ -26,7 +26,7 @@ struct TokenArgs {
 // wave by wave.
 template <bool BF, int HD>
 __global__ __launch_bounds__(64 * waves_of(HD)) void attend_token_kernel(PagePool pp, TokenArgs a) {
-  typedef WaveAttend<BF, HD, true> W;
+  typedef WaveAttend<BF, HD> W;
   constexpr int kWavesT = waves_of(HD);
   __shared__ float Os[kWavesT][16][HD + 4];
   __shared__ float Ms[kWavesT][16], Ls[kWavesT][16];
@@ -45,7 +45,6 @@ __global__ __launch_bounds__(64 * waves_of(HD)) void attend_token_kernel(PagePoo
   const int h0 = g * group + 16 * hb;
   W wv;
   wv.init();
-  wv.filled = len;
 #pragma unroll
   for (int ks = 0; ks < W::KS; ++ks) {
     wv.q[ks] = make_uint4(0, 0, 0, 0);
