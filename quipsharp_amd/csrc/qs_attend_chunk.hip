@@ -17,14 +17,14 @@ struct ChunkArgs {
   uint16_t* out;
   int64_t out_token;
   const int32_t* starts;
-  int64_t tokens;
-  int rows, heads, kv_heads, window, sinks;
+  int tokens, rows, heads, kv_heads, window, sinks;
   float scale;    // its size, times log2(e)
   uint32_t flip;  // its sign, for a pair of elements
 };
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 template <bool BF>
 __device__ __forceinline__ f32x16 mma_32x32x16(const uint4& a, const uint4& b, f32x16 c) {
@@ -44,22 +44,21 @@ __device__ __forceinline__ uint2 read_transposed(const char* at) {
 // The query columns of a work-group: columns 128 b .. of row `row`, whose
 // tokens are first .. first + count - 1.  False where there are none.
 struct Block {
-  int row;
-  int64_t b, first, count;
+  int row, b, first, count;
 };
 
-__device__ __forceinline__ bool find_block(const ChunkArgs& a, int64_t b, int group, Block& out) {
+__device__ __forceinline__ bool find_block(const ChunkArgs& a, int b, int group, Block& out) {
   const int lane = __lane_id();
   for (int r0 = 0; r0 < a.rows; r0 += 64) {
     const int r = r0 + lane;
-    int64_t first = 0, end = 0;
+    int first = 0, end = 0;
     if (r < a.rows) {
       first = a.starts[r], end = a.starts[r + 1];
       first = first < 0 ? 0 : first > a.tokens ? a.tokens : first;
       end = end > a.tokens ? a.tokens : end;
     }
-    const int count = end > first ? (int)(end - first) : 0;
-    const int n = (int)(((int64_t)count * group + kCols - 1) / kCols);
+    const int count = end > first ? end - first : 0;
+    const int n = (count * group + kCols - 1) / kCols;
     int upto = n;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -71,7 +70,7 @@ __device__ __forceinline__ bool find_block(const ChunkArgs& a, int64_t b, int gr
       const int l = __ffsll((unsigned long long)over) - 1;
       out.row = r0 + l;
       out.b = b - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
-      out.first = __builtin_amdgcn_readlane((int)first, l);
+      out.first = __builtin_amdgcn_readlane(first, l);
       out.count = __builtin_amdgcn_readlane(count, l);
       return true;
     }
@@ -103,8 +102,11 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   constexpr int RT = kT / 32, G = kT / 16;  // matrix rows of 32 positions; groups of 16, which lie on one page
   constexpr int KS = HD / 16, DT = HD / 32;
   constexpr int CPR = HD / 8;               // 16-byte pieces of a position
-  constexpr int NJ = kT * CPR / (64 * kWaves);
+  constexpr int RW = kT / kWaves;           // positions that a wave brings: on one page
+  constexpr int NJ = RW * CPR / 64;
+  constexpr int RJ = 64 / CPR;              // positions of one load of the wave
   constexpr int kRow = HD * 2;
+  constexpr int kSwz = CPR < 16 ? 7 : 15;
   __shared__ __align__(16) char Ks[2][kT * kRow];
   __shared__ __align__(16) char Vs[2][kT * kRow];
   const int group = a.heads / a.kv_heads, g = blockIdx.x % a.kv_heads;
@@ -112,75 +114,65 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   const LaneX lx = lane_x_init();
   Block blk;
   if (!find_block(a, gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads, group, blk)) return;
-  const int row = blk.row;
-  const int64_t count = blk.count, columns = count * group;
+  const int row = __builtin_amdgcn_readfirstlane(blk.row), count = __builtin_amdgcn_readfirstlane(blk.count), columns = count * group;
+  const int b0 = __builtin_amdgcn_readfirstlane(blk.b) * kCols;
   int len = pp.lengths[row];
   const int64_t most = (int64_t)pp.cols << pp.shift;
   len = __builtin_amdgcn_readfirstlane(len > most ? (int)most : len);
-  const int64_t cw = blk.b * kCols + 32 * w, c = cw + r32;
+  const int cw = b0 + 32 * w, c = cw + r32;
   const bool live = c < columns;
-  const int64_t t = live ? c / group : count - 1;
-  const int h = g * group + (int)(live ? c % group : 0);
-  const Span s = span_of(len - (int)(count - t), a.window, a.sinks);  // last may be negative: sees nothing
+  const int t = live ? c / group : count - 1;
+  const int h = g * group + (live ? c % group : 0);
+  const Span s = span_of(len - (count - t), a.window, a.sinks);  // last may be negative: sees nothing
   // the spans of the first and the last token of the wave and of the work-group
-  auto span_at = [&](int64_t col) {
-    const int64_t cc = col < columns ? col : columns - 1;
-    return span_of(len - (int)(count - cc / group), a.window, a.sinks);
+  auto span_at = [&](int col) {
+    const int cc = __builtin_amdgcn_readfirstlane(col < columns ? col : columns - 1);
+    return span_of(len - (count - cc / group), a.window, a.sinks);
   };
-  const Span s0 = span_at(cw), s1 = span_at(cw + 31);
-  const Span g0 = span_at(blk.b * kCols), g1 = span_at(blk.b * kCols + kCols - 1);
+  const Span s0 = span_at(cw), s1 = span_at(cw + 31);  // a wave without columns has the last token's
+  const Span g0 = span_at(b0), g1 = span_at(b0 + kCols - 1);
   const TileList<kT> tiles(Span{g0.low, g1.last, a.window > 0 ? (a.sinks < g0.low ? a.sinks : g0.low) : 0});
   const int last_w = s1.last, low_w = s0.low, sinks_w = a.window > 0 ? (a.sinks < s0.low ? a.sinks : s0.low) : 0;
-  const bool any = cw < columns;
   uint4 q[KS];
-  const uint16_t* qp = a.q + (blk.first + t) * a.q_token + h * a.q_head;
+  const uint16_t* qp = a.q + (int64_t)(blk.first + t) * a.q_token + h * a.q_head;
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) q[ks] = flipped(*reinterpret_cast<const uint4*>(qp + 16 * ks + 8 * hf), a.flip);
   const int32_t* trow = pp.table + row * pp.table_ld;
 
-  // a tile's entries: the page of each 16 positions, -1 for none
-  auto entries = [&](int u, int (&e)[G]) {
-    const int p0 = kT * tiles.at(u);
-#pragma unroll
-    for (int i = 0; i < G; ++i) {
-      const int col = (p0 + 16 * i) >> pp.shift;
-      const int x = col < pp.cols ? __builtin_amdgcn_readfirstlane(trow[col]) : -1;
-      e[i] = x >= 0 && x < pp.pages ? x : -1;
-    }
+  // lane i < G: the table's entry for positions 16 i .. of tile u
+  auto entry = [&](int u) {
+    const int col = (kT * tiles.at(u) + 16 * (lane < G ? lane : 0)) >> pp.shift;
+    return col < pp.cols ? trow[col] : -1;
   };
-  uint4 kr[NJ], vr[NJ];
-  const int mask = (1 << pp.shift) - 1;
-  auto fetch = [&](int u, const int (&e)[G]) {
+  // which groups of 16 positions have a page (bits), and the page of this wave's
+  auto valid = [&](int e) { return (unsigned)__ballot(lane < G && e >= 0 && e < pp.pages); };
+  constexpr unsigned kAll = (1u << G) - 1;
+  const int gw = w * RW / 16, mask = (1 << pp.shift) - 1;
+  const int rl = lane / CPR, piece = lane % CPR;  // this lane's position of a load and its piece of it
+  const unsigned ko = 2u * ((w * RW % 16 + rl) * pp.k_pos + 8 * piece), vo = 2u * ((w * RW % 16 + rl) * pp.v_pos + 8 * piece);
+  u32x4 kr[NJ], vr[NJ];
+  auto fetch = [&](int u, int e, unsigned ok) {
     const int p0 = kT * tiles.at(u);
-    bool whole = p0 + kT <= len;
+    const bool have = ok >> gw & 1;
+    const int64_t id = have ? __builtin_amdgcn_readlane(e, gw) : 0;
+    const int at = (p0 + 16 * gw) & mask;
+    const char* kb = reinterpret_cast<const char*>(pp.k + id * pp.k_page + g * pp.k_head + (int64_t)at * pp.k_pos);
+    const char* vb = reinterpret_cast<const char*>(pp.v + id * pp.v_page + g * pp.v_head + (int64_t)at * pp.v_pos);
 #pragma unroll
-    for (int i = 0; i < G; ++i) whole = whole && e[i] >= 0;
+    for (int j = 0; j < NJ; ++j) kr[j] = *reinterpret_cast<const u32x4*>(kb + (ko + 2u * j * RJ * pp.k_pos));
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) vr[j] = *reinterpret_cast<const u32x4*>(vb + (vo + 2u * j * RJ * pp.v_pos));
+  };
+  auto store = [&](int u, int buf, unsigned ok) {
+    // what lies in a place that the row has not filled may be no number, and 0 times it would be none either
+    const int fill = ok >> gw & 1 ? len - (kT * tiles.at(u) + w * RW) : 0;
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
-      const int flat = (j * kWaves + w) * 64, gi = flat / CPR / 16;
-      const int r = (flat + lane) / CPR, piece = (flat + lane) % CPR;
-      int id = e[0];
-#pragma unroll
-      for (int i = 1; i < G; ++i) id = gi == i ? e[i] : id;
-      const bool ok = id >= 0;
-      id = ok ? id : 0;
-      const int at = (p0 + r) & mask;
-      kr[j] = *reinterpret_cast<const uint4*>(pp.k + (int64_t)id * pp.k_page + g * pp.k_head + (int64_t)at * pp.k_pos + 8 * piece);
-      uint4 v = *reinterpret_cast<const uint4*>(pp.v + (int64_t)id * pp.v_page + g * pp.v_head + (int64_t)at * pp.v_pos + 8 * piece);
-      // what lies in a place that the row has not filled may be no number, and 0 times it would be none either
-      if (!whole) {
-        const bool filled = ok && p0 + r < len;
-        v.x = filled ? v.x : 0u, v.y = filled ? v.y : 0u, v.z = filled ? v.z : 0u, v.w = filled ? v.w : 0u;
-      }
-      vr[j] = v;
-    }
-  };
-  auto store = [&](int buf) {
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int flat = (j * kWaves + w) * 64 + lane, r = flat / CPR, piece = flat % CPR;
-      *reinterpret_cast<uint4*>(Ks[buf] + r * kRow + 16 * (piece ^ (r & (CPR < 16 ? 7 : 15)))) = kr[j];
-      *reinterpret_cast<uint4*>(Vs[buf] + r * kRow + 16 * (piece ^ (2 * (r & 3)))) = vr[j];
+      const int r = w * RW + j * RJ + rl;
+      *reinterpret_cast<u32x4*>(Ks[buf] + r * kRow + 16 * (piece ^ (r & kSwz))) = kr[j];
+      u32x4 v = vr[j];
+      if (fill < RW) v = j * RJ + rl < fill ? v : u32x4{0, 0, 0, 0};
+      *reinterpret_cast<u32x4*>(Vs[buf] + r * kRow + 16 * (piece ^ (2 * (r & 3)))) = v;
     }
   };
 
@@ -190,27 +182,23 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
   float top = -INFINITY, sum = 0.f;
-  int now[G], next[G];
+  unsigned ok = 0, ok_next = 0;
+  int e_next = 0;
   if (tiles.count > 0) {
-    entries(0, now);
-    fetch(0, now);
-    if (tiles.count > 1) entries(1, next);
-    store(0);
+    const int e = entry(0);
+    ok = valid(e);
+    fetch(0, e, ok);
+    e_next = entry(tiles.count > 1 ? 1 : 0);
+    store(0, 0, ok);
   }
   __syncthreads();
-  for (int u = 0; u < tiles.count; ++u) {
+  for (int u = 0; u < tiles.count; ++u, ok = ok_next) {
     const int p0 = kT * tiles.at(u), buf = u & 1;
-    const bool more = u + 1 < tiles.count;
-    int cur[G];
-#pragma unroll
-    for (int i = 0; i < G; ++i) cur[i] = now[i];
-    if (more) {
-      fetch(u + 1, next);
-#pragma unroll
-      for (int i = 0; i < G; ++i) now[i] = next[i];
-      if (u + 2 < tiles.count) entries(u + 2, next);
-    }
-    if (any && p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
+    const int next = u + 1 < tiles.count ? u + 1 : u;
+    ok_next = valid(e_next);
+    fetch(next, e_next, ok_next);
+    e_next = entry(u + 2 < tiles.count ? u + 2 : next);
+    if (p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
       f32x16 st[RT];
 #pragma unroll
       for (int r = 0; r < RT; ++r)
@@ -220,19 +208,17 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const uint4 kf = *reinterpret_cast<const uint4*>(Ks[buf] + (32 * r + r32) * kRow + 16 * ((2 * ks + hf) ^ (r32 & (CPR < 16 ? 7 : 15))));
+          const uint4 kf = *reinterpret_cast<const uint4*>(Ks[buf] + (32 * r + r32) * kRow + 16 * ((2 * ks + hf) ^ (r32 & kSwz)));
           st[r] = mma_32x32x16<BF>(kf, q[ks], st[r]);
         }
-      bool all = p0 + kT - 1 <= s0.last && (p0 >= s1.low || p0 + kT - 1 < s0.sinks);
-#pragma unroll
-      for (int i = 0; i < G; ++i) all = all && cur[i] >= 0;
+      const bool all = ok == kAll && p0 + kT - 1 <= s0.last && (p0 >= s1.low || p0 + kT - 1 < s0.sinks);
       if (!all) {
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int p = p0 + 32 * r + 8 * (i / 4) + 4 * hf + i % 4;
-            const bool see = cur[2 * r + i / 8] >= 0 && p <= s.last && (p >= s.low || p < s.sinks);
+            const bool see = (ok >> (2 * r + i / 8) & 1) && p <= s.last && (p >= s.low || p < s.sinks);
             st[r][i] = see ? st[r][i] : -INFINITY;
           }
       }
@@ -286,19 +272,19 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            const int piece = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
-            const char* at = vbase + (32 * r + 16 * x) * kRow + 16 * (piece ^ flipv);
+            const int pv = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+            const char* at = vbase + (32 * r + 16 * x) * kRow + 16 * (pv ^ flipv);
             const uint2 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
             o[d] = mma_32x32x16<BF>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[r][x], o[d]);
           }
     }
-    if (more) store(buf ^ 1);
+    store(next, buf ^ 1, ok_next);
     __syncthreads();
   }
   float l = sum + lane_xor<32>(sum, lx);
   const float rcp = l == 0.f ? 0.f : 1.f / l;
   if (!live) return;
-  uint16_t* to = a.out + (blk.first + t) * a.out_token + (int64_t)h * HD;
+  uint16_t* to = a.out + (int64_t)(blk.first + t) * a.out_token + (int64_t)h * HD;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -309,7 +295,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
 
 template <bool BF, int HD>
 int launch_chunk(const PagePool& pp, const ChunkArgs& a, hipStream_t stream) {
-  const int64_t blocks = (a.tokens * (a.heads / a.kv_heads) + kCols - 1) / kCols + a.rows;
+  const int64_t blocks = ((int64_t)a.tokens * (a.heads / a.kv_heads) + kCols - 1) / kCols + a.rows;
   hipLaunchKernelGGL((attend_chunk_kernel<BF, HD>), dim3((unsigned)(blocks * a.kv_heads)), dim3(64 * kWaves), 0, stream, pp, a);
   QS_LAUNCHED("attend_chunk_kernel");
   return QS_OK;
@@ -362,7 +348,7 @@ extern "C" int qs_attend_chunk(const void* q, int dtype, int64_t tokens, int64_t
              "qs_attend_chunk: query rows must be 16-byte aligned (strides %lld, %lld)", (long long)q_token, (long long)q_head);
   QS_REQUIRE(out_token >= (int64_t)heads * head_dim && out_token % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
              "qs_attend_chunk: output rows of %lld elements must be 16-byte aligned", (long long)out_token);
-  ChunkArgs a{static_cast<const uint16_t*>(q), q_token, q_head, static_cast<uint16_t*>(out), out_token, starts, tokens,
+  ChunkArgs a{static_cast<const uint16_t*>(q), q_token, q_head, static_cast<uint16_t*>(out), out_token, starts, (int)tokens,
               (int)rows, heads, kv_heads, window, sinks, fabsf(scale) * 1.44269504088896340736f, scale < 0 ? 0x80008000u : 0u};
   const bool bf = dtype == QS_DTYPE_BF16;
   const hipStream_t st = as_stream(stream);
