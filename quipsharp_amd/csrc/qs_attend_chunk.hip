@@ -24,7 +24,6 @@ struct ChunkArgs {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 template <bool BF>
 __device__ __forceinline__ f32x16 mma_32x32x16(const uint4& a, const uint4& b, f32x16 c) {
@@ -39,6 +38,18 @@ __device__ __forceinline__ f32x16 mma_32x32x16(const uint4& a, const uint4& b, f
 __device__ __forceinline__ uint2 read_transposed(const char* at) {
   typedef __attribute__((address_space(3))) s16x4* lds_t;
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(at)));
+}
+
+// 16 bytes per lane from base + off straight to LDS, at `lds` + 16 lane.  The
+// compiler does not count this load: wait_loads() before the barrier that
+// hands the bytes over.  (Its own form would have it wait for all such loads
+// before the next read of LDS, which here reads the other buffer.)
+__device__ __forceinline__ void load_to_lds(const char* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)(p);
 }
 
 // The query columns of a work-group: columns 128 b .. of row `row`, whose
@@ -131,7 +142,9 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   };
   const Span s0 = span_at(cw), s1 = span_at(cw + 31);  // a wave without columns has the last token's
   const Span g0 = span_at(b0), g1 = span_at(b0 + kCols - 1);
-  const TileList<kT> tiles(Span{g0.low, g1.last, a.window > 0 ? (a.sinks < g0.low ? a.sinks : g0.low) : 0});
+  TileList<kT> tiles(Span{g0.low, g1.last, a.window > 0 ? (a.sinks < g0.low ? a.sinks : g0.low) : 0});
+  tiles.sink = __builtin_amdgcn_readfirstlane(tiles.sink), tiles.low = __builtin_amdgcn_readfirstlane(tiles.low);
+  tiles.count = __builtin_amdgcn_readfirstlane(tiles.count);
   const int last_w = s1.last, low_w = s0.low, sinks_w = a.window > 0 ? (a.sinks < s0.low ? a.sinks : s0.low) : 0;
   uint4 q[KS];
   const uint16_t* qp = a.q + (int64_t)(blk.first + t) * a.q_token + h * a.q_head;
@@ -149,30 +162,43 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   constexpr unsigned kAll = (1u << G) - 1;
   const int gw = w * RW / 16, mask = (1 << pp.shift) - 1;
   const int rl = lane / CPR, piece = lane % CPR;  // this lane's position of a load and its piece of it
-  const unsigned ko = 2u * ((w * RW % 16 + rl) * pp.k_pos + 8 * piece), vo = 2u * ((w * RW % 16 + rl) * pp.v_pos + 8 * piece);
-  u32x4 kr[NJ], vr[NJ];
-  auto fetch = [&](int u, int e, unsigned ok) {
+  const unsigned k_lds = __builtin_amdgcn_readfirstlane(lds_address(Ks[0]) + w * RW * kRow);
+  const unsigned v_lds = __builtin_amdgcn_readfirstlane(lds_address(Vs[0]) + w * RW * kRow);
+  // Pieces lie swizzled in LDS (below), so a lane brings the piece that belongs at its place.
+  unsigned ko[NJ];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    const int r = w * RW + j * RJ + rl;
+    ko[j] = 2u * ((r & 15) * pp.k_pos + 8 * (piece ^ (r & kSwz)));
+  }
+  constexpr int NV = RJ % 4 == 0 ? 1 : 2;  // loads until the swizzle of the values comes round again
+  static_assert(NV * RJ % 4 == 0, "");
+  unsigned vo[NV];
+#pragma unroll
+  for (int j = 0; j < NV; ++j)
+    vo[j] = 2u * ((w * RW % 16 + rl) * pp.v_pos + 8 * (piece ^ 2 * ((j * RJ + rl) & 3)));
+  auto fetch = [&](int u, int buf, int e, unsigned ok) {
     const int p0 = kT * tiles.at(u);
-    const bool have = ok >> gw & 1;
-    const int64_t id = have ? __builtin_amdgcn_readlane(e, gw) : 0;
+    const int64_t id = ok >> gw & 1 ? __builtin_amdgcn_readlane(e, gw) : 0;
     const int at = (p0 + 16 * gw) & mask;
     const char* kb = reinterpret_cast<const char*>(pp.k + id * pp.k_page + g * pp.k_head + (int64_t)at * pp.k_pos);
     const char* vb = reinterpret_cast<const char*>(pp.v + id * pp.v_page + g * pp.v_head + (int64_t)at * pp.v_pos);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) kr[j] = *reinterpret_cast<const u32x4*>(kb + (ko + 2u * j * RJ * pp.k_pos));
+    for (int j = 0; j < NJ; ++j) load_to_lds(kb, ko[j], k_lds + buf * (kT * kRow) + 1024 * j);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) vr[j] = *reinterpret_cast<const u32x4*>(vb + (vo + 2u * j * RJ * pp.v_pos));
+    for (int j = 0; j < NJ; ++j)
+      load_to_lds(vb + (int64_t)2 * j * RJ * pp.v_pos, vo[j % NV], v_lds + buf * (kT * kRow) + 1024 * j);
   };
-  auto store = [&](int u, int buf, unsigned ok) {
-    // what lies in a place that the row has not filled may be no number, and 0 times it would be none either
+  // What lies in a place that the row has not filled may be no number, and 0
+  // times it would be none either: zeros there, by the wave that brought it.
+  auto clear = [&](int u, int buf, unsigned ok) {
     const int fill = ok >> gw & 1 ? len - (kT * tiles.at(u) + w * RW) : 0;
+    if (fill < RW) {
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const int r = w * RW + j * RJ + rl;
-      *reinterpret_cast<u32x4*>(Ks[buf] + r * kRow + 16 * (piece ^ (r & kSwz))) = kr[j];
-      u32x4 v = vr[j];
-      if (fill < RW) v = j * RJ + rl < fill ? v : u32x4{0, 0, 0, 0};
-      *reinterpret_cast<u32x4*>(Vs[buf] + r * kRow + 16 * (piece ^ (2 * (r & 3)))) = v;
+      for (int j = 0; j < NJ; ++j) {
+        const int r = j * RJ + rl;
+        if (r >= fill) *reinterpret_cast<uint4*>(Vs[buf] + (w * RW + r) * kRow + 16 * piece) = make_uint4(0, 0, 0, 0);
+      }
     }
   };
 
@@ -187,16 +213,17 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   if (tiles.count > 0) {
     const int e = entry(0);
     ok = valid(e);
-    fetch(0, e, ok);
+    fetch(0, 0, e, ok);
     e_next = entry(tiles.count > 1 ? 1 : 0);
-    store(0, 0, ok);
+    wait_loads();
+    clear(0, 0, ok);
   }
   __syncthreads();
   for (int u = 0; u < tiles.count; ++u, ok = ok_next) {
     const int p0 = kT * tiles.at(u), buf = u & 1;
     const int next = u + 1 < tiles.count ? u + 1 : u;
     ok_next = valid(e_next);
-    fetch(next, e_next, ok_next);
+    fetch(next, buf ^ 1, e_next, ok_next);
     e_next = entry(u + 2 < tiles.count ? u + 2 : next);
     if (p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
       f32x16 st[RT];
@@ -278,7 +305,8 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
             o[d] = mma_32x32x16<BF>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[r][x], o[d]);
           }
     }
-    store(next, buf ^ 1, ok_next);
+    wait_loads();
+    clear(next, buf ^ 1, ok_next);
     __syncthreads();
   }
   float l = sum + lane_xor<32>(sum, lx);

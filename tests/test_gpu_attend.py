@@ -191,6 +191,22 @@ def test_layouts_and_strides(dev, kind):
     assert not room[:, :512].any() and not room[:, 512 + heads * 128:].any()
 
 
+@pytest.mark.parametrize("dim,pad_k,pad_v", [(64, 8, 24), (128, 8, 40), (256, 72, 8)])
+def test_padded_positions(dev, dim, pad_k, pad_v):
+    """Positions that lie further apart than their elements need, keys and values each in their own way."""
+    from quipsharp_amd.pages import attend_chunk, attend_token
+    c = Cache([150, 37], 2, dim, 16, torch.bfloat16, 13)
+    k = torch.full(tuple(c.k.shape[:3]) + (dim + pad_k,), math.nan, dtype=torch.bfloat16, device=dev)[..., :dim]
+    v = torch.full(tuple(c.v.shape[:3]) + (dim + pad_v,), math.nan, dtype=torch.bfloat16, device=dev)[..., pad_v:]
+    k.copy_(c.k)
+    v.copy_(c.v)
+    _, _, table, n = c.to(dev)
+    q = torch.randn(70, 6, dim, generator=torch.Generator().manual_seed(1)).bfloat16().to(dev)
+    check(attend_token(q[:2], k, v, table, n), q[:2], c, [(0, 149), (1, 36)], dim ** -0.5, 0, 0)
+    got = attend_chunk(q, k, v, table, n, torch.tensor([0, 60, 70], dtype=torch.int32, device=dev))
+    check(got, q, c, [(0, 90 + i) for i in range(60)] + [(1, 27 + i) for i in range(10)], dim ** -0.5, 0, 0)
+
+
 @pytest.mark.parametrize("kind", ["token", "chunk"])
 def test_pages_out_of_the_window_may_be_gone(dev, kind):
     """Entries that no query of the call looks at may be -1 or name no page."""
