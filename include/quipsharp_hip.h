@@ -444,6 +444,15 @@ int qs_attend_token(const void *q, int dtype, int64_t rows, int heads, int kv_he
 int qs_attend_chunk(const void *q, int dtype, int64_t tokens, int64_t rows, int heads, int kv_heads, int head_dim,
                     int64_t q_token, int64_t q_head, const int32_t *starts, const qs_page_pool *pool, float scale,
                     int window, int sinks, void *out, int64_t out_token, qs_stream_t stream);
+/* With a workspace of qs_attend_chunk_workspace_bytes (0: no use for one) the
+ * positions of few tokens are shared by more work-groups; without one
+ * (NULL) it runs as qs_attend_chunk. */
+size_t qs_attend_chunk_workspace_bytes(int64_t tokens, int64_t rows, int heads, int kv_heads, int head_dim,
+                                       int64_t cols, int page, int window, int sinks);
+int qs_attend_chunk_ws(const void *q, int dtype, int64_t tokens, int64_t rows, int heads, int kv_heads, int head_dim,
+                       int64_t q_token, int64_t q_head, const int32_t *starts, const qs_page_pool *pool, float scale,
+                       int window, int sinks, void *out, int64_t out_token, void *workspace, size_t workspace_bytes,
+                       qs_stream_t stream);
 
 /* The whole cache of a model, for the calls that move pages: `planes` (keys
  * and values of every layer) of [pages][kv_heads][page][row_bytes], one after

@@ -113,6 +113,9 @@ _SIGNATURES = {
                          ctypes.c_size_t, _vp], _int),
     "qs_attend_chunk": ([_vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _vp, _pool_p, _f32, _int, _int, _vp,
                          _i64, _vp], _int),
+    "qs_attend_chunk_workspace_bytes": ([_i64, _i64, _int, _int, _int, _i64, _int, _int, _int], ctypes.c_size_t),
+    "qs_attend_chunk_ws": ([_vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _vp, _pool_p, _f32, _int, _int, _vp,
+                            _i64, _vp, ctypes.c_size_t, _vp], _int),
     "qs_page_advance_workspace_bytes": ([_i64], ctypes.c_size_t),
     "qs_page_advance": ([_store_p, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
                          _vp], _int),

@@ -18,6 +18,8 @@ struct ChunkArgs {
   int64_t out_token;
   const int32_t* starts;
   int tokens, rows, heads, kv_heads, window, sinks;
+  float* part;
+  int splits;
   float scale;    // its size, times log2(e)
   uint32_t flip;  // its sign, for a pair of elements
 };
@@ -40,54 +42,93 @@ __device__ __forceinline__ uint2 read_transposed(const char* at) {
   return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_t)(at)));
 }
 
-// 16 bytes per lane from base + off straight to LDS, at `lds` + 16 lane.  The
-// compiler does not count this load: wait_loads() before the barrier that
-// hands the bytes over.  (Its own form would have it wait for all such loads
-// before the next read of LDS, which here reads the other buffer.)
-__device__ __forceinline__ void load_to_lds(const char* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
-}
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
-__device__ __forceinline__ unsigned lds_address(const void* p) {
-  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)(p);
+__device__ __forceinline__ int wave_total(int v, LaneX lx) {
+  auto other = [&](auto x) { return __builtin_bit_cast(int, x); };
+  auto f = [&]() { return __builtin_bit_cast(float, v); };
+  v += other(lane_xor<32>(f(), lx));
+  v += other(lane_xor<16>(f(), lx));
+  v += other(lane_xor<8>(f(), lx));
+  v += other(lane_xor<4>(f(), lx));
+  v += other(lane_xor<2>(f(), lx));
+  v += other(lane_xor<1>(f(), lx));
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
 // The query columns of a work-group: columns 128 b .. of row `row`, whose
-// tokens are first .. first + count - 1.  False where there are none.
+// tokens are first .. first + count - 1.
 struct Block {
   int row, b, first, count;
 };
 
-__device__ __forceinline__ bool find_block(const ChunkArgs& a, int b, int group, Block& out) {
+// The k-th block of the call, those that end at the latest position first: a
+// long one that begins last would have the chip wait for it.  False where
+// there are fewer.  The block at hand is found by its end: the largest x such
+// that more than k blocks end at x or beyond.
+__device__ __forceinline__ bool find_block(const ChunkArgs& a, const PagePool& pp, int k, int group, LaneX lx, Block& out) {
   const int lane = __lane_id();
-  for (int r0 = 0; r0 < a.rows; r0 += 64) {
-    const int r = r0 + lane;
-    int first = 0, end = 0;
+  // a lane's row: its tokens, its blocks, the position of its first token
+  int first, count, n, p0;
+  auto row_of = [&](int r) {
+    first = count = n = p0 = 0;
     if (r < a.rows) {
-      first = a.starts[r], end = a.starts[r + 1];
+      int end = a.starts[r + 1];
+      first = a.starts[r];
       first = first < 0 ? 0 : first > a.tokens ? a.tokens : first;
       end = end > a.tokens ? a.tokens : end;
+      count = end > first ? end - first : 0;
+      n = (count * group + kCols - 1) / kCols;
+      const int64_t most = (int64_t)pp.cols << pp.shift;
+      const int len = pp.lengths[r];
+      p0 = (len < 0 ? 0 : len > most ? (int)most : len) - count;
     }
-    const int count = end > first ? end - first : 0;
-    const int n = (count * group + kCols - 1) / kCols;
-    int upto = n;
+  };
+  // how many of the row's blocks end at position x or beyond
+  auto from = [&](int x) {
+    const int t = x - p0;  // from this token on
+    return t <= 0 ? n : t >= count ? 0 : n - t * group / kCols;
+  };
+  const int rounds = (a.rows + 63) / 64;
+  auto blocks_from = [&](int x) {
+    int v = 0;
+    for (int i = 0; i < rounds; ++i) {
+      if (rounds > 1) row_of(64 * i + lane);
+      v += from(x);
+    }
+    return wave_total(v, lx);
+  };
+  row_of(lane);
+  if (a.rows == 1) {
+    out = Block{0, __builtin_amdgcn_readfirstlane(n) - 1 - k, __builtin_amdgcn_readfirstlane(first), __builtin_amdgcn_readfirstlane(count)};
+    return out.b >= 0;
+  }
+  // blocks_from(lo) > k >= blocks_from(hi)
+  int lo = -a.tokens, hi = (int)((int64_t)pp.cols << pp.shift) + 1;
+  if (k >= blocks_from(lo)) return false;
+  while (hi - lo > 1) {
+    const int mid = lo + (hi - lo) / 2;
+    if (blocks_from(mid) > k) lo = mid; else hi = mid;
+  }
+  k -= blocks_from(hi);  // among those that end at lo, by row
+  for (int i = 0;; ++i) {
+    if (rounds > 1) row_of(64 * i + lane);
+    const int beyond = from(hi), here = from(lo) - beyond;
+    int upto = here;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const int y = __shfl_up(upto, d, 64);
       if (lane >= d) upto += y;
     }
-    const uint64_t over = __ballot(b < upto);
+    const uint64_t over = __ballot(k < upto);
     if (over) {
       const int l = __ffsll((unsigned long long)over) - 1;
-      out.row = r0 + l;
-      out.b = b - (__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(n, l));
+      out.row = 64 * i + l;
+      out.b = __builtin_amdgcn_readlane(n - beyond - here + upto, l) - 1 - k;
       out.first = __builtin_amdgcn_readlane(first, l);
       out.count = __builtin_amdgcn_readlane(count, l);
       return true;
     }
-    b -= __builtin_amdgcn_readlane(upto, 63);
+    k -= __builtin_amdgcn_readlane(upto, 63);
   }
-  return false;
 }
 
 // out[t][h] = sum_p w_p v_p, w = softmax(scale q_t,h . k_p) over the positions
@@ -124,7 +165,8 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r32 = lane & 31, hf = lane >> 5;
   const LaneX lx = lane_x_init();
   Block blk;
-  if (!find_block(a, gridDim.x / a.kv_heads - 1 - blockIdx.x / a.kv_heads, group, blk)) return;
+  if (!find_block(a, pp, blockIdx.x / a.kv_heads, group, lx, blk)) return;
+  const int split = blockIdx.y;
   const int row = __builtin_amdgcn_readfirstlane(blk.row), count = __builtin_amdgcn_readfirstlane(blk.count), columns = count * group;
   const int b0 = __builtin_amdgcn_readfirstlane(blk.b) * kCols;
   int len = pp.lengths[row];
@@ -146,6 +188,8 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   tiles.sink = __builtin_amdgcn_readfirstlane(tiles.sink), tiles.low = __builtin_amdgcn_readfirstlane(tiles.low);
   tiles.count = __builtin_amdgcn_readfirstlane(tiles.count);
   const int last_w = s1.last, low_w = s0.low, sinks_w = a.window > 0 ? (a.sinks < s0.low ? a.sinks : s0.low) : 0;
+  // this split's share of the tiles
+  const int u0 = (int)((int64_t)split * tiles.count / a.splits), n = (int)((int64_t)(split + 1) * tiles.count / a.splits);
   uint4 q[KS];
   const uint16_t* qp = a.q + (int64_t)(blk.first + t) * a.q_token + h * a.q_head;
 #pragma unroll
@@ -202,6 +246,9 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
     }
   };
 
+  const int i16 = lane & 15;
+  const unsigned k_at = r32 * kRow + 16 * (hf ^ (r32 & kSwz));
+  const unsigned v_at = (4 * hf + (i16 >> 2)) * kRow + 16 * ((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ 2 * (i16 >> 2)) + 8 * (i16 & 1);
   f32x16 o[DT];
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -210,22 +257,24 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   float top = -INFINITY, sum = 0.f;
   unsigned ok = 0, ok_next = 0;
   int e_next = 0;
-  if (tiles.count > 0) {
-    const int e = entry(0);
+  if (u0 < n) {
+    const int e = entry(u0);
     ok = valid(e);
-    fetch(0, 0, e, ok);
-    e_next = entry(tiles.count > 1 ? 1 : 0);
-    wait_loads();
-    clear(0, 0, ok);
+    fetch(u0, u0 & 1, e, ok);
+    e_next = entry(u0 + 1 < n ? u0 + 1 : u0);
+    wait_loads<0>();
+    clear(u0, u0 & 1, ok);
   }
   __syncthreads();
-  for (int u = 0; u < tiles.count; ++u, ok = ok_next) {
+  for (int u = u0; u < n; ++u, ok = ok_next) {
     const int p0 = kT * tiles.at(u), buf = u & 1;
-    const int next = u + 1 < tiles.count ? u + 1 : u;
+    const int next = u + 1 < n ? u + 1 : u;
     ok_next = valid(e_next);
     fetch(next, buf ^ 1, e_next, ok_next);
-    e_next = entry(u + 2 < tiles.count ? u + 2 : next);
+    e_next = entry(u + 2 < n ? u + 2 : next);
     if (p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
+      unsigned ka = k_at, va = v_at;
+      asm volatile("" : "+v"(ka), "+v"(va));  // the addresses made of these are not kept over the loop
       f32x16 st[RT];
 #pragma unroll
       for (int r = 0; r < RT; ++r)
@@ -235,17 +284,19 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
-          const uint4 kf = *reinterpret_cast<const uint4*>(Ks[buf] + (32 * r + r32) * kRow + 16 * ((2 * ks + hf) ^ (r32 & kSwz)));
+          const uint4 kf = *reinterpret_cast<const uint4*>(Ks[buf] + 32 * r * kRow + (ka ^ 32 * ks));
           st[r] = mma_32x32x16<BF>(kf, q[ks], st[r]);
         }
       const bool all = ok == kAll && p0 + kT - 1 <= s0.last && (p0 >= s1.low || p0 + kT - 1 < s0.sinks);
       if (!all) {
+        // the span from this lane's first position on
+        const int at = p0 + 4 * hf, hi = s.last - at, lo = s.low - at, sk = s.sinks - at;
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const int p = p0 + 32 * r + 8 * (i / 4) + 4 * hf + i % 4;
-            const bool see = (ok >> (2 * r + i / 8) & 1) && p <= s.last && (p >= s.low || p < s.sinks);
+            const int p = 32 * r + 8 * (i / 4) + i % 4;
+            const bool see = p <= (ok >> (2 * r + i / 8) & 1 ? hi : -1) && (p >= lo || p < sk);
             st[r][i] = see ? st[r][i] : -INFINITY;
           }
       }
@@ -291,27 +342,34 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
                                 pack16<BF>(st[r][8 * x + 4], st[r][8 * x + 5]), pack16<BF>(st[r][8 * x + 6], st[r][8 * x + 7]));
       }
       // positions 32 r + 16 x + 4 hf + {0 .. 3, 8 .. 11} are this lane's operand of a step
-      const int i16 = lane & 15, vrow = 4 * hf + (i16 >> 2), flipv = 2 * (i16 >> 2);
-      const char* vbase = Vs[buf] + vrow * kRow + 8 * (i16 & 1);
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int x = 0; x < 2; ++x)
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            const int pv = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
-            const char* at = vbase + (32 * r + 16 * x) * kRow + 16 * (pv ^ flipv);
+            const char* at = Vs[buf] + (32 * r + 16 * x) * kRow + (va ^ 64 * d);
             const uint2 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
             o[d] = mma_32x32x16<BF>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[r][x], o[d]);
           }
     }
-    wait_loads();
+    wait_loads<0>();
     clear(next, buf ^ 1, ok_next);
     __syncthreads();
   }
-  float l = sum + lane_xor<32>(sum, lx);
-  const float rcp = l == 0.f ? 0.f : 1.f / l;
+  const float l = sum + lane_xor<32>(sum, lx);
   if (!live) return;
+  if (a.splits > 1) {
+    float* to = a.part + (((int64_t)(blk.first + t) * a.heads + h) * a.splits + split) * part_floats(HD);
+    if (hf == 0) to[0] = top, to[1] = l;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2)
+        *reinterpret_cast<float2*>(to + kPartHead + 32 * d + 2 * (i & ~3) + 4 * hf + i % 4) = make_float2(o[d][i], o[d][i + 1]);
+    return;
+  }
+  const float rcp = l == 0.f ? 0.f : 1.f / l;
   uint16_t* to = a.out + (int64_t)(blk.first + t) * a.out_token + (int64_t)h * HD;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
@@ -321,11 +379,29 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
           make_uint2(pack16<BF>(o[d][i] * rcp, o[d][i + 1] * rcp), pack16<BF>(o[d][i + 2] * rcp, o[d][i + 3] * rcp));
 }
 
+int64_t chunk_blocks(int64_t tokens, int64_t rows, int heads, int kv_heads) {
+  return (tokens * (heads / kv_heads) + kCols - 1) / kCols + rows;
+}
+
+// Into how many shares the tiles of a block are cut.  A share is a work-group;
+// two of them fill a CU, so cutting pays where the blocks' heads are fewer
+// than the chip's 512 places, and shares of less than 4 tiles do not repay the
+// second launch that joins them (16 tokens of 8 kv heads over 6000 positions:
+// %%A us whole, %%B us in shares; a prompt of 512 with 64 heads: %%C us whole,
+// %%D us in two).
+int chunk_splits(int64_t tokens, int64_t rows, int heads, int kv_heads, int64_t cols, int page, int window, int sinks) {
+  const int64_t blocks = (tokens * (heads / kv_heads) + kCols - 1) / kCols, wgs = blocks * kv_heads;
+  const int64_t seen = seen_positions(cols * page, window, sinks, (tokens - 1 < kCols ? tokens - 1 : kCols));
+  const int64_t most = seen / 512, n = 256 / wgs;
+  return (int)(n < 2 || most < 2 ? 1 : n < most ? n : most);
+}
+
 template <bool BF, int HD>
 int launch_chunk(const PagePool& pp, const ChunkArgs& a, hipStream_t stream) {
-  const int64_t blocks = ((int64_t)a.tokens * (a.heads / a.kv_heads) + kCols - 1) / kCols + a.rows;
-  hipLaunchKernelGGL((attend_chunk_kernel<BF, HD>), dim3((unsigned)(blocks * a.kv_heads)), dim3(64 * kWaves), 0, stream, pp, a);
+  const int64_t blocks = chunk_blocks(a.tokens, a.rows, a.heads, a.kv_heads);
+  hipLaunchKernelGGL((attend_chunk_kernel<BF, HD>), dim3((unsigned)(blocks * a.kv_heads), (unsigned)a.splits), dim3(64 * kWaves), 0, stream, pp, a);
   QS_LAUNCHED("attend_chunk_kernel");
+  if (a.splits > 1) return join_parts(a.part, a.splits, a.tokens, a.heads, HD, BF, a.scale, a.out, a.out_token, stream);
   return QS_OK;
 }
 
@@ -363,10 +439,25 @@ int page_pool_checks(const char* fn, const qs_page_pool* p, int dtype, int64_t r
 
 using namespace qs;
 
+extern "C" size_t qs_attend_chunk_workspace_bytes(int64_t tokens, int64_t rows, int heads, int kv_heads, int head_dim,
+                                                  int64_t cols, int page, int window, int sinks) {
+  if (tokens < 1 || rows < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || cols < 1 || page < 1) return 0;
+  const int n = chunk_splits(tokens, rows, heads, kv_heads, cols, page, window, sinks);
+  return n == 1 ? 0 : (size_t)tokens * heads * n * part_floats(head_dim) * sizeof(float);
+}
+
 extern "C" int qs_attend_chunk(const void* q, int dtype, int64_t tokens, int64_t rows, int heads, int kv_heads,
                                int head_dim, int64_t q_token, int64_t q_head, const int32_t* starts,
                                const qs_page_pool* pool, float scale, int window, int sinks, void* out,
                                int64_t out_token, qs_stream_t stream) {
+  return qs_attend_chunk_ws(q, dtype, tokens, rows, heads, kv_heads, head_dim, q_token, q_head, starts, pool, scale,
+                            window, sinks, out, out_token, nullptr, 0, stream);
+}
+
+extern "C" int qs_attend_chunk_ws(const void* q, int dtype, int64_t tokens, int64_t rows, int heads, int kv_heads,
+                                  int head_dim, int64_t q_token, int64_t q_head, const int32_t* starts,
+                                  const qs_page_pool* pool, float scale, int window, int sinks, void* out,
+                                  int64_t out_token, void* workspace, size_t workspace_bytes, qs_stream_t stream) {
   if (tokens == 0 || rows == 0) return QS_OK;
   PagePool pp;
   if (const int rc = page_pool_checks("qs_attend_chunk", pool, dtype, rows, heads, kv_heads, head_dim, scale, window, sinks, pp)) return rc;
@@ -376,8 +467,12 @@ extern "C" int qs_attend_chunk(const void* q, int dtype, int64_t tokens, int64_t
              "qs_attend_chunk: query rows must be 16-byte aligned (strides %lld, %lld)", (long long)q_token, (long long)q_head);
   QS_REQUIRE(out_token >= (int64_t)heads * head_dim && out_token % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0,
              "qs_attend_chunk: output rows of %lld elements must be 16-byte aligned", (long long)out_token);
+  const size_t need = qs_attend_chunk_workspace_bytes(tokens, rows, heads, kv_heads, head_dim, pool->cols, pool->page, window, sinks);
+  QS_REQUIRE(!workspace || (workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+             "qs_attend_chunk: workspace of %zu bytes (16-byte aligned), %zu needed", workspace_bytes, need);
+  const int splits = workspace && need ? chunk_splits(tokens, rows, heads, kv_heads, pool->cols, pool->page, window, sinks) : 1;
   ChunkArgs a{static_cast<const uint16_t*>(q), q_token, q_head, static_cast<uint16_t*>(out), out_token, starts, (int)tokens,
-              (int)rows, heads, kv_heads, window, sinks, fabsf(scale) * 1.44269504088896340736f, scale < 0 ? 0x80008000u : 0u};
+              (int)rows, heads, kv_heads, window, sinks, static_cast<float*>(workspace), splits, fabsf(scale) * 1.44269504088896340736f, scale < 0 ? 0x80008000u : 0u};
   const bool bf = dtype == QS_DTYPE_BF16;
   const hipStream_t st = as_stream(stream);
   if (head_dim == 64) return bf ? launch_chunk<true, 64>(pp, a, st) : launch_chunk<false, 64>(pp, a, st);

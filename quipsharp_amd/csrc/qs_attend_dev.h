@@ -16,6 +16,8 @@ namespace qs {
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 struct PagePool {
   const uint16_t *k, *v;
@@ -95,6 +97,21 @@ __device__ __forceinline__ uint4 flipped(uint4 x, uint32_t flip) {
   return make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
 }
 
+// 16 bytes per lane from base + off straight to LDS, at `lds` + 16 lane.  The
+// compiler does not count this load: wait_loads before the bytes are read.
+// (Its own form would have it wait for all such loads before the next read of
+// LDS, whatever place that reads.)
+__device__ __forceinline__ void load_to_lds(const char* base, unsigned off, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+}
+// All but the last N of the wave's loads are there (loads that are written in
+// the program between two of these calls stay between them).
+template <int N>
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+__device__ __forceinline__ unsigned lds_address(const void* p) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) const char*)(p);
+}
+
 // One wave's attention of 16 query columns (the heads of a token) over
 // tiles of 32 positions, with the running maximum and sum of the softmax.
 //
@@ -104,83 +121,104 @@ __device__ __forceinline__ uint4 flipped(uint4 x, uint32_t flip) {
 // + j of each 16, which is what it hands to the second product as its 8 of 32
 // positions -- the order of the positions inside a sum is free -- and the
 // maximum, the sum and the rescaling of O are the lane's own registers.
-// Values are read as they lie, 16 lanes to a row; the operand wants 8
-// positions of one dimension, so the lane takes rows 4 qd + j and 16 + 4 qd +
-// j and puts halves together, and the dimension of operand row m of tile j is
-// DPL m + j.  Nothing goes through LDS.
 //
-// All columns are heads of one token and see the same positions.
-template <bool BF, int HD>
+// The loads are the whole cost, so each of them takes whole rows: keys go
+// straight to the wave's own part of LDS (a lane's operand is 16 bytes of each
+// of 16 rows, and loads in that shape took 288 us instead of 281 over 1.6 GB,
+// 10.3 instead of 7.2 us over 577 positions), values lie as they are used, 16
+// lanes to a row: the operand wants 8 positions of one dimension, so the lane
+// takes rows 4 qd + j and 16 + 4 qd + j and puts halves together, and the
+// dimension of operand row m of tile j is DPL m + j.
+//
+// All columns are heads of one token and see the same positions.  NT: values
+// are loaded past the caches.
+template <bool BF, int HD, bool NT>
 struct WaveAttend {
-  static constexpr int DPL = HD / 16;  // dimensions per lane of a value row
-  static constexpr int KS = HD / 32;   // steps of the score product
+  static constexpr int DPL = HD / 16;   // dimensions per lane of a value row
+  static constexpr int KS = HD / 32;    // steps of the score product
+  static constexpr int kRow = HD * 2;   // bytes of a position in LDS
+  static constexpr int kKeys = 32 * kRow;
+  static constexpr int CPR = HD / 8;    // 16-byte pieces of a position
+  static constexpr int NJ = 16 * CPR / 64, RJ = 64 / CPR;  // loads of 16 positions, positions of a load
+  static constexpr int kSwz = CPR < 16 ? 7 : 15;
+  static constexpr int NV = DPL == 4 ? 8 : DPL;  // loads of the values
   uint4 q[KS];
   f32x4 o[DPL];
-  float top, sum;  // of the products q k; the sum is over this lane's positions
+  float top, sum;   // of the products q k; the sum is over this lane's positions
+  unsigned ko[NJ];  // where the lane's piece of a load lies behind the first of 16 positions
+  unsigned lds;     // the wave's part
+  const char* keys;
 
-  __device__ __forceinline__ void init() {
+  __device__ __forceinline__ void init(const PagePool& pp, const char* at) {
+    const int lane = __lane_id();
 #pragma unroll
     for (int j = 0; j < DPL; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
     top = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      const int r = j * RJ + lane / CPR;
+      ko[j] = 2u * (r * pp.k_pos + 8 * ((lane % CPR) ^ (r & kSwz)));
+    }
+    keys = at;
+    lds = __builtin_amdgcn_readfirstlane(lds_address(at));
   }
 
-  // Positions p0 .. p0 + 31 (p0 a multiple of 32) of kv head g; s is the
-  // column's span, `all` (uniform) that every column sees every position.
-  __device__ __forceinline__ void step(const PagePool& pp, const int32_t* trow, int g, int p0, const Span& s, bool all,
+  // Positions p0 .. p0 + 31 (p0 a multiple of 32) of kv head g, the pages of
+  // whose halves are e (-1: none); s is the columns' span, `all` that it
+  // holds every position.  e, p0, s and all are the same for the whole wave.
+  __device__ __forceinline__ void step(const PagePool& pp, const int (&e)[2], int g, int p0, const Span& s, bool all,
                                        float scale, LaneX lx) {
     const int lane = __lane_id(), r16 = lane & 15, qd = lane >> 4;
     const int mask = (1 << pp.shift) - 1;
-    int64_t id[2];
-    bool ok[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int col = (p0 + 16 * t) >> pp.shift;
-      const int e = col < pp.cols ? trow[col] : -1;
-      ok[t] = e >= 0 && e < pp.pages;
-      id[t] = ok[t] ? e : 0;
+      const int64_t id = e[t] < 0 ? 0 : e[t];
+      const char* kb = reinterpret_cast<const char*>(pp.k + id * pp.k_page + g * pp.k_head + (int64_t)((p0 + 16 * t) & mask) * pp.k_pos);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) load_to_lds(kb, ko[j], lds + 16 * t * kRow + 1024 * j);
     }
-    uint4 kf[2][KS];
     uint32_t vr[8][DPL / 2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const uint16_t* kb = pp.k + id[t] * pp.k_page + g * pp.k_head + (int64_t)((p0 + 16 * t) & mask) * pp.k_pos;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-        kf[t][ks] = *reinterpret_cast<const uint4*>(kb + r16 * pp.k_pos + 32 * ks + 8 * qd);
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const uint16_t* vb = pp.v + id[t] * pp.v_page + g * pp.v_head + (int64_t)((p0 + 16 * t) & mask) * pp.v_pos;
+      const int64_t id = e[t] < 0 ? 0 : e[t];
+      const uint16_t* vb = pp.v + id * pp.v_page + g * pp.v_head + (int64_t)((p0 + 16 * t) & mask) * pp.v_pos;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint16_t* a = vb + (4 * qd + j) * pp.v_pos + DPL * r16;
+        const uint16_t* a = vb + (unsigned)((4 * qd + j) * pp.v_pos + DPL * r16);
         uint32_t* to = vr[4 * t + j];
         if constexpr (DPL == 4) {
-          const uint2 x = *reinterpret_cast<const uint2*>(a);
-          to[0] = x.x, to[1] = x.y;
+          const u32x2 x = *reinterpret_cast<const u32x2*>(a);
+          to[0] = x[0], to[1] = x[1];
         } else {
 #pragma unroll
           for (int i = 0; i < DPL / 8; ++i) {
-            const uint4 x = *reinterpret_cast<const uint4*>(a + 8 * i);
-            to[4 * i] = x.x, to[4 * i + 1] = x.y, to[4 * i + 2] = x.z, to[4 * i + 3] = x.w;
+            const u32x4* from = reinterpret_cast<const u32x4*>(a + 8 * i);
+            u32x4 x;
+            if constexpr (NT) x = __builtin_nontemporal_load(from);
+            else x = *from;
+            to[4 * i] = x[0], to[4 * i + 1] = x[1], to[4 * i + 2] = x[2], to[4 * i + 3] = x[3];
           }
         }
       }
     }
+    wait_loads<NV>();
     f32x4 st[2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       st[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) st[t] = mma_16x16x32<BF>(kf[t][ks], q[ks], st[t]);
+      for (int ks = 0; ks < KS; ++ks) {
+        const uint4 kf = *reinterpret_cast<const uint4*>(keys + (16 * t + r16) * kRow + 16 * ((4 * ks + qd) ^ (r16 & kSwz)));
+        st[t] = mma_16x16x32<BF>(kf, q[ks], st[t]);
+      }
     }
-    if (!all || !ok[0] || !ok[1]) {
+    if (!all || (e[0] | e[1]) < 0) {
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int p = p0 + 16 * t + 4 * qd + j;
-          const bool see = ok[t] && p <= s.last && (p >= s.low || p < s.sinks);
+          const bool see = e[t] >= 0 && p <= s.last && (p >= s.low || p < s.sinks);
           st[t][j] = see ? st[t][j] : -INFINITY;
           // what lies in a place that is not seen may be no number, and 0 times it would be none either
 #pragma unroll
@@ -226,6 +264,21 @@ struct WaveAttend {
     return t + lane_xor<32>(t, lx);
   }
 };
+
+// The positions that `span` + 1 tokens in a row see at most, of `room`.
+inline int64_t seen_positions(int64_t room, int window, int sinks, int64_t span) {
+  const int64_t n = (int64_t)window + sinks + span;
+  return window > 0 && n < room ? n : room;
+}
+
+// A part of a token's head: its maximum, its sum, two words that keep what
+// follows 16-byte aligned, and head_dim sums of weighted values.
+constexpr int kPartHead = 4;
+constexpr int part_floats(int head_dim) { return kPartHead + head_dim; }
+
+// The parts (part[token][head][split]) of `tokens` tokens' heads together.
+int join_parts(const float* part, int splits, int64_t tokens, int heads, int head_dim, bool bf, float scale,
+               uint16_t* out, int64_t out_token, hipStream_t stream);
 
 // The argument checks of the attention calls; fills `out`.
 int page_pool_checks(const char* fn, const qs_page_pool* p, int dtype, int64_t rows, int heads, int kv_heads,

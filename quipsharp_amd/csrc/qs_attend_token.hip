@@ -7,8 +7,10 @@ namespace qs {
 namespace {
 
 constexpr int kTile = 32;  // positions of one step of a wave
-// waves of a work-group: their results meet in LDS, 64 KB at most
-constexpr int waves_of(int hd) { return hd == 256 ? 2 : 4; }
+// Waves of a work-group, whose results meet in LDS.  A few where a row's
+// tiles are split over work-groups, many where one work-group takes them all.
+constexpr int few_waves(int hd) { return hd == 256 ? 2 : 4; }
+constexpr int many_waves(int hd) { return hd == 256 ? 8 : 16; }
 
 struct TokenArgs {
   const uint16_t* q;
@@ -24,19 +26,24 @@ struct TokenArgs {
 // One work-group per (split, kv head and block of 16 of its heads, row): the
 // row's visible tiles are dealt in runs of ceil(tiles / splits), within a run
 // wave by wave.
-template <bool BF, int HD>
-__global__ __launch_bounds__(64 * waves_of(HD)) void attend_token_kernel(PagePool pp, TokenArgs a) {
-  typedef WaveAttend<BF, HD> W;
-  constexpr int kWavesT = waves_of(HD);
-  __shared__ float Os[kWavesT][16][HD + 4];
+template <bool BF, int HD, int kWavesT, bool NT>
+__global__ __launch_bounds__(64 * kWavesT) void attend_token_kernel(PagePool pp, TokenArgs a) {
+  typedef WaveAttend<BF, HD, NT> W;
+  // the keys at hand, a part for every wave; at the end the waves' results
+  union Shared {
+    char keys[kWavesT][W::kKeys];
+    float Os[kWavesT][16][HD + 4];
+  };
+  __shared__ __align__(16) Shared sh;
   __shared__ float Ms[kWavesT][16], Ls[kWavesT][16];
+  auto& Os = sh.Os;
   const int group = a.heads / a.kv_heads, blocks = (group + 15) / 16;
   const int split = blockIdx.x, g = blockIdx.y / blocks, hb = blockIdx.y % blocks, row = blockIdx.z;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r16 = lane & 15, qd = lane >> 4;
   const LaneX lx = lane_x_init();
   int len = pp.lengths[row];
   const int64_t most = (int64_t)pp.cols << pp.shift;
-  len = len > most ? (int)most : len;
+  len = __builtin_amdgcn_readfirstlane(len > most ? (int)most : len);
   const Span s = span_of(len - 1, a.window, a.sinks);
   const TileList<kTile> tiles(s);
   const int run = (tiles.count + a.splits - 1) / a.splits;
@@ -44,20 +51,35 @@ __global__ __launch_bounds__(64 * waves_of(HD)) void attend_token_kernel(PagePoo
   const int nh = group - 16 * hb < 16 ? group - 16 * hb : 16;
   const int h0 = g * group + 16 * hb;
   W wv;
-  wv.init();
+  wv.init(pp, sh.keys[w]);
 #pragma unroll
   for (int ks = 0; ks < W::KS; ++ks) {
     wv.q[ks] = make_uint4(0, 0, 0, 0);
     if (r16 < nh) wv.q[ks] = flipped(*reinterpret_cast<const uint4*>(a.q + row * a.q_row + (h0 + r16) * a.q_head + 32 * ks + 8 * qd), a.flip);
   }
-  const int32_t* trow = pp.table + row * pp.table_ld;
+  typedef const __attribute__((address_space(4))) int32_t* const_t;  // the same for the wave: scalar loads
+  const const_t trow = (const_t)(pp.table + row * pp.table_ld);
+  auto look_up = [&](int u, int (&e)[2]) {
+    const int p0 = kTile * tiles.at(u);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int col = (p0 + 16 * t) >> pp.shift;
+      const int x = trow[col < pp.cols ? col : pp.cols - 1];
+      e[t] = col < pp.cols && x >= 0 && x < pp.pages ? x : -1;
+    }
+  };
+  int e[2], next[2];
+  if (u0 + w < u1) look_up(u0 + w, next);
   for (int u = u0 + w; u < u1; u += kWavesT) {
     const int p0 = kTile * tiles.at(u);
     const bool all = p0 + kTile - 1 <= s.last && (p0 >= s.low || p0 + kTile - 1 < s.sinks);
-    wv.step(pp, trow, g, p0, s, all, a.scale, lx);
+    e[0] = next[0], e[1] = next[1];
+    if (u + kWavesT < u1) look_up(u + kWavesT, next);
+    wv.step(pp, e, g, p0, s, all, a.scale, lx);
   }
   // the waves' results together
   const float sum = wv.total(lx);
+  __syncthreads();  // other waves' keys lie where the results go
   if (qd == 0) Ms[w][r16] = wv.top, Ls[w][r16] = sum;
 #pragma unroll
   for (int j = 0; j < W::DPL; ++j)
@@ -80,56 +102,127 @@ __global__ __launch_bounds__(64 * waves_of(HD)) void attend_token_kernel(PagePoo
       const float r = l == 0.f ? 0.f : o / l;
       a.out[row * a.out_row + (int64_t)(h0 + h) * HD + d] = (uint16_t)pack16<BF>(r, r);
     } else {
-      float* to = a.part + (((int64_t)row * a.heads + h0 + h) * a.splits + split) * (HD + 2);
-      to[2 + d] = o;
+      float* to = a.part + (((int64_t)row * a.heads + h0 + h) * a.splits + split) * part_floats(HD);
+      to[kPartHead + d] = o;
       if (d == 0) to[0] = m, to[1] = l;
     }
   }
 }
 
-// The splits' results of one head together.
-template <bool BF, int HD>
-__global__ __launch_bounds__(HD) void attend_join_kernel(TokenArgs a) {
-  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
-  const float* from = a.part + ((int64_t)row * a.heads + h) * a.splits * (HD + 2);
-  float m = -INFINITY;
-  for (int i = 0; i < a.splits; ++i) m = fmaxf(m, from[i * (HD + 2)]);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, o = 0.f;
-  for (int i = 0; i < a.splits; ++i) {
-    const float* p = from + i * (HD + 2);
-    const float f = weight(p[0] - base, a.scale);
-    l += f * p[1], o += f * p[2 + d];
-  }
-  const float r = l == 0.f ? 0.f : o / l;
-  a.out[row * a.out_row + (int64_t)h * HD + d] = (uint16_t)pack16<BF>(r, r);
+template <int N, typename V>
+__device__ __forceinline__ float vec_at(const V& x, int i) {
+  if constexpr (N == 1) return x[0];
+  else return x[i];
 }
 
-int token_splits(int64_t rows, int heads, int kv_heads, int64_t cols, int page, int window, int sinks) {
+// One wave per head of a token: lane i has the weights of splits i, i + 64
+// .., and HD / 64 dimensions.
+template <bool BF, int HD>
+__global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, int64_t pairs, int heads, float scale,
+                                                   uint16_t* out, int64_t out_token) {
+  constexpr int N = HD / 64;
+  typedef float vec __attribute__((ext_vector_type(N)));
+  const LaneX lx = lane_x_init();
+  const int lane = threadIdx.x & 63;
+  const int64_t pair = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (pair >= pairs) return;
+  const float* from = part + pair * splits * part_floats(HD);
+  float top = -INFINITY, sum = 0.f, o[N] = {};
+  for (int s0 = 0; s0 < splits; s0 += 64) {
+    const int left = splits - s0 < 64 ? splits - s0 : 64;
+    float m = -INFINITY, l = 0.f;
+    if (lane < left) {
+      const float2 ml = *reinterpret_cast<const float2*>(from + (int64_t)(s0 + lane) * part_floats(HD));
+      m = ml.x, l = ml.y;
+    }
+    float mx = fmaxf(m, lane_xor<32>(m, lx));
+    mx = fmaxf(mx, lane_xor<16>(mx, lx));
+    mx = fmaxf(mx, lane_xor<8>(mx, lx));
+    mx = fmaxf(mx, lane_xor<4>(mx, lx));
+    mx = fmaxf(mx, lane_xor<2>(mx, lx));
+    mx = fmaxf(mx, lane_xor<1>(mx, lx));
+    mx = fmaxf(mx, top);
+    const float base = mx == -INFINITY ? 0.f : mx;
+    const float back = weight(top - base, scale), f = weight(m - base, scale);
+    top = mx;
+    sum = sum * back + wave_sum(f * l, lx);
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] *= back;
+    // four parts at a time, whose loads do not wait for each other
+    for (int s = 0; s < left; s += 4) {
+      vec x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int at = s + j < left ? s + j : left - 1;
+        x[j] = *reinterpret_cast<const vec*>(from + (int64_t)(s0 + at) * part_floats(HD) + kPartHead + N * lane);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float fj = s + j < left ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s + j)) : 0.f;
+        // a part without weight may hold no number where its values do
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[i] = fj == 0.f ? o[i] : o[i] + fj * vec_at<N>(x[j], i);
+      }
+    }
+  }
+  const float r = sum == 0.f ? 0.f : 1.f / sum;
+  uint16_t* to = out + pair / heads * out_token + pair % heads * HD + N * lane;
+  if constexpr (N == 1) {
+    *to = (uint16_t)pack16<BF>(o[0] * r, 0.f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) *reinterpret_cast<uint32_t*>(to + i) = pack16<BF>(o[i] * r, o[i + 1] * r);
+  }
+}
+
+// How many work-groups share a row's tiles, and whether they have many waves.
+struct Shares {
+  int splits;
+  bool many;
+};
+
+Shares token_shares(int64_t rows, int heads, int kv_heads, int64_t cols, int page, int window, int sinks) {
   const int64_t wgs = rows * kv_heads * ((heads / kv_heads + 15) / 16);
-  int64_t seen = cols * page;
-  if (window > 0 && window + (int64_t)sinks < seen) seen = window + (int64_t)sinks;
-  const int64_t tiles = seen / kTile + 2;
-  int64_t n = (1024 + wgs - 1) / wgs;
-  const int64_t most = (tiles + 3) / 4;
+  const int64_t tiles = seen_positions(cols * page, window, sinks, 0) / kTile + 2;
+  if (wgs <= 256 && tiles <= 24) return {1, true};
+  int64_t n = (4096 + wgs - 1) / wgs;
+  const int64_t most = (tiles + 7) / 8;
   n = n < most ? n : most;
-  return (int)(n < 1 ? 1 : n);
+  return {(int)(n < 1 ? 1 : n), false};
 }
 
 template <bool BF, int HD>
-int launch_token(const PagePool& pp, const TokenArgs& a, int64_t rows, hipStream_t stream) {
+int launch_token(const PagePool& pp, const TokenArgs& a, int64_t rows, bool many, bool past_caches, hipStream_t stream) {
   const int blocks = (a.heads / a.kv_heads + 15) / 16;
-  hipLaunchKernelGGL((attend_token_kernel<BF, HD>), dim3((unsigned)a.splits, (unsigned)(a.kv_heads * blocks), (unsigned)rows),
-                     dim3(64 * waves_of(HD)), 0, stream, pp, a);
+  const dim3 grid((unsigned)a.splits, (unsigned)(a.kv_heads * blocks), (unsigned)rows);
+  const dim3 few(64 * few_waves(HD));
+  if (many) hipLaunchKernelGGL((attend_token_kernel<BF, HD, many_waves(HD), false>), grid, dim3(64 * many_waves(HD)), 0, stream, pp, a);
+  else if (past_caches) hipLaunchKernelGGL((attend_token_kernel<BF, HD, few_waves(HD), true>), grid, few, 0, stream, pp, a);
+  else hipLaunchKernelGGL((attend_token_kernel<BF, HD, few_waves(HD), false>), grid, few, 0, stream, pp, a);
   QS_LAUNCHED("attend_token_kernel");
-  if (a.splits > 1) {
-    hipLaunchKernelGGL((attend_join_kernel<BF, HD>), dim3((unsigned)a.heads, (unsigned)rows), dim3(HD), 0, stream, a);
-    QS_LAUNCHED("attend_join_kernel");
-  }
+  if (a.splits > 1) return join_parts(a.part, a.splits, rows, a.heads, HD, BF, a.scale, a.out, a.out_row, stream);
   return QS_OK;
 }
 
 }  // namespace
+
+int join_parts(const float* part, int splits, int64_t tokens, int heads, int head_dim, bool bf, float scale,
+               uint16_t* out, int64_t out_token, hipStream_t stream) {
+  const int64_t pairs = tokens * heads;
+  const dim3 grid((unsigned)((pairs + 3) / 4)), block(256);
+  if (head_dim == 64) {
+    if (bf) hipLaunchKernelGGL((join_kernel<true, 64>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
+    else hipLaunchKernelGGL((join_kernel<false, 64>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
+  } else if (head_dim == 128) {
+    if (bf) hipLaunchKernelGGL((join_kernel<true, 128>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
+    else hipLaunchKernelGGL((join_kernel<false, 128>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
+  } else {
+    if (bf) hipLaunchKernelGGL((join_kernel<true, 256>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
+    else hipLaunchKernelGGL((join_kernel<false, 256>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
+  }
+  QS_LAUNCHED("join_kernel");
+  return QS_OK;
+}
 }  // namespace qs
 
 using namespace qs;
@@ -137,8 +230,8 @@ using namespace qs;
 extern "C" size_t qs_attend_token_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim, int64_t cols,
                                                   int page, int window, int sinks) {
   if (rows < 1 || heads < 1 || kv_heads < 1 || heads % kv_heads || cols < 1 || page < 1) return 0;
-  const int n = token_splits(rows, heads, kv_heads, cols, page, window, sinks);
-  return n == 1 ? 0 : (size_t)rows * heads * n * (head_dim + 2) * sizeof(float);
+  const int n = token_shares(rows, heads, kv_heads, cols, page, window, sinks).splits;
+  return n == 1 ? 0 : (size_t)rows * heads * n * part_floats(head_dim) * sizeof(float);
 }
 
 extern "C" int qs_attend_token(const void* q, int dtype, int64_t rows, int heads, int kv_heads, int head_dim,
@@ -156,13 +249,18 @@ extern "C" int qs_attend_token(const void* q, int dtype, int64_t rows, int heads
   const size_t need = qs_attend_token_workspace_bytes(rows, heads, kv_heads, head_dim, pool->cols, pool->page, window, sinks);
   QS_REQUIRE(workspace_bytes >= need && (workspace || !need) && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
              "qs_attend_token: workspace of %zu bytes (16-byte aligned), %zu needed", workspace_bytes, need);
+  const Shares sh = token_shares(rows, heads, kv_heads, pool->cols, pool->page, window, sinks);
   TokenArgs a{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<uint16_t*>(out), out_row,
-              static_cast<float*>(workspace), heads, kv_heads,
-              token_splits(rows, heads, kv_heads, pool->cols, pool->page, window, sinks), window, sinks,
+              static_cast<float*>(workspace), heads, kv_heads, sh.splits, window, sinks,
               fabsf(scale) * 1.44269504088896340736f, scale < 0 ? 0x80008000u : 0u};
+  // A layer's pages that exceed the chip's 256 MB cache are not found in it by
+  // the next call, and values that go past it leave it to the keys: 311 us
+  // with, 287 us without over 1.6 GB; where they fit, 26.4 and 27.4 us over
+  // 100 MB.
+  const bool past_caches = (int64_t)pp.pages * pool->page * kv_heads * head_dim * 4 > (256 << 20);
   const bool bf = dtype == QS_DTYPE_BF16;
   const hipStream_t st = as_stream(stream);
-  if (head_dim == 64) return bf ? launch_token<true, 64>(pp, a, rows, st) : launch_token<false, 64>(pp, a, rows, st);
-  if (head_dim == 128) return bf ? launch_token<true, 128>(pp, a, rows, st) : launch_token<false, 128>(pp, a, rows, st);
-  return bf ? launch_token<true, 256>(pp, a, rows, st) : launch_token<false, 256>(pp, a, rows, st);
+  if (head_dim == 64) return bf ? launch_token<true, 64>(pp, a, rows, sh.many, past_caches, st) : launch_token<false, 64>(pp, a, rows, sh.many, past_caches, st);
+  if (head_dim == 128) return bf ? launch_token<true, 128>(pp, a, rows, sh.many, past_caches, st) : launch_token<false, 128>(pp, a, rows, sh.many, past_caches, st);
+  return bf ? launch_token<true, 256>(pp, a, rows, sh.many, past_caches, st) : launch_token<false, 256>(pp, a, rows, sh.many, past_caches, st);
 }

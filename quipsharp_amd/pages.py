@@ -137,6 +137,13 @@ def token_workspace_bytes(rows, heads, k_pages: Tensor, table: Tensor, window=0,
                                                           table.shape[1], k_pages.shape[2], window, sinks))
 
 
+def chunk_workspace_bytes(tokens, heads, k_pages: Tensor, table: Tensor, window=0, sinks=0) -> int:
+    """Bytes of workspace that ``attend_chunk`` takes for calls of this shape."""
+    return int(_lib.lib().qs_attend_chunk_workspace_bytes(tokens, table.shape[0], heads, k_pages.shape[1],
+                                                          k_pages.shape[3], table.shape[1], k_pages.shape[2], window,
+                                                          sinks))
+
+
 def attend_token(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, *, scale: float = None,
                  window: int = 0, sinks: int = 0, out: Tensor = None, workspace: Tensor = None) -> Tensor:
     """Attention of one new token per row over the row's pages.
@@ -164,7 +171,8 @@ def attend_token(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
 
 
 def attend_chunk(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, starts: Tensor, *,
-                 scale: float = None, window: int = 0, sinks: int = 0, out: Tensor = None) -> Tensor:
+                 scale: float = None, window: int = 0, sinks: int = 0, out: Tensor = None,
+                 workspace: Tensor = None) -> Tensor:
     """Causal attention of several new tokens per row over the row's pages.
 
     q: (tokens, heads, head dim); the tokens of row r are ``starts[r]`` ..
@@ -173,17 +181,21 @@ def attend_chunk(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     the pages already.  Each sees the positions up to its own, as in
     ``attend_token``.  Returns (tokens, heads, head dim) in q's type."""
     pool = _pool(k_pages, v_pages, table, lengths)
-    dev, (_, kv_heads, _, dim) = k_pages.device, k_pages.shape
+    dev, (_, kv_heads, page, dim) = k_pages.device, k_pages.shape
     _heads("q", q, None, dim, k_pages.dtype, dev)
     rows = table.shape[0]
     _int32("starts", starts, (rows + 1,), dev)
     window, sinks = _visible(window, sinks)
     out = _output(out, q)
     _lib.require_gpu(k_pages, what="attend_chunk")
-    _lib.check(_lib.lib().qs_attend_chunk(q.data_ptr(), _lib.dtype_code(q.dtype), q.shape[0], rows, q.shape[1],
-                                          kv_heads, dim, q.stride(0), q.stride(1), starts.data_ptr(), pool,
-                                          dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
-                                          out.stride(0), _lib.stream_of(q)))
+    L, tokens, heads = _lib.lib(), q.shape[0], q.shape[1]
+    need = L.qs_attend_chunk_workspace_bytes(tokens, rows, heads, kv_heads, dim, table.shape[1], page, window, sinks)
+    workspace = _workspace(workspace, need, dev)
+    _lib.check(L.qs_attend_chunk_ws(q.data_ptr(), _lib.dtype_code(q.dtype), tokens, rows, heads, kv_heads, dim,
+                                    q.stride(0), q.stride(1), starts.data_ptr(), pool,
+                                    dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+                                    out.stride(0), _lib.ptr(workspace),
+                                    0 if workspace is None else workspace.numel(), _lib.stream_of(q)))
     return out
 
 
