@@ -6,15 +6,16 @@
 // needs (the running maximum and sum) and each slice's best `keep`; the
 // second launch adds the slices' sums and chooses among the slices' bests by
 // the score in fp64.
-#include "qs_common.h"
+#include <type_traits>
+
+#include "qs_chunk_dev.h"
 
 namespace qs {
 namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxKeep = 128;
-constexpr int kPer = 16;                  // logits per thread
-constexpr int kSlice = kThreads * kPer;   // logits per work-group
+constexpr int kRoom = 4096;  // candidates of a slice
 
 // Order-preserving bits of a float; -0 counts as 0, NaN as -inf.
 __device__ __forceinline__ uint32_t order_bits(float f) {
@@ -47,65 +48,166 @@ struct SelectArgs {
   int beams, vocab, keep, slices, dtype;
 };
 
-// One work-group per slice of a row of logits.
+// exp(x - m) for x <= m, zero where there is nothing yet.  log2(e) in two
+// parts: the rounding of one alone would be the same for all terms of a sum.
+__device__ __forceinline__ float exp_below(float x, float m) {
+  const float d = x - (m == -INFINITY ? 0.f : m);
+  return __builtin_amdgcn_exp2f(__builtin_fmaf(d, 1.44269502f, d * 1.92596299e-8f));
+}
+
+// The largest u such that at least n lanes (1 .. 64) have a key of u or more.
+__device__ __forceinline__ uint32_t nth_key(uint32_t key, int n) {
+  uint32_t u = 0;
+#pragma unroll
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t v = u | 1u << bit;
+    if (__popcll(__ballot(key >= v)) >= n) u = v;
+  }
+  return u;
+}
+
+// The logits of a thread: number (i * 256 + tid) * W + e of the slice, which
+// begins at t0, is x[i * W + e].
+template <typename T, bool WIDE, int E>
+struct Slice {
+  static constexpr int W = WIDE ? 16 / sizeof(T) : 1;
+  float x[E];
+  __device__ __forceinline__ static int token(int t0, int i) { return t0 + (i / W * kThreads + (int)threadIdx.x) * W + i % W; }
+  __device__ __forceinline__ void load(const T* row, int t0, int vocab) {
+    if (WIDE && t0 + E * kThreads <= vocab) {
+      uint4 v[E / W];
+#pragma unroll
+      for (int i = 0; i < E / W; ++i) v[i] = *reinterpret_cast<const uint4*>(row + token(t0, i * W));
+#pragma unroll
+      for (int i = 0; i < E / W; ++i) {
+        const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          if constexpr (sizeof(T) == 4) x[i * W + e] = __uint_as_float(u[e]);
+          else if constexpr (std::is_same<T, _Float16>::value) x[i * W + e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u[e / 2] >> 16 * (e & 1)));
+          else x[i * W + e] = __uint_as_float(e & 1 ? u[e / 2] & 0xFFFF0000u : u[e / 2] << 16);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int t = token(t0, i);
+        float f = -INFINITY;
+        if (t < vocab) {
+          if constexpr (sizeof(T) == 4) f = row[t];
+          else if constexpr (std::is_same<T, _Float16>::value) f = (float)row[t];
+          else f = __uint_as_float((uint32_t)row[t] << 16);
+        }
+        x[i] = f;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = fmaxf(x[i], -INFINITY);  // NaN counts as -inf
+  }
+};
+
+// One work-group per slice of 256 E logits, which stay in registers.
+//
+// A logit is among the slice's best only if it is not below the edge: the
+// keep-th largest of the threads' largest, or (up to 64) the largest of the
+// waves' keep-th largest, which takes no exchange.  Above the edge lie at
+// most (keep - 1) E logits by the first rule and four times as many by the
+// second, which slice_size keeps below kRoom, and few in most cases; those at
+// the edge may be any number, and the lowest tokens of them are taken.
+template <typename T, bool WIDE, int E>
 __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
-  __shared__ uint64_t tops[kThreads];
-  __shared__ uint64_t cand[kMaxKeep * kPer];
-  __shared__ float red[kThreads / 64];
-  __shared__ uint64_t edge;
+  typedef Slice<T, WIDE, E> S;
+  __shared__ uint64_t room[kRoom];
+  __shared__ float tops[kThreads];
+  __shared__ float red[3][4];
+  __shared__ float line;
   __shared__ int count;
-  const int tid = threadIdx.x, slice = blockIdx.x;
+  const LaneX lx = lane_x_init();
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, slice = blockIdx.x;
   const int64_t row = blockIdx.y;
   if (a.finished && a.finished[row]) return;  // its one continuation needs no logits
-  float x[kPer];
-  uint64_t key[kPer], top = 0;
+  const int t0 = slice * (E * kThreads), keep = a.keep;
+  S s;
+  s.load(static_cast<const T*>(a.logits) + row * a.ld, t0, a.vocab);
   float m = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int t = slice * kSlice + i * kThreads + tid;
-    x[i] = t < a.vocab ? load_as_float(a.logits, a.dtype, row * a.ld + t) : -INFINITY;
-    x[i] = x[i] != x[i] ? -INFINITY : x[i];
-    key[i] = t < a.vocab ? (uint64_t)order_bits(x[i]) << 32 | (uint32_t)~t : 0;
-    top = key[i] > top ? key[i] : top;
-    m = fmaxf(m, x[i]);
-  }
-#pragma unroll
-  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-  tops[tid] = top;
-  if ((tid & 63) == 0) red[tid >> 6] = m;
-  if (tid == 0) count = 0, edge = 0;
+  for (int i = 0; i < E; ++i) m = fmaxf(m, s.x[i]);
+  float top = m;
+  top = fmaxf(top, lane_xor<32>(top, lx));
+  top = fmaxf(top, lane_xor<16>(top, lx));
+  top = fmaxf(top, lane_xor<8>(top, lx));
+  top = fmaxf(top, lane_xor<4>(top, lx));
+  top = fmaxf(top, lane_xor<2>(top, lx));
+  top = fmaxf(top, lane_xor<1>(top, lx));
+  const float edge_w = keep <= 64 ? order_float(nth_key(order_bits(m), keep)) : -INFINITY;
+  if (keep > 64) tops[tid] = m;
+  if (lane == 0) red[0][w] = top, red[1][w] = edge_w;
+  if (tid == 0) count = 0;
   __syncthreads();
-  m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float all = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float edge = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+  if (keep > 64) {
+    int above = 0, same = 0;
+    for (int i = 0; i < kThreads; ++i) above += tops[i] > m, same += tops[i] == m;
+    if (above < keep && keep <= above + same) line = m;  // all that write it write the same
+    __syncthreads();
+    edge = line;
+  }
   float sum = 0.f;
-  if (fabsf(m) != INFINITY) {
+  if (all < INFINITY) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) sum += expf(x[i] - m);
+    for (int p = 0; p < E; p += 16) {
+      float part = 0.f;
+#pragma unroll
+      for (int i = p; i < p + 16; ++i) part += exp_below(s.x[i], all);
+      sum += part;
+    }
   }
+  sum = wave_sum(sum, lx);
+  if (lane == 0) red[2][w] = sum;
+  auto add = [&](int i) {
+    const int at = atomicAdd(&count, 1);
+    if (at < kRoom) room[at] = (uint64_t)order_bits(s.x[i]) << 32 | (uint32_t)~S::token(t0, i);
+  };
+  if (__any(m >= edge)) {
 #pragma unroll
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-  // the keep-th largest of the threads' largest: at least `keep` keys are not below it, and only `keep` threads hold
-  // such keys, kPer each at most
-  int above = 0;
-  for (int i = 0; i < kThreads; ++i) above += tops[i] > top;
-  if (above == a.keep - 1 && top) edge = top;
+    for (int i = 0; i < E; ++i)
+      if (s.x[i] >= edge && S::token(t0, i) < a.vocab) add(i);
+  }
   __syncthreads();
-  if ((tid & 63) == 0) red[tid >> 6] = sum;
-  const uint64_t least = edge ? edge : 1;
+  int n = count;
+  if (n > kRoom) {
+    // too many at the edge: those above it, then the others by rising tokens until there are enough
+    __syncthreads();
+    if (tid == 0) count = 0;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kPer; ++i)
-    if (key[i] >= least) cand[atomicAdd(&count, 1)] = key[i];
-  __syncthreads();
-  const int n = count;
-  uint64_t* best = a.best + (row * a.slices + slice) * a.keep;
+    for (int i = 0; i < E; ++i)
+      if (s.x[i] > edge) add(i);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < E; i += S::W) {
+      const bool enough = count >= keep;
+      __syncthreads();
+      if (enough) continue;
+#pragma unroll
+      for (int e = i; e < i + S::W; ++e)
+        if (s.x[e] == edge && S::token(t0, e) < a.vocab) add(e);
+      __syncthreads();
+    }
+    n = count;
+  }
+  uint64_t* best = a.best + (row * a.slices + slice) * keep;
   for (int c = tid; c < n; c += kThreads) {
-    int rank = 0;
-    for (int i = 0; i < n; ++i) rank += cand[i] > cand[c];
-    if (rank < a.keep) best[rank] = cand[c];
+    const uint64_t me = room[c];
+    int place = 0;
+    for (int i = 0; i < n; ++i) place += room[i] > me;
+    if (place < keep) best[place] = me;
   }
-  for (int c = n + tid; c < a.keep; c += kThreads) best[c] = 0;
+  for (int c = n + tid; c < keep; c += kThreads) best[c] = 0;
   if (tid == 0) {
     float* st = a.stats + 2 * (row * a.slices + slice);
-    st[0] = m, st[1] = (red[0] + red[1]) + (red[2] + red[3]);
+    st[0] = all, st[1] = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
   }
 }
 
@@ -119,11 +221,14 @@ __device__ __forceinline__ bool over(const Candidate& x, const Candidate& y) {
 
 // One work-group per request.
 __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a, Candidate* spill) {
-  __shared__ Candidate tops[kThreads];
+  constexpr int kList = 512;
   __shared__ double base[1024];  // score - log sum; of a beam without continuations -inf
   __shared__ uint8_t state[1024];
-  __shared__ Candidate edge;
+  __shared__ Candidate list[kList];
+  __shared__ uint32_t tops[kThreads];
+  __shared__ uint32_t edge;
   __shared__ int count;
+  const LaneX lx = lane_x_init();
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int64_t b = blockIdx.x;
   for (int j = w; j < a.beams; j += kThreads / 64) {
@@ -135,33 +240,40 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a, Candi
       if (done) {
         c = s;
       } else {
-        const float* st = a.stats + 2 * row * a.slices;
-        float m = -INFINITY;
-        for (int i = lane; i < a.slices; i += 64) m = fmaxf(m, st[2 * i]);
-#pragma unroll
-        for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-        double sum = 0;
-        if (fabsf(m) < INFINITY)
-          for (int i = lane; i < a.slices; i += 64) sum += exp((double)st[2 * i] - m) * st[2 * i + 1];
-#pragma unroll
-        for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
-        if (fabsf(m) < INFINITY) c = (double)s - ((double)m + log(sum));
+        // lane i: slices i, i + 64 ..
+        const float2* st = reinterpret_cast<const float2*>(a.stats) + row * a.slices;
+        float m = -INFINITY, l = 0.f;
+        for (int i = lane; i < a.slices; i += 64) {
+          const float2 x = st[i];
+          const float up = fmaxf(m, x.x);
+          l = l * exp_below(m, up) + x.y * exp_below(x.x, up);
+          m = up;
+        }
+        float top = m;
+        top = fmaxf(top, lane_xor<32>(top, lx));
+        top = fmaxf(top, lane_xor<16>(top, lx));
+        top = fmaxf(top, lane_xor<8>(top, lx));
+        top = fmaxf(top, lane_xor<4>(top, lx));
+        top = fmaxf(top, lane_xor<2>(top, lx));
+        top = fmaxf(top, lane_xor<1>(top, lx));
+        const float sum = wave_sum(fabsf(top) < INFINITY ? l * exp_below(m, top) : 0.f, lx);
+        if (fabsf(top) < INFINITY) c = (double)s - ((double)top + log((double)sum));
       }
     }
     if (lane == 0) base[j] = c, state[j] = done ? 1 : c == -INFINITY ? 2 : 0;
   }
-  if (tid == 0) count = 0, edge = Candidate{0, 0};
+  if (tid == 0) count = 0, edge = 0;
   __syncthreads();
   // a beam offers slices * keep candidates; one that is finished or has none keep + 1: eos and the first tokens
-  const int per = a.slices * a.keep > a.keep + 1 ? a.slices * a.keep : a.keep + 1, all = a.beams * per;
+  const int some = a.slices * a.keep, per = some > a.keep + 1 ? some : a.keep + 1, all = a.beams * per;
   auto get = [&](int e) {
     const int j = e / per, i = e % per;
     const int64_t row = b * a.beams + j;
     int64_t t = -1;
     double v = -INFINITY;
     if (state[j] == 0) {
-      if (i >= a.slices * a.keep) return Candidate{0, 0};
-      const uint64_t k = a.best[row * a.slices * a.keep + i];
+      if (i >= some) return Candidate{0, 0};
+      const uint64_t k = a.best[row * some + i];
       if (!k) return Candidate{0, 0};
       t = (uint32_t)~k;
       v = base[j] + (double)order_float((uint32_t)(k >> 32));
@@ -174,30 +286,41 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a, Candi
     }
     return Candidate{order_bits64(v), ~(uint32_t)(j * (int64_t)a.vocab + t)};
   };
-  Candidate top{0, 0};
+  // The upper half of a score's order bits is enough to leave most out: at
+  // least `keep` candidates have the edge's or more, and so have the best.
+  uint32_t top = 0;
   for (int e = tid; e < all; e += kThreads) {
-    const Candidate c = get(e);
-    if (over(c, top)) top = c;
+    const uint32_t hi = (uint32_t)(get(e).score >> 32);
+    top = hi > top ? hi : top;
   }
-  tops[tid] = top;
+  if (a.keep <= 64) {
+    const uint32_t u = nth_key(top, a.keep);
+    if (lane == 0) atomicMax(&edge, u);
+  } else {
+    tops[tid] = top;
+    __syncthreads();
+    int above = 0, same = 0;
+    for (int i = 0; i < kThreads; ++i) above += tops[i] > top, same += tops[i] == top && i < tid;
+    if (above + same == a.keep - 1) edge = top;
+  }
   __syncthreads();
-  int above = 0;
-  for (int i = 0; i < kThreads; ++i) above += over(tops[i], top);
-  if (above == a.keep - 1 && top.score) edge = top;
-  __syncthreads();
-  const Candidate least = edge;
-  Candidate* cand = spill + b * (int64_t)all;
+  const uint32_t least = edge;
+  Candidate* more = spill + b * (int64_t)all;
   for (int e = tid; e < all; e += kThreads) {
     const Candidate c = get(e);
-    if (c.score && !over(least, c)) cand[atomicAdd(&count, 1)] = c;
+    if (!c.score || (uint32_t)(c.score >> 32) < least) continue;
+    const int at = atomicAdd(&count, 1);
+    (at < kList ? list[at] : more[at]) = c;
   }
   __threadfence();
   __syncthreads();
   const int n = count;
   for (int c = tid; c < n; c += kThreads) {
-    const Candidate x = cand[c];
+    const Candidate x = c < kList ? list[c] : more[c];
     int rank = 0;
-    for (int i = 0; i < n; ++i) rank += over(cand[i], x);
+    const int near = n < kList ? n : kList;
+    for (int i = 0; i < near; ++i) rank += over(list[i], x);
+    for (int i = kList; i < n; ++i) rank += over(more[i], x);
     if (rank < a.keep) {
       const uint32_t at = ~x.at;
       a.scores_out[b * a.keep + rank] = (float)order_double(x.score);
@@ -207,21 +330,40 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a, Candi
   }
 }
 
+// Logits per thread: as many as leave a work-group for each CU, since a
+// slice's selection costs the same whatever its length, and few enough that
+// what lies above the edge fits (see beam_slice_kernel).
+int slice_size(int64_t rows, int64_t vocab, int keep) {
+  const int most = keep <= 16 ? 64 : keep <= 32 ? 32 : keep <= 64 ? 16 : 32;
+  int e = 16;
+  while (e < most && rows * ((vocab + 2 * kThreads * e - 1) / (2 * kThreads * e)) >= 512) e *= 2;
+  return e;
+}
+
 struct Layout {
-  int slices;
+  int slices, each;
   size_t stats, best, spill, bytes;
 };
 
 Layout layout_of(int64_t batch, int beams, int64_t vocab, int keep) {
   Layout l;
-  l.slices = (int)((vocab + kSlice - 1) / kSlice);
-  const int64_t rows = batch * beams, per = (int64_t)l.slices * keep > keep + 1 ? (int64_t)l.slices * keep : keep + 1;
+  const int64_t rows = batch * beams;
+  l.each = slice_size(rows, vocab, keep);
+  const int64_t slice = (int64_t)kThreads * l.each;
+  l.slices = (int)((vocab + slice - 1) / slice);
+  const int64_t per = (int64_t)l.slices * keep > keep + 1 ? (int64_t)l.slices * keep : keep + 1;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   l.stats = 0;
   l.best = up((size_t)rows * l.slices * 2 * sizeof(float));
   l.spill = l.best + up((size_t)rows * l.slices * keep * sizeof(uint64_t));
   l.bytes = l.spill + up((size_t)rows * per * sizeof(Candidate));
   return l;
+}
+
+template <typename T>
+auto slice_kernel(bool wide, int each) {
+  if (wide) return each == 64 ? beam_slice_kernel<T, true, 64> : each == 32 ? beam_slice_kernel<T, true, 32> : beam_slice_kernel<T, true, 16>;
+  return each == 64 ? beam_slice_kernel<T, false, 64> : each == 32 ? beam_slice_kernel<T, false, 32> : beam_slice_kernel<T, false, 16>;
 }
 
 // ---------------------------------------------------------------------------
@@ -288,7 +430,13 @@ extern "C" int qs_beam_select(const void* logits, int dtype, int64_t ld, int64_t
   const SelectArgs a{logits, ld, scores, finished, reinterpret_cast<float*>(ws + l.stats),
                      reinterpret_cast<uint64_t*>(ws + l.best), scores_out, parents_out, tokens_out, eos, beams,
                      (int)vocab, keep, l.slices, dtype};
-  hipLaunchKernelGGL(beam_slice_kernel, dim3((unsigned)l.slices, (unsigned)(batch * beams)), dim3(kThreads), 0, as_stream(stream), a);
+  const size_t size = dtype == QS_DTYPE_F32 ? 4 : 2;
+  const bool wide = (reinterpret_cast<uintptr_t>(logits) & 15) == 0 && ld * size % 16 == 0;
+  const dim3 grid((unsigned)l.slices, (unsigned)(batch * beams));
+  const auto slice = dtype == QS_DTYPE_F32   ? slice_kernel<float>(wide, l.each)
+                     : dtype == QS_DTYPE_F16 ? slice_kernel<_Float16>(wide, l.each)
+                                             : slice_kernel<uint16_t>(wide, l.each);
+  hipLaunchKernelGGL(slice, grid, dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("beam_slice_kernel");
   hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)batch), dim3(kThreads), 0, as_stream(stream), a,
                      reinterpret_cast<Candidate*>(ws + l.spill));

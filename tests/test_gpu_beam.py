@@ -68,6 +68,21 @@ def test_ties_and_orders(dev, order):
     check(dev, logits.half(), torch.zeros(2, 3), 7)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("keep", [3, 16, 40, 128])
+@pytest.mark.parametrize("kind", ["equal", "few allowed", "periodic", "steps"])
+def test_many_at_the_edge(dev, kind, keep, dtype):
+    """Rows enough for the longest slices, and more candidates in one than it has room for: all equal, all but some
+    banned, the large ones in few threads, and runs of equal values."""
+    V, rows = 34000, 300
+    t = torch.arange(V)
+    x = {"equal": torch.zeros(V), "few allowed": torch.where(t % 4999 == 7, 1.0, -math.inf),
+         "periodic": torch.where(t % 1024 < 12, (t % 997) / 997.0, -5.0), "steps": (t // 5000 % 2).float()}[kind]
+    logits = x.repeat(rows, 1)
+    logits[1::2, 100] = 3.0
+    check(dev, logits.to(dtype), -(torch.arange(rows) % 5).float().view(100, 3), keep)
+
+
 def test_zeros_of_both_signs_tie(dev):
     logits = torch.zeros(2, 100)
     logits[0, ::2] = -0.0
