@@ -7,7 +7,11 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .pages import _int32, _rows_flag, _workspace
+from .pages import _int32, _room, _rows_flag, _workspace
+
+# argument arrays for 0 .. QS_MAX_STATES states
+_WORDS = [ctypes.c_int64 * k for k in range(_lib.QS_MAX_STATES + 1)]
+_POINTERS = [ctypes.c_void_p * k for k in range(_lib.QS_MAX_STATES + 1)]
 
 
 def beam_select(logits: Tensor, scores: Tensor, keep: int = None, finished: Tensor = None, eos: int = -1, *,
@@ -29,17 +33,18 @@ def beam_select(logits: Tensor, scores: Tensor, keep: int = None, finished: Tens
         raise ValueError(f"scores must be a contiguous float32 (batch, beams), got {tuple(scores.shape)} x {scores.dtype}")
     batch, beams = scores.shape
     vocab = logits.shape[-1]
-    if tuple(logits.shape) not in ((batch * beams, vocab), (batch, beams, vocab)):
+    if logits.shape not in ((batch * beams, vocab), (batch, beams, vocab)):
         raise ValueError(f"logits {tuple(logits.shape)} do not fit scores {tuple(scores.shape)}")
-    if logits.dim() == 3:
-        if batch > 1 and beams > 1 and logits.stride(0) != beams * logits.stride(1):
+    strides = logits.stride()
+    if len(strides) == 3:
+        if batch > 1 and beams > 1 and strides[0] != beams * strides[1]:
             raise ValueError("the rows of logits must lie one stride apart")
-        ld = logits.stride(1) if beams > 1 else logits.stride(0)
+        ld = strides[1] if beams > 1 else strides[0]
     else:
-        ld = logits.stride(0)
+        ld = strides[0]
     if batch * beams == 1:
         ld = vocab
-    if logits.stride(-1) != 1 and vocab > 1:
+    if strides[-1] != 1 and vocab > 1:
         raise ValueError("the logits of a row must lie together (stride 1)")
     dev = logits.device
     if scores.device != dev:
@@ -51,15 +56,14 @@ def beam_select(logits: Tensor, scores: Tensor, keep: int = None, finished: Tens
         raise ValueError(f"keep {keep} must be 1 or more")
     code = _lib.dtype_code(logits.dtype)
     _lib.require_gpu(logits, what="beam_select")
-    out = torch.empty(3, batch, keep, dtype=torch.int32, device=dev)
-    best, parents, tokens = out.unbind()
-    best = best.view(torch.float32)
+    best = scores.new_empty((batch, keep))
+    parents, tokens = torch.empty_like(best, dtype=torch.int32), torch.empty_like(best, dtype=torch.int32)
     L = _lib.lib()
     workspace = _workspace(workspace, L.qs_beam_select_workspace_bytes(batch, beams, vocab, keep), dev)
     _lib.check(L.qs_beam_select(logits.data_ptr(), code, ld, batch, beams, vocab,
                                 scores.data_ptr(), _lib.ptr(finished), -1 if eos is None else eos, keep,
-                                best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), _lib.ptr(workspace),
-                                0 if workspace is None else workspace.numel(), _lib.stream_of(logits)))
+                                best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), *_room(workspace),
+                                _lib.stream_of(logits)))
     return best, parents, tokens
 
 
@@ -73,20 +77,22 @@ def reorder_states(states, parents: Tensor):
     dev, n = states[0].device, parents.numel()
     _int32("parents", parents, parents.shape, dev)
     rows = states[0].shape[0]
-    size, stride = [], []
+    size, stride, out = [], [], []
     for s in states:
-        if s.device != dev or s.dim() < 1 or s.shape[0] != rows:
-            raise ValueError(f"every state must have {rows} rows on {dev}, got {tuple(s.shape)} on {s.device}")
-        row = s[0].numel() if rows else 0
-        if rows and not s[0].is_contiguous():
+        shape = s.shape
+        if s.device != dev or not shape or shape[0] != rows:
+            raise ValueError(f"every state must have {rows} rows on {dev}, got {tuple(shape)} on {s.device}")
+        if not s.is_contiguous() and rows and not s[0].is_contiguous():
             raise ValueError("the elements of a state's row must lie together")
-        size.append(row * s.element_size())
-        stride.append(s.stride(0) * s.element_size() if rows > 1 else size[-1])
+        each = s.element_size()
+        size.append(s.numel() // rows * each if rows else 0)
+        stride.append(s.stride()[0] * each if rows > 1 else size[-1])
     _lib.require_gpu(*states, what="reorder_states")
-    out = [torch.empty((n,) + tuple(s.shape[1:]), dtype=s.dtype, device=dev) for s in states]
+    for s in states:
+        out.append(s.new_empty((n,) + s.shape[1:]))
     k = len(states)
-    _lib.check(_lib.lib().qs_reorder_states(k, (ctypes.c_void_p * k)(*[s.data_ptr() for s in states]),
-                                            (ctypes.c_void_p * k)(*[o.data_ptr() for o in out]),
-                                            (ctypes.c_int64 * k)(*size), (ctypes.c_int64 * k)(*stride),
+    words, pointers = _WORDS[k], _POINTERS[k]
+    _lib.check(_lib.lib().qs_reorder_states(k, pointers(*[s.data_ptr() for s in states]),
+                                            pointers(*[o.data_ptr() for o in out]), words(*size), words(*stride),
                                             parents.data_ptr(), n, rows, _lib.stream_of(states[0])))
     return out

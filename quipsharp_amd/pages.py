@@ -24,10 +24,11 @@ from torch import Tensor
 from . import _lib
 
 _HALF = (torch.bfloat16, torch.float16)
+_FLAGS = (torch.bool, torch.uint8)
 
 
 def _int32(name, t, shape, device):
-    if not isinstance(t, Tensor) or t.dtype != torch.int32 or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if not isinstance(t, Tensor) or t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous():
         got = f"{tuple(t.shape)} x {t.dtype}" if isinstance(t, Tensor) else type(t).__name__
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)}, got {got}")
     if t.device != device:
@@ -36,7 +37,7 @@ def _int32(name, t, shape, device):
 
 
 def _rows_flag(name, t, shape, device):
-    if t.dtype not in (torch.bool, torch.uint8) or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.dtype not in _FLAGS or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous bool tensor of shape {tuple(shape)}, got {tuple(t.shape)} x {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
@@ -55,6 +56,20 @@ def _visible(window, sinks):
 def _pool(k_pages, v_pages, table, lengths):
     """The library's description of one layer's pages, with the checks that
     keep its kernels inside the tensors."""
+    shape, dev, rows = k_pages.shape, k_pages.device, table.shape
+    ks, vs = k_pages.stride(), v_pages.stride()
+    # a decode step of one layer takes microseconds: what is refused is looked into only where something is
+    if not (len(shape) == 4 and shape == v_pages.shape and k_pages.dtype is v_pages.dtype and k_pages.dtype in _HALF
+            and ks[3] == 1 and vs[3] == 1 and v_pages.device == dev and len(rows) == 2
+            and table.dtype is torch.int32 and table.is_contiguous() and table.device == dev
+            and isinstance(lengths, Tensor) and lengths.dtype is torch.int32 and lengths.shape == rows[:1] and lengths.is_contiguous()
+            and lengths.device == dev):
+        _refuse_pool(k_pages, v_pages, table, lengths)
+    return _lib.PagePool(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], shape[0],
+                         shape[2], table.data_ptr(), rows[1], rows[1], lengths.data_ptr())
+
+
+def _refuse_pool(k_pages, v_pages, table, lengths):
     if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
         raise ValueError(f"k_pages and v_pages must be (pages, kv heads, page, head dim) of one type, got "
                          f"{tuple(k_pages.shape)} x {k_pages.dtype} and {tuple(v_pages.shape)} x {v_pages.dtype}")
@@ -69,28 +84,26 @@ def _pool(k_pages, v_pages, table, lengths):
         raise ValueError(f"table must be (rows, columns), got {tuple(table.shape)}")
     _int32("table", table, table.shape, dev)
     _int32("lengths", lengths, (table.shape[0],), dev)
-    ks, vs = k_pages.stride(), v_pages.stride()
-    return _lib.PagePool(k_pages.data_ptr(), v_pages.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-                         k_pages.shape[0], k_pages.shape[2], table.data_ptr(), table.shape[1], table.shape[1],
-                         lengths.data_ptr())
+    raise AssertionError("one of the checks above holds")
 
 
 def _heads(name, x, rows, dim, dtype, device):
-    """(rows, heads, dim) with the elements of a head together."""
-    if x.dim() != 3 or x.shape[2] != dim or (rows is not None and x.shape[0] != rows):
-        raise ValueError(f"{name} must be ({'tokens' if rows is None else rows}, heads, {dim}), got {tuple(x.shape)}")
-    if x.dtype != dtype:
+    """The strides of (rows, heads, dim) with the elements of a head together."""
+    shape, st = x.shape, x.stride()
+    if len(shape) != 3 or shape[2] != dim or (rows is not None and shape[0] != rows):
+        raise ValueError(f"{name} must be ({'tokens' if rows is None else rows}, heads, {dim}), got {tuple(shape)}")
+    if x.dtype is not dtype:
         raise TypeError(f"{name} is {x.dtype}, the cache {dtype}")
     if x.device != device:
         raise ValueError(f"{name} is on {x.device}, the cache on {device}")
-    if x.shape[1] and x.stride(2) != 1:
+    if st[2] != 1 and shape[1]:
         raise ValueError(f"the elements of a head of {name} must lie together (stride 1)")
-    return x
+    return st
 
 
 def _output(out, q):
     if out is None:
-        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError(f"out must be {tuple(q.shape)} x {q.dtype} on {q.device}, got {tuple(out.shape)} x {out.dtype} on {out.device}")
     if out.stride(2) != 1 or out.stride(1) != out.shape[2]:
@@ -110,6 +123,10 @@ def _workspace(workspace, need, device):
     return workspace
 
 
+def _room(workspace):
+    return (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+
+
 def append_pages(k_pages: Tensor, v_pages: Tensor, k: Tensor, v: Tensor, table: Tensor, lengths: Tensor,
                  starts: Tensor = None) -> None:
     """Store new tokens' keys and values, (tokens, kv heads, head dim) each, in
@@ -119,16 +136,15 @@ def append_pages(k_pages: Tensor, v_pages: Tensor, k: Tensor, v: Tensor, table: 
     pool = _pool(k_pages, v_pages, table, lengths)
     dev, dim = k_pages.device, k_pages.shape[3]
     rows = table.shape[0]
-    _heads("k", k, None if starts is not None else rows, dim, k_pages.dtype, dev)
-    _heads("v", v, k.shape[0], dim, k_pages.dtype, dev)
+    ks = _heads("k", k, None if starts is not None else rows, dim, k_pages.dtype, dev)
+    vs = _heads("v", v, k.shape[0], dim, k_pages.dtype, dev)
     if k.shape[1] != k_pages.shape[1] or v.shape[1] != k_pages.shape[1]:
         raise ValueError(f"{k.shape[1]} and {v.shape[1]} heads for a cache of {k_pages.shape[1]}")
     if starts is not None:
         _int32("starts", starts, (rows + 1,), dev)
     _lib.require_gpu(k_pages, what="append_pages")
-    _lib.check(_lib.lib().qs_page_append(k.data_ptr(), v.data_ptr(), k.shape[0], rows, k.shape[1], dim, k.stride(0),
-                                         k.stride(1), v.stride(0), v.stride(1), _lib.ptr(starts), pool,
-                                         _lib.stream_of(k_pages)))
+    _lib.check(_lib.lib().qs_page_append(k.data_ptr(), v.data_ptr(), k.shape[0], rows, k.shape[1], dim, ks[0], ks[1],
+                                         vs[0], vs[1], _lib.ptr(starts), pool, _lib.stream_of(k_pages)))
 
 
 def token_workspace_bytes(rows, heads, k_pages: Tensor, table: Tensor, window=0, sinks=0) -> int:
@@ -155,18 +171,18 @@ def attend_token(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     Returns (rows, heads, head dim) in q's type; zeros for a row that sees
     nothing.  ``scale`` defaults to ``head_dim ** -0.5``."""
     pool = _pool(k_pages, v_pages, table, lengths)
-    dev, (_, kv_heads, page, dim) = k_pages.device, k_pages.shape
-    _heads("q", q, table.shape[0], dim, k_pages.dtype, dev)
+    dev, (_, kv_heads, page, dim), (rows, cols) = k_pages.device, k_pages.shape, table.shape
+    dtype = k_pages.dtype
+    st = _heads("q", q, rows, dim, dtype, dev)
     window, sinks = _visible(window, sinks)
     out = _output(out, q)
     _lib.require_gpu(k_pages, what="attend_token")
-    L, rows, heads = _lib.lib(), q.shape[0], q.shape[1]
-    need = L.qs_attend_token_workspace_bytes(rows, heads, kv_heads, dim, table.shape[1], page, window, sinks)
+    L, heads = _lib.lib(), q.shape[1]
+    need = L.qs_attend_token_workspace_bytes(rows, heads, kv_heads, dim, cols, page, window, sinks)
     workspace = _workspace(workspace, need, dev)
-    _lib.check(L.qs_attend_token(q.data_ptr(), _lib.dtype_code(q.dtype), rows, heads, kv_heads, dim, q.stride(0),
-                                 q.stride(1), pool, dim ** -0.5 if scale is None else scale, window, sinks,
-                                 out.data_ptr(), out.stride(0), _lib.ptr(workspace),
-                                 0 if workspace is None else workspace.numel(), _lib.stream_of(q)))
+    _lib.check(L.qs_attend_token(q.data_ptr(), _lib.dtype_code(dtype), rows, heads, kv_heads, dim, st[0], st[1], pool,
+                                 dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+                                 out.stride(0), *_room(workspace), _lib.stream_of(q)))
     return out
 
 
@@ -181,21 +197,19 @@ def attend_chunk(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     the pages already.  Each sees the positions up to its own, as in
     ``attend_token``.  Returns (tokens, heads, head dim) in q's type."""
     pool = _pool(k_pages, v_pages, table, lengths)
-    dev, (_, kv_heads, page, dim) = k_pages.device, k_pages.shape
-    _heads("q", q, None, dim, k_pages.dtype, dev)
-    rows = table.shape[0]
+    dev, (_, kv_heads, page, dim), (rows, cols) = k_pages.device, k_pages.shape, table.shape
+    dtype = k_pages.dtype
+    st = _heads("q", q, None, dim, dtype, dev)
     _int32("starts", starts, (rows + 1,), dev)
     window, sinks = _visible(window, sinks)
     out = _output(out, q)
     _lib.require_gpu(k_pages, what="attend_chunk")
-    L, tokens, heads = _lib.lib(), q.shape[0], q.shape[1]
-    need = L.qs_attend_chunk_workspace_bytes(tokens, rows, heads, kv_heads, dim, table.shape[1], page, window, sinks)
+    L, (tokens, heads, _) = _lib.lib(), q.shape
+    need = L.qs_attend_chunk_workspace_bytes(tokens, rows, heads, kv_heads, dim, cols, page, window, sinks)
     workspace = _workspace(workspace, need, dev)
-    _lib.check(L.qs_attend_chunk_ws(q.data_ptr(), _lib.dtype_code(q.dtype), tokens, rows, heads, kv_heads, dim,
-                                    q.stride(0), q.stride(1), starts.data_ptr(), pool,
-                                    dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
-                                    out.stride(0), _lib.ptr(workspace),
-                                    0 if workspace is None else workspace.numel(), _lib.stream_of(q)))
+    _lib.check(L.qs_attend_chunk_ws(q.data_ptr(), _lib.dtype_code(dtype), tokens, rows, heads, kv_heads, dim, st[0],
+                                    st[1], starts.data_ptr(), pool, dim ** -0.5 if scale is None else scale, window,
+                                    sinks, out.data_ptr(), out.stride(0), *_room(workspace), _lib.stream_of(q)))
     return out
 
 
@@ -203,7 +217,7 @@ def _store(kv):
     if kv.dim() < 4 or not kv.is_contiguous():
         raise ValueError(f"kv must be a contiguous (..., pages, kv heads, page, head dim) tensor, got {tuple(kv.shape)}")
     pages, heads, page, dim = kv.shape[-4:]
-    planes = kv.numel() // max(1, pages * heads * page * dim)
+    planes = kv.numel() // (pages * heads * page * dim or 1)
     return _lib.PageStore(kv.data_ptr(), planes, pages, heads, page, dim * kv.element_size())
 
 
@@ -250,8 +264,7 @@ def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, toke
     workspace = _workspace(workspace, L.qs_page_advance_workspace_bytes(rows), dev)
     _lib.check(L.qs_page_advance(store, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), _lib.ptr(parents),
                                  rows, cols, tokens, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
-                                 out[3].data_ptr(), _lib.ptr(workspace),
-                                 0 if workspace is None else workspace.numel(), _lib.stream_of(kv)))
+                                 out[3].data_ptr(), *_room(workspace), _lib.stream_of(kv)))
     return tuple(out)
 
 
