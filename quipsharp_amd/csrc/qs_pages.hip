@@ -137,6 +137,7 @@ dim3 copy_grid(const Store& st, int64_t count) {
 
 struct AdvanceArgs {
   const int32_t *table, *lengths, *refs, *parents;
+  const int32_t* row_tokens;  // per row, or null: `tokens` for all
   int32_t *table_out, *lengths_out, *refs_out, *short_pages, *plan;
   int rows, cols, pages, page, tokens;
 };
@@ -172,8 +173,12 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
     for (int p = tid; p < a.pages; p += kThreads) near_refs[p] = a.refs[p];
   else if (a.refs_out != a.refs)
     for (int p = tid; p < a.pages; p += kThreads) ref_store(a.refs_out + p, a.refs[p]);
-  int old_len = 0;
+  int old_len = 0, tokens = a.tokens;
   if (tid < a.rows) {
+    if (a.row_tokens) {
+      const int n = a.row_tokens[tid];
+      tokens = n < 0 ? 0 : n > (1 << 30) ? 1 << 30 : n;
+    }
     int par = a.parents ? a.parents[tid] : tid;
     par = par >= 0 && par < a.rows ? par : -1;
     from[tid] = par;
@@ -210,7 +215,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   if (tid < a.rows) {
     c0 = old_len / a.page, used = old_len % a.page;
     int p = -1;
-    if (a.tokens > 0 && used > 0) p = entry((int64_t)tid * a.cols + c0);
+    if (tokens > 0 && used > 0) p = entry((int64_t)tid * a.cols + c0);
     mine[tid] = p >= 0 && ref_at(p) > 1 ? p : -1;
   }
   __syncthreads();
@@ -227,10 +232,10 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   if (tid < a.rows) {
     copy = shared_page[tid];
     first = c0 + (used > 0);
-    int64_t last = a.tokens > 0 ? ((int64_t)old_len + a.tokens - 1) / a.page : -1;
+    int64_t last = tokens > 0 ? ((int64_t)old_len + tokens - 1) / a.page : -1;
     if (last >= a.cols) atomicAdd(&lost, (int)(last - a.cols + 1)), last = a.cols - 1;
     wants = copy + (last >= first ? (int)(last - first + 1) : 0);
-    const int64_t end = (int64_t)old_len + a.tokens;
+    const int64_t end = (int64_t)old_len + tokens;
     a.lengths_out[tid] = (int)(end < room ? end : room);
   }
   int total;
@@ -596,6 +601,15 @@ extern "C" int qs_page_advance(const qs_page_store* store, const int32_t* table,
                                const int32_t* refs, const int32_t* parents, int64_t rows, int64_t cols, int tokens,
                                int32_t* table_out, int32_t* lengths_out, int32_t* refs_out, int32_t* short_pages,
                                void* workspace, size_t workspace_bytes, qs_stream_t stream) {
+  return qs_page_advance_rows(store, table, lengths, refs, parents, rows, cols, tokens, nullptr, table_out, lengths_out,
+                              refs_out, short_pages, workspace, workspace_bytes, stream);
+}
+
+extern "C" int qs_page_advance_rows(const qs_page_store* store, const int32_t* table, const int32_t* lengths,
+                                    const int32_t* refs, const int32_t* parents, int64_t rows, int64_t cols, int tokens,
+                                    const int32_t* row_tokens, int32_t* table_out, int32_t* lengths_out,
+                                    int32_t* refs_out, int32_t* short_pages, void* workspace, size_t workspace_bytes,
+                                    qs_stream_t stream) {
   Store st;
   if (const int rc = store_checks("qs_page_advance", store, st)) return rc;
   if (const int rc = table_checks("qs_page_advance", rows, cols, st.pages, st.page)) return rc;
@@ -606,7 +620,7 @@ extern "C" int qs_page_advance(const qs_page_store* store, const int32_t* table,
              "qs_page_advance: workspace of %zu bytes (16-byte aligned), %zu needed", workspace_bytes,
              qs_page_advance_workspace_bytes(rows));
   int32_t* plan = static_cast<int32_t*>(workspace);
-  const AdvanceArgs a{table, lengths, refs, parents, table_out, lengths_out, refs_out, short_pages, plan,
+  const AdvanceArgs a{table, lengths, refs, parents, row_tokens, table_out, lengths_out, refs_out, short_pages, plan,
                       (int)rows, (int)cols, (int)st.pages, st.page, tokens};
   if (st.pages <= kNearPages && rows * cols <= kTileInts) hipLaunchKernelGGL(page_advance_kernel<true>, dim3(1), dim3(kThreads), 0, as_stream(stream), a);
   else hipLaunchKernelGGL(page_advance_kernel<false>, dim3(1), dim3(kThreads), 0, as_stream(stream), a);

@@ -230,13 +230,13 @@ def _books(table, lengths, refs, pages, device):
     _int32("refs", refs, (pages,), device)
 
 
-def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, tokens: int = 1, parents: Tensor = None,
-                  *, out=None, workspace: Tensor = None):
+def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, tokens=1, parents: Tensor = None, *,
+                  out=None, workspace: Tensor = None):
     """One step of every row of a cache ``kv`` (..., pages, kv heads, page,
     head dim): row i takes the pages and the length of row ``parents[i]``
     (int32; None: its own; no row of the table: an empty one), gives back pages
-    beyond that length, and gets room for ``tokens`` more positions, by which
-    its length grows.
+    beyond that length, and gets room for ``tokens`` more positions (a number,
+    or an int32 tensor with one for every row), by which its length grows.
 
     The partly filled page that a row writes next is copied where several rows
     hold it, for each of them but the longest (the first of the longest); full
@@ -250,7 +250,10 @@ def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, toke
     rows, cols = table.shape
     if parents is not None:
         _int32("parents", parents, (rows,), dev)
-    if not 0 <= tokens <= 1 << 30:
+    each = None
+    if isinstance(tokens, Tensor):
+        each, tokens = _int32("tokens", tokens, (rows,), dev), 0
+    elif not 0 <= tokens <= 1 << 30:
         raise ValueError(f"{tokens} tokens")
     if out is None:
         out = (torch.empty_like(table), torch.empty_like(lengths), torch.empty_like(refs),
@@ -262,9 +265,9 @@ def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, toke
     _lib.require_gpu(kv, what="advance_pages")
     L = _lib.lib()
     workspace = _workspace(workspace, L.qs_page_advance_workspace_bytes(rows), dev)
-    _lib.check(L.qs_page_advance(store, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), _lib.ptr(parents),
-                                 rows, cols, tokens, out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
-                                 out[3].data_ptr(), *_room(workspace), _lib.stream_of(kv)))
+    _lib.check(L.qs_page_advance_rows(store, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), _lib.ptr(parents),
+                                      rows, cols, tokens, _lib.ptr(each), out[0].data_ptr(), out[1].data_ptr(),
+                                      out[2].data_ptr(), out[3].data_ptr(), *_room(workspace), _lib.stream_of(kv)))
     return tuple(out)
 
 

@@ -183,6 +183,38 @@ def test_entries_that_name_no_page(dev):
     assert cache.kv.shape == kv.shape
 
 
+def test_a_number_of_tokens_for_every_row(dev):
+    """Rows that begin, go on and wait in one call give what one call after the other gives where no page is shared,
+    and the rows that wait keep what they share."""
+    from quipsharp_amd.pages import PagedCache
+    cache, books = filled(5, 9, 60, 16, dev)
+    r = random.Random(2)
+    for step in range(12):
+        each = [r.choice([0, 0, 1, 5, 17, 33]) for _ in range(5)]
+        cache.advance(torch.tensor(each, dtype=torch.int32, device=dev))
+        taken = sum(-(-n // 16) - -(-m // 16) for n, m in zip(cache.lengths.tolist(), books.length))
+        free = [p for p in range(60) if books.refs()[p] == 0][:taken]
+        for i, n in enumerate(each):
+            n0, n1 = books.length[i], min(books.length[i] + n, 9 * 16)
+            for c in range(-(-n0 // 16), -(-n1 // 16)):
+                books.table[i][c] = free.pop(0)
+            books.length[i] = n1
+        books.same(cache)
+    # two rows of one parent: the one that writes copies the page, the one that waits keeps it
+    cache = PagedCache(1, 20, 1, 64, 2, 4, page=16, device=dev)
+    cache.advance(torch.tensor([20, 0], dtype=torch.int32, device=dev))
+    cache.kv.copy_(torch.randn(cache.kv.shape, generator=torch.Generator().manual_seed(1)))
+    zero = torch.zeros(2, dtype=torch.int32, device=dev)
+    cache.advance(0, zero)
+    kept = cache.table[0].tolist()
+    cache.advance(torch.tensor([0, 3], dtype=torch.int32, device=dev))
+    assert cache.table[0].tolist() == kept and cache.lengths.tolist() == [20, 23]
+    assert cache.table[1, 0] == kept[0] and cache.table[1, 1] != kept[1]
+    assert torch.equal(cache.kv[:, :, cache.table[1, 1].item(), :, :4], cache.kv[:, :, kept[1], :, :4])
+    cache.advance(torch.tensor([-7, 0], dtype=torch.int32, device=dev))
+    assert cache.lengths.tolist() == [20, 23]
+
+
 def test_many_rows_and_pages(dev):
     """The largest number of rows, and a pool that takes many rounds to look through."""
     from quipsharp_amd.pages import PagedCache
