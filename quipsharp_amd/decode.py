@@ -130,7 +130,7 @@ class StaticDecoder:
     (several tokens per row) runs transformers' modules with the same bf16
     cache (attention in fp32)."""
 
-    def __init__(self, model, batch, max_len):
+    def __init__(self, model, batch, max_len, cache=True):
         from . import _lib
         cfg = model.config
         self.model = model
@@ -143,8 +143,9 @@ class StaticDecoder:
         dev = model.lm_head.weight.device
         self.dev = dev
         bf = torch.bfloat16
-        self.k = [torch.zeros(batch, self.nkv, max_len, self.hd, device=dev, dtype=bf) for _ in self.layers]
-        self.v = [torch.zeros(batch, self.nkv, max_len, self.hd, device=dev, dtype=bf) for _ in self.layers]
+        if cache:
+            self.k = [torch.zeros(batch, self.nkv, max_len, self.hd, device=dev, dtype=bf) for _ in self.layers]
+            self.v = [torch.zeros(batch, self.nkv, max_len, self.hd, device=dev, dtype=bf) for _ in self.layers]
         self.kpos = torch.arange(max_len, device=dev)
         # rotary tables of every cache position, as transformers computes them
         m = model.model
@@ -153,8 +154,9 @@ class StaticDecoder:
         self.cos, self.sin = cos[0].to(bf).contiguous(), sin[0].to(bf).contiguous()
         L = _lib.lib()
         self._L, self._lib = L, _lib
-        nbytes = L.qs_dec_attention_workspace_bytes(batch, self.nkv, max_len)
-        self.attn_ws = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
+        if cache:
+            nbytes = L.qs_dec_attention_workspace_bytes(batch, self.nkv, max_len)
+            self.attn_ws = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
         self.fused_ok = self.hd == 128 and self.nh % self.nkv == 0 and self.nh // self.nkv <= 16 \
             and self.hidden % 8 == 0
 
@@ -201,7 +203,7 @@ class StaticDecoder:
         L, lib = self._L, self._lib
         m = self.model.model
         B = ids.shape[0]
-        H, nh, nkv, hd = self.hidden, self.nh, self.nkv, self.hd
+        H, nh, hd = self.hidden, self.nh, self.hd
         stream = lib.stream_of(ids)
         vp = lib.ptr
         h = m.embed_tokens(ids).reshape(B, H)
@@ -221,12 +223,8 @@ class StaticDecoder:
                                              {"kind": "rmsnorm", "delta": delta, "h_out": h_alt, "eps": self.eps,
                                               "weight": self._weight(Ly.input_layernorm)})
             h, h_alt = h_alt, h
-            # q/k norm, rotary and the cache write inside the attention's launches
-            lib.check(L.qs_dec_attention_rope(vp(qo.contiguous()), vp(ko.contiguous()), vp(vo.contiguous()),
-                                              vp(self._weight(a.q_norm)), vp(self._weight(a.k_norm)), vp(self.cos),
-                                              vp(self.sin), vp(pos), vp(self.k[i]), vp(self.v[i]), vp(attn), nh * hd,
-                                              vp(self.attn_ws), self.attn_ws.numel(), B, nh, nkv, hd, self.max_len,
-                                              self.eps, self.scale, stream))
+            self._attend(i, qo.contiguous(), ko.contiguous(), vo.contiguous(),
+                         (self._weight(a.q_norm), self._weight(a.k_norm)), pos, attn, stream)
             o = a.o_proj(attn).contiguous()
             go, uo = grouped_forward_pre(h, [Ly.mlp.gate_proj, Ly.mlp.up_proj],
                                          {"kind": "rmsnorm", "delta": o, "h_out": h_alt, "eps": self.eps,
@@ -240,6 +238,14 @@ class StaticDecoder:
         x = torch.empty_like(h)
         lib.check(L.qs_dec_rmsnorm(vp(h), vp(delta), vp(h), vp(self._weight(m.norm)), vp(x), B, H, H, self.eps, stream))
         return self.model.lm_head(x)
+
+    def _attend(self, i, qo, ko, vo, norms, pos, out, stream):
+        """q/k norm, rotary and the cache write inside the attention's launches."""
+        L, vp = self._L, self._lib.ptr
+        self._lib.check(L.qs_dec_attention_rope(vp(qo), vp(ko), vp(vo), vp(norms[0]), vp(norms[1]), vp(self.cos),
+                                                vp(self.sin), vp(pos), vp(self.k[i]), vp(self.v[i]), vp(out),
+                                                self.nh * self.hd, vp(self.attn_ws), self.attn_ws.numel(), self.B,
+                                                self.nh, self.nkv, self.hd, self.max_len, self.eps, self.scale, stream))
 
 
 @torch.no_grad()
@@ -283,6 +289,147 @@ def greedy_decode_static(model, prompt_ids, new_tokens, use_graph=True):
         toks.append(nxt.clone())
     torch.cuda.synchronize()
     return torch.cat(toks, 1), t1 - t0, time.perf_counter() - t2
+
+
+class PagedDecoder(StaticDecoder):
+    """StaticDecoder's layers over a paged cache (pages.PagedCache): rows of
+    different lengths, prompts that begin while other rows wait, rows that fork
+    (beam search) and, with ``window``, streams far longer than what is kept
+    visible (the last ``window`` positions and the first ``sinks``; pages that
+    fell out are given back).  Everything that a step needs to know of its rows
+    lies on the GPU, so a step can be captured once and replayed."""
+
+    def __init__(self, model, rows, max_len, page=64, pages=None, window=0, sinks=0):
+        from .pages import PagedCache
+        super().__init__(model, rows, max_len, cache=False)
+        if not self.fused_ok:
+            raise ValueError("the paged decode step takes head_dim 128 and at most 16 query heads per kv head")
+        columns = -(-max_len // page)
+        self.window, self.sinks = window, sinks
+        self.cache = PagedCache(len(self.layers), rows * columns if pages is None else pages, self.nkv, self.hd, rows,
+                                columns, page, torch.bfloat16, self.dev)
+        self.spans = {"window": window, "sinks": sinks}
+
+    @torch.no_grad()
+    def prompt(self, ids, counts):
+        """``counts[r]`` new tokens of row r (0: the row waits), their ids one
+        row after the other in ``ids``.  Logits of every row's last token, for
+        the rows with tokens."""
+        from transformers.models.qwen3.modeling_qwen3 import apply_rotary_pos_emb
+        m, cache = self.model.model, self.cache
+        T = int(sum(counts))
+        if ids.shape != (T,) or len(counts) != self.B:
+            raise ValueError(f"ids {tuple(ids.shape)} for {T} tokens in {len(counts)} of {self.B} rows")
+        count = torch.tensor(counts, dtype=torch.int32)
+        starts = torch.cat([torch.zeros(1, dtype=torch.int32), count.cumsum(0, dtype=torch.int32)]).to(self.dev)
+        last = (count.cumsum(0) - 1)[count > 0].to(self.dev)
+        row = torch.repeat_interleave(torch.arange(self.B), count).to(self.dev)
+        cache.advance(count.to(self.dev))
+        pos = cache.lengths[row] - starts[row + 1] + torch.arange(T, device=self.dev)
+        h = m.embed_tokens(ids)[None]
+        cos, sin = m.rotary_emb(h, pos[None])
+        for i, L in enumerate(self.layers):
+            a = L.self_attn
+            x = L.input_layernorm(h)
+            qo, ko, vo = grouped_forward(x, [a.q_proj, a.k_proj, a.v_proj])
+            q = a.q_norm(qo.view(1, T, self.nh, self.hd)).transpose(1, 2)
+            k = a.k_norm(ko.view(1, T, self.nkv, self.hd)).transpose(1, 2)
+            q, k = apply_rotary_pos_emb(q, k, cos, sin)
+            bf = torch.bfloat16
+            cache.append(i, k[0].transpose(0, 1).to(bf).contiguous(), vo.view(T, self.nkv, self.hd).to(bf), starts)
+            o = cache.attend_chunk(i, q[0].transpose(0, 1).to(bf).contiguous(), starts, scale=self.scale, **self.spans)
+            h = h + a.o_proj(o.view(1, T, self.nh * self.hd).to(h.dtype))
+            x = L.post_attention_layernorm(h)
+            go, uo = grouped_forward(x, [L.mlp.gate_proj, L.mlp.up_proj])
+            h = h + L.mlp.down_proj(L.mlp.act_fn(go) * uo)
+        if self.window:
+            cache.free(window=self.window, sinks=self.sinks)
+        return self.model.lm_head(m.norm(h[0, last]))
+
+    @torch.no_grad()
+    def step(self, ids, parents=None):
+        """One new token for every row, ids (rows,) or (rows, 1): row i goes on
+        from row ``parents[i]`` (int32; None: its own).  Logits (rows, vocab)."""
+        self.cache.advance(1, parents)
+        logits = self._decode_step(ids.reshape(-1, 1), None)
+        if self.window:
+            self.cache.free(window=self.window, sinks=self.sinks)
+        return logits
+
+    def _attend(self, i, qo, ko, vo, norms, pos, out, stream):
+        from .pages import _pool
+        c, vp = self.cache, self._lib.ptr
+        q = torch.empty_like(out)
+        self._lib.check(self._L.qs_page_append_rope(
+            vp(qo), vp(ko), vp(vo), vp(norms[0]), vp(norms[1]), vp(self.cos), vp(self.sin), self.cos.shape[0], vp(q),
+            self.B, self.nh, self.nkv, self.hd, _pool(c.keys(i), c.values(i), c.table, c.lengths), self.eps, stream))
+        heads = (self.B, self.nh, self.hd)
+        c.attend_token(i, q.view(heads), scale=self.scale, out=out.view(heads), **self.spans)
+
+
+@torch.no_grad()
+def beam_decode(model, prompts, beams, new_tokens, eos=-1, use_graph=True, page=64):
+    """Beam search: the ``beams`` best continuations of each prompt (a list of
+    1-D id tensors, of any lengths) by ``new_tokens`` tokens, a beam that took
+    ``eos`` going on with it at its score.  Steps are replays of one HIP graph
+    unless use_graph=False.  Returns (tokens (prompts, beams, new_tokens) in
+    descending order of scores (prompts, beams), prompt s, decode s)."""
+    from .beam import beam_select, reorder_states
+    R, dev = len(prompts), prompts[0].device
+    longest = max(len(p) for p in prompts)
+    columns = -(-(longest + new_tokens) // page)
+    # every beam may come to hold all its pages after the prompt's last full one, and a copy of what it goes on from
+    pages = sum(len(p) // page + 1 for p in prompts) + R * beams * (-(-new_tokens // page) + 2)
+    dec = PagedDecoder(model, R * beams, columns * page, page, pages)
+    counts = [0] * (R * beams)
+    counts[::beams] = [len(p) for p in prompts]
+    torch.cuda.synchronize()
+    t0 = time.perf_counter()
+    logits = dec.prompt(torch.cat(list(prompts)), counts)
+    torch.cuda.synchronize()
+    t1 = time.perf_counter()
+    # a prompt's row is its first beam, the only one that counts in the first selection
+    scores = torch.full((R, beams), float("-inf"), device=dev)
+    scores[:, 0] = 0
+    scores, parents, last = beam_select(logits.repeat_interleave(beams, 0), scores)
+    finished = last == eos
+    tokens = torch.zeros(R * beams, new_tokens, dtype=torch.int32, device=dev)
+    tokens[:, 0] = last.view(-1)
+    at = torch.ones(1, dtype=torch.long, device=dev)
+
+    def step():
+        logits = dec.step(last.view(-1).long(), parents.view(-1))
+        s, p, t = beam_select(logits, scores, finished=finished, eos=eos)
+        old, ended = reorder_states([tokens, finished.view(-1, 1)], p)
+        tokens.copy_(old.index_copy(1, at, t.view(-1, 1)))
+        finished.copy_(ended.view(R, beams) | (t == eos))
+        for keep, new in ((scores, s), (parents, p), (last, t)):
+            keep.copy_(new)
+        at.add_(1)
+
+    if use_graph and new_tokens > 2:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        torch.cuda.synchronize()
+        t1, t0 = time.perf_counter(), t0 + time.perf_counter() - t1  # the capture is no part of either time
+        todo, go = new_tokens - 2, graph.replay
+    else:
+        todo, go = new_tokens - 1, step
+    for _ in range(todo):
+        go()
+    torch.cuda.synchronize()
+    t2 = time.perf_counter()
+    short = dec.cache.short.item()
+    if short:
+        raise RuntimeError(f"the cache is short of {short} pages")
+    return tokens.view(R, beams, new_tokens).long(), scores, t1 - t0, t2 - t1
 
 
 def linear_bytes(m, n, B):
@@ -442,6 +589,7 @@ def main():
     ap.add_argument("--batch", type=int, nargs="+", default=[1, 8])
     ap.add_argument("--prompt", type=int, default=512)
     ap.add_argument("--new", type=int, default=256)
+    ap.add_argument("--beams", type=int, default=0, help="also decode each batch by a search with this many beams")
     ap.add_argument("--eager", action="store_true", help="decode steps launched eagerly (no HIP graph)")
     args = ap.parse_args()
     from transformers import Qwen3Config
@@ -463,6 +611,10 @@ def main():
         res["runs"].append({"batch": B, "graph": not args.eager, "prefill_s": round(pre_s, 3), "decode_s": round(dec_s, 3),
                             "tok_per_s": round(B * steps / dec_s, 2), "ms_per_step": round(1e3 * dec_s / steps, 3),
                             "first_tokens": toks[0, :8].tolist()})
+        if args.beams:
+            toks, scores, pre_s, dec_s = beam_decode(model, list(ids), args.beams, args.new, use_graph=not args.eager)
+            res["runs"][-1]["beams"] = {"beams": args.beams, "prefill_s": round(pre_s, 3), "decode_s": round(dec_s, 3),
+                                        "best_scores": [round(x, 3) for x in scores[:, 0].tolist()]}
     res["per_linear"] = linear_gbps(model, args.batch)
     print(json.dumps(res), flush=True)
 
