@@ -439,8 +439,7 @@ int qs_attend_token(const void *q, int dtype, int64_t rows, int heads, int kv_he
  * its own: the tokens of row r are starts[r] .. starts[r + 1] - 1 of q and
  * out, the last of them at position lengths[r] - 1, their keys and values in
  * the pages already.  starts: [rows + 1], not decreasing, starts[rows] =
- * tokens.  Values at the row's positions have to be finite where another
- * query of the call sees them. */
+ * tokens. */
 int qs_attend_chunk(const void *q, int dtype, int64_t tokens, int64_t rows, int heads, int kv_heads, int head_dim,
                     int64_t q_token, int64_t q_head, const int32_t *starts, const qs_page_pool *pool, float scale,
                     int window, int sinks, void *out, int64_t out_token, qs_stream_t stream);

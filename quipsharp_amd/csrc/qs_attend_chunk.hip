@@ -2,6 +2,7 @@
 // (qs_attend_chunk).  The tokens of row r are q[starts[r]] .. q[starts[r + 1]
 // - 1]; the last of them is at position lengths[r] - 1.
 #include <cmath>
+#include <type_traits>
 
 #include "qs_attend_dev.h"
 
@@ -26,6 +27,7 @@ struct ChunkArgs {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 template <bool BF>
 __device__ __forceinline__ f32x16 mma_32x32x16(const uint4& a, const uint4& b, f32x16 c) {
@@ -34,6 +36,32 @@ __device__ __forceinline__ f32x16 mma_32x32x16(const uint4& a, const uint4& b, f
   else
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+
+template <bool BF>
+__device__ __forceinline__ float from16(uint16_t x) {
+  if constexpr (BF) return __uint_as_float((uint32_t)x << 16);
+  else return (float)__builtin_bit_cast(_Float16, x);
+}
+
+// The bits of two elements' exponents: all of them set for infinities and no
+// numbers.
+template <bool BF>
+constexpr uint32_t exponents() { return BF ? 0x7F807F80u : 0x7C007C00u; }
+
+// Two elements as finite ones (0 for the others) and ones at +inf and at -inf;
+// no number counts as both, whose sum is none.
+template <bool BF>
+struct Parted {
+  uint32_t finite, plus, minus;
+  __device__ __forceinline__ explicit Parted(uint32_t two) {
+    const uint32_t lack = ~two & exponents<BF>(), one = BF ? 0x3F80u : 0x3C00u;
+    const uint32_t odd = (lack - 0x00010001u) & ~lack & 0x80008000u;  // bits 15 and 31: nothing lacks
+    const uint32_t none = odd & ((two & (BF ? 0x007F007Fu : 0x03FF03FFu)) + 0x7FFF7FFFu);
+    finite = two & ~((odd >> 15) * 0xFFFFu);
+    plus = ((odd & (~two | none)) >> 15) * one;
+    minus = ((odd & (two | none)) >> 15) * one;
+  }
+};
 
 // 4 rows of 16 elements from LDS, transposed: lane i of 16 gives the address
 // of elements 4 (i % 4) .. + 3 of row i / 4 and gets element i of the rows.
@@ -135,21 +163,28 @@ __device__ __forceinline__ bool find_block(const ChunkArgs& a, const PagePool& p
 // that token t sees, in one pass with the running maximum and sum.
 //
 // One work-group per kv head and 128 columns of a row, column c being head c %
-// group of the row's token c / group; one wave per 32 of them.  Tiles of kT
-// positions go through LDS, which all four waves read (straight from the L1
-// every wave loads every tile, 4 times the bytes that its rate allows beside
-// the products); the next tile is on its way in registers while one is worked
-// on.  As in WaveAttend both products are transposed, so that a column stays
-// the lane's own (lane & 31): a 32x32 result of K Q^T leaves lane (hf = lane /
-// 32) with positions 8 a + 4 hf + {0 .. 3}, and the second product takes 8 of
-// them at a step, with the values read through LDS's transposing load.
+// group of the row's token c / group; one wave per 32 of them, whose sums stay
+// in its registers.  Tiles of kT positions go through LDS, which all four
+// waves read (straight from the L1 every wave would load every tile: 616 us
+// for 8192 tokens under a window of 1024 instead of 192), past the registers
+// (through them 242 us); the next tile is on its way while one is worked on.
+// Two work-groups share a CU, so that one's softmax runs beside the other's
+// products.  Both products are transposed, so that a column stays the lane's
+// own (lane & 31): a 32x32 result of K Q^T leaves lane (hf = lane / 32) with
+// positions 8 a + 4 hf + {0 .. 3}, and the second product takes 8 of them at a
+// step, with the values read through LDS's transposing load.
 //
 // The weights refer to a base that follows the running maximum only where it
 // has fallen 2^8 behind, so that most tiles rescale nothing; in fp16 they
 // carry a factor of 2^7 too, which keeps 2^-21 of the largest from being
 // subnormal and the largest below 2^15.
+//
+// Bound by the matrix and vector instructions together, at the clock that
+// their power leaves: 129 GFLOP in 192 us (8192 tokens, window 1024) and 237
+// in 286 (six rows), 670 and 830 TFLOP/s, where the products alone would run
+// at 1750.
 template <bool BF, int HD>
-__global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_kernel(PagePool pp, ChunkArgs a) {
+__global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) void attend_chunk_kernel(PagePool pp, ChunkArgs a) {
   constexpr int kT = HD == 256 ? 32 : 64;   // positions of a tile
   constexpr int RT = kT / 32, G = kT / 16;  // matrix rows of 32 positions; groups of 16, which lie on one page
   constexpr int KS = HD / 16, DT = HD / 32;
@@ -161,6 +196,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   constexpr int kSwz = CPR < 16 ? 7 : 15;
   __shared__ __align__(16) char Ks[2][kT * kRow];
   __shared__ __align__(16) char Vs[2][kT * kRow];
+  __shared__ int odd[kWaves];  // whether a wave has results that are infinite or no number
   const int group = a.heads / a.kv_heads, g = blockIdx.x % a.kv_heads;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r32 = lane & 31, hf = lane >> 5;
   const LaneX lx = lane_x_init();
@@ -249,134 +285,232 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : 2) void attend_chunk_k
   const int i16 = lane & 15;
   const unsigned k_at = r32 * kRow + 16 * (hf ^ (r32 & kSwz));
   const unsigned v_at = (4 * hf + (i16 >> 2)) * kRow + 16 * ((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ 2 * (i16 >> 2)) + 8 * (i16 & 1);
-  f32x16 o[DT];
+  // In a tile that not every column sees all of, a value that is infinite or
+  // no number must not meet the columns that do not see it, whose weight of 0
+  // would make it NaN.  Where results are not finite the tiles are gone over
+  // again (in a loop of its own: looking in the first one took 2 to 7 %), the
+  // wave that brings such a value puts a zero in its place, and at the end
+  // they are brought to the columns that see them.
+  auto partial = [&](int u) {
+    const int p0 = kT * tiles.at(u);
+    return p0 + kT - 1 > g0.last || (p0 < g1.low && p0 + kT - 1 >= g0.sinks);
+  };
+  auto take_out = [&](int u, int buf) {
+    if (!partial(u)) return;
+    char* v = Vs[buf] + w * RW * kRow + 16 * lane;
+    uint4 x[NJ];
 #pragma unroll
-  for (int d = 0; d < DT; ++d)
+    for (int j = 0; j < NJ; ++j) x[j] = *reinterpret_cast<const uint4*>(v + 1024 * j);
+    // the least of what the exponents lack of all bits set: of the low elements and of the high ones
+    u16x2 least = {0xFFFF, 0xFFFF};
 #pragma unroll
-    for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
-  float top = -INFINITY, sum = 0.f;
-  unsigned ok = 0, ok_next = 0;
-  int e_next = 0;
-  if (u0 < n) {
-    const int e = entry(u0);
-    ok = valid(e);
-    fetch(u0, u0 & 1, e, ok);
-    e_next = entry(u0 + 1 < n ? u0 + 1 : u0);
-    wait_loads<0>();
-    clear(u0, u0 & 1, ok);
-  }
-  __syncthreads();
-  for (int u = u0; u < n; ++u, ok = ok_next) {
-    const int p0 = kT * tiles.at(u), buf = u & 1;
-    const int next = u + 1 < n ? u + 1 : u;
-    ok_next = valid(e_next);
-    fetch(next, buf ^ 1, e_next, ok_next);
-    e_next = entry(u + 2 < n ? u + 2 : next);
-    if (p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
-      unsigned ka = k_at, va = v_at;
-      asm volatile("" : "+v"(ka), "+v"(va));  // the addresses made of these are not kept over the loop
-      f32x16 st[RT];
+    for (int j = 0; j < NJ; ++j) {
+      const uint32_t words[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) st[r][i] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const uint4 kf = *reinterpret_cast<const uint4*>(Ks[buf] + 32 * r * kRow + (ka ^ 32 * ks));
-          st[r] = mma_32x32x16<BF>(kf, q[ks], st[r]);
-        }
-      const bool all = ok == kAll && p0 + kT - 1 <= s0.last && (p0 >= s1.low || p0 + kT - 1 < s0.sinks);
-      if (!all) {
-        // the span from this lane's first position on
-        const int at = p0 + 4 * hf, hi = s.last - at, lo = s.low - at, sk = s.sinks - at;
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int p = 32 * r + 8 * (i / 4) + i % 4;
-            const bool see = p <= (ok >> (2 * r + i / 8) & 1 ? hi : -1) && (p >= lo || p < sk);
-            st[r][i] = see ? st[r][i] : -INFINITY;
-          }
-      }
-      float mx = st[0][0];
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[r][i]);
-      mx = fmaxf(mx, lane_xor<32>(mx, lx));
-      // the base of the weights follows the maximum only where it has fallen 2^8 behind
-      if (__any((mx - top) * a.scale > 8.f)) {
-        const float up = fmaxf(mx, top), f = up == -INFINITY ? 1.f : weight(top - up, a.scale);
-        top = up;
-        sum *= f;
-#pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[d][i] *= f;
-      }
-      const float base = top == -INFINITY ? 0.f : top;
-      float back = BF ? -base * a.scale : __builtin_fmaf(-base, a.scale, 7.f);
-      if (__any(fabsf(base) > 1e36f)) {
-        // the product with scale could leave the range of fp32: the difference first
-#pragma unroll
-        for (int r = 0; r < RT; ++r)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) st[r][i] -= base;
-        back = BF ? 0.f : 7.f;
-      }
-      uint4 pb[RT][2];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        float part = 0.f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          st[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r][i], a.scale, back));
-          part += st[r][i];
-        }
-        sum += part;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          pb[r][x] = make_uint4(pack16<BF>(st[r][8 * x], st[r][8 * x + 1]), pack16<BF>(st[r][8 * x + 2], st[r][8 * x + 3]),
-                                pack16<BF>(st[r][8 * x + 4], st[r][8 * x + 5]), pack16<BF>(st[r][8 * x + 6], st[r][8 * x + 7]));
-      }
-      // positions 32 r + 16 x + 4 hf + {0 .. 3, 8 .. 11} are this lane's operand of a step
-#pragma unroll
-      for (int r = 0; r < RT; ++r)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const char* at = Vs[buf] + (32 * r + 16 * x) * kRow + (va ^ 64 * d);
-            const uint2 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
-            o[d] = mma_32x32x16<BF>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[r][x], o[d]);
-          }
+      for (int i = 0; i < 4; ++i) least = __builtin_elementwise_min(least, __builtin_bit_cast(u16x2, ~words[i] & exponents<BF>()));
     }
-    wait_loads<0>();
-    clear(next, buf ^ 1, ok_next);
-    __syncthreads();
-  }
-  const float l = sum + lane_xor<32>(sum, lx);
-  if (!live) return;
-  if (a.splits > 1) {
-    float* to = a.part + (((int64_t)(blk.first + t) * a.heads + h) * a.splits + split) * part_floats(HD);
-    if (hf == 0) to[0] = top, to[1] = l;
+    if (!__any(least[0] == 0 || least[1] == 0)) return;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      *reinterpret_cast<uint4*>(v + 1024 * j) =
+          make_uint4(Parted<BF>(x[j].x).finite, Parted<BF>(x[j].y).finite, Parted<BF>(x[j].z).finite, Parted<BF>(x[j].w).finite);
+  };
+
+  f32x16 o[DT];
+  float top, sum;
+  // One pass over the tiles; CLEAN: with values taken out.
+  auto sweep = [&](auto clean_values) {
+    constexpr bool CLEAN = decltype(clean_values)::value;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
-      for (int i = 0; i < 16; i += 2)
-        *reinterpret_cast<float2*>(to + kPartHead + 32 * d + 2 * (i & ~3) + 4 * hf + i % 4) = make_float2(o[d][i], o[d][i + 1]);
-    return;
-  }
-  const float rcp = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* to = a.out + (int64_t)(blk.first + t) * a.out_token + (int64_t)h * HD;
+      for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
+    top = -INFINITY, sum = 0.f;
+    unsigned ok = 0, ok_next = 0;
+    int e_next = 0;
+    if (u0 < n) {
+      const int e = entry(u0);
+      ok = valid(e);
+      fetch(u0, u0 & 1, e, ok);
+      e_next = entry(u0 + 1 < n ? u0 + 1 : u0);
+      wait_loads<0>();
+      clear(u0, u0 & 1, ok);
+      if (CLEAN) take_out(u0, u0 & 1);
+    }
+    __syncthreads();
+    for (int u = u0; u < n; ++u, ok = ok_next) {
+      const int p0 = kT * tiles.at(u), buf = u & 1;
+      const int next = u + 1 < n ? u + 1 : u;
+      ok_next = valid(e_next);
+      fetch(next, buf ^ 1, e_next, ok_next);
+      e_next = entry(u + 2 < n ? u + 2 : next);
+      if (cw < columns && p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
+        unsigned ka = k_at, va = v_at;
+        asm volatile("" : "+v"(ka), "+v"(va));  // the addresses made of these are not kept over the loop
+        f32x16 st[RT];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) st[r][i] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int r = 0; r < RT; ++r) {
+            const uint4 kf = *reinterpret_cast<const uint4*>(Ks[buf] + 32 * r * kRow + (ka ^ 32 * ks));
+            st[r] = mma_32x32x16<BF>(kf, q[ks], st[r]);
+          }
+        const bool all = ok == kAll && p0 + kT - 1 <= s0.last && (p0 >= s1.low || p0 + kT - 1 < s0.sinks);
+        if (!all) {
+          // the span from this lane's first position on
+          const int at = p0 + 4 * hf, hi = s.last - at, lo = s.low - at, sk = s.sinks - at;
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int p = 32 * r + 8 * (i / 4) + i % 4;
+              const bool see = p <= (ok >> (2 * r + i / 8) & 1 ? hi : -1) && (p >= lo || p < sk);
+              st[r][i] = see ? st[r][i] : -INFINITY;
+            }
+        }
+        float mx = st[0][0];
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, st[r][i]);
+        mx = fmaxf(mx, lane_xor<32>(mx, lx));
+        // the base of the weights follows the maximum only where it has fallen 2^8 behind
+        if (__any((mx - top) * a.scale > 8.f)) {
+          const float up = fmaxf(mx, top), f = up == -INFINITY ? 1.f : weight(top - up, a.scale);
+          top = up;
+          sum *= f;
+#pragma unroll
+          for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[d][i] *= f;
+        }
+        const float base = top == -INFINITY ? 0.f : top;
+        float back = BF ? -base * a.scale : __builtin_fmaf(-base, a.scale, 7.f);
+        if (__any(fabsf(base) > 1e36f)) {
+          // the product with scale could leave the range of fp32: the difference first
+#pragma unroll
+          for (int r = 0; r < RT; ++r)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) st[r][i] -= base;
+          back = BF ? 0.f : 7.f;
+        }
+        uint4 pb[RT][2];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          float part = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            st[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r][i], a.scale, back));
+            part += st[r][i];
+          }
+          sum += part;
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            pb[r][x] = make_uint4(pack16<BF>(st[r][8 * x], st[r][8 * x + 1]), pack16<BF>(st[r][8 * x + 2], st[r][8 * x + 3]),
+                                  pack16<BF>(st[r][8 * x + 4], st[r][8 * x + 5]), pack16<BF>(st[r][8 * x + 6], st[r][8 * x + 7]));
+        }
+        // positions 32 r + 16 x + 4 hf + {0 .. 3, 8 .. 11} are this lane's operand of a step
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              const char* at = Vs[buf] + (32 * r + 16 * x) * kRow + (va ^ 64 * d);
+              const uint2 lo = read_transposed(at), hi = read_transposed(at + 8 * kRow);
+              o[d] = mma_32x32x16<BF>(make_uint4(lo.x, lo.y, hi.x, hi.y), pb[r][x], o[d]);
+            }
+      }
+      wait_loads<0>();
+      clear(next, buf ^ 1, ok_next);
+      if (CLEAN) take_out(next, buf ^ 1);
+      __syncthreads();
+    }
+  };
+  sweep(std::false_type());
+  // infinite or no number?
+  float zero = 0.f;
 #pragma unroll
   for (int d = 0; d < DT; ++d)
 #pragma unroll
-    for (int i = 0; i < 16; i += 4)
-      *reinterpret_cast<uint2*>(to + 32 * d + 2 * i + 4 * hf) =
-          make_uint2(pack16<BF>(o[d][i] * rcp, o[d][i + 1] * rcp), pack16<BF>(o[d][i + 2] * rcp, o[d][i + 3] * rcp));
+    for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(o[d][i], 0.f, zero);
+  if (lane == 0) odd[w] = 0;
+  if (zero != 0.f) odd[w] = 1;
+  __syncthreads();
+  const bool again = __builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]);
+  if (again) sweep(std::true_type());
+  const float l = sum + lane_xor<32>(sum, lx);
+  // element i of o[d] is dimension 32 d + 2 (i & ~3) + 4 hf + i % 4
+  float* part = a.part + (((int64_t)(blk.first + t) * a.heads + h) * a.splits + split) * part_floats(HD) + kPartHead + 4 * hf;
+  uint16_t* out = a.out + (int64_t)(blk.first + t) * a.out_token + (int64_t)h * HD + 4 * hf;
+  if (live && a.splits > 1) {
+    if (hf == 0) part[-kPartHead] = top, part[1 - kPartHead] = l;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<f32x4*>(part + 32 * d + 2 * i) = f32x4{o[d][i], o[d][i + 1], o[d][i + 2], o[d][i + 3]};
+  } else if (live) {
+    const float rcp = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<uint2*>(out + 32 * d + 2 * i) =
+            make_uint2(pack16<BF>(o[d][i] * rcp, o[d][i + 1] * rcp), pack16<BF>(o[d][i + 2] * rcp, o[d][i + 3] * rcp));
+  }
+  if (!again) return;
+  // Ones at the infinite values (no number counts as +inf and -inf) times
+  // ones at the positions that a column sees say what its sums get.
+  f32x16 up[DT], down[DT];
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) up[d][i] = down[d][i] = 0.f;
+  for (int u = u0; u < n; ++u) {
+    if (!partial(u)) continue;
+    __syncthreads();
+    const int e = entry(u);
+    fetch(u, 0, e, valid(e));
+    wait_loads<0>();
+    clear(u, 0, valid(e));
+    __syncthreads();
+    const int at = kT * tiles.at(u) + 4 * hf, hi = s.last - at, lo = s.low - at, sk = s.sinks - at;
+    constexpr uint32_t one = BF ? 0x3F80u : 0x3C00u;
+#pragma unroll 1
+    for (int r = 0; r < 2 * RT; ++r) {
+      uint32_t sees[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int p = 16 * r + 8 * (i / 4) + i % 4;
+        sees[i / 2] |= p <= hi && (p >= lo || p < sk) ? one << 16 * (i % 2) : 0u;
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        const char* v = Vs[0] + 16 * r * kRow + (v_at ^ 64 * d);
+        const uint2 x = read_transposed(v), y = read_transposed(v + 8 * kRow);
+        const Parted<BF> x0(x.x), x1(x.y), y0(y.x), y1(y.y);
+        const uint4 b = make_uint4(sees[0], sees[1], sees[2], sees[3]);
+        up[d] = mma_32x32x16<BF>(make_uint4(x0.plus, x1.plus, y0.plus, y1.plus), b, up[d]);
+        down[d] = mma_32x32x16<BF>(make_uint4(x0.minus, x1.minus, y0.minus, y1.minus), b, down[d]);
+      }
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int d = 0; d < DT; ++d)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (!(up[d][i] > 0.f || down[d][i] > 0.f)) continue;
+      const int at = 32 * d + 2 * (i & ~3) + i % 4;
+      const float gets = (up[d][i] > 0.f ? INFINITY : 0.f) - (down[d][i] > 0.f ? INFINITY : 0.f);
+      if (a.splits > 1) part[at] += gets;
+      else out[at] = (uint16_t)pack16<BF>(from16<BF>(out[at]) + gets, 0.f);
+    }
 }
 
 int64_t chunk_blocks(int64_t tokens, int64_t rows, int heads, int kv_heads) {
@@ -384,11 +518,11 @@ int64_t chunk_blocks(int64_t tokens, int64_t rows, int heads, int kv_heads) {
 }
 
 // Into how many shares the tiles of a block are cut.  A share is a work-group;
-// two of them fill a CU, so cutting pays where the blocks' heads are fewer
-// than the chip's 512 places, and shares of less than 4 tiles do not repay the
-// second launch that joins them (16 tokens of 8 kv heads over 6000 positions:
-// %%A us whole, %%B us in shares; a prompt of 512 with 64 heads: %%C us whole,
-// %%D us in two).
+// a CU has room for two, so cutting pays where the blocks' heads are fewer
+// than half the chip's CUs, and shares of less than 8 tiles do not repay the
+// second launch and the parts that it joins (16 tokens of 8 kv heads behind
+// 6000 positions: 136 us whole, 26 us in shares; a prompt of 512 with 64 heads:
+// 21 us whole, 36 us in two).
 int chunk_splits(int64_t tokens, int64_t rows, int heads, int kv_heads, int64_t cols, int page, int window, int sinks) {
   const int64_t blocks = (tokens * (heads / kv_heads) + kCols - 1) / kCols, wgs = blocks * kv_heads;
   const int64_t seen = seen_positions(cols * page, window, sinks, (tokens - 1 < kCols ? tokens - 1 : kCols));

@@ -256,6 +256,78 @@ def test_infinite_keys_outside_the_window(dev):
     check(got, q, c, [(0, 199)], 128 ** -0.5, 48, 10)
 
 
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("heads,kv_heads,dim,window,sinks", [(4, 1, 128, 0, 0), (4, 2, 64, 40, 3), (8, 8, 128, 90, 0),
+                                                             (2, 1, 256, 33, 20)])
+def test_values_that_are_no_numbers(dev, heads, kv_heads, dim, window, sinks, dtype):
+    """Infinities and NaN reach the tokens that see their position, and no other."""
+    from quipsharp_amd.pages import attend_chunk
+    dt, n, new = TYPES[dtype], 300, 200
+    c = Cache([n], kv_heads, dim, 32, dt, 21)
+    k, v, table, length = c.to(dev)
+    bad = {290: math.nan, 150: math.inf, 130: -math.inf, 199: math.nan, 64: math.inf, 1: math.nan if window else 0.5}
+    for p, x in bad.items():
+        v[int(c.table[0, p // 32]), kv_heads - 1, p % 32, 5::7] = x
+        c.rows[0][1][p, kv_heads - 1, 5::7] = x
+    q = torch.randn(new, heads, dim, generator=torch.Generator().manual_seed(1)).to(dt).to(dev)
+    got = attend_chunk(q, k, v, table, length, torch.tensor([0, new], dtype=torch.int32, device=dev), window=window,
+                       sinks=sinks).cpu().double()
+    group = heads // kv_heads
+    for t in range(new):
+        see = seen_by(n - new + t, window, sinks)
+        for g in range(kv_heads):
+            rv = c.rows[0][1][see, g]
+            out, tol = want_and_tolerance(q[t, g * group:(g + 1) * group].cpu(), c.rows[0][0][see, g],
+                                          torch.nan_to_num(rv, 0, 0, 0), dim ** -0.5)
+            fine = torch.isfinite(rv).all(0)  # dimensions without such a value
+            mine = got[t, g * group:(g + 1) * group]
+            assert torch.equal(torch.isfinite(mine), fine.expand(group, -1)), (t, g)
+            assert ((mine - out).abs() <= tol)[:, fine].all(), (t, g)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("rows,heads,kv_heads,dim,page,window,sinks", [
+    ([(1, 6000)], 8, 1, 128, 64, 0, 0), ([(5, 4096), (0, 300), (3, 20), (2, 2500)], 4, 2, 64, 32, 0, 0),
+    ([(7, 5000)], 6, 2, 256, 16, 0, 0), ([(9, 7000), (4, 5)], 7, 1, 128, 128, 3000, 20)])
+def test_few_tokens_behind_a_long_cache(dev, rows, heads, kv_heads, dim, page, window, sinks, dtype):
+    """Positions shared by several work-groups, some of whose shares hold nothing that a row sees; without a
+    workspace one takes them all."""
+    from quipsharp_amd import _lib
+    from quipsharp_amd.pages import _pool, attend_chunk, chunk_workspace_bytes
+    dt = TYPES[dtype]
+    lengths = [a + b for a, b in rows]
+    c = Cache(lengths, kv_heads, dim, page, dt, sum(lengths))
+    starts = [0]
+    for a, _ in rows:
+        starts.append(starts[-1] + a)
+    k, v, table, n = c.to(dev)
+    q = torch.randn(starts[-1], heads, dim, generator=torch.Generator().manual_seed(dim)).to(dt).to(dev)
+    begin = torch.tensor(starts, dtype=torch.int32, device=dev)
+    assert chunk_workspace_bytes(starts[-1], heads, k, table, window, sinks) > 0
+    where = [(r, b + i) for r, (a, b) in enumerate(rows) for i in range(a)]
+    check(attend_chunk(q, k, v, table, n, begin, window=window, sinks=sinks), q, c, where, dim ** -0.5, window, sinks)
+    whole = torch.empty_like(q)
+    _lib.check(_lib.lib().qs_attend_chunk(q.data_ptr(), _lib.dtype_code(dt), starts[-1], len(rows), heads, kv_heads, dim,
+                                          heads * dim, dim, begin.data_ptr(), _pool(k, v, table, n), dim ** -0.5, window,
+                                          sinks, whole.data_ptr(), heads * dim, _lib.stream_of(q)))
+    check(whole, q, c, where, dim ** -0.5, window, sinks)
+
+
+@pytest.mark.parametrize("rows", [70, 200])
+def test_many_rows_of_several_tokens(dev, rows):
+    """More rows than a wave has lanes, of mixed lengths, some without new tokens."""
+    from quipsharp_amd.pages import attend_chunk
+    new = [(7 * r) % 5 for r in range(rows)]
+    cached = [(13 * r) % 60 for r in range(rows)]
+    c = Cache([a + b for a, b in zip(new, cached)], 1, 64, 16, torch.bfloat16, rows)
+    starts = [0]
+    for a in new:
+        starts.append(starts[-1] + a)
+    q = torch.randn(starts[-1], 3, 64, generator=torch.Generator().manual_seed(1)).bfloat16().to(dev)
+    got = attend_chunk(q, *c.to(dev), torch.tensor(starts, dtype=torch.int32, device=dev))
+    check(got, q, c, [(r, cached[r] + i) for r in range(rows) for i in range(new[r])], 0.125, 0, 0)
+
+
 def test_lowest_and_equal_scores(dev):
     """Scores that are all the type's lowest, and all the same."""
     from quipsharp_amd.pages import attend_chunk, attend_token
