@@ -89,7 +89,8 @@ def reorder_states(states, parents: Tensor):
         stride.append(s.stride()[0] * each if rows > 1 else size[-1])
     _lib.require_gpu(*states, what="reorder_states")
     for s in states:
-        out.append(s.new_empty((n,) + s.shape[1:]))
+        out.append(torch.empty_like(s, memory_format=torch.contiguous_format) if n == rows
+                   else s.new_empty((n,) + s.shape[1:]))
     k = len(states)
     words, pointers = _WORDS[k], _POINTERS[k]
     _lib.check(_lib.lib().qs_reorder_states(k, pointers(*[s.data_ptr() for s in states]),

@@ -14,8 +14,10 @@ namespace qs {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kJoin = 256;  // threads of the join
 constexpr int kMaxKeep = 128;
-constexpr int kRoom = 4096;  // candidates of a slice
+constexpr int kRoom = 2304;  // candidates of a slice (what lies above the edge, or 128 of it and a row of ties)
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Order-preserving bits of a float; -0 counts as 0, NaN as -inf.
 __device__ __forceinline__ uint32_t order_bits(float f) {
@@ -75,12 +77,12 @@ struct Slice {
   __device__ __forceinline__ static int token(int t0, int i) { return t0 + (i / W * kThreads + (int)threadIdx.x) * W + i % W; }
   __device__ __forceinline__ void load(const T* row, int t0, int vocab) {
     if (WIDE && t0 + E * kThreads <= vocab) {
-      uint4 v[E / W];
+      u32x4 v[E / W];
 #pragma unroll
-      for (int i = 0; i < E / W; ++i) v[i] = *reinterpret_cast<const uint4*>(row + token(t0, i * W));
+      for (int i = 0; i < E / W; ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(row + token(t0, i * W)));
 #pragma unroll
       for (int i = 0; i < E / W; ++i) {
-        const uint32_t u[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+        const u32x4 u = v[i];
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           if constexpr (sizeof(T) == 4) x[i * W + e] = __uint_as_float(u[e]);
@@ -109,11 +111,14 @@ struct Slice {
 // One work-group per slice of 256 E logits, which stay in registers.
 //
 // A logit is among the slice's best only if it is not below the edge: the
-// keep-th largest of the threads' largest, or (up to 64) the largest of the
+// keep-th largest of the threads' largest, or (up to 32) the largest of the
 // waves' keep-th largest, which takes no exchange.  Above the edge lie at
 // most (keep - 1) E logits by the first rule and four times as many by the
 // second, which slice_size keeps below kRoom, and few in most cases; those at
 // the edge may be any number, and the lowest tokens of them are taken.
+//
+// Bound by the logits' way from memory: 26 us for 155 MB (256 rows of 151936
+// fp32).
 template <typename T, bool WIDE, int E>
 __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
   typedef Slice<T, WIDE, E> S;
@@ -139,14 +144,14 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
   top = fmaxf(top, lane_xor<4>(top, lx));
   top = fmaxf(top, lane_xor<2>(top, lx));
   top = fmaxf(top, lane_xor<1>(top, lx));
-  const float edge_w = keep <= 64 ? order_float(nth_key(order_bits(m), keep)) : -INFINITY;
-  if (keep > 64) tops[tid] = m;
+  const float edge_w = keep <= 32 ? order_float(nth_key(order_bits(m), keep)) : -INFINITY;
+  if (keep > 32) tops[tid] = m;
   if (lane == 0) red[0][w] = top, red[1][w] = edge_w;
   if (tid == 0) count = 0;
   __syncthreads();
   const float all = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   float edge = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
-  if (keep > 64) {
+  if (keep > 32) {
     int above = 0, same = 0;
     for (int i = 0; i < kThreads; ++i) above += tops[i] > m, same += tops[i] == m;
     if (above < keep && keep <= above + same) line = m;  // all that write it write the same
@@ -220,60 +225,64 @@ __device__ __forceinline__ bool over(const Candidate& x, const Candidate& y) {
 }
 
 // One work-group per request.
-__global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a, Candidate* spill) {
-  constexpr int kList = 512;
-  __shared__ double base[1024];  // score - log sum; of a beam without continuations -inf
+__global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidate* spill) {
+  constexpr int kList = 512, kAhead = 4;
+  __shared__ double base[1024];  // the sum; then score - log sum, of a beam without continuations -inf
+  __shared__ float largest[1024];
   __shared__ uint8_t state[1024];
   __shared__ Candidate list[kList];
-  __shared__ uint32_t tops[kThreads];
+  __shared__ uint32_t tops[kJoin];
   __shared__ uint32_t edge;
   __shared__ int count;
   const LaneX lx = lane_x_init();
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const int64_t b = blockIdx.x;
-  for (int j = w; j < a.beams; j += kThreads / 64) {
-    const int64_t row = b * a.beams + j;
-    const bool done = a.finished && a.finished[row];
-    const float s = a.scores[row];
-    double c = -INFINITY;
-    if (fabsf(s) < INFINITY) {
-      if (done) {
-        c = s;
-      } else {
-        // lane i: slices i, i + 64 ..
-        const float2* st = reinterpret_cast<const float2*>(a.stats) + row * a.slices;
-        float m = -INFINITY, l = 0.f;
-        for (int i = lane; i < a.slices; i += 64) {
-          const float2 x = st[i];
-          const float up = fmaxf(m, x.x);
-          l = l * exp_below(m, up) + x.y * exp_below(x.x, up);
-          m = up;
-        }
-        float top = m;
-        top = fmaxf(top, lane_xor<32>(top, lx));
-        top = fmaxf(top, lane_xor<16>(top, lx));
-        top = fmaxf(top, lane_xor<8>(top, lx));
-        top = fmaxf(top, lane_xor<4>(top, lx));
-        top = fmaxf(top, lane_xor<2>(top, lx));
-        top = fmaxf(top, lane_xor<1>(top, lx));
-        const float sum = wave_sum(fabsf(top) < INFINITY ? l * exp_below(m, top) : 0.f, lx);
-        if (fabsf(top) < INFINITY) c = (double)s - ((double)top + log((double)sum));
-      }
+  const int some = a.slices * a.keep, per = some > a.keep + 1 ? some : a.keep + 1, all = a.beams * per;
+  // a thread's first candidates are on their way while the sums are made
+  uint64_t ahead[kAhead];
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    const int e = tid + i * kJoin, j = e / per;
+    ahead[i] = e < all && e - j * per < some ? a.best[(b * a.beams + j) * some + e - j * per] : 0;
+  }
+  for (int j = w; j < a.beams; j += kJoin / 64) {
+    // lane i: slices i, i + 64 ..
+    const float2* st = reinterpret_cast<const float2*>(a.stats) + (b * a.beams + j) * a.slices;
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < a.slices; i += 64) {
+      const float2 x = st[i];
+      const float up = fmaxf(m, x.x);
+      l = l * exp_below(m, up) + x.y * exp_below(x.x, up);
+      m = up;
     }
-    if (lane == 0) base[j] = c, state[j] = done ? 1 : c == -INFINITY ? 2 : 0;
+    float top = m;
+    top = fmaxf(top, lane_xor<32>(top, lx));
+    top = fmaxf(top, lane_xor<16>(top, lx));
+    top = fmaxf(top, lane_xor<8>(top, lx));
+    top = fmaxf(top, lane_xor<4>(top, lx));
+    top = fmaxf(top, lane_xor<2>(top, lx));
+    top = fmaxf(top, lane_xor<1>(top, lx));
+    const float sum = wave_sum(fabsf(top) < INFINITY ? l * exp_below(m, top) : 0.f, lx);
+    if (lane == 0) base[j] = sum, largest[j] = top;
   }
   if (tid == 0) count = 0, edge = 0;
   __syncthreads();
-  // a beam offers slices * keep candidates; one that is finished or has none keep + 1: eos and the first tokens
-  const int some = a.slices * a.keep, per = some > a.keep + 1 ? some : a.keep + 1, all = a.beams * per;
-  auto get = [&](int e) {
-    const int j = e / per, i = e % per;
+  for (int j = tid; j < a.beams; j += kJoin) {
     const int64_t row = b * a.beams + j;
+    const bool done = a.finished && a.finished[row];
+    const float s = a.scores[row], top = largest[j];
+    double c = -INFINITY;
+    if (fabsf(s) < INFINITY && done) c = s;
+    else if (fabsf(s) < INFINITY && fabsf(top) < INFINITY) c = (double)s - ((double)top + log(base[j]));
+    base[j] = c, state[j] = done ? 1 : c == -INFINITY ? 2 : 0;
+  }
+  __syncthreads();
+  // a beam offers slices * keep candidates; one that is finished or has none keep + 1: eos and the first tokens
+  auto get = [&](int e, uint64_t k) {
+    const int j = e / per, i = e - j * per;
     int64_t t = -1;
     double v = -INFINITY;
     if (state[j] == 0) {
-      if (i >= some) return Candidate{0, 0};
-      const uint64_t k = a.best[row * some + i];
       if (!k) return Candidate{0, 0};
       t = (uint32_t)~k;
       v = base[j] + (double)order_float((uint32_t)(k >> 32));
@@ -286,13 +295,22 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a, Candi
     }
     return Candidate{order_bits64(v), ~(uint32_t)(j * (int64_t)a.vocab + t)};
   };
+  auto each = [&](auto use) {
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (tid + i * kJoin < all) use(get(tid + i * kJoin, ahead[i]));
+    for (int e = tid + kAhead * kJoin; e < all; e += kJoin) {
+      const int j = e / per;
+      use(get(e, e - j * per < some ? a.best[(b * a.beams + j) * some + e - j * per] : 0));
+    }
+  };
   // The upper half of a score's order bits is enough to leave most out: at
   // least `keep` candidates have the edge's or more, and so have the best.
   uint32_t top = 0;
-  for (int e = tid; e < all; e += kThreads) {
-    const uint32_t hi = (uint32_t)(get(e).score >> 32);
+  each([&](const Candidate& c) {
+    const uint32_t hi = (uint32_t)(c.score >> 32);
     top = hi > top ? hi : top;
-  }
+  });
   if (a.keep <= 64) {
     const uint32_t u = nth_key(top, a.keep);
     if (lane == 0) atomicMax(&edge, u);
@@ -300,22 +318,21 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a, Candi
     tops[tid] = top;
     __syncthreads();
     int above = 0, same = 0;
-    for (int i = 0; i < kThreads; ++i) above += tops[i] > top, same += tops[i] == top && i < tid;
+    for (int i = 0; i < kJoin; ++i) above += tops[i] > top, same += tops[i] == top && i < tid;
     if (above + same == a.keep - 1) edge = top;
   }
   __syncthreads();
   const uint32_t least = edge;
   Candidate* more = spill + b * (int64_t)all;
-  for (int e = tid; e < all; e += kThreads) {
-    const Candidate c = get(e);
-    if (!c.score || (uint32_t)(c.score >> 32) < least) continue;
+  each([&](const Candidate& c) {
+    if (!c.score || (uint32_t)(c.score >> 32) < least) return;
     const int at = atomicAdd(&count, 1);
     (at < kList ? list[at] : more[at]) = c;
-  }
+  });
   __threadfence();
   __syncthreads();
   const int n = count;
-  for (int c = tid; c < n; c += kThreads) {
+  for (int c = tid; c < n; c += kJoin) {
     const Candidate x = c < kList ? list[c] : more[c];
     int rank = 0;
     const int near = n < kList ? n : kList;
@@ -330,14 +347,13 @@ __global__ __launch_bounds__(kThreads) void beam_join_kernel(SelectArgs a, Candi
   }
 }
 
-// Logits per thread: as many as leave a work-group for each CU, since a
-// slice's selection costs the same whatever its length, and few enough that
-// what lies above the edge fits (see beam_slice_kernel).
+// Logits per thread: 32 where that leaves work-groups enough to fill the chip
+// (256 rows of 151936: 40 us for the whole selection, with 16 48 us, with 64
+// 42 us), 16 otherwise and where what lies above the edge would not fit
+// (beam_slice_kernel).
 int slice_size(int64_t rows, int64_t vocab, int keep) {
-  const int most = keep <= 16 ? 64 : keep <= 32 ? 32 : keep <= 64 ? 16 : 32;
-  int e = 16;
-  while (e < most && rows * ((vocab + 2 * kThreads * e - 1) / (2 * kThreads * e)) >= 512) e *= 2;
-  return e;
+  const bool fits = keep <= 16 || (keep > 32 && keep <= 64);
+  return fits && rows * ((vocab + 32 * kThreads - 1) / (32 * kThreads)) >= 512 ? 32 : 16;
 }
 
 struct Layout {
@@ -362,8 +378,8 @@ Layout layout_of(int64_t batch, int beams, int64_t vocab, int keep) {
 
 template <typename T>
 auto slice_kernel(bool wide, int each) {
-  if (wide) return each == 64 ? beam_slice_kernel<T, true, 64> : each == 32 ? beam_slice_kernel<T, true, 32> : beam_slice_kernel<T, true, 16>;
-  return each == 64 ? beam_slice_kernel<T, false, 64> : each == 32 ? beam_slice_kernel<T, false, 32> : beam_slice_kernel<T, false, 16>;
+  if (wide) return each == 32 ? beam_slice_kernel<T, true, 32> : beam_slice_kernel<T, true, 16>;
+  return each == 32 ? beam_slice_kernel<T, false, 32> : beam_slice_kernel<T, false, 16>;
 }
 
 // ---------------------------------------------------------------------------
@@ -438,7 +454,7 @@ extern "C" int qs_beam_select(const void* logits, int dtype, int64_t ld, int64_t
                                              : slice_kernel<uint16_t>(wide, l.each);
   hipLaunchKernelGGL(slice, grid, dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("beam_slice_kernel");
-  hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)batch), dim3(kThreads), 0, as_stream(stream), a,
+  hipLaunchKernelGGL(beam_join_kernel, dim3((unsigned)batch), dim3(kJoin), 0, as_stream(stream), a,
                      reinterpret_cast<Candidate*>(ws + l.spill));
   QS_LAUNCHED("beam_join_kernel");
   return QS_OK;
