@@ -232,9 +232,10 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
   for (int ks = 0; ks < KS; ++ks) q[ks] = flipped(*reinterpret_cast<const uint4*>(qp + 16 * ks + 8 * hf), a.flip);
   const int32_t* trow = pp.table + row * pp.table_ld;
 
-  // lane i < G: the table's entry for positions 16 i .. of tile u
-  auto entry = [&](int u) {
-    const int col = (kT * tiles.at(u) + 16 * (lane < G ? lane : 0)) >> pp.shift;
+  // lane i < G: the table's entry for positions 16 i .. of the tile at p0
+  const int lane_at = 16 * (lane < G ? lane : 0);
+  auto entry = [&](int p0) {
+    const int col = (p0 + lane_at) >> pp.shift;
     return col < pp.cols ? trow[col] : -1;
   };
   // which groups of 16 positions have a page (bits), and the page of this wave's
@@ -251,28 +252,28 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
     const int r = w * RW + j * RJ + rl;
     ko[j] = 2u * ((r & 15) * pp.k_pos + 8 * (piece ^ (r & kSwz)));
   }
-  constexpr int NV = RJ % 4 == 0 ? 1 : 2;  // loads until the swizzle of the values comes round again
-  static_assert(NV * RJ % 4 == 0, "");
-  unsigned vo[NV];
+  unsigned vo[NJ];
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
-    vo[j] = 2u * ((w * RW % 16 + rl) * pp.v_pos + 8 * (piece ^ 2 * ((j * RJ + rl) & 3)));
-  auto fetch = [&](int u, int buf, int e, unsigned ok) {
-    const int p0 = kT * tiles.at(u);
-    const int64_t id = ok >> gw & 1 ? __builtin_amdgcn_readlane(e, gw) : 0;
-    const int at = (p0 + 16 * gw) & mask;
-    const char* kb = reinterpret_cast<const char*>(pp.k + id * pp.k_page + g * pp.k_head + (int64_t)at * pp.k_pos);
-    const char* vb = reinterpret_cast<const char*>(pp.v + id * pp.v_page + g * pp.v_head + (int64_t)at * pp.v_pos);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) load_to_lds(kb, ko[j], k_lds + buf * (kT * kRow) + 1024 * j);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      load_to_lds(vb + (int64_t)2 * j * RJ * pp.v_pos, vo[j % NV], v_lds + buf * (kT * kRow) + 1024 * j);
+  for (int j = 0; j < NJ; ++j) {
+    const int r = w * RW + j * RJ + rl;
+    vo[j] = 2u * ((r & 15) * pp.v_pos + 8 * (piece ^ 2 * (r & 3)));
+  }
+  // the head's first page; bytes from page to page and from position to position
+  const char* const k_head = reinterpret_cast<const char*>(pp.k + g * pp.k_head);
+  const char* const v_head = reinterpret_cast<const char*>(pp.v + g * pp.v_head);
+  const unsigned k_page = 2u * (unsigned)pp.k_page, v_page = 2u * (unsigned)pp.v_page;
+  const unsigned k_pos = 2u * pp.k_pos, v_pos = 2u * pp.v_pos;
+  // this wave's positions of the tile at p0
+  auto fetch = [&](int p0, int buf, int e, unsigned ok) {
+    const unsigned id = ok >> gw & 1 ? __builtin_amdgcn_readlane(e, gw) : 0;
+    const unsigned at = (p0 + 16 * gw) & mask;
+    load_rows(k_head + ((uint64_t)id * k_page + at * k_pos), ko, k_lds + buf * (kT * kRow));
+    load_rows(v_head + ((uint64_t)id * v_page + at * v_pos), vo, v_lds + buf * (kT * kRow));
   };
   // What lies in a place that the row has not filled may be no number, and 0
   // times it would be none either: zeros there, by the wave that brought it.
-  auto clear = [&](int u, int buf, unsigned ok) {
-    const int fill = ok >> gw & 1 ? len - (kT * tiles.at(u) + w * RW) : 0;
+  auto clear = [&](int p0, int buf, unsigned ok) {
+    const int fill = ok >> gw & 1 ? len - (p0 + w * RW) : 0;
     if (fill < RW) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -291,12 +292,11 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
   // again (in a loop of its own: looking in the first one took 2 to 7 %), the
   // wave that brings such a value puts a zero in its place, and at the end
   // they are brought to the columns that see them.
-  auto partial = [&](int u) {
-    const int p0 = kT * tiles.at(u);
+  auto partial = [&](int p0) {
     return p0 + kT - 1 > g0.last || (p0 < g1.low && p0 + kT - 1 >= g0.sinks);
   };
-  auto take_out = [&](int u, int buf) {
-    if (!partial(u)) return;
+  auto take_out = [&](int p0, int buf) {
+    if (!partial(p0)) return;
     char* v = Vs[buf] + w * RW * kRow + 16 * lane;
     uint4 x[NJ];
 #pragma unroll
@@ -326,24 +326,27 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[d][i] = 0.f;
     top = -INFINITY, sum = 0.f;
-    unsigned ok = 0, ok_next = 0;
-    int e_next = 0;
+    unsigned ok = 0;
+    int e_next = 0, p0 = 0, p1 = 0, p2 = 0;  // the tile at hand, the next one (the last again), the one after it
+    float back = BF ? 0.f : 7.f;             // what the scaled scores get added: the lift less the base of the weights
+    bool far = false;                        // whether a base times scale could leave the range of fp32
     if (u0 < n) {
-      const int e = entry(u0);
+      p0 = kT * tiles.at(u0), p1 = kT * tiles.at(u0 + 1 < n ? u0 + 1 : u0);
+      const int e = entry(p0);
       ok = valid(e);
-      fetch(u0, u0 & 1, e, ok);
-      e_next = entry(u0 + 1 < n ? u0 + 1 : u0);
+      fetch(p0, u0 & 1, e, ok);
+      e_next = entry(p1);
       wait_loads<0>();
-      clear(u0, u0 & 1, ok);
-      if (CLEAN) take_out(u0, u0 & 1);
+      clear(p0, u0 & 1, ok);
+      if (CLEAN) take_out(p0, u0 & 1);
     }
     __syncthreads();
-    for (int u = u0; u < n; ++u, ok = ok_next) {
-      const int p0 = kT * tiles.at(u), buf = u & 1;
-      const int next = u + 1 < n ? u + 1 : u;
-      ok_next = valid(e_next);
-      fetch(next, buf ^ 1, e_next, ok_next);
-      e_next = entry(u + 2 < n ? u + 2 : next);
+    for (int u = u0; u < n; ++u) {
+      const int buf = u & 1;
+      const unsigned ok_next = valid(e_next);
+      fetch(p1, buf ^ 1, e_next, ok_next);
+      p2 = u + 2 < n ? kT * tiles.at(u + 2) : p1;
+      e_next = entry(p2);
       if (cw < columns && p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
         unsigned ka = k_at, va = v_at;
         asm volatile("" : "+v"(ka), "+v"(va));  // the addresses made of these are not kept over the loop
@@ -387,16 +390,19 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
           for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int i = 0; i < 16; ++i) o[d][i] *= f;
+          const float base = top == -INFINITY ? 0.f : top;
+          back = BF ? -base * a.scale : __builtin_fmaf(-base, a.scale, 7.f);
+          far = __any(fabsf(base) > 1e36f);
         }
-        const float base = top == -INFINITY ? 0.f : top;
-        float back = BF ? -base * a.scale : __builtin_fmaf(-base, a.scale, 7.f);
-        if (__any(fabsf(base) > 1e36f)) {
-          // the product with scale could leave the range of fp32: the difference first
+        float plus = back;
+        if (far) {
+          // the difference first
+          const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
           for (int r = 0; r < RT; ++r)
 #pragma unroll
             for (int i = 0; i < 16; ++i) st[r][i] -= base;
-          back = BF ? 0.f : 7.f;
+          plus = BF ? 0.f : 7.f;
         }
         uint4 pb[RT][2];
 #pragma unroll
@@ -404,7 +410,7 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
           float part = 0.f;
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            st[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r][i], a.scale, back));
+            st[r][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(st[r][i], a.scale, plus));
             part += st[r][i];
           }
           sum += part;
@@ -426,9 +432,10 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
             }
       }
       wait_loads<0>();
-      clear(next, buf ^ 1, ok_next);
-      if (CLEAN) take_out(next, buf ^ 1);
+      clear(p1, buf ^ 1, ok_next);
+      if (CLEAN) take_out(p1, buf ^ 1);
       __syncthreads();
+      p0 = p1, p1 = p2, ok = ok_next;
     }
   };
   sweep(std::false_type());
@@ -472,14 +479,15 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
 #pragma unroll
     for (int i = 0; i < 16; ++i) up[d][i] = down[d][i] = 0.f;
   for (int u = u0; u < n; ++u) {
-    if (!partial(u)) continue;
+    const int p0 = kT * tiles.at(u);
+    if (!partial(p0)) continue;
     __syncthreads();
-    const int e = entry(u);
-    fetch(u, 0, e, valid(e));
+    const int e = entry(p0);
+    fetch(p0, 0, e, valid(e));
     wait_loads<0>();
-    clear(u, 0, valid(e));
+    clear(p0, 0, valid(e));
     __syncthreads();
-    const int at = kT * tiles.at(u) + 4 * hf, hi = s.last - at, lo = s.low - at, sk = s.sinks - at;
+    const int at = p0 + 4 * hf, hi = s.last - at, lo = s.low - at, sk = s.sinks - at;
     constexpr uint32_t one = BF ? 0x3F80u : 0x3C00u;
 #pragma unroll 1
     for (int r = 0; r < 2 * RT; ++r) {
@@ -558,6 +566,10 @@ int page_pool_checks(const char* fn, const qs_page_pool* p, int dtype, int64_t r
   QS_REQUIRE(window >= 0 && sinks >= 0 && (sinks == 0 || window > 0), "%s: window %d, sinks %d", fn, window, sinks);
   const int64_t st[6] = {p->k_page, p->k_head, p->k_pos, p->v_page, p->v_head, p->v_pos};
   for (int64_t x : st) QS_REQUIRE(x >= 0 && x % 8 == 0, "%s: pool strides must be multiples of 8 elements, got %lld", fn, (long long)x);
+  QS_SUPPORTED(p->k_page < ((int64_t)1 << 31) && p->v_page < ((int64_t)1 << 31) && p->page * p->k_pos <= (1 << 30) &&
+                   p->page * p->v_pos <= (1 << 30),
+               "%s: pages %lld and %lld elements apart, positions %lld and %lld (at most 2^31, a page's 2^30)", fn,
+               (long long)p->k_page, (long long)p->v_page, (long long)p->k_pos, (long long)p->v_pos);
   QS_REQUIRE(p->k_pos >= head_dim && p->k_pos <= (1 << 24) && p->v_pos >= head_dim && p->v_pos <= (1 << 24),
              "%s: position strides %lld, %lld", fn, (long long)p->k_pos, (long long)p->v_pos);
   QS_REQUIRE(((reinterpret_cast<uintptr_t>(p->k) | reinterpret_cast<uintptr_t>(p->v)) & 15) == 0,

@@ -97,12 +97,22 @@ __device__ __forceinline__ uint4 flipped(uint4 x, uint32_t flip) {
   return make_uint4(x.x ^ flip, x.y ^ flip, x.z ^ flip, x.w ^ flip);
 }
 
-// 16 bytes per lane from base + off straight to LDS, at `lds` + 16 lane.  The
+// 16 bytes per lane from base + off straight to LDS, at `lds` + AT + 16 lane.  The
 // compiler does not count this load: wait_loads before the bytes are read.
 // (Its own form would have it wait for all such loads before the next read of
 // LDS, whatever place that reads.)
+template <int AT>
 __device__ __forceinline__ void load_to_lds(const char* base, unsigned off, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base), "n"(AT)
+               : "memory", "m0", "scc");
+}
+// N loads whose lanes' places behind base are off, one after the other in LDS.
+template <int N, int AT = 0>
+__device__ __forceinline__ void load_rows(const char* base, const unsigned (&off)[N], unsigned lds) {
+  if constexpr (AT < N) {
+    load_to_lds<1024 * AT>(base, off[AT], lds);
+    load_rows<N, AT + 1>(base, off, lds);
+  }
 }
 // All but the last N of the wave's loads are there (loads that are written in
 // the program between two of these calls stay between them).
@@ -174,8 +184,7 @@ struct WaveAttend {
     for (int t = 0; t < 2; ++t) {
       const int64_t id = e[t] < 0 ? 0 : e[t];
       const char* kb = reinterpret_cast<const char*>(pp.k + id * pp.k_page + g * pp.k_head + (int64_t)((p0 + 16 * t) & mask) * pp.k_pos);
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) load_to_lds(kb, ko[j], lds + 16 * t * kRow + 1024 * j);
+      load_rows<NJ>(kb, ko, lds + 16 * t * kRow);
     }
     uint32_t vr[8][DPL / 2];
 #pragma unroll

@@ -223,3 +223,10 @@ def test_empty_calls_do_nothing():
     assert L.qs_page_append(None, None, 0, 0, 2, 128, 0, 0, 0, 0, None, None, None) == 0
     assert L.qs_page_copy(None, None, None, 0, None) == 0
     assert L.qs_beam_select(None, 0, 0, 0, 3, 10, None, None, -1, 3, None, None, None, None, 0, None) == 0
+
+
+@pytest.mark.parametrize("over", [dict(k_page=1 << 31), dict(v_page=1 << 31), dict(k_pos=1 << 24, page=128),
+                                  dict(v_pos=1 << 20, page=2048)])
+def test_pages_too_far_apart(over):
+    L = _lib.lib()
+    assert token(L, **over) == 3 and b"elements apart" in L.qs_last_error()
