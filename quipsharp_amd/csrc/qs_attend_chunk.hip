@@ -183,8 +183,12 @@ __device__ __forceinline__ bool find_block(const ChunkArgs& a, const PagePool& p
 // their power leaves: 129 GFLOP in 192 us (8192 tokens, window 1024) and 237
 // in 286 (six rows), 670 and 830 TFLOP/s, where the products alone would run
 // at 1750.
-template <bool BF, int HD>
-__global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) void attend_chunk_kernel(PagePool pp, ChunkArgs a) {
+//
+// GR = 2: eight waves, of which the second four take every other tile; their
+// results meet in LDS at the end.  For calls whose work-groups do not fill
+// the chip, where a block's own tiles are what takes the time.
+template <bool BF, int HD, int GR>
+__global__ __launch_bounds__(64 * kWaves * GR, HD == 256 ? 1 : HD == 128 || GR == 2 ? 2 : 3) void attend_chunk_kernel(PagePool pp, ChunkArgs a) {
   constexpr int kT = HD == 256 ? 32 : 64;   // positions of a tile
   constexpr int RT = kT / 32, G = kT / 16;  // matrix rows of 32 positions; groups of 16, which lie on one page
   constexpr int KS = HD / 16, DT = HD / 32;
@@ -194,12 +198,15 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
   constexpr int RJ = 64 / CPR;              // positions of one load of the wave
   constexpr int kRow = HD * 2;
   constexpr int kSwz = CPR < 16 ? 7 : 15;
-  __shared__ __align__(16) char Ks[2][kT * kRow];
-  __shared__ __align__(16) char Vs[2][kT * kRow];
-  __shared__ int odd[kWaves];  // whether a wave has results that are infinite or no number
+  __shared__ __align__(16) char all_keys[GR][2][kT * kRow];
+  __shared__ __align__(16) char all_values[GR][2][kT * kRow];
+  __shared__ int odd[kWaves * GR];  // whether a wave has results that are infinite or no number
   const int group = a.heads / a.kv_heads, g = blockIdx.x % a.kv_heads;
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r32 = lane & 31, hf = lane >> 5;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), w = wave % kWaves, gr = wave / kWaves;
+  const int lane = tid & 63, r32 = lane & 31, hf = lane >> 5;
   const LaneX lx = lane_x_init();
+  auto& Ks = all_keys[gr];
+  auto& Vs = all_values[gr];
   Block blk;
   if (!find_block(a, pp, blockIdx.x / a.kv_heads, group, lx, blk)) return;
   const int split = blockIdx.y;
@@ -209,9 +216,9 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
   const int64_t most = (int64_t)pp.cols << pp.shift;
   len = __builtin_amdgcn_readfirstlane(len > most ? (int)most : len);
   const int cw = b0 + 32 * w, c = cw + r32;
-  const bool live = c < columns;
-  const int t = live ? c / group : count - 1;
-  const int h = g * group + (live ? c % group : 0);
+  const bool column = c < columns;
+  const int t = column ? c / group : count - 1;
+  const int h = g * group + (column ? c % group : 0);
   const Span s = span_of(len - (count - t), a.window, a.sinks);  // last may be negative: sees nothing
   // the spans of the first and the last token of the wave and of the work-group
   auto span_at = [&](int col) {
@@ -331,23 +338,24 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
     float back = BF ? 0.f : 7.f;             // what the scaled scores get added: the lift less the base of the weights
     bool far = false;                        // whether a base times scale could leave the range of fp32
     if (u0 < n) {
-      p0 = kT * tiles.at(u0), p1 = kT * tiles.at(u0 + 1 < n ? u0 + 1 : u0);
+      const int first = u0 + gr < n ? u0 + gr : u0;
+      p0 = kT * tiles.at(first), p1 = kT * tiles.at(first + GR < n ? first + GR : first);
       const int e = entry(p0);
       ok = valid(e);
-      fetch(p0, u0 & 1, e, ok);
+      fetch(p0, 0, e, ok);
       e_next = entry(p1);
       wait_loads<0>();
-      clear(p0, u0 & 1, ok);
-      if (CLEAN) take_out(p0, u0 & 1);
+      clear(p0, 0, ok);
+      if (CLEAN) take_out(p0, 0);
     }
     __syncthreads();
-    for (int u = u0; u < n; ++u) {
-      const int buf = u & 1;
+    int buf = 0;
+    for (int u = u0 + gr; u - gr < n; u += GR, buf ^= 1) {
       const unsigned ok_next = valid(e_next);
       fetch(p1, buf ^ 1, e_next, ok_next);
-      p2 = u + 2 < n ? kT * tiles.at(u + 2) : p1;
+      p2 = u + 2 * GR < n ? kT * tiles.at(u + 2 * GR) : p1;
       e_next = entry(p2);
-      if (cw < columns && p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
+      if ((GR == 1 || u < n) && cw < columns && p0 <= last_w && (p0 + kT - 1 >= low_w || p0 < sinks_w)) {
         unsigned ka = k_at, va = v_at;
         asm volatile("" : "+v"(ka), "+v"(va));  // the addresses made of these are not kept over the loop
         f32x16 st[RT];
@@ -445,11 +453,38 @@ __global__ __launch_bounds__(64 * kWaves, HD == 256 ? 1 : HD == 128 ? 2 : 3) voi
   for (int d = 0; d < DT; ++d)
 #pragma unroll
     for (int i = 0; i < 16; ++i) zero = __builtin_fmaf(o[d][i], 0.f, zero);
-  if (lane == 0) odd[w] = 0;
-  if (zero != 0.f) odd[w] = 1;
+  if (lane == 0) odd[wave] = 0;
+  if (zero != 0.f) odd[wave] = 1;
   __syncthreads();
-  const bool again = __builtin_amdgcn_readfirstlane(odd[0] | odd[1] | odd[2] | odd[3]);
+  int some = odd[0];
+#pragma unroll
+  for (int i = 1; i < kWaves * GR; ++i) some |= odd[i];
+  const bool again = __builtin_amdgcn_readfirstlane(some);
   if (again) sweep(std::true_type());
+  if constexpr (GR == 2) {
+    // a wave's sums lie register by register, its lanes side by side
+    float* sums = reinterpret_cast<float*>(all_keys) + w * (DT * 16 * 64) + lane;
+    float* tops = reinterpret_cast<float*>(all_values) + w * 128 + lane;
+    static_assert(sizeof(all_keys) >= kWaves * DT * 16 * 64 * sizeof(float), "");
+    if (gr == 1) {
+      tops[0] = top, tops[64] = sum;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sums[(16 * d + i) * 64] = o[d][i];
+    }
+    __syncthreads();
+    if (gr == 0) {
+      const float up = fmaxf(top, tops[0]), base = up == -INFINITY ? 0.f : up;
+      const float f0 = weight(top - base, a.scale), f1 = weight(tops[0] - base, a.scale);
+      top = up, sum = f0 * sum + f1 * tops[64];
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[d][i] = f0 * o[d][i] + f1 * sums[(16 * d + i) * 64];
+    }
+  }
+  const bool live = column && gr == 0;
   const float l = sum + lane_xor<32>(sum, lx);
   // element i of o[d] is dimension 32 d + 2 (i & ~3) + 4 hf + i % 4
   float* part = a.part + (((int64_t)(blk.first + t) * a.heads + h) * a.splits + split) * part_floats(HD) + kPartHead + 4 * hf;
@@ -541,7 +576,22 @@ int chunk_splits(int64_t tokens, int64_t rows, int heads, int kv_heads, int64_t 
 template <bool BF, int HD>
 int launch_chunk(const PagePool& pp, const ChunkArgs& a, hipStream_t stream) {
   const int64_t blocks = chunk_blocks(a.tokens, a.rows, a.heads, a.kv_heads);
-  hipLaunchKernelGGL((attend_chunk_kernel<BF, HD>), dim3((unsigned)(blocks * a.kv_heads), (unsigned)a.splits), dim3(64 * kWaves), 0, stream, pp, a);
+  const dim3 grid((unsigned)(blocks * a.kv_heads), (unsigned)a.splits);
+  if constexpr (HD < 256) {  // whose registers leave no room for a second wave on a SIMD
+    // One work-group for a CU at most, with tiles for both halves: eight waves
+    // (a prompt of 512 with 64 heads: 19.2 us against 20.7, 300 tokens behind
+    // 6000 positions 105 against 146; with one or two tiles the second half
+    // only costs, 10.9 against 9.1 us for a prompt of 64).  The blocks counted
+    // are those that there are if the rows' tokens fill theirs.
+    const int64_t seen = seen_positions((int64_t)pp.cols << pp.shift, a.window, a.sinks, a.tokens - 1 < kCols ? a.tokens - 1 : kCols);
+    if ((blocks - a.rows) * a.kv_heads * a.splits <= 256 && seen / a.splits >= 256) {
+      hipLaunchKernelGGL((attend_chunk_kernel<BF, HD, 2>), grid, dim3(128 * kWaves), 0, stream, pp, a);
+      QS_LAUNCHED("attend_chunk_kernel");
+      if (a.splits > 1) return join_parts(a.part, a.splits, a.tokens, a.heads, HD, BF, a.scale, a.out, a.out_token, stream);
+      return QS_OK;
+    }
+  }
+  hipLaunchKernelGGL((attend_chunk_kernel<BF, HD, 1>), grid, dim3(64 * kWaves), 0, stream, pp, a);
   QS_LAUNCHED("attend_chunk_kernel");
   if (a.splits > 1) return join_parts(a.part, a.splits, a.tokens, a.heads, HD, BF, a.scale, a.out, a.out_token, stream);
   return QS_OK;

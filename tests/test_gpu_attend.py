@@ -258,7 +258,7 @@ def test_infinite_keys_outside_the_window(dev):
 
 @pytest.mark.parametrize("dtype", sorted(TYPES))
 @pytest.mark.parametrize("heads,kv_heads,dim,window,sinks", [(4, 1, 128, 0, 0), (4, 2, 64, 40, 3), (8, 8, 128, 90, 0),
-                                                             (2, 1, 256, 33, 20)])
+                                                             (2, 1, 256, 33, 20), (136, 136, 64, 70, 3)])
 def test_values_that_are_no_numbers(dev, heads, kv_heads, dim, window, sinks, dtype):
     """Infinities and NaN reach the tokens that see their position, and no other."""
     from quipsharp_amd.pages import attend_chunk
