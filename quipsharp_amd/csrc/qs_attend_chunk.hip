@@ -198,6 +198,8 @@ __global__ __launch_bounds__(64 * kWaves * GR, HD == 256 ? 1 : HD == 128 || GR =
   constexpr int RJ = 64 / CPR;              // positions of one load of the wave
   constexpr int kRow = HD * 2;
   constexpr int kSwz = CPR < 16 ? 7 : 15;
+  // a transposing load of half a wave takes 64 bytes of four positions: all 64 banks once
+  auto value_swizzle = [](int r) { return HD == 64 ? 2 * (r & 2) : 4 * (r & 3); };
   __shared__ __align__(16) char all_keys[GR][2][kT * kRow];
   __shared__ __align__(16) char all_values[GR][2][kT * kRow];
   __shared__ int odd[kWaves * GR];  // whether a wave has results that are infinite or no number
@@ -263,7 +265,7 @@ __global__ __launch_bounds__(64 * kWaves * GR, HD == 256 ? 1 : HD == 128 || GR =
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
     const int r = w * RW + j * RJ + rl;
-    vo[j] = 2u * ((r & 15) * pp.v_pos + 8 * (piece ^ 2 * (r & 3)));
+    vo[j] = 2u * ((r & 15) * pp.v_pos + 8 * (piece ^ value_swizzle(r)));
   }
   // the head's first page; bytes from page to page and from position to position
   const char* const k_head = reinterpret_cast<const char*>(pp.k + g * pp.k_head);
@@ -292,7 +294,7 @@ __global__ __launch_bounds__(64 * kWaves * GR, HD == 256 ? 1 : HD == 128 || GR =
 
   const int i16 = lane & 15;
   const unsigned k_at = r32 * kRow + 16 * (hf ^ (r32 & kSwz));
-  const unsigned v_at = (4 * hf + (i16 >> 2)) * kRow + 16 * ((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ 2 * (i16 >> 2)) + 8 * (i16 & 1);
+  const unsigned v_at = (4 * hf + (i16 >> 2)) * kRow + 16 * ((2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1)) ^ value_swizzle(i16 >> 2)) + 8 * (i16 & 1);
   // In a tile that not every column sees all of, a value that is infinite or
   // no number must not meet the columns that do not see it, whose weight of 0
   // would make it NaN.  Where results are not finite the tiles are gone over
