@@ -285,8 +285,24 @@ inline int64_t seen_positions(int64_t room, int window, int sinks, int64_t span)
 constexpr int kPartHead = 4;
 constexpr int part_floats(int head_dim) { return kPartHead + head_dim; }
 
-// The parts (part[token][head][split]) of `tokens` tokens' heads together.
-int join_parts(const float* part, int splits, int64_t tokens, int heads, int head_dim, bool bf, float scale,
+// The tiles of one share of a single token's: at least one for each wave, so
+// that a short row in a table of many columns uses few of the shares.
+constexpr int kShareTiles = 4;
+__host__ __device__ __forceinline__ int share_tiles(int count, int splits) {
+  const int n = (count + splits - 1) / splits;
+  return n < kShareTiles ? kShareTiles : n;
+}
+
+// Which parts of a single token's head there are: those of its row's tiles.
+struct Used {
+  const int32_t* lengths;
+  int64_t most;  // positions that the table has room for
+  int window, sinks;
+};
+
+// The parts (part[token][head][split]) of `tokens` tokens' heads together;
+// used: null where all are there.
+int join_parts(const float* part, int splits, const Used* used, int64_t tokens, int heads, int head_dim, bool bf, float scale,
                uint16_t* out, int64_t out_token, hipStream_t stream);
 
 // The argument checks of the attention calls; fills `out`.

@@ -41,12 +41,12 @@ __global__ __launch_bounds__(64 * kWavesT) void attend_token_kernel(PagePool pp,
   const int split = blockIdx.x, g = blockIdx.y / blocks, hb = blockIdx.y % blocks, row = blockIdx.z;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r16 = lane & 15, qd = lane >> 4;
   const LaneX lx = lane_x_init();
-  int len = pp.lengths[row];
   const int64_t most = (int64_t)pp.cols << pp.shift;
-  len = __builtin_amdgcn_readfirstlane(len > most ? (int)most : len);
+  const int len = __builtin_amdgcn_readfirstlane(pp.lengths[row] > most ? (int)most : pp.lengths[row]);
   const Span s = span_of(len - 1, a.window, a.sinks);
   const TileList<kTile> tiles(s);
-  const int run = (tiles.count + a.splits - 1) / a.splits;
+  const int run = share_tiles(tiles.count, a.splits);
+  if (split > 0 && split * run >= tiles.count) return;  // the join does not look for it
   const int u0 = split * run, u1 = u0 + run < tiles.count ? u0 + run : tiles.count;
   const int nh = group - 16 * hb < 16 ? group - 16 * hb : 16;
   const int h0 = g * group + 16 * hb;
@@ -118,8 +118,8 @@ __device__ __forceinline__ float vec_at(const V& x, int i) {
 // One wave per head of a token: lane i has the weights of splits i, i + 64
 // .., and HD / 64 dimensions.
 template <bool BF, int HD>
-__global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, int64_t pairs, int heads, float scale,
-                                                   uint16_t* out, int64_t out_token) {
+__global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, Used used, int64_t pairs, int heads,
+                                                   float scale, uint16_t* out, int64_t out_token) {
   constexpr int N = HD / 64;
   typedef float vec __attribute__((ext_vector_type(N)));
   const LaneX lx = lane_x_init();
@@ -127,6 +127,12 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
   const int64_t pair = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (pair >= pairs) return;
   const float* from = part + pair * splits * part_floats(HD);
+  if (used.lengths) {
+    const int n = used.lengths[pair / heads], len = n > used.most ? (int)used.most : n;
+    const int count = TileList<kTile>(span_of(len - 1, used.window, used.sinks)).count, run = share_tiles(count, splits);
+    const int there = __builtin_amdgcn_readfirstlane((count + run - 1) / run);
+    splits = there < 1 ? 1 : there;
+  }
   float top = -INFINITY, sum = 0.f, o[N] = {};
   for (int s0 = 0; s0 < splits; s0 += 64) {
     const int left = splits - s0 < 64 ? splits - s0 : 64;
@@ -181,6 +187,13 @@ struct Shares {
   bool many;
 };
 
+// A work-group of many waves takes all of a short row in one launch (32 rows
+// of up to 577 positions 12.5 us against 16.3 with shares and their join, one
+// row 8.0 against 9.2); from about 700 positions on its waves' turns take
+// longer than the join (1000: 14.4 against 9.2).  Shares: as many as make 4096
+// work-groups, which even out rows of different lengths (48 rows of up to
+// 16384: 273 us, with 1024 304), of 8 tiles or more (of 16: 12.4 us instead of
+// 10 for one row of 2000).
 Shares token_shares(int64_t rows, int heads, int kv_heads, int64_t cols, int page, int window, int sinks) {
   const int64_t wgs = rows * kv_heads * ((heads / kv_heads + 15) / 16);
   const int64_t tiles = seen_positions(cols * page, window, sinks, 0) / kTile + 2;
@@ -200,25 +213,27 @@ int launch_token(const PagePool& pp, const TokenArgs& a, int64_t rows, bool many
   else if (past_caches) hipLaunchKernelGGL((attend_token_kernel<BF, HD, few_waves(HD), true>), grid, few, 0, stream, pp, a);
   else hipLaunchKernelGGL((attend_token_kernel<BF, HD, few_waves(HD), false>), grid, few, 0, stream, pp, a);
   QS_LAUNCHED("attend_token_kernel");
-  if (a.splits > 1) return join_parts(a.part, a.splits, rows, a.heads, HD, BF, a.scale, a.out, a.out_row, stream);
+  const Used used{pp.lengths, (int64_t)pp.cols << pp.shift, a.window, a.sinks};
+  if (a.splits > 1) return join_parts(a.part, a.splits, &used, rows, a.heads, HD, BF, a.scale, a.out, a.out_row, stream);
   return QS_OK;
 }
 
 }  // namespace
 
-int join_parts(const float* part, int splits, int64_t tokens, int heads, int head_dim, bool bf, float scale,
+int join_parts(const float* part, int splits, const Used* there, int64_t tokens, int heads, int head_dim, bool bf, float scale,
                uint16_t* out, int64_t out_token, hipStream_t stream) {
   const int64_t pairs = tokens * heads;
+  const Used used = there ? *there : Used{nullptr, 0, 0, 0};
   const dim3 grid((unsigned)((pairs + 3) / 4)), block(256);
   if (head_dim == 64) {
-    if (bf) hipLaunchKernelGGL((join_kernel<true, 64>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
-    else hipLaunchKernelGGL((join_kernel<false, 64>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
+    if (bf) hipLaunchKernelGGL((join_kernel<true, 64>), grid, block, 0, stream, part, splits, used, pairs, heads, scale, out, out_token);
+    else hipLaunchKernelGGL((join_kernel<false, 64>), grid, block, 0, stream, part, splits, used, pairs, heads, scale, out, out_token);
   } else if (head_dim == 128) {
-    if (bf) hipLaunchKernelGGL((join_kernel<true, 128>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
-    else hipLaunchKernelGGL((join_kernel<false, 128>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
+    if (bf) hipLaunchKernelGGL((join_kernel<true, 128>), grid, block, 0, stream, part, splits, used, pairs, heads, scale, out, out_token);
+    else hipLaunchKernelGGL((join_kernel<false, 128>), grid, block, 0, stream, part, splits, used, pairs, heads, scale, out, out_token);
   } else {
-    if (bf) hipLaunchKernelGGL((join_kernel<true, 256>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
-    else hipLaunchKernelGGL((join_kernel<false, 256>), grid, block, 0, stream, part, splits, pairs, heads, scale, out, out_token);
+    if (bf) hipLaunchKernelGGL((join_kernel<true, 256>), grid, block, 0, stream, part, splits, used, pairs, heads, scale, out, out_token);
+    else hipLaunchKernelGGL((join_kernel<false, 256>), grid, block, 0, stream, part, splits, used, pairs, heads, scale, out, out_token);
   }
   QS_LAUNCHED("join_kernel");
   return QS_OK;

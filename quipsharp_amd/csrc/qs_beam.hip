@@ -14,7 +14,7 @@ namespace qs {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kJoin = 256;  // threads of the join
+constexpr int kJoin = 256;  // threads of the join (32 requests of 8 beams: 9.0 us, with 1024 13)
 constexpr int kMaxKeep = 128;
 constexpr int kRoom = 2304;  // candidates of a slice (what lies above the edge, or 128 of it and a row of ties)
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));

@@ -168,6 +168,18 @@ def test_chunk_with_more_tokens_than_the_row_holds(dev):
     check(got, q, c, [(0, i - 30) for i in range(50)], 128 ** -0.5, 0, 0)
 
 
+@pytest.mark.parametrize("window,sinks", [(0, 0), (700, 5)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 1, 128), (3, 3, 64), (4, 2, 256)])
+def test_token_in_a_wide_table(dev, heads, kv_heads, dim, window, sinks):
+    """Short and long rows in a table with columns for far longer ones: most shares of a row have nothing to do."""
+    from quipsharp_amd.pages import attend_token
+    lengths = [1, 0, 577, 130, 3000, 33]
+    c = Cache(lengths, kv_heads, dim, 16, torch.bfloat16, 31, cols=2500)
+    q = torch.randn(len(lengths), heads, dim, generator=torch.Generator().manual_seed(dim)).bfloat16().to(dev)
+    got = attend_token(q, *c.to(dev), window=window, sinks=sinks)
+    check(got, q, c, [(r, n - 1) for r, n in enumerate(lengths)], dim ** -0.5, window, sinks)
+
+
 @pytest.mark.parametrize("kind", ["token", "chunk"])
 def test_layouts_and_strides(dev, kind):
     """Heads of a position together in the pool, queries as a slice of a wider projection, output into a view."""
@@ -313,7 +325,7 @@ def test_few_tokens_behind_a_long_cache(dev, rows, heads, kv_heads, dim, page, w
     check(whole, q, c, where, dim ** -0.5, window, sinks)
 
 
-@pytest.mark.parametrize("rows", [70, 200])
+@pytest.mark.parametrize("rows", [64, 65, 70, 200, 4200])
 def test_many_rows_of_several_tokens(dev, rows):
     """More rows than a wave has lanes, of mixed lengths, some without new tokens."""
     from quipsharp_amd.pages import attend_chunk
