@@ -127,6 +127,9 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
   const int64_t pair = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (pair >= pairs) return;
   const float* from = part + pair * splits * part_floats(HD);
+  // the first parts' maxima and sums, before it is known how many there are
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (lane < splits) ml = *reinterpret_cast<const float2*>(from + (int64_t)lane * part_floats(HD));
   if (used.lengths) {
     const int n = used.lengths[pair / heads], len = n > used.most ? (int)used.most : n;
     const int count = TileList<kTile>(span_of(len - 1, used.window, used.sinks)).count, run = share_tiles(count, splits);
@@ -136,11 +139,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
   float top = -INFINITY, sum = 0.f, o[N] = {};
   for (int s0 = 0; s0 < splits; s0 += 64) {
     const int left = splits - s0 < 64 ? splits - s0 : 64;
-    float m = -INFINITY, l = 0.f;
-    if (lane < left) {
-      const float2 ml = *reinterpret_cast<const float2*>(from + (int64_t)(s0 + lane) * part_floats(HD));
-      m = ml.x, l = ml.y;
-    }
+    if (s0 > 0 && lane < left) ml = *reinterpret_cast<const float2*>(from + (int64_t)(s0 + lane) * part_floats(HD));
+    const float m = lane < left ? ml.x : -INFINITY, l = lane < left ? ml.y : 0.f;
     float mx = fmaxf(m, lane_xor<32>(m, lx));
     mx = fmaxf(mx, lane_xor<16>(mx, lx));
     mx = fmaxf(mx, lane_xor<8>(mx, lx));
