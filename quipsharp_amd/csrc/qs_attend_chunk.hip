@@ -126,8 +126,7 @@ __device__ __forceinline__ bool find_block(const ChunkArgs& a, const PagePool& p
     count = end > first ? end - first : 0;
     n = (count * group + kCols - 1) / kCols;
     const int64_t most = (int64_t)pp.cols << pp.shift;
-    const int len = pp.lengths[lane];
-    p0 = (len < 0 ? 0 : len > most ? (int)most : len) - count;
+    p0 = length_of(pp.lengths[lane], most) - count;
   }
   if (a.rows == 1) {
     out = Block{0, __builtin_amdgcn_readfirstlane(n) - 1 - k, __builtin_amdgcn_readfirstlane(first), __builtin_amdgcn_readfirstlane(count)};
@@ -219,9 +218,7 @@ __global__ __launch_bounds__(64 * kWaves * GR, HD == 256 ? 1 : HD == 128 || GR =
   const int split = blockIdx.y;
   const int row = __builtin_amdgcn_readfirstlane(blk.row), count = __builtin_amdgcn_readfirstlane(blk.count), columns = count * group;
   const int b0 = __builtin_amdgcn_readfirstlane(blk.b) * kCols;
-  int len = pp.lengths[row];
-  const int64_t most = (int64_t)pp.cols << pp.shift;
-  len = __builtin_amdgcn_readfirstlane(len > most ? (int)most : len);
+  const int len = __builtin_amdgcn_readfirstlane(length_of(pp.lengths[row], (int64_t)pp.cols << pp.shift));
   const int cw = b0 + 32 * w, c = cw + r32;
   const bool column = c < columns;
   const int t = column ? c / group : count - 1;

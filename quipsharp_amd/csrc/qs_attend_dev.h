@@ -30,6 +30,9 @@ struct PagePool {
   const int32_t* lengths;
 };
 
+// A row's length as its table can hold it.
+__device__ __forceinline__ int length_of(int n, int64_t most) { return n < 0 ? 0 : n > most ? (int)most : n; }
+
 // What a query at position `last` sees: positions low .. last and those below
 // sinks (sinks <= low; zero without a window).
 struct Span {

@@ -42,7 +42,7 @@ __global__ __launch_bounds__(64 * kWavesT) void attend_token_kernel(PagePool pp,
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r16 = lane & 15, qd = lane >> 4;
   const LaneX lx = lane_x_init();
   const int64_t most = (int64_t)pp.cols << pp.shift;
-  const int len = __builtin_amdgcn_readfirstlane(pp.lengths[row] > most ? (int)most : pp.lengths[row]);
+  const int len = __builtin_amdgcn_readfirstlane(length_of(pp.lengths[row], most));
   const Span s = span_of(len - 1, a.window, a.sinks);
   const TileList<kTile> tiles(s);
   const int run = share_tiles(tiles.count, a.splits);
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
   float2 ml = make_float2(-INFINITY, 0.f);
   if (lane < splits) ml = *reinterpret_cast<const float2*>(from + (int64_t)lane * part_floats(HD));
   if (used.lengths) {
-    const int n = used.lengths[pair / heads], len = n > used.most ? (int)used.most : n;
+    const int len = length_of(used.lengths[pair / heads], used.most);
     const int count = TileList<kTile>(span_of(len - 1, used.window, used.sinks)).count, run = share_tiles(count, splits);
     const int there = __builtin_amdgcn_readfirstlane((count + run - 1) / run);
     splits = there < 1 ? 1 : there;

@@ -410,3 +410,20 @@ def test_same_call_gives_the_same_bits(dev):
     for _ in range(5):
         assert torch.equal(first[0], attend_token(q[:3], k, v, table, n))
         assert torch.equal(first[1], attend_chunk(q, k, v, table, n, starts))
+
+
+@pytest.mark.parametrize("cols", [4, 200])
+def test_lengths_below_zero(dev, cols):
+    """A row whose length is below zero, down to the type's lowest, sees nothing."""
+    from quipsharp_amd import pages
+    cache = Cache([40, 40, 40], 2, 64, 16, torch.bfloat16, 29, cols=cols)
+    k, v, table, _ = cache.to(dev)
+    lengths = torch.tensor([-1, -2 ** 31, 40], dtype=torch.int32, device=dev)
+    q = torch.randn(3, 4, 64, generator=torch.Generator().manual_seed(30)).to(torch.bfloat16)
+    where = [(0, -1), (1, -1), (2, 39)]
+    for window, sinks in [(0, 0), (20, 3)]:
+        got = pages.attend_token(q.to(dev), k, v, table, lengths, window=window, sinks=sinks)
+        check(got, q, cache, where, 64 ** -0.5, window, sinks)
+        starts = torch.arange(4, dtype=torch.int32, device=dev)
+        got = pages.attend_chunk(q.to(dev), k, v, table, lengths, starts, window=window, sinks=sinks)
+        check(got, q, cache, where, 64 ** -0.5, window, sinks)
