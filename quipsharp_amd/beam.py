@@ -2,6 +2,7 @@
 beams and vocabulary, and the states that follow them.  No counterpart in the
 reference.  The computation runs in libquipsharp_hip.so (csrc/qs_beam.hip)."""
 import ctypes
+import math
 
 import torch
 from torch import Tensor
@@ -85,7 +86,7 @@ def reorder_states(states, parents: Tensor):
         if not s.is_contiguous() and rows and not s[0].is_contiguous():
             raise ValueError("the elements of a state's row must lie together")
         each = s.element_size()
-        size.append(s.numel() // rows * each if rows else 0)
+        size.append((s.numel() // rows if rows else math.prod(shape[1:])) * each)
         stride.append(s.stride()[0] * each if rows > 1 else size[-1])
     _lib.require_gpu(*states, what="reorder_states")
     for s in states:

@@ -470,7 +470,7 @@ extern "C" int qs_reorder_states(int count, const void* const* src, void* const*
   ReorderArgs a{};
   int64_t most = 0;
   for (int s = 0; s < count; ++s) {
-    QS_REQUIRE(row_bytes[s] >= 0 && src_stride[s] >= row_bytes[s] && ((src[s] && dst[s]) || row_bytes[s] == 0),
+    QS_REQUIRE(row_bytes[s] >= 0 && src_stride[s] >= row_bytes[s] && (((src[s] || rows_in == 0) && dst[s]) || row_bytes[s] == 0),
                "qs_reorder_states: state %d: rows of %lld bytes, %lld apart", s, (long long)row_bytes[s], (long long)src_stride[s]);
     const uintptr_t bits = reinterpret_cast<uintptr_t>(src[s]) | reinterpret_cast<uintptr_t>(dst[s]) | (uintptr_t)row_bytes[s] | (uintptr_t)src_stride[s];
     a.src[s] = static_cast<const char*>(src[s]), a.dst[s] = static_cast<char*>(dst[s]);

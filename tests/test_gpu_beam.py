@@ -148,6 +148,14 @@ def test_reorder_states(dev):
         assert o.shape == want.shape and torch.equal(o.cpu(), want)
 
 
+def test_states_without_rows(dev):
+    """No parent names a row of an empty state."""
+    from quipsharp_amd.beam import reorder_states
+    torch.full((3, 9), 7.0, device=dev)  # what the output's place may hold
+    got, = reorder_states([torch.zeros(0, 9, device=dev)], torch.tensor([0, -1, 2], dtype=torch.int32, device=dev))
+    assert got.tolist() == [[0.0] * 9] * 3
+
+
 def test_captured_select(dev):
     """A captured selection with its states: every replay equals the eager call."""
     from quipsharp_amd.beam import beam_select, reorder_states
