@@ -658,7 +658,8 @@ extern "C" int qs_attend_chunk_ws(const void* q, int dtype, int64_t tokens, int6
                                   int head_dim, int64_t q_token, int64_t q_head, const int32_t* starts,
                                   const qs_page_pool* pool, float scale, int window, int sinks, void* out,
                                   int64_t out_token, void* workspace, size_t workspace_bytes, qs_stream_t stream) {
-  if (tokens == 0 || rows == 0) return QS_OK;
+  if (tokens == 0) return QS_OK;
+  QS_REQUIRE(rows != 0, "qs_attend_chunk: %lld tokens of no row", (long long)tokens);
   PagePool pp;
   if (const int rc = page_pool_checks("qs_attend_chunk", pool, dtype, rows, heads, kv_heads, head_dim, scale, window, sinks, pp)) return rc;
   QS_REQUIRE(q && out && starts, "qs_attend_chunk: null pointer");

@@ -152,7 +152,8 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   __shared__ int32_t len[kMaxRows], from[kMaxRows], need[kMaxRows + 1], mine[kMaxRows];
   __shared__ uint8_t shared_page[kMaxRows];
   __shared__ int part[kThreads / 64];
-  __shared__ int copies, lost;
+  __shared__ int copies;
+  __shared__ unsigned long long lost;  // pages in columns that the table does not have
   const int tid = threadIdx.x;
   const int64_t room = (int64_t)a.cols * a.page;
   auto sync = [&]() {
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
     copy = shared_page[tid];
     first = c0 + (used > 0);
     int64_t last = tokens > 0 ? ((int64_t)old_len + tokens - 1) / a.page : -1;
-    if (last >= a.cols) atomicAdd(&lost, (int)(last - a.cols + 1)), last = a.cols - 1;
+    if (last >= a.cols) atomicAdd(&lost, (unsigned long long)(last - a.cols + 1)), last = a.cols - 1;
     wants = copy + (last >= first ? (int)(last - first + 1) : 0);
     const int64_t end = (int64_t)old_len + tokens;
     a.lengths_out[tid] = (int)(end < room ? end : room);
@@ -285,7 +286,8 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   }
   if (tid == 0) {
     a.plan[0] = copies;
-    a.short_pages[0] = lost + (total > found ? total - found : 0);
+    const unsigned long long missing = lost + (total > found ? total - found : 0);
+    a.short_pages[0] = missing < INT32_MAX ? (int)missing : INT32_MAX;
   }
 }
 
@@ -613,7 +615,8 @@ extern "C" int qs_page_advance_rows(const qs_page_store* store, const int32_t* t
   Store st;
   if (const int rc = store_checks("qs_page_advance", store, st)) return rc;
   if (const int rc = table_checks("qs_page_advance", rows, cols, st.pages, st.page)) return rc;
-  QS_SUPPORTED(rows <= kMaxRows, "qs_page_advance: %lld rows (at most %d)", (long long)rows, kMaxRows);
+  QS_SUPPORTED(rows <= kMaxRows && rows * cols <= INT32_MAX, "qs_page_advance: %lld rows of %lld columns (at most %d, 2^31 entries)",
+               (long long)rows, (long long)cols, kMaxRows);
   QS_REQUIRE(table && lengths && refs && table_out && lengths_out && refs_out && short_pages, "qs_page_advance: null pointer");
   QS_REQUIRE(tokens >= 0 && tokens <= (1 << 30), "qs_page_advance: %d tokens", tokens);
   QS_REQUIRE(workspace && workspace_bytes >= qs_page_advance_workspace_bytes(rows) && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,

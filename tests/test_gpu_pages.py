@@ -359,3 +359,13 @@ def test_captured_steps(dev):
         assert torch.equal(got, want), i
         assert torch.equal(a.table, b.table) and torch.equal(a.lengths, b.lengths) and torch.equal(a.refs, b.refs)
         assert torch.equal(a.kv, b.kv) and a.short.item() == 0
+
+
+@pytest.mark.parametrize("rows", [8, 64])
+def test_far_more_tokens_than_columns(dev, rows):
+    """The pages that are missing are counted up to the largest int32."""
+    cache, _ = filled(rows, 2, 4, 16, dev, layers=1, heads=1)
+    cache.advance(1 << 30)
+    assert cache.short.item() == min(rows * 2 ** 26 - 4, 2 ** 31 - 1)
+    assert cache.lengths.tolist() == [32] * rows
+    assert cache.table.view(-1).tolist() == [0, 1, 2, 3] + [-1] * (2 * rows - 4)

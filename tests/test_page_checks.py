@@ -230,3 +230,13 @@ def test_empty_calls_do_nothing():
 def test_pages_too_far_apart(over):
     L = _lib.lib()
     assert token(L, **over) == 3 and b"elements apart" in L.qs_last_error()
+
+
+def test_tables_and_tokens_out_of_range():
+    L = _lib.lib()
+    store = _lib.PageStore(64, 4, 16, 2, 16, 128)
+    cols = 1 << 21
+    assert L.qs_page_advance(store, P, P, P, None, 1024, cols, 1, P, P, P, P, P, 1 << 20, None) == 3
+    assert b"2097152 columns" in L.qs_last_error()
+    assert L.qs_attend_chunk(P, 2, 4, 0, 8, 2, 128, 1024, 128, P, pool(), 0.1, 0, 0, P, 1024, None) == 1
+    assert b"4 tokens of no row" in L.qs_last_error()
