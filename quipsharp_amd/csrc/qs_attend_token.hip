@@ -120,14 +120,22 @@ __device__ __forceinline__ float vec_at(const V& x, int i) {
 template <bool BF, int HD>
 __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits, Used used, int64_t pairs, int heads,
                                                    float scale, uint16_t* out, int64_t out_token) {
-  constexpr int N = HD / 64;
+  constexpr int N = HD / 64, kAhead = 8;
   typedef float vec __attribute__((ext_vector_type(N)));
   const LaneX lx = lane_x_init();
   const int lane = threadIdx.x & 63;
   const int64_t pair = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (pair >= pairs) return;
   const float* from = part + pair * splits * part_floats(HD);
-  // the first parts' maxima and sums, before it is known how many there are
+  // kAhead parts' values at a time, whose loads do not wait for each other
+  auto bring = [&](vec (&x)[kAhead], int s) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      x[j] = *reinterpret_cast<const vec*>(from + (int64_t)(s + j < splits ? s + j : splits - 1) * part_floats(HD) + kPartHead + N * lane);
+  };
+  // the first parts, before it is known how many there are
+  vec x[kAhead];
+  bring(x, 0);
   float2 ml = make_float2(-INFINITY, 0.f);
   if (lane < splits) ml = *reinterpret_cast<const float2*>(from + (int64_t)lane * part_floats(HD));
   if (used.lengths) {
@@ -154,21 +162,18 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
     sum = sum * back + wave_sum(f * l, lx);
 #pragma unroll
     for (int i = 0; i < N; ++i) o[i] *= back;
-    // four parts at a time, whose loads do not wait for each other
-    for (int s = 0; s < left; s += 4) {
-      vec x[4];
+    for (int s = 0; s < left; s += kAhead) {
+      vec next[kAhead] = {};
+      if (s0 + s + kAhead < splits) bring(next, s0 + s + kAhead);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int at = s + j < left ? s + j : left - 1;
-        x[j] = *reinterpret_cast<const vec*>(from + (int64_t)(s0 + at) * part_floats(HD) + kPartHead + N * lane);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < kAhead; ++j) {
         const float fj = s + j < left ? __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), s + j)) : 0.f;
         // a part without weight may hold no number where its values do
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] = fj == 0.f ? o[i] : o[i] + fj * vec_at<N>(x[j], i);
       }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) x[j] = next[j];
     }
   }
   const float r = sum == 0.f ? 0.f : 1.f / sum;
