@@ -189,3 +189,19 @@ def test_captured_select(dev):
         if i % 2:
             torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, step())), i
+
+
+@pytest.mark.parametrize("keep", [5, 64, 100, 128])
+@pytest.mark.parametrize("kind", ["spread", "equal", "one ahead", "close"])
+def test_many_beams(dev, kind, keep):
+    """Hundreds of beams, whose slices' bests are far more than the join ranks at once.  Sums of different beams lie
+    2^-15 apart at least, those of "close" agree in the upper half of an fp64."""
+    K, V = 300, 9000
+    g = torch.Generator().manual_seed(keep)
+    x = torch.randint(0, 200, (V,), generator=g).float() / 64
+    beam = torch.arange(K).float()
+    scores = {"spread": -torch.randint(0, 500, (K,), generator=g).float() / 64 - beam / 2 ** 15, "equal": torch.zeros(K),
+              "one ahead": torch.where(beam == 123, 50.0, -beam / 2 ** 15), "close": -1024.0 - beam / 2 ** 13}[kind]
+    if kind in ("equal", "close"):
+        x = torch.zeros(V)
+    check(dev, x.repeat(K, 1), scores.view(1, K), keep)
