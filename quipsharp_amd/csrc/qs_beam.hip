@@ -110,12 +110,14 @@ struct Slice {
 
 // One work-group per slice of 256 E logits, which stay in registers.
 //
-// A logit is among the slice's best only if it is not below the edge: the
-// keep-th largest of the threads' largest, or (up to 32) the largest of the
-// waves' keep-th largest, which takes no exchange.  Above the edge lie at
-// most (keep - 1) E logits by the first rule and four times as many by the
-// second, which slice_size keeps below kRoom, and few in most cases; those at
-// the edge may be any number, and the lowest tokens of them are taken.
+// A logit is among the slice's best only if it is not below the edge, the
+// keep-th largest of the threads' largest, or something lower that is found
+// without an exchange: up to 32, the largest of the waves' keep-th largest
+// and, from 9 on, the least of their keep / 4-th (256 rows of 151936 bf16,
+// keep 32: 47.5 us with both instead of 59).  Few logits lie above it in most
+// cases; where they and those at it are more than kRoom, the edge is taken from
+// the threads, above which lie (keep - 1) E at most, which slice_size keeps
+// below kRoom, and of those at it the lowest tokens are taken.
 //
 // Bound by the logits' way from memory: 26 us for 155 MB (256 rows of 151936
 // fp32).
@@ -124,7 +126,7 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
   typedef Slice<T, WIDE, E> S;
   __shared__ uint64_t room[kRoom];
   __shared__ float tops[kThreads];
-  __shared__ float red[3][4];
+  __shared__ float red[4][4];
   __shared__ float line;
   __shared__ int count;
   const LaneX lx = lane_x_init();
@@ -145,19 +147,22 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
   top = fmaxf(top, lane_xor<2>(top, lx));
   top = fmaxf(top, lane_xor<1>(top, lx));
   const float edge_w = keep <= 32 ? order_float(nth_key(order_bits(m), keep)) : -INFINITY;
-  if (keep > 32) tops[tid] = m;
-  if (lane == 0) red[0][w] = top, red[1][w] = edge_w;
+  const float part_w = keep <= 32 && keep > 8 ? order_float(nth_key(order_bits(m), (keep + 3) / 4)) : -INFINITY;
+  tops[tid] = m;
+  if (lane == 0) red[0][w] = top, red[1][w] = edge_w, red[3][w] = part_w;
   if (tid == 0) count = 0;
   __syncthreads();
   const float all = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   float edge = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
-  if (keep > 32) {
+  edge = fmaxf(edge, fminf(fminf(red[3][0], red[3][1]), fminf(red[3][2], red[3][3])));
+  auto threads_edge = [&]() {
     int above = 0, same = 0;
     for (int i = 0; i < kThreads; ++i) above += tops[i] > m, same += tops[i] == m;
     if (above < keep && keep <= above + same) line = m;  // all that write it write the same
     __syncthreads();
-    edge = line;
-  }
+    return line;
+  };
+  if (keep > 32) edge = threads_edge();
   float sum = 0.f;
   if (all < INFINITY) {
 #pragma unroll
@@ -183,6 +188,7 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
   int n = count;
   if (n > kRoom) {
     // too many at the edge: those above it, then the others by rising tokens until there are enough
+    if (keep <= 32) edge = threads_edge();
     __syncthreads();
     if (tid == 0) count = 0;
     __syncthreads();
@@ -438,8 +444,7 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidat
 // 42 us), 16 otherwise and where what lies above the edge would not fit
 // (beam_slice_kernel).
 int slice_size(int64_t rows, int64_t vocab, int keep) {
-  const bool fits = keep <= 16 || (keep > 32 && keep <= 64);
-  return fits && rows * ((vocab + 32 * kThreads - 1) / (32 * kThreads)) >= 512 ? 32 : 16;
+  return keep <= 64 && rows * ((vocab + 32 * kThreads - 1) / (32 * kThreads)) >= 512 ? 32 : 16;
 }
 
 struct Layout {

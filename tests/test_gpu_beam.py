@@ -205,3 +205,19 @@ def test_many_beams(dev, kind, keep):
     if kind in ("equal", "close"):
         x = torch.zeros(V)
     check(dev, x.repeat(K, 1), scores.view(1, K), keep)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("keep", [9, 17, 32])
+@pytest.mark.parametrize("kind", ["lanes", "steps", "equal"])
+def test_far_more_above_the_edge_than_room(dev, kind, keep, dtype):
+    """"lanes": three of a slice's four waves have large logits, each in fewer threads than are kept, so that all of
+    them lie above what the waves agree on."""
+    V, rows = 34000, 300
+    t, wide = torch.arange(V), 128 // torch.finfo(dtype).bits
+    thread = t // wide % 256
+    x = {"lanes": torch.where((thread < 192) & (thread % 64 < keep - 1), 1.0 + t % 7, (t % 5) / 8.0),
+         "steps": (t // 5000 % 2).float(), "equal": torch.zeros(V)}[kind]
+    logits = x.repeat(rows, 1)
+    logits[1::2, 100] = 9.5
+    check(dev, logits.to(dtype), -(torch.arange(rows) % 5).float().view(100, 3), keep)
