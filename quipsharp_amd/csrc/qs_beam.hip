@@ -250,7 +250,11 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidat
   // 1530 us, turned 66).
   auto place = [&](int k) { return k * kJoin + ((tid + 37 * k) & (kJoin - 1)); };
   const int some = a.slices * a.keep, per = some > a.keep + 1 ? some : a.keep + 1, all = a.beams * per;
-  const bool lists = a.beams * a.slices >= kJoin;
+  // More candidates than the threads have at hand at first, and lists enough for
+  // a close edge: by lists (the request above 22 us, 300 beams of 20000 tokens,
+  // keep 128, 91 instead of 540, 32 x 8 beams, keep 8, 35.4 instead of 37.8;
+  // 4 beams of 151936, keep 4, of 592 candidates, 11.0 by lists, 10.7 without).
+  const bool lists = all > kAhead * kJoin && a.beams * a.slices >= 64 && a.beams * a.slices >= 2 * a.keep;
   // a thread's first candidates are on their way while the sums are made
   uint64_t ahead[kAhead];
 #pragma unroll
@@ -324,9 +328,8 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidat
         if (place(i + x) < all) use(get(place(i + x) / per, place(i + x) % per, k[x]));
     }
   };
-  // Where there is a list (of a slice) for every thread, only the lists' first
-  // entries are looked at for the edge, and of each list what is not below it
-  // (the request above 22 us, 300 beams of 20000 tokens, keep 128, 91 instead of 540).
+  // `lists`: only the first entry of each slice's list is looked at for the
+  // edge, and of each list what is not below it.
   auto list_of = [&](int u, auto use) {
     const int j = u / a.slices, s = u - j * a.slices;
     use(j, s * a.keep, a.best + ((b * a.beams + j) * a.slices + s) * a.keep);
@@ -379,7 +382,9 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidat
   };
   if (lists) firsts(highest);
   else each(highest);
-  if (a.keep <= 64) {
+  // Of a wave's threads, or of all (one request of 40 beams, keep 64: 66 us and
+  // 32; 8 of 10 beams, keep 40: 28.5 and 31.6).
+  if (a.keep <= 48) {
     const uint32_t u = nth_key(top, a.keep);
     if (lane == 0) atomicMax(&edge, u);
   } else {
