@@ -14,7 +14,7 @@ namespace qs {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kJoin = 256;  // threads of the join (32 requests of 8 beams: 9.0 us, with 1024 13)
+constexpr int kJoin = 256;  // threads of the join (selection of 32 requests of 8 beams: 35.4 us, with 512 38, with 1024 41)
 constexpr int kMaxKeep = 128;
 constexpr int kRoom = 2304;  // candidates of a slice (what lies above the edge, or 128 of it and a row of ties)
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -114,10 +114,11 @@ struct Slice {
 // keep-th largest of the threads' largest, or something lower that is found
 // without an exchange: up to 32, the largest of the waves' keep-th largest
 // and, from 9 on, the least of their keep / 4-th (256 rows of 151936 bf16,
-// keep 32: 47.5 us with both instead of 59).  Few logits lie above it in most
-// cases; where they and those at it are more than kRoom, the edge is taken from
-// the threads, above which lie (keep - 1) E at most, which slice_size keeps
-// below kRoom, and of those at it the lowest tokens are taken.
+// keep 32: 59 us for the selection with both instead of 70, 48 with longer
+// slices).  Few logits lie above it in most cases; where they and those at it
+// are more than kRoom, the edge is taken from the threads, above which lie
+// (keep - 1) E at most, which slice_size keeps below kRoom, and of those at it
+// the lowest tokens are taken.
 //
 // Bound by the logits' way from memory: 26 us for 155 MB (256 rows of 151936
 // fp32).
@@ -445,9 +446,9 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidat
 }
 
 // Logits per thread: 32 where that leaves work-groups enough to fill the chip
-// (256 rows of 151936: 40 us for the whole selection, with 16 48 us, with 64
-// 42 us), 16 otherwise and where what lies above the edge would not fit
-// (beam_slice_kernel).
+// (256 rows of 151936 fp32, keep 8: 35.4 us for the whole selection, with 16 42;
+// bf16, keep 32: 48 and 59), 16 otherwise and where what lies above the edge
+// would not fit (beam_slice_kernel).
 int slice_size(int64_t rows, int64_t vocab, int keep) {
   return keep <= 64 && rows * ((vocab + 32 * kThreads - 1) / (32 * kThreads)) >= 512 ? 32 : 16;
 }
