@@ -40,6 +40,21 @@ __device__ __forceinline__ void ref_store(int32_t* p, int v) {
   __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
+// The counts of all pages, for a kernel's own work on them: loads of eight
+// pages of a thread are on their way together (the stores, which may be to the
+// same place, would have each wait for the one before).
+__device__ __forceinline__ void ref_copy(const int32_t* from, int32_t* to, int pages) {
+  constexpr int kN = 8;
+  for (int p0 = threadIdx.x; p0 < pages; p0 += kN * blockDim.x) {
+    int n[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) n[i] = p0 + i * (int)blockDim.x < pages ? from[p0 + i * blockDim.x] : 0;
+#pragma unroll
+    for (int i = 0; i < kN; ++i)
+      if (p0 + i * (int)blockDim.x < pages) ref_store(to + p0 + i * blockDim.x, n[i]);
+  }
+}
+
 // Every global access of the work-group before the barrier is done when a
 // thread goes on after it (loads and atomics of another wave see it in the L2).
 __device__ __forceinline__ void group_sync() {
@@ -173,7 +188,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   if (NEAR)
     for (int p = tid; p < a.pages; p += kThreads) near_refs[p] = a.refs[p];
   else if (a.refs_out != a.refs)
-    for (int p = tid; p < a.pages; p += kThreads) ref_store(a.refs_out + p, a.refs[p]);
+    ref_copy(a.refs, a.refs_out, a.pages);
   int old_len = 0, tokens = a.tokens;
   if (tid < a.rows) {
     if (a.row_tokens) {
@@ -220,11 +235,15 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
     mine[tid] = p >= 0 && ref_at(p) > 1 ? p : -1;
   }
   __syncthreads();
-  for (int e = tid; e < a.rows * a.rows; e += kThreads) {
-    const int i = e / a.rows, j = e % a.rows;
-    if (mine[i] < 0 || i == j) continue;
-    if (len[j] > len[i] || (len[j] == len[i] && j < i))
-      if (entry((int64_t)j * a.cols + len[i] / a.page) == mine[i]) shared_page[i] = 1;
+  // a wave for a row, against all others (1024 rows and no new page: 54 us; with
+  // a thread for every pair 212)
+  for (int i = tid >> 6; i < a.rows; i += kThreads / 64) {
+    const int p = mine[i], n = len[i];
+    if (p < 0) continue;
+    const int c = n / a.page;
+    for (int j = tid & 63; j < a.rows; j += 64)
+      if (len[j] > n || (len[j] == n && j < i))
+        if (entry((int64_t)j * a.cols + c) == p) shared_page[i] = 1;
   }
   __syncthreads();
   // pages that a row needs: a copy's, then those of columns first .. last
@@ -247,13 +266,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   // free pages in ascending order; the page of rank k goes to the row whose
   // share of the ranks holds k
   int found = 0;
-  for (int p0 = 0; p0 < a.pages && found < total; p0 += kThreads) {
-    const int p = p0 + tid;
-    const bool is_free = p < a.pages && ref_at(p) <= 0;
-    int n;
-    const int k = found + scan1024(is_free, part, &n);
-    found += n;
-    if (!is_free || k >= total) continue;
+  auto give = [&](int p, int k) {
     int lo = 0, hi = a.rows;  // need[lo] <= k < need[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) / 2;
@@ -273,6 +286,22 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
     set_entry((int64_t)lo * a.cols + col, p);
     if (NEAR) near_refs[p] = 1;
     else ref_store(a.refs_out + p, 1);
+  };
+  constexpr int kEach = NEAR ? 1 : 4;  // pages of a thread at a time, next to each other (70000 to look through: 33 us, one by one 65)
+  for (int p0 = 0; p0 < a.pages && found < total; p0 += kEach * kThreads) {
+    const int p = p0 + kEach * tid;
+    bool is_free[kEach];
+    int mine_free = 0, n;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) mine_free += is_free[i] = p + i < a.pages && ref_at(p + i) <= 0;
+    int k = found + scan1024(mine_free, part, &n);
+    found += n;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+      if (is_free[i]) {
+        if (k < total) give(p + i, k);
+        ++k;
+      }
   }
   // a copy that got no page: the row loses its hold
   if (tid < a.rows && copy && mark >= found) {
@@ -310,8 +339,7 @@ __global__ __launch_bounds__(kThreads) void page_free_kernel(FreeArgs a) {
     for (int p = tid; p < a.pages; p += kThreads) near_refs[p] = a.refs[p];
     __syncthreads();
   } else {
-    if (a.refs_out != a.refs)
-      for (int p = tid; p < a.pages; p += kThreads) ref_store(a.refs_out + p, a.refs[p]);
+    if (a.refs_out != a.refs) ref_copy(a.refs, a.refs_out, a.pages);
     group_sync();
   }
   const int64_t all = (int64_t)a.rows * a.cols;
@@ -413,8 +441,7 @@ __global__ __launch_bounds__(kThreads) void page_compact_kernel(CompactArgs a) {
     free_before += n & 0xFFFF, high_before += n >> 16;
   }
   group_sync();
-  if (a.refs_out != a.refs)
-    for (int p = tid; p < a.pages; p += kThreads) a.refs_out[p] = a.refs[p];
+  if (a.refs_out != a.refs) ref_copy(a.refs, a.refs_out, a.pages);
   group_sync();
   for (int k = tid; k < high_before; k += kThreads) {
     const int s = copies[k].src, d = copies[k].dst;
