@@ -463,7 +463,7 @@ typedef struct qs_page_store {
   int64_t row_bytes;
 } qs_page_store;
 
-/* A step of every row (at most 1024): row i takes the pages and the length of
+/* A step of every row (at most 1024, and 2^31 table entries): row i takes the pages and the length of
  * row parents[i] (its own where parents is NULL; none where parents[i] names
  * no row), gives back pages beyond that length, and gets room for `tokens`
  * more, by which its length grows.  The partly filled page that is written
@@ -471,7 +471,8 @@ typedef struct qs_page_store {
  * it, for each of them but the longest, or the first of the longest.  New
  * pages are the free ones in ascending order, given out by row, then by
  * column.  short_pages[0] gets the number of pages that were asked for and
- * could not be given (none free, or the table full): those entries are -1.
+ * could not be given (none free, or the table full), at most 2^31 - 1: those
+ * entries are -1.
  * Outputs may be the inputs.  workspace: qs_page_advance_workspace_bytes. */
 size_t qs_page_advance_workspace_bytes(int64_t rows);
 int qs_page_advance(const qs_page_store *store, const int32_t *table, const int32_t *lengths, const int32_t *refs,

@@ -242,9 +242,9 @@ def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, toke
     hold it, for each of them but the longest (the first of the longest); full
     pages stay shared.  New pages are the free ones in ascending order, given
     out by row, then by column.  Returns ``(table, lengths, refs, short)``;
-    ``short`` (int32, 1) is the number of pages that were wanted and could not
-    be given, because none is free or the table has no column left: their
-    entries are -1."""
+    ``short`` (int32, 1; at most 2^31 - 1) is the number of pages that were
+    wanted and could not be given, because none is free or the table has no
+    column left: their entries are -1."""
     store, dev = _store(kv), kv.device
     _books(table, lengths, refs, store.pages, dev)
     rows, cols = table.shape
