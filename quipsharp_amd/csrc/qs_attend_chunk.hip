@@ -564,16 +564,26 @@ int64_t chunk_blocks(int64_t tokens, int64_t rows, int heads, int kv_heads) {
   return (tokens * (heads / kv_heads) + kCols - 1) / kCols + rows;
 }
 
+// The blocks that there are if the rows' tokens fill theirs and every row has some.
+int64_t likely_blocks(int64_t tokens, int64_t rows, int heads, int kv_heads) {
+  const int64_t full = (tokens * (heads / kv_heads) + kCols - 1) / kCols, some = rows < tokens ? rows : tokens;
+  return full > some ? full : some;
+}
+
 // Into how many shares the tiles of a block are cut.  A share is a work-group;
 // a CU has room for two, so cutting pays where the blocks' heads are fewer
 // than half the chip's CUs, and shares of less than 8 tiles do not repay the
 // second launch and the parts that it joins (16 tokens of 8 kv heads behind
 // 6000 positions: 136 us whole, 26 us in shares; a prompt of 512 with 64 heads:
-// 21 us whole, 36 us in two).
+// 21 us whole, 36 us in two).  Blocks that are not full leave few parts to
+// join, so that twice the shares pay (16 rows of up to 8 tokens behind up to
+// 4000 positions: 38.5 us instead of 45; full ones, 100 tokens behind 6000
+// positions: 59 us instead of 41).
 int chunk_splits(int64_t tokens, int64_t rows, int heads, int kv_heads, int64_t cols, int page, int window, int sinks) {
-  const int64_t blocks = (tokens * (heads / kv_heads) + kCols - 1) / kCols, wgs = blocks * kv_heads;
+  const int64_t blocks = likely_blocks(tokens, rows, heads, kv_heads), wgs = blocks * kv_heads;
+  const int64_t slots = tokens * (heads / kv_heads) * 4 <= blocks * kCols * 3 ? 512 : 256;
   const int64_t seen = seen_positions(cols * page, window, sinks, (tokens - 1 < kCols ? tokens - 1 : kCols));
-  const int64_t most = seen / 512, n = 256 / wgs;
+  const int64_t most = seen / 512, n = slots / wgs;
   return (int)(n < 2 || most < 2 ? 1 : n < most ? n : most);
 }
 
@@ -585,10 +595,10 @@ int launch_chunk(const PagePool& pp, const ChunkArgs& a, hipStream_t stream) {
     // One work-group for a CU at most, with tiles for both halves: eight waves
     // (a prompt of 512 with 64 heads: 19.2 us against 20.7, 300 tokens behind
     // 6000 positions 105 against 146; with one or two tiles the second half
-    // only costs, 10.9 against 9.1 us for a prompt of 64).  The blocks counted
-    // are those that there are if the rows' tokens fill theirs.
+    // only costs, 10.9 against 9.1 us for a prompt of 64; 64 rows of up to 2
+    // tokens behind up to 1000 positions, 8 kv heads: 34 us, with eight waves 59).
     const int64_t seen = seen_positions((int64_t)pp.cols << pp.shift, a.window, a.sinks, a.tokens - 1 < kCols ? a.tokens - 1 : kCols);
-    if ((blocks - a.rows) * a.kv_heads * a.splits <= 256 && seen / a.splits >= 256) {
+    if (likely_blocks(a.tokens, a.rows, a.heads, a.kv_heads) * a.kv_heads * a.splits <= 256 && seen / a.splits >= 256) {
       hipLaunchKernelGGL((attend_chunk_kernel<BF, HD, 2>), grid, dim3(128 * kWaves), 0, stream, pp, a);
       QS_LAUNCHED("attend_chunk_kernel");
       if (a.splits > 1) return join_parts(a.part, a.splits, nullptr, a.tokens, a.heads, HD, BF, a.scale, a.out, a.out_token, stream);

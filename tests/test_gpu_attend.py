@@ -427,3 +427,18 @@ def test_lengths_below_zero(dev, cols):
         starts = torch.arange(4, dtype=torch.int32, device=dev)
         got = pages.attend_chunk(q.to(dev), k, v, table, lengths, starts, window=window, sinks=sinks)
         check(got, q, cache, where, 64 ** -0.5, window, sinks)
+
+
+@pytest.mark.parametrize("rows,new,cached,heads,kv_heads,dim", [(16, 3, 2500, 8, 2, 128), (40, 2, 300, 16, 8, 64),
+                                                              (5, 20, 1100, 7, 1, 256)])
+def test_rows_of_few_tokens(dev, rows, new, cached, heads, kv_heads, dim):
+    """Blocks that are mostly empty, with and without shares of the positions; some rows have no token."""
+    from quipsharp_amd.pages import attend_chunk
+    g = torch.Generator().manual_seed(rows)
+    news = torch.randint(0, new + 1, (rows,), generator=g).tolist()
+    lengths = [n + m for n, m in zip(news, torch.randint(0, cached, (rows,), generator=g).tolist())]
+    c = Cache(lengths, kv_heads, dim, 16, torch.bfloat16, rows + 1)
+    starts = torch.tensor([0] + news).cumsum(0).to(torch.int32)
+    q = torch.randn(sum(news), heads, dim, generator=g).bfloat16()
+    got = attend_chunk(q.to(dev), *c.to(dev), starts.to(dev))
+    check(got, q, c, [(r, lengths[r] - news[r] + i) for r in range(rows) for i in range(news[r])], dim ** -0.5, 0, 0)
