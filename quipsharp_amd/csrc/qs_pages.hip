@@ -13,6 +13,9 @@ namespace {
 
 constexpr int kMaxRows = 1024;
 constexpr int kThreads = 1024;
+// Loops over pages and copies count in int: a step beyond the last stays below 2^31.
+constexpr int kPageStep = 8 * kThreads;  // the longest step (ref_copy)
+constexpr int kCopyStep = 64;            // work-groups that deal copies
 
 struct Store {
   char* data;
@@ -44,7 +47,7 @@ __device__ __forceinline__ void ref_store(int32_t* p, int v) {
 // pages of a thread are on their way together (the stores, which may be to the
 // same place, would have each wait for the one before).
 __device__ __forceinline__ void ref_copy(const int32_t* from, int32_t* to, int pages) {
-  constexpr int kN = 8;
+  constexpr int kN = kPageStep / kThreads;
   for (int p0 = threadIdx.x; p0 < pages; p0 += kN * blockDim.x) {
     int n[kN];
 #pragma unroll
@@ -140,7 +143,7 @@ __global__ __launch_bounds__(256) void page_list_kernel(Store st, const int32_t*
 // Work-groups for up to `count` copies: 4096 in all, each with a few pieces.
 dim3 copy_grid(const Store& st, int64_t count) {
   const int64_t pieces = (st.page * st.row_bytes + kPiece - 1) / kPiece, per = st.planes * st.kv_heads * pieces;
-  int64_t x = count < 64 ? count : 64;
+  int64_t x = count < kCopyStep ? count : kCopyStep;
   int64_t y = 4096 / x;
   y = y < per ? y : per;
   return dim3((unsigned)x, (unsigned)y);
@@ -552,7 +555,7 @@ int store_checks(const char* fn, const qs_page_store* s, Store& out) {
 }
 
 int table_checks(const char* fn, int64_t rows, int64_t cols, int64_t pages, int page) {
-  QS_REQUIRE(rows >= 1 && cols >= 1 && cols <= (1 << 24) && pages >= 1 && pages <= INT32_MAX - kThreads && page >= 1 &&
+  QS_REQUIRE(rows >= 1 && cols >= 1 && cols <= (1 << 24) && pages >= 1 && pages <= INT32_MAX - kPageStep && page >= 1 &&
                  cols * page <= INT32_MAX - 65536,
              "%s: table of %lld x %lld, %lld pages of %d", fn, (long long)rows, (long long)cols, (long long)pages, page);
   return QS_OK;
@@ -707,7 +710,7 @@ extern "C" int qs_page_copy(const qs_page_store* store, const int32_t* src, cons
   if (count == 0) return QS_OK;
   Store st;
   if (const int rc = store_checks("qs_page_copy", store, st)) return rc;
-  QS_REQUIRE(src && dst && count >= 1 && count <= INT32_MAX, "qs_page_copy: null pointer or %lld pairs", (long long)count);
+  QS_REQUIRE(src && dst && count >= 1 && count <= INT32_MAX - kCopyStep, "qs_page_copy: null pointer or %lld pairs", (long long)count);
   hipLaunchKernelGGL(page_list_kernel, copy_grid(st, count), dim3(256), 0, as_stream(stream), st, src, dst, (int)count);
   QS_LAUNCHED("page_list_kernel");
   return QS_OK;

@@ -240,3 +240,18 @@ def test_tables_and_tokens_out_of_range():
     assert b"2097152 columns" in L.qs_last_error()
     assert L.qs_attend_chunk(P, 2, 4, 0, 8, 2, 128, 1024, 128, P, pool(), 0.1, 0, 0, P, 1024, None) == 1
     assert b"4 tokens of no row" in L.qs_last_error()
+
+
+def test_pools_whose_pages_no_int_counts():
+    """The kernels' loops step over pages and copies by up to 8192 and 64 at a time, in 32 bits."""
+    L = _lib.lib()
+    for pages in (2 ** 31 - 1024, 2 ** 31 - 8192):
+        store = _lib.PageStore(64, 1, pages, 1, 1, 16)
+        assert L.qs_page_advance(store, P, P, P, None, 8, 4, 1, P, P, P, P, P, 1 << 20, None) == 1
+        assert b"%d pages" % pages in L.qs_last_error()
+        assert L.qs_page_free(P, P, P, None, 8, 4, pages, 1, 0, 0, P, P, P, None) == 1
+        assert b"%d pages" % pages in L.qs_last_error()
+        assert L.qs_page_compact(store, P, P, 8, 4, P, P, P, 1 << 40, None) == 1
+        assert b"%d pages" % pages in L.qs_last_error()
+    store = _lib.PageStore(64, 1, 4, 1, 1, 16)
+    assert L.qs_page_copy(store, P, P, 2 ** 31 - 64, None) == 1 and b"2147483584 pairs" in L.qs_last_error()
