@@ -125,8 +125,9 @@ __device__ __forceinline__ bool find_block(const ChunkArgs& a, const PagePool& p
     const int end = first_of(a, lane + 1);
     count = end > first ? end - first : 0;
     n = (count * group + kCols - 1) / kCols;
-    const int64_t most = (int64_t)pp.cols << pp.shift;
-    p0 = length_of(pp.lengths[lane], most) - count;
+    // for the order alone: a row that ends beyond its table counts as one that ends with it
+    const int len = length_of(pp.lengths[lane]), most = pp.cols << pp.shift;
+    p0 = (len < most ? len : most) - count;
   }
   if (a.rows == 1) {
     out = Block{0, __builtin_amdgcn_readfirstlane(n) - 1 - k, __builtin_amdgcn_readfirstlane(first), __builtin_amdgcn_readfirstlane(count)};
@@ -218,23 +219,23 @@ __global__ __launch_bounds__(64 * kWaves * GR, HD == 256 ? 1 : HD == 128 || GR =
   const int split = blockIdx.y;
   const int row = __builtin_amdgcn_readfirstlane(blk.row), count = __builtin_amdgcn_readfirstlane(blk.count), columns = count * group;
   const int b0 = __builtin_amdgcn_readfirstlane(blk.b) * kCols;
-  const int len = __builtin_amdgcn_readfirstlane(length_of(pp.lengths[row], (int64_t)pp.cols << pp.shift));
+  const int len = __builtin_amdgcn_readfirstlane(length_of(pp.lengths[row])), most = pp.cols << pp.shift;
   const int cw = b0 + 32 * w, c = cw + r32;
   const bool column = c < columns;
   const int t = column ? c / group : count - 1;
   const int h = g * group + (column ? c % group : 0);
-  const Span s = span_of(len - (count - t), a.window, a.sinks);  // last may be negative: sees nothing
+  const Span s = span_of(len - (count - t), a.window, a.sinks, most);  // last may be negative: sees nothing
   // the spans of the first and the last token of the wave and of the work-group
   auto span_at = [&](int col) {
     const int cc = __builtin_amdgcn_readfirstlane(col < columns ? col : columns - 1);
-    return span_of(len - (count - cc / group), a.window, a.sinks);
+    return span_of(len - (count - cc / group), a.window, a.sinks, most);
   };
   const Span s0 = span_at(cw), s1 = span_at(cw + 31);  // a wave without columns has the last token's
   const Span g0 = span_at(b0), g1 = span_at(b0 + kCols - 1);
-  TileList<kT> tiles(Span{g0.low, g1.last, a.window > 0 ? (a.sinks < g0.low ? a.sinks : g0.low) : 0});
+  TileList<kT> tiles(Span{g0.low, g1.last, g0.sinks});
   tiles.sink = __builtin_amdgcn_readfirstlane(tiles.sink), tiles.low = __builtin_amdgcn_readfirstlane(tiles.low);
   tiles.count = __builtin_amdgcn_readfirstlane(tiles.count);
-  const int last_w = s1.last, low_w = s0.low, sinks_w = a.window > 0 ? (a.sinks < s0.low ? a.sinks : s0.low) : 0;
+  const int last_w = s1.last, low_w = s0.low, sinks_w = s0.sinks;
   // this split's share of the tiles
   const int u0 = (int)((int64_t)split * tiles.count / a.splits), n = (int)((int64_t)(split + 1) * tiles.count / a.splits);
   uint4 q[KS];

@@ -30,20 +30,24 @@ struct PagePool {
   const int32_t* lengths;
 };
 
-// A row's length as its table can hold it.
-__device__ __forceinline__ int length_of(int n, int64_t most) { return n < 0 ? 0 : n > most ? (int)most : n; }
+// A row's length, which may lie beyond what its table has room for.
+__device__ __forceinline__ int length_of(int n) { return n < 0 ? 0 : n; }
 
-// What a query at position `last` sees: positions low .. last and those below
-// sinks (sinks <= low; zero without a window).
+// What a query at position `at` sees of a table with room for `most`
+// positions: positions low .. last and those below sinks (sinks <= low; zero
+// without a window).  The window goes by where the query is; of what it holds,
+// positions beyond the table are left out here, so that no kernel looks for
+// them (low may lie beyond last then).
 struct Span {
   int low, last, sinks;
 };
 
-__device__ __forceinline__ Span span_of(int last, int window, int sinks) {
+__device__ __forceinline__ Span span_of(int at, int window, int sinks, int most) {
   Span s;
-  s.last = last;
-  s.low = window > 0 && last >= window ? last - window + 1 : 0;
+  s.last = at < most ? at : most - 1;
+  s.low = window > 0 && at >= window ? at - window + 1 : 0;
   s.sinks = sinks < s.low ? sinks : s.low;
+  if (s.sinks > most) s.sinks = most;
   return s;
 }
 
@@ -53,10 +57,11 @@ template <int T>
 struct TileList {
   int sink, low, count;
   __device__ __forceinline__ explicit TileList(const Span& s) {
+    const bool window = s.low <= s.last;
     low = s.low / T;
     sink = (s.sinks + T - 1) / T;
-    if (sink > low) sink = low;
-    count = s.last < 0 ? 0 : sink + s.last / T - low + 1;
+    if (window && sink > low) sink = low;
+    count = sink + (window ? s.last / T - low + 1 : 0);
   }
   __device__ __forceinline__ int at(int u) const { return u < sink ? u : low + u - sink; }
 };
@@ -299,7 +304,7 @@ __host__ __device__ __forceinline__ int share_tiles(int count, int splits) {
 // Which parts of a single token's head there are: those of its row's tiles.
 struct Used {
   const int32_t* lengths;
-  int64_t most;  // positions that the table has room for
+  int most;  // positions that the table has room for
   int window, sinks;
 };
 

@@ -41,9 +41,8 @@ __global__ __launch_bounds__(64 * kWavesT) void attend_token_kernel(PagePool pp,
   const int split = blockIdx.x, g = blockIdx.y / blocks, hb = blockIdx.y % blocks, row = blockIdx.z;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r16 = lane & 15, qd = lane >> 4;
   const LaneX lx = lane_x_init();
-  const int64_t most = (int64_t)pp.cols << pp.shift;
-  const int len = __builtin_amdgcn_readfirstlane(length_of(pp.lengths[row], most));
-  const Span s = span_of(len - 1, a.window, a.sinks);
+  const int len = __builtin_amdgcn_readfirstlane(length_of(pp.lengths[row]));
+  const Span s = span_of(len - 1, a.window, a.sinks, pp.cols << pp.shift);
   const TileList<kTile> tiles(s);
   const int run = share_tiles(tiles.count, a.splits);
   if (split > 0 && split * run >= tiles.count) return;  // the join does not look for it
@@ -139,8 +138,8 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
   float2 ml = make_float2(-INFINITY, 0.f);
   if (lane < splits) ml = *reinterpret_cast<const float2*>(from + (int64_t)lane * part_floats(HD));
   if (used.lengths) {
-    const int len = length_of(used.lengths[pair / heads], used.most);
-    const int count = TileList<kTile>(span_of(len - 1, used.window, used.sinks)).count, run = share_tiles(count, splits);
+    const int len = length_of(used.lengths[pair / heads]);
+    const int count = TileList<kTile>(span_of(len - 1, used.window, used.sinks, used.most)).count, run = share_tiles(count, splits);
     const int there = __builtin_amdgcn_readfirstlane((count + run - 1) / run);
     splits = there < 1 ? 1 : there;
   }
@@ -218,7 +217,7 @@ int launch_token(const PagePool& pp, const TokenArgs& a, int64_t rows, bool many
   else if (past_caches) hipLaunchKernelGGL((attend_token_kernel<BF, HD, few_waves(HD), true>), grid, few, 0, stream, pp, a);
   else hipLaunchKernelGGL((attend_token_kernel<BF, HD, few_waves(HD), false>), grid, few, 0, stream, pp, a);
   QS_LAUNCHED("attend_token_kernel");
-  const Used used{pp.lengths, (int64_t)pp.cols << pp.shift, a.window, a.sinks};
+  const Used used{pp.lengths, pp.cols << pp.shift, a.window, a.sinks};
   if (a.splits > 1) return join_parts(a.part, a.splits, &used, rows, a.heads, HD, BF, a.scale, a.out, a.out_row, stream);
   return QS_OK;
 }
