@@ -394,7 +394,12 @@ int qs_dec_silu_mul(const void *gate, const void *up, void *out, int64_t rows, i
 /* One layer's keys and values.  Strides in elements, multiples of 8; the
  * head_dim elements of a position lie together.  page: a power of two from 16
  * to 4096.  A table entry that names no page of the pool, and a position
- * beyond the table, is left out of an attention and not written. */
+ * beyond the table, is left out of an attention and not written.
+ *
+ * The calls ..._over take, per row, how many of its newest tokens lie beyond
+ * the table (`over`, as qs_page_advance_over leaves it): where lengths[r] is
+ * the table's room, the row ends at lengths[r] + over[r] instead of
+ * lengths[r].  over NULL: as the calls of the same name without it. */
 typedef struct qs_page_pool {
   void *k, *v;
   int64_t k_page, k_head, k_pos;
@@ -414,6 +419,10 @@ int qs_page_append(const void *k, const void *v, int64_t tokens, int64_t rows, i
                    int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t *starts,
                    const qs_page_pool *pool, qs_stream_t stream);
 
+int qs_page_append_over(const void *k, const void *v, int64_t tokens, int64_t rows, int kv_heads, int head_dim,
+                        int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t *starts,
+                        const qs_page_pool *pool, const int32_t *over, qs_stream_t stream);
+
 /* qs_dec_qk_norm_rope for a paged cache, one token per row, each at its own
  * position lengths[r] - 1 (the row of the cos / sin tables, of table_rows
  * rows, too): q and k heads get their norm and the rotary embedding, q into
@@ -421,6 +430,10 @@ int qs_page_append(const void *k, const void *v, int64_t tokens, int64_t rows, i
 int qs_page_append_rope(const void *q, const void *k, const void *v, const void *q_norm_w, const void *k_norm_w,
                         const void *cos_table, const void *sin_table, int64_t table_rows, void *q_out, int64_t rows,
                         int nh, int nkv, int head_dim, const qs_page_pool *pool, float eps, qs_stream_t stream);
+int qs_page_append_rope_over(const void *q, const void *k, const void *v, const void *q_norm_w, const void *k_norm_w,
+                             const void *cos_table, const void *sin_table, int64_t table_rows, void *q_out,
+                             int64_t rows, int nh, int nkv, int head_dim, const qs_page_pool *pool,
+                             const int32_t *over, float eps, qs_stream_t stream);
 
 /* Attention of one new token per row, at position lengths[r] - 1, over the
  * row's pages: out[r][h * head_dim + d] = sum_p softmax_p(scale q_h . k_p)
@@ -434,6 +447,10 @@ size_t qs_attend_token_workspace_bytes(int64_t rows, int heads, int kv_heads, in
 int qs_attend_token(const void *q, int dtype, int64_t rows, int heads, int kv_heads, int head_dim, int64_t q_row,
                     int64_t q_head, const qs_page_pool *pool, float scale, int window, int sinks, void *out,
                     int64_t out_row, void *workspace, size_t workspace_bytes, qs_stream_t stream);
+int qs_attend_token_over(const void *q, int dtype, int64_t rows, int heads, int kv_heads, int head_dim, int64_t q_row,
+                         int64_t q_head, const qs_page_pool *pool, const int32_t *over, float scale, int window,
+                         int sinks, void *out, int64_t out_row, void *workspace, size_t workspace_bytes,
+                         qs_stream_t stream);
 
 /* The same for several new tokens per row, each seeing the positions up to
  * its own: the tokens of row r are starts[r] .. starts[r + 1] - 1 of q and
@@ -452,6 +469,10 @@ int qs_attend_chunk_ws(const void *q, int dtype, int64_t tokens, int64_t rows, i
                        int64_t q_token, int64_t q_head, const int32_t *starts, const qs_page_pool *pool, float scale,
                        int window, int sinks, void *out, int64_t out_token, void *workspace, size_t workspace_bytes,
                        qs_stream_t stream);
+int qs_attend_chunk_over(const void *q, int dtype, int64_t tokens, int64_t rows, int heads, int kv_heads, int head_dim,
+                         int64_t q_token, int64_t q_head, const int32_t *starts, const qs_page_pool *pool,
+                         const int32_t *over, float scale, int window, int sinks, void *out, int64_t out_token,
+                         void *workspace, size_t workspace_bytes, qs_stream_t stream);
 
 /* The whole cache of a model, for the calls that move pages: `planes` (keys
  * and values of every layer) of [pages][kv_heads][page][row_bytes], one after
@@ -472,7 +493,8 @@ typedef struct qs_page_store {
  * pages are the free ones in ascending order, given out by row, then by
  * column.  short_pages[0] gets the number of pages that were asked for and
  * could not be given (none free, or the table full), at most 2^31 - 1: those
- * entries are -1.
+ * entries are -1.  Lengths count tokens beyond the table too (up to 2^31 -
+ * 1), so that the calls above leave those out and keep what is cached.
  * Outputs may be the inputs.  workspace: qs_page_advance_workspace_bytes. */
 size_t qs_page_advance_workspace_bytes(int64_t rows);
 int qs_page_advance(const qs_page_store *store, const int32_t *table, const int32_t *lengths, const int32_t *refs,
@@ -485,6 +507,13 @@ int qs_page_advance_rows(const qs_page_store *store, const int32_t *table, const
                          const int32_t *parents, int64_t rows, int64_t cols, int tokens, const int32_t *row_tokens,
                          int32_t *table_out, int32_t *lengths_out, int32_t *refs_out, int32_t *short_pages,
                          void *workspace, size_t workspace_bytes, qs_stream_t stream);
+/* The same with lengths cut to the table's room, and over [rows] set to how
+ * many of a row's new tokens lie beyond it; those are gone with the next step.
+ * over NULL: as qs_page_advance_rows. */
+int qs_page_advance_over(const qs_page_store *store, const int32_t *table, const int32_t *lengths, const int32_t *refs,
+                         const int32_t *parents, int64_t rows, int64_t cols, int tokens, const int32_t *row_tokens,
+                         int32_t *table_out, int32_t *lengths_out, int32_t *refs_out, int32_t *short_pages,
+                         int32_t *over, void *workspace, size_t workspace_bytes, qs_stream_t stream);
 
 /* Gives pages back: all of the rows with keep[i] == 0 (their length becomes
  * 0; keep may be NULL), and with a window the pages that no token at position

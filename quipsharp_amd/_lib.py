@@ -106,20 +106,29 @@ _SIGNATURES = {
                                _int, _int, _i64, _f32, _f32, _vp], _int),
     "qs_dec_silu_mul": ([_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp], _int),
     "qs_page_append": ([_vp, _vp, _i64, _i64, _int, _int, _i64, _i64, _i64, _i64, _vp, _pool_p, _vp], _int),
+    "qs_page_append_over": ([_vp, _vp, _i64, _i64, _int, _int, _i64, _i64, _i64, _i64, _vp, _pool_p, _vp, _vp], _int),
     "qs_page_append_rope": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _int, _int, _int, _pool_p, _f32,
                              _vp], _int),
+    "qs_page_append_rope_over": ([_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _int, _int, _int, _pool_p, _vp,
+                                  _f32, _vp], _int),
     "qs_attend_token_workspace_bytes": ([_i64, _int, _int, _int, _i64, _int, _int, _int], ctypes.c_size_t),
     "qs_attend_token": ([_vp, _int, _i64, _int, _int, _int, _i64, _i64, _pool_p, _f32, _int, _int, _vp, _i64, _vp,
                          ctypes.c_size_t, _vp], _int),
+    "qs_attend_token_over": ([_vp, _int, _i64, _int, _int, _int, _i64, _i64, _pool_p, _vp, _f32, _int, _int, _vp, _i64,
+                              _vp, ctypes.c_size_t, _vp], _int),
     "qs_attend_chunk": ([_vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _vp, _pool_p, _f32, _int, _int, _vp,
                          _i64, _vp], _int),
     "qs_attend_chunk_workspace_bytes": ([_i64, _i64, _int, _int, _int, _i64, _int, _int, _int], ctypes.c_size_t),
     "qs_attend_chunk_ws": ([_vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _vp, _pool_p, _f32, _int, _int, _vp,
                             _i64, _vp, ctypes.c_size_t, _vp], _int),
+    "qs_attend_chunk_over": ([_vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _vp, _pool_p, _vp, _f32, _int, _int,
+                              _vp, _i64, _vp, ctypes.c_size_t, _vp], _int),
     "qs_page_advance_workspace_bytes": ([_i64], ctypes.c_size_t),
     "qs_page_advance": ([_store_p, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, ctypes.c_size_t,
                          _vp], _int),
     "qs_page_advance_rows": ([_store_p, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, _vp,
+                              ctypes.c_size_t, _vp], _int),
+    "qs_page_advance_over": ([_store_p, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                               ctypes.c_size_t, _vp], _int),
     "qs_page_free": ([_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp], _int),
     "qs_page_compact_workspace_bytes": ([_i64], ctypes.c_size_t),

@@ -126,7 +126,7 @@ __device__ __forceinline__ bool find_block(const ChunkArgs& a, const PagePool& p
     count = end > first ? end - first : 0;
     n = (count * group + kCols - 1) / kCols;
     // for the order alone: a row that ends beyond its table counts as one that ends with it
-    const int len = length_of(pp.lengths[lane]), most = pp.cols << pp.shift;
+    const int len = pp.lengths[lane] < 0 ? 0 : pp.lengths[lane], most = pp.cols << pp.shift;
     p0 = (len < most ? len : most) - count;
   }
   if (a.rows == 1) {
@@ -219,7 +219,7 @@ __global__ __launch_bounds__(64 * kWaves * GR, HD == 256 ? 1 : HD == 128 || GR =
   const int split = blockIdx.y;
   const int row = __builtin_amdgcn_readfirstlane(blk.row), count = __builtin_amdgcn_readfirstlane(blk.count), columns = count * group;
   const int b0 = __builtin_amdgcn_readfirstlane(blk.b) * kCols;
-  const int len = __builtin_amdgcn_readfirstlane(length_of(pp.lengths[row])), most = pp.cols << pp.shift;
+  const int most = pp.cols << pp.shift, len = __builtin_amdgcn_readfirstlane(end_of(pp.lengths, pp.over, most, row));
   const int cw = b0 + 32 * w, c = cw + r32;
   const bool column = c < columns;
   const int t = column ? c / group : count - 1;
@@ -615,7 +615,7 @@ int launch_chunk(const PagePool& pp, const ChunkArgs& a, hipStream_t stream) {
 }  // namespace
 
 int page_pool_checks(const char* fn, const qs_page_pool* p, int dtype, int64_t rows, int heads, int kv_heads,
-                     int head_dim, float scale, int window, int sinks, PagePool& out) {
+                     int head_dim, float scale, int window, int sinks, const int32_t* over, PagePool& out) {
   QS_REQUIRE(std::isfinite(scale) && scale != 0.f, "%s: scale %g", fn, (double)scale);
   QS_SUPPORTED(dtype == QS_DTYPE_BF16 || dtype == QS_DTYPE_F16, "%s: dtype %d (bf16 and fp16 only)", fn, dtype);
   QS_SUPPORTED(head_dim == 64 || head_dim == 128 || head_dim == 256, "%s: head_dim %d (64, 128 or 256)", fn, head_dim);
@@ -642,7 +642,7 @@ int page_pool_checks(const char* fn, const qs_page_pool* p, int dtype, int64_t r
   int shift = 0;
   while ((1 << shift) < p->page) ++shift;
   out = PagePool{static_cast<const uint16_t*>(p->k), static_cast<const uint16_t*>(p->v), p->k_page, p->k_head, p->v_page,
-                 p->v_head, (int)p->k_pos, (int)p->v_pos, (int)p->pages, shift, p->table, p->table_ld, (int)p->cols, p->lengths};
+                 p->v_head, (int)p->k_pos, (int)p->v_pos, (int)p->pages, shift, p->table, p->table_ld, (int)p->cols, p->lengths, over};
   return QS_OK;
 }
 
@@ -661,18 +661,27 @@ extern "C" int qs_attend_chunk(const void* q, int dtype, int64_t tokens, int64_t
                                int head_dim, int64_t q_token, int64_t q_head, const int32_t* starts,
                                const qs_page_pool* pool, float scale, int window, int sinks, void* out,
                                int64_t out_token, qs_stream_t stream) {
-  return qs_attend_chunk_ws(q, dtype, tokens, rows, heads, kv_heads, head_dim, q_token, q_head, starts, pool, scale,
-                            window, sinks, out, out_token, nullptr, 0, stream);
+  return qs_attend_chunk_over(q, dtype, tokens, rows, heads, kv_heads, head_dim, q_token, q_head, starts, pool, nullptr,
+                              scale, window, sinks, out, out_token, nullptr, 0, stream);
 }
 
 extern "C" int qs_attend_chunk_ws(const void* q, int dtype, int64_t tokens, int64_t rows, int heads, int kv_heads,
                                   int head_dim, int64_t q_token, int64_t q_head, const int32_t* starts,
                                   const qs_page_pool* pool, float scale, int window, int sinks, void* out,
                                   int64_t out_token, void* workspace, size_t workspace_bytes, qs_stream_t stream) {
+  return qs_attend_chunk_over(q, dtype, tokens, rows, heads, kv_heads, head_dim, q_token, q_head, starts, pool, nullptr,
+                              scale, window, sinks, out, out_token, workspace, workspace_bytes, stream);
+}
+
+extern "C" int qs_attend_chunk_over(const void* q, int dtype, int64_t tokens, int64_t rows, int heads, int kv_heads,
+                                    int head_dim, int64_t q_token, int64_t q_head, const int32_t* starts,
+                                    const qs_page_pool* pool, const int32_t* over, float scale, int window, int sinks,
+                                    void* out, int64_t out_token, void* workspace, size_t workspace_bytes,
+                                    qs_stream_t stream) {
   if (tokens == 0) return QS_OK;
   QS_REQUIRE(rows != 0, "qs_attend_chunk: %lld tokens of no row", (long long)tokens);
   PagePool pp;
-  if (const int rc = page_pool_checks("qs_attend_chunk", pool, dtype, rows, heads, kv_heads, head_dim, scale, window, sinks, pp)) return rc;
+  if (const int rc = page_pool_checks("qs_attend_chunk", pool, dtype, rows, heads, kv_heads, head_dim, scale, window, sinks, over, pp)) return rc;
   QS_REQUIRE(q && out && starts, "qs_attend_chunk: null pointer");
   QS_REQUIRE(tokens >= 1 && tokens * heads <= INT32_MAX, "qs_attend_chunk: %lld tokens", (long long)tokens);
   QS_REQUIRE(q_head >= head_dim && q_head % 8 == 0 && q_token >= 0 && q_token % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0,

@@ -27,11 +27,18 @@ struct PagePool {
   const int32_t* table;
   int64_t table_ld;
   int cols;
-  const int32_t* lengths;
+  const int32_t *lengths, *over;  // over: per row, or null
 };
 
-// A row's length, which may lie beyond what its table has room for.
-__device__ __forceinline__ int length_of(int n) { return n < 0 ? 0 : n; }
+// Where a row's tokens end, which may lie beyond the `most` positions that its
+// table has room for: at its length, or where that is the table's end, `over`
+// further.
+__device__ __forceinline__ int end_of(const int32_t* lengths, const int32_t* over, int most, int64_t row) {
+  const int n = lengths[row] < 0 ? 0 : lengths[row];
+  if (!over || n < most) return n;
+  const int o = over[row] < 0 ? 0 : over[row];
+  return o < INT32_MAX - n ? n + o : INT32_MAX;
+}
 
 // What a query at position `at` sees of a table with room for `most`
 // positions: positions low .. last and those below sinks (sinks <= low; zero
@@ -303,7 +310,7 @@ __host__ __device__ __forceinline__ int share_tiles(int count, int splits) {
 
 // Which parts of a single token's head there are: those of its row's tiles.
 struct Used {
-  const int32_t* lengths;
+  const int32_t *lengths, *over;
   int most;  // positions that the table has room for
   int window, sinks;
 };
@@ -315,6 +322,6 @@ int join_parts(const float* part, int splits, const Used* used, int64_t tokens, 
 
 // The argument checks of the attention calls; fills `out`.
 int page_pool_checks(const char* fn, const qs_page_pool* p, int dtype, int64_t rows, int heads, int kv_heads,
-                     int head_dim, float scale, int window, int sinks, PagePool& out);
+                     int head_dim, float scale, int window, int sinks, const int32_t* over, PagePool& out);
 
 }  // namespace qs

@@ -41,8 +41,9 @@ __global__ __launch_bounds__(64 * kWavesT) void attend_token_kernel(PagePool pp,
   const int split = blockIdx.x, g = blockIdx.y / blocks, hb = blockIdx.y % blocks, row = blockIdx.z;
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, r16 = lane & 15, qd = lane >> 4;
   const LaneX lx = lane_x_init();
-  const int len = __builtin_amdgcn_readfirstlane(length_of(pp.lengths[row]));
-  const Span s = span_of(len - 1, a.window, a.sinks, pp.cols << pp.shift);
+  const int most = pp.cols << pp.shift;
+  const int len = __builtin_amdgcn_readfirstlane(end_of(pp.lengths, pp.over, most, row));
+  const Span s = span_of(len - 1, a.window, a.sinks, most);
   const TileList<kTile> tiles(s);
   const int run = share_tiles(tiles.count, a.splits);
   if (split > 0 && split * run >= tiles.count) return;  // the join does not look for it
@@ -138,7 +139,7 @@ __global__ __launch_bounds__(256) void join_kernel(const float* part, int splits
   float2 ml = make_float2(-INFINITY, 0.f);
   if (lane < splits) ml = *reinterpret_cast<const float2*>(from + (int64_t)lane * part_floats(HD));
   if (used.lengths) {
-    const int len = length_of(used.lengths[pair / heads]);
+    const int len = end_of(used.lengths, used.over, used.most, pair / heads);
     const int count = TileList<kTile>(span_of(len - 1, used.window, used.sinks, used.most)).count, run = share_tiles(count, splits);
     const int there = __builtin_amdgcn_readfirstlane((count + run - 1) / run);
     splits = there < 1 ? 1 : there;
@@ -217,7 +218,7 @@ int launch_token(const PagePool& pp, const TokenArgs& a, int64_t rows, bool many
   else if (past_caches) hipLaunchKernelGGL((attend_token_kernel<BF, HD, few_waves(HD), true>), grid, few, 0, stream, pp, a);
   else hipLaunchKernelGGL((attend_token_kernel<BF, HD, few_waves(HD), false>), grid, few, 0, stream, pp, a);
   QS_LAUNCHED("attend_token_kernel");
-  const Used used{pp.lengths, pp.cols << pp.shift, a.window, a.sinks};
+  const Used used{pp.lengths, pp.over, pp.cols << pp.shift, a.window, a.sinks};
   if (a.splits > 1) return join_parts(a.part, a.splits, &used, rows, a.heads, HD, BF, a.scale, a.out, a.out_row, stream);
   return QS_OK;
 }
@@ -227,7 +228,7 @@ int launch_token(const PagePool& pp, const TokenArgs& a, int64_t rows, bool many
 int join_parts(const float* part, int splits, const Used* there, int64_t tokens, int heads, int head_dim, bool bf, float scale,
                uint16_t* out, int64_t out_token, hipStream_t stream) {
   const int64_t pairs = tokens * heads;
-  const Used used = there ? *there : Used{nullptr, 0, 0, 0};
+  const Used used = there ? *there : Used{nullptr, nullptr, 0, 0, 0};
   const dim3 grid((unsigned)((pairs + 3) / 4)), block(256);
   if (head_dim == 64) {
     if (bf) hipLaunchKernelGGL((join_kernel<true, 64>), grid, block, 0, stream, part, splits, used, pairs, heads, scale, out, out_token);
@@ -257,9 +258,17 @@ extern "C" int qs_attend_token(const void* q, int dtype, int64_t rows, int heads
                                int64_t q_row, int64_t q_head, const qs_page_pool* pool, float scale, int window,
                                int sinks, void* out, int64_t out_row, void* workspace, size_t workspace_bytes,
                                qs_stream_t stream) {
+  return qs_attend_token_over(q, dtype, rows, heads, kv_heads, head_dim, q_row, q_head, pool, nullptr, scale, window,
+                              sinks, out, out_row, workspace, workspace_bytes, stream);
+}
+
+extern "C" int qs_attend_token_over(const void* q, int dtype, int64_t rows, int heads, int kv_heads, int head_dim,
+                                    int64_t q_row, int64_t q_head, const qs_page_pool* pool, const int32_t* over,
+                                    float scale, int window, int sinks, void* out, int64_t out_row, void* workspace,
+                                    size_t workspace_bytes, qs_stream_t stream) {
   if (rows == 0) return QS_OK;
   PagePool pp;
-  if (const int rc = page_pool_checks("qs_attend_token", pool, dtype, rows, heads, kv_heads, head_dim, scale, window, sinks, pp)) return rc;
+  if (const int rc = page_pool_checks("qs_attend_token", pool, dtype, rows, heads, kv_heads, head_dim, scale, window, sinks, over, pp)) return rc;
   QS_REQUIRE(q && out, "qs_attend_token: null pointer");
   QS_REQUIRE(q_head >= head_dim && q_head % 8 == 0 && q_row >= 0 && q_row % 8 == 0 && (reinterpret_cast<uintptr_t>(q) & 15) == 0,
              "qs_attend_token: query rows must be 16-byte aligned (strides %lld, %lld)", (long long)q_row, (long long)q_head);

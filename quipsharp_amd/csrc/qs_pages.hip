@@ -157,6 +157,7 @@ struct AdvanceArgs {
   const int32_t *table, *lengths, *refs, *parents;
   const int32_t* row_tokens;  // per row, or null: `tokens` for all
   int32_t *table_out, *lengths_out, *refs_out, *short_pages, *plan;
+  int32_t* over;  // per row, or null: lengths go on beyond the table
   int rows, cols, pages, page, tokens;
 };
 
@@ -193,6 +194,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   else if (a.refs_out != a.refs)
     ref_copy(a.refs, a.refs_out, a.pages);
   int old_len = 0, tokens = a.tokens;
+  int64_t start = 0;  // where the new tokens begin: at old_len, or beyond the table
   if (tid < a.rows) {
     if (a.row_tokens) {
       const int n = a.row_tokens[tid];
@@ -201,8 +203,9 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
     int par = a.parents ? a.parents[tid] : tid;
     par = par >= 0 && par < a.rows ? par : -1;
     from[tid] = par;
-    int n = par >= 0 ? a.lengths[par] : 0;
+    const int n = par >= 0 ? a.lengths[par] : 0;
     old_len = n < 0 ? 0 : n > room ? (int)room : n;
+    start = a.over || n < old_len ? old_len : n;
     len[tid] = old_len;
     shared_page[tid] = 0;
   }
@@ -255,11 +258,17 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   if (tid < a.rows) {
     copy = shared_page[tid];
     first = c0 + (used > 0);
-    int64_t last = tokens > 0 ? ((int64_t)old_len + tokens - 1) / a.page : -1;
-    if (last >= a.cols) atomicAdd(&lost, (unsigned long long)(last - a.cols + 1)), last = a.cols - 1;
+    const int64_t end = start + tokens;
+    int64_t last = tokens > 0 ? (end - 1) / a.page : -1;
+    if (last >= a.cols) {
+      const int64_t from_col = start / a.page;
+      atomicAdd(&lost, (unsigned long long)(last - (from_col < a.cols ? a.cols : from_col) + 1));
+      last = a.cols - 1;
+    }
     wants = copy + (last >= first ? (int)(last - first + 1) : 0);
-    const int64_t end = (int64_t)old_len + tokens;
-    a.lengths_out[tid] = (int)(end < room ? end : room);
+    const int64_t cut = a.over ? room : INT32_MAX;
+    a.lengths_out[tid] = (int)(end < cut ? end : cut);
+    if (a.over) a.over[tid] = end <= room ? 0 : (int)(end < INT32_MAX ? end - room : INT32_MAX - room);
   }
   int total;
   const int mark = scan1024(wants, part, &total);
@@ -469,10 +478,16 @@ __global__ __launch_bounds__(256) void page_remap_kernel(const int32_t* table, i
 // new tokens
 // ---------------------------------------------------------------------------
 
+// Where a row's tokens end, as the attention has it.
+__device__ __forceinline__ int64_t row_end(const qs_page_pool& pool, const int32_t* over, int64_t row) {
+  const int64_t n = pool.lengths[row];
+  return over && n >= pool.cols * pool.page && over[row] > 0 ? n + over[row] : n;
+}
+
 struct AppendArgs {
   const uint16_t *k, *v;
   int64_t k_token, k_head, v_token, v_head, tokens;
-  const int32_t* starts;
+  const int32_t *starts, *over;
   int rows, kv_heads, head_dim;
 };
 
@@ -504,7 +519,7 @@ __global__ __launch_bounds__(256) void page_append_kernel(qs_page_pool pool, App
     back = a.starts[row + 1] - t;
     if (a.starts[row] > t || back <= 0) return;
   }
-  const int64_t p = pool.lengths[row] - back;
+  const int64_t p = row_end(pool, a.over, row) - back;
   if (uint16_t* to = place(pool.k, pool.k_page, pool.k_head, pool.k_pos, pool, row, p, head))
     *reinterpret_cast<uint4*>(to + d) = *reinterpret_cast<const uint4*>(a.k + t * a.k_token + head * a.k_head + d);
   if (uint16_t* to = place(pool.v, pool.v_page, pool.v_head, pool.v_pos, pool, row, p, head))
@@ -516,11 +531,11 @@ __global__ __launch_bounds__(256) void page_append_rope_kernel(const uint16_t* q
                                                                const uint16_t* qw, const uint16_t* kw,
                                                                const uint16_t* cos_t, const uint16_t* sin_t,
                                                                int64_t table_rows, uint16_t* q_out, qs_page_pool pool,
-                                                               int nh, int nkv, float eps) {
+                                                               const int32_t* over, int nh, int nkv, float eps) {
   const LaneX lx = lane_x_init();
   const int b = blockIdx.x, hh = blockIdx.y * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
   if (hh >= nh + 2 * nkv) return;
-  const int64_t pos = (int64_t)pool.lengths[b] - 1;
+  const int64_t pos = row_end(pool, over, b) - 1;
   if (hh >= nh + nkv) {
     const int g = hh - nh - nkv;
     const uint16_t* src = v + ((int64_t)b * nkv + g) * 128;
@@ -589,6 +604,14 @@ using namespace qs;
 extern "C" int qs_page_append(const void* k, const void* v, int64_t tokens, int64_t rows, int kv_heads, int head_dim,
                               int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head, const int32_t* starts,
                               const qs_page_pool* pool, qs_stream_t stream) {
+  return qs_page_append_over(k, v, tokens, rows, kv_heads, head_dim, k_token, k_head, v_token, v_head, starts, pool,
+                             nullptr, stream);
+}
+
+extern "C" int qs_page_append_over(const void* k, const void* v, int64_t tokens, int64_t rows, int kv_heads, int head_dim,
+                                   int64_t k_token, int64_t k_head, int64_t v_token, int64_t v_head,
+                                   const int32_t* starts, const qs_page_pool* pool, const int32_t* over,
+                                   qs_stream_t stream) {
   if (tokens == 0 || rows == 0) return QS_OK;
   if (const int rc = pool_checks("qs_page_append", pool, rows, kv_heads, head_dim)) return rc;
   QS_REQUIRE(k && v && tokens >= 1 && (starts || tokens == rows), "qs_page_append: %lld tokens of %lld rows",
@@ -600,7 +623,7 @@ extern "C" int qs_page_append(const void* k, const void* v, int64_t tokens, int6
   const int64_t threads = tokens * kv_heads * (head_dim / 8);
   QS_REQUIRE(threads <= ((int64_t)INT32_MAX << 8), "qs_page_append: %lld tokens", (long long)tokens);
   const AppendArgs a{static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v), k_token, k_head, v_token, v_head,
-                     tokens, starts, (int)rows, kv_heads, head_dim};
+                     tokens, starts, over, (int)rows, kv_heads, head_dim};
   hipLaunchKernelGGL(page_append_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, as_stream(stream), *pool, a);
   QS_LAUNCHED("page_append_kernel");
   return QS_OK;
@@ -610,6 +633,14 @@ extern "C" int qs_page_append_rope(const void* q, const void* k, const void* v, 
                                    const void* k_norm_w, const void* cos_table, const void* sin_table,
                                    int64_t table_rows, void* q_out, int64_t rows, int nh, int nkv, int head_dim,
                                    const qs_page_pool* pool, float eps, qs_stream_t stream) {
+  return qs_page_append_rope_over(q, k, v, q_norm_w, k_norm_w, cos_table, sin_table, table_rows, q_out, rows, nh, nkv,
+                                  head_dim, pool, nullptr, eps, stream);
+}
+
+extern "C" int qs_page_append_rope_over(const void* q, const void* k, const void* v, const void* q_norm_w,
+                                        const void* k_norm_w, const void* cos_table, const void* sin_table,
+                                        int64_t table_rows, void* q_out, int64_t rows, int nh, int nkv, int head_dim,
+                                        const qs_page_pool* pool, const int32_t* over, float eps, qs_stream_t stream) {
   if (rows == 0) return QS_OK;
   QS_REQUIRE(q && k && v && q_norm_w && k_norm_w && cos_table && sin_table && q_out, "qs_page_append_rope: null pointer");
   QS_SUPPORTED(head_dim == 128, "qs_page_append_rope: head_dim %d (128 only)", head_dim);
@@ -620,7 +651,7 @@ extern "C" int qs_page_append_rope(const void* q, const void* k, const void* v, 
                      as_stream(stream), static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k),
                      static_cast<const uint16_t*>(v), static_cast<const uint16_t*>(q_norm_w),
                      static_cast<const uint16_t*>(k_norm_w), static_cast<const uint16_t*>(cos_table),
-                     static_cast<const uint16_t*>(sin_table), table_rows, static_cast<uint16_t*>(q_out), *pool, nh, nkv, eps);
+                     static_cast<const uint16_t*>(sin_table), table_rows, static_cast<uint16_t*>(q_out), *pool, over, nh, nkv, eps);
   QS_LAUNCHED("page_append_rope_kernel");
   return QS_OK;
 }
@@ -642,6 +673,15 @@ extern "C" int qs_page_advance_rows(const qs_page_store* store, const int32_t* t
                                     const int32_t* row_tokens, int32_t* table_out, int32_t* lengths_out,
                                     int32_t* refs_out, int32_t* short_pages, void* workspace, size_t workspace_bytes,
                                     qs_stream_t stream) {
+  return qs_page_advance_over(store, table, lengths, refs, parents, rows, cols, tokens, row_tokens, table_out, lengths_out,
+                              refs_out, short_pages, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int qs_page_advance_over(const qs_page_store* store, const int32_t* table, const int32_t* lengths,
+                                    const int32_t* refs, const int32_t* parents, int64_t rows, int64_t cols, int tokens,
+                                    const int32_t* row_tokens, int32_t* table_out, int32_t* lengths_out,
+                                    int32_t* refs_out, int32_t* short_pages, int32_t* over, void* workspace,
+                                    size_t workspace_bytes, qs_stream_t stream) {
   Store st;
   if (const int rc = store_checks("qs_page_advance", store, st)) return rc;
   if (const int rc = table_checks("qs_page_advance", rows, cols, st.pages, st.page)) return rc;
@@ -654,7 +694,7 @@ extern "C" int qs_page_advance_rows(const qs_page_store* store, const int32_t* t
              qs_page_advance_workspace_bytes(rows));
   int32_t* plan = static_cast<int32_t*>(workspace);
   const AdvanceArgs a{table, lengths, refs, parents, row_tokens, table_out, lengths_out, refs_out, short_pages, plan,
-                      (int)rows, (int)cols, (int)st.pages, st.page, tokens};
+                      over, (int)rows, (int)cols, (int)st.pages, st.page, tokens};
   if (st.pages <= kNearPages && rows * cols <= kTileInts) hipLaunchKernelGGL(page_advance_kernel<true>, dim3(1), dim3(kThreads), 0, as_stream(stream), a);
   else hipLaunchKernelGGL(page_advance_kernel<false>, dim3(1), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("page_advance_kernel");

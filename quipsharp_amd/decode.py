@@ -325,7 +325,7 @@ class PagedDecoder(StaticDecoder):
         last = (count.cumsum(0) - 1)[count > 0].to(self.dev)
         row = torch.repeat_interleave(torch.arange(self.B), count).to(self.dev)
         cache.advance(count.to(self.dev))
-        pos = cache.lengths[row] - starts[row + 1] + torch.arange(T, device=self.dev)
+        pos = (cache.lengths + cache.over)[row] - starts[row + 1] + torch.arange(T, device=self.dev)
         h = m.embed_tokens(ids)[None]
         cos, sin = m.rotary_emb(h, pos[None])
         for i, L in enumerate(self.layers):
@@ -360,9 +360,10 @@ class PagedDecoder(StaticDecoder):
         from .pages import _pool
         c, vp = self.cache, self._lib.ptr
         q = torch.empty_like(out)
-        self._lib.check(self._L.qs_page_append_rope(
+        self._lib.check(self._L.qs_page_append_rope_over(
             vp(qo), vp(ko), vp(vo), vp(norms[0]), vp(norms[1]), vp(self.cos), vp(self.sin), self.cos.shape[0], vp(q),
-            self.B, self.nh, self.nkv, self.hd, _pool(c.keys(i), c.values(i), c.table, c.lengths), self.eps, stream))
+            self.B, self.nh, self.nkv, self.hd, _pool(c.keys(i), c.values(i), c.table, c.lengths), vp(c.over), self.eps,
+            stream))
         heads = (self.B, self.nh, self.hd)
         c.attend_token(i, q.view(heads), scale=self.scale, out=out.view(heads), **self.spans)
 

@@ -11,6 +11,11 @@ holds, ``refs[i]`` the number of table entries that hold page i; a page with
 none is free.  All three are int32 tensors on the GPU that only kernels read
 and write, so a step that uses them can be captured in a HIP graph.
 
+A row that runs out of columns keeps what it has: tokens at positions beyond
+the table are stored nowhere and seen by none.  ``lengths`` count them, or,
+where a call is given ``over`` (int32, a number for every row), stop at the
+table's room, and ``over`` has how many of the row's newest tokens lie beyond.
+
 The functions return new tables and leave their arguments as they are, unless
 ``out`` names the tensors to write, which may be the arguments themselves;
 the pool is changed in place.  ``PagedCache`` keeps the tensors together and
@@ -128,11 +133,12 @@ def _room(workspace):
 
 
 def append_pages(k_pages: Tensor, v_pages: Tensor, k: Tensor, v: Tensor, table: Tensor, lengths: Tensor,
-                 starts: Tensor = None) -> None:
+                 starts: Tensor = None, over: Tensor = None) -> None:
     """Store new tokens' keys and values, (tokens, kv heads, head dim) each, in
     the pages: the tokens of row r are ``starts[r]`` .. ``starts[r + 1] - 1``
     (int32, rows + 1; None: one token per row), and the last of them goes to
-    position ``lengths[r] - 1``.  Positions without a page are left out."""
+    position ``lengths[r] - 1`` (``over[r]`` further where the row is over).
+    Positions without a page are left out."""
     pool = _pool(k_pages, v_pages, table, lengths)
     dev, dim = k_pages.device, k_pages.shape[3]
     rows = table.shape[0]
@@ -142,9 +148,12 @@ def append_pages(k_pages: Tensor, v_pages: Tensor, k: Tensor, v: Tensor, table: 
         raise ValueError(f"{k.shape[1]} and {v.shape[1]} heads for a cache of {k_pages.shape[1]}")
     if starts is not None:
         _int32("starts", starts, (rows + 1,), dev)
+    if over is not None:
+        _int32("over", over, (rows,), dev)
     _lib.require_gpu(k_pages, what="append_pages")
-    _lib.check(_lib.lib().qs_page_append(k.data_ptr(), v.data_ptr(), k.shape[0], rows, k.shape[1], dim, ks[0], ks[1],
-                                         vs[0], vs[1], _lib.ptr(starts), pool, _lib.stream_of(k_pages)))
+    _lib.check(_lib.lib().qs_page_append_over(k.data_ptr(), v.data_ptr(), k.shape[0], rows, k.shape[1], dim, ks[0],
+                                              ks[1], vs[0], vs[1], _lib.ptr(starts), pool, _lib.ptr(over),
+                                              _lib.stream_of(k_pages)))
 
 
 def token_workspace_bytes(rows, heads, k_pages: Tensor, table: Tensor, window=0, sinks=0) -> int:
@@ -161,11 +170,13 @@ def chunk_workspace_bytes(tokens, heads, k_pages: Tensor, table: Tensor, window=
 
 
 def attend_token(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, *, scale: float = None,
-                 window: int = 0, sinks: int = 0, out: Tensor = None, workspace: Tensor = None) -> Tensor:
+                 window: int = 0, sinks: int = 0, over: Tensor = None, out: Tensor = None,
+                 workspace: Tensor = None) -> Tensor:
     """Attention of one new token per row over the row's pages.
 
     q: (rows, heads, head dim), the token of row r at position ``lengths[r] -
-    1``, its key and value in the pages already.  It sees the positions up to
+    1`` (``over[r]`` further where the row is over), its key and value in the
+    pages already.  It sees the positions up to
     its own: all of them, or with ``window`` the last ``window`` and the first
     ``sinks``.  Query head h reads kv head ``h // (heads / kv heads)``.
     Returns (rows, heads, head dim) in q's type; zeros for a row that sees
@@ -175,19 +186,21 @@ def attend_token(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     dtype = k_pages.dtype
     st = _heads("q", q, rows, dim, dtype, dev)
     window, sinks = _visible(window, sinks)
+    if over is not None:
+        _int32("over", over, (rows,), dev)
     out = _output(out, q)
     _lib.require_gpu(k_pages, what="attend_token")
     L, heads = _lib.lib(), q.shape[1]
     need = L.qs_attend_token_workspace_bytes(rows, heads, kv_heads, dim, cols, page, window, sinks)
     workspace = _workspace(workspace, need, dev)
-    _lib.check(L.qs_attend_token(q.data_ptr(), _lib.dtype_code(dtype), rows, heads, kv_heads, dim, st[0], st[1], pool,
-                                 dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
-                                 out.stride(0), *_room(workspace), _lib.stream_of(q)))
+    _lib.check(L.qs_attend_token_over(q.data_ptr(), _lib.dtype_code(dtype), rows, heads, kv_heads, dim, st[0], st[1],
+                                      pool, _lib.ptr(over), dim ** -0.5 if scale is None else scale, window, sinks,
+                                      out.data_ptr(), out.stride(0), *_room(workspace), _lib.stream_of(q)))
     return out
 
 
 def attend_chunk(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor, starts: Tensor, *,
-                 scale: float = None, window: int = 0, sinks: int = 0, out: Tensor = None,
+                 scale: float = None, window: int = 0, sinks: int = 0, over: Tensor = None, out: Tensor = None,
                  workspace: Tensor = None) -> Tensor:
     """Causal attention of several new tokens per row over the row's pages.
 
@@ -202,14 +215,17 @@ def attend_chunk(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     st = _heads("q", q, None, dim, dtype, dev)
     _int32("starts", starts, (rows + 1,), dev)
     window, sinks = _visible(window, sinks)
+    if over is not None:
+        _int32("over", over, (rows,), dev)
     out = _output(out, q)
     _lib.require_gpu(k_pages, what="attend_chunk")
     L, (tokens, heads, _) = _lib.lib(), q.shape
     need = L.qs_attend_chunk_workspace_bytes(tokens, rows, heads, kv_heads, dim, cols, page, window, sinks)
     workspace = _workspace(workspace, need, dev)
-    _lib.check(L.qs_attend_chunk_ws(q.data_ptr(), _lib.dtype_code(dtype), tokens, rows, heads, kv_heads, dim, st[0],
-                                    st[1], starts.data_ptr(), pool, dim ** -0.5 if scale is None else scale, window,
-                                    sinks, out.data_ptr(), out.stride(0), *_room(workspace), _lib.stream_of(q)))
+    _lib.check(L.qs_attend_chunk_over(q.data_ptr(), _lib.dtype_code(dtype), tokens, rows, heads, kv_heads, dim, st[0],
+                                      st[1], starts.data_ptr(), pool, _lib.ptr(over),
+                                      dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+                                      out.stride(0), *_room(workspace), _lib.stream_of(q)))
     return out
 
 
@@ -231,7 +247,7 @@ def _books(table, lengths, refs, pages, device):
 
 
 def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, tokens=1, parents: Tensor = None, *,
-                  out=None, workspace: Tensor = None):
+                  out=None, over: Tensor = None, workspace: Tensor = None):
     """One step of every row of a cache ``kv`` (..., pages, kv heads, page,
     head dim): row i takes the pages and the length of row ``parents[i]``
     (int32; None: its own; no row of the table: an empty one), gives back pages
@@ -244,7 +260,9 @@ def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, toke
     out by row, then by column.  Returns ``(table, lengths, refs, short)``;
     ``short`` (int32, 1; at most 2^31 - 1) is the number of pages that were
     wanted and could not be given, because none is free or the table has no
-    column left: their entries are -1."""
+    column left: their entries are -1.  With ``over`` (int32, rows; written)
+    lengths stop at the table's room and ``over`` gets how many of a row's new
+    tokens lie beyond it, which are gone with the next step."""
     store, dev = _store(kv), kv.device
     _books(table, lengths, refs, store.pages, dev)
     rows, cols = table.shape
@@ -262,12 +280,15 @@ def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, toke
         _books(out[0], out[1], out[2], store.pages, dev)
         _int32("out[0]", out[0], table.shape, dev)
         _int32("out[3]", out[3], (1,), dev)
+    if over is not None:
+        _int32("over", over, (rows,), dev)
     _lib.require_gpu(kv, what="advance_pages")
     L = _lib.lib()
     workspace = _workspace(workspace, L.qs_page_advance_workspace_bytes(rows), dev)
-    _lib.check(L.qs_page_advance_rows(store, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), _lib.ptr(parents),
+    _lib.check(L.qs_page_advance_over(store, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), _lib.ptr(parents),
                                       rows, cols, tokens, _lib.ptr(each), out[0].data_ptr(), out[1].data_ptr(),
-                                      out[2].data_ptr(), out[3].data_ptr(), *_room(workspace), _lib.stream_of(kv)))
+                                      out[2].data_ptr(), out[3].data_ptr(), _lib.ptr(over), *_room(workspace),
+                                      _lib.stream_of(kv)))
     return tuple(out)
 
 
@@ -329,7 +350,9 @@ def copy_pages(kv: Tensor, src: Tensor, dst: Tensor) -> None:
 class PagedCache:
     """The pages of a whole decoder: ``kv`` (layers, 2, pages, kv heads, page,
     head dim) with the table, lengths and reference counts of ``rows`` rows of
-    at most ``columns`` pages.  The methods work in place."""
+    at most ``columns`` pages.  The methods work in place.  ``lengths`` stop at
+    the table's room; ``over`` has how many of a row's newest tokens lie beyond,
+    which no page holds and no token sees."""
 
     def __init__(self, layers, pages, kv_heads, head_dim, rows, columns, page=64, dtype=torch.bfloat16, device="cuda"):
         self.page = page
@@ -338,6 +361,7 @@ class PagedCache:
         self.table = torch.full((rows, columns), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.zeros(rows, dtype=torch.int32, device=dev)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=dev)
+        self.over = torch.zeros(rows, dtype=torch.int32, device=dev)
         self.short = torch.zeros(1, dtype=torch.int32, device=dev)
 
     def keys(self, layer):
@@ -349,7 +373,7 @@ class PagedCache:
     def advance(self, tokens=1, parents=None):
         """``advance_pages``; ``self.short`` gets the pages that were missing."""
         advance_pages(self.kv, self.table, self.lengths, self.refs, tokens, parents,
-                      out=(self.table, self.lengths, self.refs, self.short))
+                      out=(self.table, self.lengths, self.refs, self.short), over=self.over)
 
     def free(self, keep=None, window=0, sinks=0):
         free_pages(self.table, self.lengths, self.refs, page=self.page, keep=keep, window=window, sinks=sinks,
@@ -359,10 +383,11 @@ class PagedCache:
         compact_pages(self.kv, self.table, self.refs, out=(self.table, self.refs))
 
     def append(self, layer, k, v, starts=None):
-        append_pages(self.kv[layer, 0], self.kv[layer, 1], k, v, self.table, self.lengths, starts)
+        append_pages(self.kv[layer, 0], self.kv[layer, 1], k, v, self.table, self.lengths, starts, self.over)
 
     def attend_token(self, layer, q, **options):
-        return attend_token(q, self.kv[layer, 0], self.kv[layer, 1], self.table, self.lengths, **options)
+        return attend_token(q, self.kv[layer, 0], self.kv[layer, 1], self.table, self.lengths, over=self.over, **options)
 
     def attend_chunk(self, layer, q, starts, **options):
-        return attend_chunk(q, self.kv[layer, 0], self.kv[layer, 1], self.table, self.lengths, starts, **options)
+        return attend_chunk(q, self.kv[layer, 0], self.kv[layer, 1], self.table, self.lengths, starts, over=self.over,
+                            **options)

@@ -18,6 +18,17 @@ def ints(values, dev):
     return torch.tensor(values, dtype=torch.int32, device=dev)
 
 
+def filled(lengths, dev, pages=12, heads=2, dim=64, parents=None):
+    """A cache whose rows hold these lengths (or their parents'), every place of the pool a number of its own."""
+    from quipsharp_amd.pages import PagedCache
+    cache = PagedCache(1, pages, heads, dim, len(lengths), COLS, page=PAGE, device=dev)
+    cache.kv.copy_(torch.randn(cache.kv.shape, generator=torch.Generator().manual_seed(11)))
+    cache.advance(ints(lengths, dev))
+    if parents:
+        cache.advance(0, ints(parents, dev))
+    return cache
+
+
 def held(pool, table, row):
     """(positions, heads, dim) of a row's pages in order, on the CPU."""
     pages = [p for p in table[row].tolist() if p >= 0]
@@ -29,6 +40,90 @@ def near(got, q, k, v, see, dim):
     for g in range(k.shape[1]):
         want, tol = want_and_tolerance(q[g * group:(g + 1) * group], k[see, g], v[see, g], dim ** -0.5)
         assert ((got[g * group:(g + 1) * group].double() - want).abs() <= tol).all()
+
+
+def tokens_of(n, heads, dim, seed, dev):
+    g = torch.Generator().manual_seed(seed)
+    return [torch.randn(n, h, dim, generator=g).to(BF).to(dev) for h in (heads, heads, 2 * heads)]
+
+
+@pytest.mark.parametrize("calls", ["cache", "functions"])
+def test_more_tokens_than_the_table_has_room_for(dev, calls):
+    """Row 0 goes on from 40 by 20 where 8 have room: those 8 are stored, nothing else changes, row 1, which shares
+    the first pages, least of all; each query sees the positions up to its own that there are."""
+    from quipsharp_amd.pages import advance_pages, append_pages, attend_chunk
+    cache = filled([40, 0], dev, parents=[0, 0])
+    before = cache.kv.clone()
+    k, v, q = tokens_of(20, 2, 64, 1, dev)
+    starts = ints([0, 20, 20], dev)
+    if calls == "cache":
+        cache.advance(ints([20, 0], dev))
+        table = cache.table
+        cache.append(0, k, v, starts)
+        got = cache.attend_chunk(0, q, starts)
+        lead = cache.attend_chunk(0, q, starts, window=12, sinks=2)
+    else:
+        table, lengths, _, short = advance_pages(cache.kv, cache.table, cache.lengths, cache.refs, ints([20, 0], dev))
+        assert short.item() == 1
+        append_pages(cache.keys(0), cache.values(0), k, v, table, lengths, starts)
+        pools = (cache.keys(0), cache.values(0), table, lengths, starts)
+        got, lead = attend_chunk(q, *pools), attend_chunk(q, *pools, window=12, sinks=2)
+    want = before.clone()
+    last = table[0, 2].item()
+    if last != table[1, 2].item():  # copied before it is written
+        want[0, :, last, :, :8] = before[0, :, table[1, 2].item(), :, :8]
+    want[0, 0, last, :, 8:] = k[:8].transpose(0, 1)
+    want[0, 1, last, :, 8:] = v[:8].transpose(0, 1)
+    assert torch.equal(cache.kv, want)
+    rk, rv = held(want[0, 0], table, 0), held(want[0, 1], table, 0)
+    for i in range(20):
+        near(got[i].cpu(), q[i].cpu(), rk, rv, list(range(min(41 + i, ROOM))), 64)
+        near(lead[i].cpu(), q[i].cpu(), rk, rv, [p for p in range(min(41 + i, ROOM)) if p > 28 + i or p < 2], 64)
+
+
+@pytest.mark.parametrize("calls", ["cache", "functions"])
+def test_steps_of_a_full_row(dev, calls):
+    """Single tokens of a row without room, several of them: nothing is stored, and the row attends to what it has."""
+    from quipsharp_amd.pages import advance_pages, append_pages, attend_token
+    cache = filled([ROOM, 5], dev)
+    table, lengths, refs = cache.table, cache.lengths, cache.refs
+    for step in range(3):
+        k, v, q = tokens_of(2, 2, 64, 2 + step, dev)
+        before = cache.kv.clone()
+        if calls == "cache":
+            cache.advance(1)
+            short = cache.short
+            cache.append(0, k, v)
+            got, lead = cache.attend_token(0, q), cache.attend_token(0, q, window=10)
+            n = ROOM
+        else:
+            table, lengths, refs, short = advance_pages(cache.kv, table, lengths, refs, 1)
+            append_pages(cache.keys(0), cache.values(0), k, v, table, lengths)
+            pools = (cache.keys(0), cache.values(0), table, lengths)
+            got, lead = attend_token(q, *pools), attend_token(q, *pools, window=10)
+            n = ROOM + step
+        assert short.item() == 1
+        at = table[1, 0].item()
+        before[0, 0, at, :, 5 + step], before[0, 1, at, :, 5 + step] = k[1], v[1]
+        assert torch.equal(cache.kv, before)
+        rk, rv = held(cache.keys(0), table, 0), held(cache.values(0), table, 0)
+        near(got[0].cpu(), q[0].cpu(), rk, rv, list(range(ROOM)), 64)
+        near(lead[0].cpu(), q[0].cpu(), rk, rv, list(range(n - 9, ROOM)), 64)
+
+
+def test_full_rows_that_share_their_pages(dev):
+    """Rows forked from a full one write nothing, together or one after the other."""
+    cache = filled([ROOM, 0, 0], dev, parents=[0, 0, 0])
+    before = cache.kv.clone()
+    k, v, q = tokens_of(3, 2, 64, 6, dev)
+    for parents in (None, [2, 0, 1]):
+        cache.advance(1, None if parents is None else ints(parents, dev))
+        cache.append(0, k, v)
+        assert torch.equal(cache.kv, before) and cache.short.item() == 3
+        got = cache.attend_token(0, q)
+        rk, rv = held(cache.keys(0), cache.table, 0), held(cache.values(0), cache.table, 0)
+        for r in range(3):
+            near(got[r].cpu(), q[r].cpu(), rk, rv, list(range(ROOM)), 64)
 
 
 @pytest.mark.parametrize("far", [1, 100, 2 ** 31 - 1 - ROOM])

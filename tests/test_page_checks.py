@@ -255,3 +255,15 @@ def test_pools_whose_pages_no_int_counts():
         assert b"%d pages" % pages in L.qs_last_error()
     store = _lib.PageStore(64, 1, 4, 1, 1, 16)
     assert L.qs_page_copy(store, P, P, 2 ** 31 - 64, None) == 1 and b"2147483584 pairs" in L.qs_last_error()
+
+
+@pytest.mark.parametrize("over,message", [(torch.zeros(3, dtype=I32), "over must be"), (torch.zeros(2), "over must be"),
+                                          (torch.zeros(2, dtype=I32, device="meta"), "over is on")])
+def test_tokens_over_the_table_refuse(over, message):
+    a = attention(over=over)
+    new = torch.zeros(2, 2, 128, dtype=BF)
+    for call in (lambda: attend_token(**a), lambda: attend_chunk(starts=torch.tensor([0, 1, 2], dtype=I32), **a),
+                 lambda: append_pages(a["k_pages"], a["v_pages"], new, new, a["table"], a["lengths"], over=over),
+                 lambda: advance_pages(*books(), over=over)):
+        with pytest.raises(ValueError, match=message):
+            call()
