@@ -493,8 +493,11 @@ typedef struct qs_page_store {
  * pages are the free ones in ascending order, given out by row, then by
  * column.  short_pages[0] gets the number of pages that were asked for and
  * could not be given (none free, or the table full), at most 2^31 - 1: those
- * entries are -1.  Lengths count tokens beyond the table too (up to 2^31 -
- * 1), so that the calls above leave those out and keep what is cached.
+ * entries are -1.  A page that a row did not get is not given later, because
+ * the positions before in it are lost; it counts in every step whose tokens go
+ * to it, so that short_pages[0] is 0 only if every new token has its place.
+ * Lengths count tokens beyond the table too (up to 2^31 - 1), so that the
+ * calls above leave those out and keep what is cached.
  * Outputs may be the inputs.  workspace: qs_page_advance_workspace_bytes. */
 size_t qs_page_advance_workspace_bytes(int64_t rows);
 int qs_page_advance(const qs_page_store *store, const int32_t *table, const int32_t *lengths, const int32_t *refs,

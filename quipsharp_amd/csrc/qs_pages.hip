@@ -172,7 +172,7 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   __shared__ uint8_t shared_page[kMaxRows];
   __shared__ int part[kThreads / 64];
   __shared__ int copies;
-  __shared__ unsigned long long lost;  // pages in columns that the table does not have
+  __shared__ unsigned long long lost;  // pages in columns that the table does not have, and those missing since an earlier step
   const int tid = threadIdx.x;
   const int64_t room = (int64_t)a.cols * a.page;
   auto sync = [&]() {
@@ -237,7 +237,11 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
   if (tid < a.rows) {
     c0 = old_len / a.page, used = old_len % a.page;
     int p = -1;
-    if (tokens > 0 && used > 0) p = entry((int64_t)tid * a.cols + c0);
+    if (tokens > 0 && used > 0) {
+      p = entry((int64_t)tid * a.cols + c0);
+      // the positions before are lost, and a page now would have their places hold anything
+      if (p < 0) atomicAdd(&lost, 1ull);
+    }
     mine[tid] = p >= 0 && ref_at(p) > 1 ? p : -1;
   }
   __syncthreads();

@@ -260,7 +260,10 @@ def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, toke
     out by row, then by column.  Returns ``(table, lengths, refs, short)``;
     ``short`` (int32, 1; at most 2^31 - 1) is the number of pages that were
     wanted and could not be given, because none is free or the table has no
-    column left: their entries are -1.  With ``over`` (int32, rows; written)
+    column left: their entries are -1.  A page that a row did not get is not
+    given later (the positions before in it are lost); it counts in every step
+    whose tokens go to it, so that 0 says that every new token has its place.
+    With ``over`` (int32, rows; written)
     lengths stop at the table's room and ``over`` gets how many of a row's new
     tokens lie beyond it, which are gone with the next step."""
     store, dev = _store(kv), kv.device

@@ -149,3 +149,30 @@ def test_lengths_beyond_the_table(dev, dim, cols, window, sinks, far):
     got = attend_chunk(q.to(dev), *args, ints([0, new], dev), window=window, sinks=sinks).cpu()
     for i in range(new):
         near(got[i], q[i], rk, rv, seen(n - new + i), dim)
+
+
+def test_pages_that_are_missing_are_counted_in_every_step(dev):
+    """A token that goes to a page which its row did not get is counted as the one that should have opened it."""
+    cache = filled([16, 16], dev, pages=2)
+    for step in range(3):
+        cache.advance(1)
+        assert cache.short.item() == 2, step
+    assert cache.table.tolist() == [[0, -1, -1], [1, -1, -1]]
+    cache.free(torch.tensor([True, False], device=dev))
+    cache.advance(ints([1, 0], dev))  # positions before it in its page are lost: a page now would not bring them back
+    assert cache.short.item() == 1 and cache.table[0].tolist() == [0, -1, -1]
+    cache.advance(ints([0, 0], dev))
+    assert cache.short.item() == 0
+    cache.advance(ints([12, 0], dev))
+    assert cache.short.item() == 1 and cache.lengths.tolist() == [32, 0]
+    cache.advance(ints([1, 0], dev))
+    assert cache.short.item() == 0 and cache.table[0].tolist() == [0, -1, 1]
+
+
+def test_a_copy_that_gets_no_page_is_counted_in_every_step(dev):
+    """So is the page that a row lost because there was none for its copy."""
+    cache = filled([20, 0], dev, pages=2, parents=[0, 0])
+    for step in range(2):
+        cache.advance(1)
+        assert cache.short.item() == 1, step
+        assert cache.table.tolist() == [[0, 1, -1], [0, -1, -1]]
