@@ -426,7 +426,9 @@ int qs_page_append_over(const void *k, const void *v, int64_t tokens, int64_t ro
 /* qs_dec_qk_norm_rope for a paged cache, one token per row, each at its own
  * position lengths[r] - 1 (the row of the cos / sin tables, of table_rows
  * rows, too): q and k heads get their norm and the rotary embedding, q into
- * q_out, k and v into the pages.  bf16, head_dim 128; the same bits. */
+ * q_out, k and v into the pages.  A row whose position is below 0 or beyond
+ * the tables gets zero queries and stores nothing.  bf16, head_dim 128; the
+ * same bits. */
 int qs_page_append_rope(const void *q, const void *k, const void *v, const void *q_norm_w, const void *k_norm_w,
                         const void *cos_table, const void *sin_table, int64_t table_rows, void *q_out, int64_t rows,
                         int nh, int nkv, int head_dim, const qs_page_pool *pool, float eps, qs_stream_t stream);

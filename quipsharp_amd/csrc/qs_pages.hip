@@ -540,14 +540,15 @@ __global__ __launch_bounds__(256) void page_append_rope_kernel(const uint16_t* q
   const int b = blockIdx.x, hh = blockIdx.y * 4 + (threadIdx.x >> 6), l = threadIdx.x & 63;
   if (hh >= nh + 2 * nkv) return;
   const int64_t pos = row_end(pool, over, b) - 1;
+  // a row without tokens, or a position beyond the tables, has no rotation: its queries are zeros and nothing is stored
+  const bool inside = pos >= 0 && pos < table_rows, isq = hh < nh;
   if (hh >= nh + nkv) {
+    if (!inside) return;
     const int g = hh - nh - nkv;
     const uint16_t* src = v + ((int64_t)b * nkv + g) * 128;
     if (uint16_t* to = place(pool.v, pool.v_page, pool.v_head, pool.v_pos, pool, b, pos, g)) to[l] = src[l], to[l + 64] = src[l + 64];
     return;
   }
-  // a row without tokens, or a position beyond the tables, has no rotation: its queries are zeros and nothing is stored
-  const bool inside = pos >= 0 && pos < table_rows, isq = hh < nh;
   const int g = isq ? hh : hh - nh;
   uint16_t o0 = 0, o1 = 0;
   if (inside) {

@@ -176,3 +176,28 @@ def test_a_copy_that_gets_no_page_is_counted_in_every_step(dev):
         cache.advance(1)
         assert cache.short.item() == 1, step
         assert cache.table.tolist() == [[0, 1, -1], [0, -1, -1]]
+
+
+def test_append_rope_stores_no_half_of_a_position(dev):
+    """A row without tokens and a position beyond the rotary tables: zero queries, and the pools as they were."""
+    from quipsharp_amd import _lib
+    from quipsharp_amd.pages import _pool
+    L = _lib.lib()
+    rows, nh, nkv = 3, 4, 2
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(rows, h * 128, generator=g).to(BF).to(dev) for h in (nh, nkv, nkv))
+    qw, kw = (torch.ones(128, dtype=BF, device=dev) for _ in range(2))
+    cos, sin = (torch.randn(20, 128, generator=g).to(BF).to(dev) for _ in range(2))
+    pools = [torch.randn(9, nkv, PAGE, 128, generator=g).to(BF).to(dev) for _ in range(2)]
+    before = [p.clone() for p in pools]
+    table = ints([[4, 1, 2], [0, 3, 5], [6, 7, 8]], dev)
+    lengths = ints([0, 21, 20], dev)
+    qo = torch.full_like(q, 7)
+    _lib.check(L.qs_page_append_rope(*(t.data_ptr() for t in (q, k, v, qw, kw, cos, sin)), 20, qo.data_ptr(), rows, nh,
+                                     nkv, 128, _pool(*pools, table, lengths), 1e-6, _lib.stream_of(q)))
+    assert (qo[:2] == 0).all() and (qo[2] != 7).any()
+    assert not torch.equal(pools[0][7, :, 3], before[0][7, :, 3])
+    assert torch.equal(pools[1][7, :, 3], v[2].view(nkv, 128))
+    for pool, old in zip(pools, before):
+        pool[7, :, 3] = old[7, :, 3]
+        assert torch.equal(pool, old)
