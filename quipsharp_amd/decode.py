@@ -301,10 +301,10 @@ class PagedDecoder(StaticDecoder):
 
     def __init__(self, model, rows, max_len, page=64, pages=None, window=0, sinks=0):
         from .pages import PagedCache
-        super().__init__(model, rows, max_len, cache=False)
+        columns = -(-max_len // page)
+        super().__init__(model, rows, columns * page, cache=False)  # rotary tables to the last page's end
         if not self.fused_ok:
             raise ValueError("the paged decode step takes head_dim 128 and at most 16 query heads per kv head")
-        columns = -(-max_len // page)
         self.window, self.sinks = window, sinks
         self.cache = PagedCache(len(self.layers), rows * columns if pages is None else pages, self.nkv, self.hd, rows,
                                 columns, page, torch.bfloat16, self.dev)

@@ -117,3 +117,21 @@ def test_one_beam_is_greedy(model, dev):
     for i in range(12):
         assert tokens[0, 0, i] == last[0]
         last = dec.step(last).argmax(-1)
+
+
+def test_the_last_page_of_a_row_is_whole(model, dev):
+    """max_len ends inside a page: the positions up to the page's end work like the others, and a step beyond them is
+    counted."""
+    from quipsharp_amd.decode import PagedDecoder
+    dec = PagedDecoder(model, 2, 20, page=16)
+    rows = [ids_of(17, 13, dev), ids_of(9, 14, dev)]
+    dec.prompt(torch.cat(rows), [17, 9])
+    for step in range(15):
+        new = ids_of(2, 200 + step, dev)
+        got = dec.step(new)
+        rows = [torch.cat([t, new[r:r + 1]]) for r, t in enumerate(rows)]
+        for r in range(2):
+            near(got[r], whole(model, rows[r])[-1])
+    assert dec.cache.short.item() == 0 and dec.cache.lengths.tolist() == [32, 24]
+    dec.step(ids_of(2, 300, dev))
+    assert dec.cache.short.item() == 1
