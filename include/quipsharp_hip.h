@@ -513,12 +513,15 @@ int qs_page_advance_rows(const qs_page_store *store, const int32_t *table, const
                          int32_t *table_out, int32_t *lengths_out, int32_t *refs_out, int32_t *short_pages,
                          void *workspace, size_t workspace_bytes, qs_stream_t stream);
 /* The same with lengths cut to the table's room, and over [rows] set to how
- * many of a row's new tokens lie beyond it; those are gone with the next step.
- * over NULL: as qs_page_advance_rows. */
+ * many of a row's new tokens lie beyond it; those are gone with the next step
+ * (over NULL: as qs_page_advance_rows).  short_pages[0] is added to missing[0]
+ * (at most 2^31 - 1; NULL: to nothing), which a caller can look at after many
+ * steps. */
 int qs_page_advance_over(const qs_page_store *store, const int32_t *table, const int32_t *lengths, const int32_t *refs,
                          const int32_t *parents, int64_t rows, int64_t cols, int tokens, const int32_t *row_tokens,
                          int32_t *table_out, int32_t *lengths_out, int32_t *refs_out, int32_t *short_pages,
-                         int32_t *over, void *workspace, size_t workspace_bytes, qs_stream_t stream);
+                         int32_t *over, int32_t *missing, void *workspace, size_t workspace_bytes,
+                         qs_stream_t stream);
 
 /* Gives pages back: all of the rows with keep[i] == 0 (their length becomes
  * 0; keep may be NULL), and with a window the pages that no token at position

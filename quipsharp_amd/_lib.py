@@ -128,7 +128,7 @@ _SIGNATURES = {
                          _vp], _int),
     "qs_page_advance_rows": ([_store_p, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, _vp,
                               ctypes.c_size_t, _vp], _int),
-    "qs_page_advance_over": ([_store_p, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+    "qs_page_advance_over": ([_store_p, _vp, _vp, _vp, _vp, _i64, _i64, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                               ctypes.c_size_t, _vp], _int),
     "qs_page_free": ([_vp, _vp, _vp, _vp, _i64, _i64, _i64, _int, _int, _int, _vp, _vp, _vp, _vp], _int),
     "qs_page_compact_workspace_bytes": ([_i64], ctypes.c_size_t),

@@ -157,7 +157,8 @@ struct AdvanceArgs {
   const int32_t *table, *lengths, *refs, *parents;
   const int32_t* row_tokens;  // per row, or null: `tokens` for all
   int32_t *table_out, *lengths_out, *refs_out, *short_pages, *plan;
-  int32_t* over;  // per row, or null: lengths go on beyond the table
+  int32_t* over;     // per row, or null: lengths go on beyond the table
+  int32_t* missing;  // the sum of short_pages over the steps, or null
   int rows, cols, pages, page, tokens;
 };
 
@@ -333,6 +334,10 @@ __global__ __launch_bounds__(kThreads) void page_advance_kernel(AdvanceArgs a) {
     a.plan[0] = copies;
     const unsigned long long missing = lost + (total > found ? total - found : 0);
     a.short_pages[0] = missing < INT32_MAX ? (int)missing : INT32_MAX;
+    if (a.missing) {
+      const unsigned long long sum = missing + (a.missing[0] < 0 ? 0 : a.missing[0]);
+      a.missing[0] = sum < INT32_MAX ? (int)sum : INT32_MAX;
+    }
   }
 }
 
@@ -679,14 +684,14 @@ extern "C" int qs_page_advance_rows(const qs_page_store* store, const int32_t* t
                                     int32_t* refs_out, int32_t* short_pages, void* workspace, size_t workspace_bytes,
                                     qs_stream_t stream) {
   return qs_page_advance_over(store, table, lengths, refs, parents, rows, cols, tokens, row_tokens, table_out, lengths_out,
-                              refs_out, short_pages, nullptr, workspace, workspace_bytes, stream);
+                              refs_out, short_pages, nullptr, nullptr, workspace, workspace_bytes, stream);
 }
 
 extern "C" int qs_page_advance_over(const qs_page_store* store, const int32_t* table, const int32_t* lengths,
                                     const int32_t* refs, const int32_t* parents, int64_t rows, int64_t cols, int tokens,
                                     const int32_t* row_tokens, int32_t* table_out, int32_t* lengths_out,
-                                    int32_t* refs_out, int32_t* short_pages, int32_t* over, void* workspace,
-                                    size_t workspace_bytes, qs_stream_t stream) {
+                                    int32_t* refs_out, int32_t* short_pages, int32_t* over, int32_t* missing,
+                                    void* workspace, size_t workspace_bytes, qs_stream_t stream) {
   Store st;
   if (const int rc = store_checks("qs_page_advance", store, st)) return rc;
   if (const int rc = table_checks("qs_page_advance", rows, cols, st.pages, st.page)) return rc;
@@ -699,7 +704,7 @@ extern "C" int qs_page_advance_over(const qs_page_store* store, const int32_t* t
              qs_page_advance_workspace_bytes(rows));
   int32_t* plan = static_cast<int32_t*>(workspace);
   const AdvanceArgs a{table, lengths, refs, parents, row_tokens, table_out, lengths_out, refs_out, short_pages, plan,
-                      over, (int)rows, (int)cols, (int)st.pages, st.page, tokens};
+                      over, missing, (int)rows, (int)cols, (int)st.pages, st.page, tokens};
   if (st.pages <= kNearPages && rows * cols <= kTileInts) hipLaunchKernelGGL(page_advance_kernel<true>, dim3(1), dim3(kThreads), 0, as_stream(stream), a);
   else hipLaunchKernelGGL(page_advance_kernel<false>, dim3(1), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("page_advance_kernel");

@@ -297,7 +297,11 @@ class PagedDecoder(StaticDecoder):
     (beam search) and, with ``window``, streams far longer than what is kept
     visible (the last ``window`` positions and the first ``sinks``; pages that
     fell out are given back).  Everything that a step needs to know of its rows
-    lies on the GPU, so a step can be captured once and replayed."""
+    lies on the GPU, so a step can be captured once and replayed.
+
+    Rows of at most ``max_len`` positions (rounded up to whole pages).  A step
+    that runs out of pages or of positions leaves tokens out; it does not wait
+    to say so, ``cache.check()`` and the next ``prompt`` raise for it."""
 
     def __init__(self, model, rows, max_len, page=64, pages=None, window=0, sinks=0):
         from .pages import PagedCache
@@ -325,6 +329,7 @@ class PagedDecoder(StaticDecoder):
         last = (count.cumsum(0) - 1)[count > 0].to(self.dev)
         row = torch.repeat_interleave(torch.arange(self.B), count).to(self.dev)
         cache.advance(count.to(self.dev))
+        cache.check()
         pos = (cache.lengths + cache.over)[row] - starts[row + 1] + torch.arange(T, device=self.dev)
         h = m.embed_tokens(ids)[None]
         cos, sin = m.rotary_emb(h, pos[None])
@@ -427,9 +432,7 @@ def beam_decode(model, prompts, beams, new_tokens, eos=-1, use_graph=True, page=
         go()
     torch.cuda.synchronize()
     t2 = time.perf_counter()
-    short = dec.cache.short.item()
-    if short:
-        raise RuntimeError(f"the cache is short of {short} pages")
+    dec.cache.check()
     return tokens.view(R, beams, new_tokens).long(), scores, t1 - t0, t2 - t1
 
 

@@ -247,7 +247,7 @@ def _books(table, lengths, refs, pages, device):
 
 
 def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, tokens=1, parents: Tensor = None, *,
-                  out=None, over: Tensor = None, workspace: Tensor = None):
+                  out=None, over: Tensor = None, missing: Tensor = None, workspace: Tensor = None):
     """One step of every row of a cache ``kv`` (..., pages, kv heads, page,
     head dim): row i takes the pages and the length of row ``parents[i]``
     (int32; None: its own; no row of the table: an empty one), gives back pages
@@ -265,7 +265,8 @@ def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, toke
     whose tokens go to it, so that 0 says that every new token has its place.
     With ``over`` (int32, rows; written)
     lengths stop at the table's room and ``over`` gets how many of a row's new
-    tokens lie beyond it, which are gone with the next step."""
+    tokens lie beyond it, which are gone with the next step.  ``missing``
+    (int32, 1) gets ``short`` added to it."""
     store, dev = _store(kv), kv.device
     _books(table, lengths, refs, store.pages, dev)
     rows, cols = table.shape
@@ -285,13 +286,15 @@ def advance_pages(kv: Tensor, table: Tensor, lengths: Tensor, refs: Tensor, toke
         _int32("out[3]", out[3], (1,), dev)
     if over is not None:
         _int32("over", over, (rows,), dev)
+    if missing is not None:
+        _int32("missing", missing, (1,), dev)
     _lib.require_gpu(kv, what="advance_pages")
     L = _lib.lib()
     workspace = _workspace(workspace, L.qs_page_advance_workspace_bytes(rows), dev)
     _lib.check(L.qs_page_advance_over(store, table.data_ptr(), lengths.data_ptr(), refs.data_ptr(), _lib.ptr(parents),
                                       rows, cols, tokens, _lib.ptr(each), out[0].data_ptr(), out[1].data_ptr(),
-                                      out[2].data_ptr(), out[3].data_ptr(), _lib.ptr(over), *_room(workspace),
-                                      _lib.stream_of(kv)))
+                                      out[2].data_ptr(), out[3].data_ptr(), _lib.ptr(over), _lib.ptr(missing),
+                                      *_room(workspace), _lib.stream_of(kv)))
     return tuple(out)
 
 
@@ -355,7 +358,8 @@ class PagedCache:
     head dim) with the table, lengths and reference counts of ``rows`` rows of
     at most ``columns`` pages.  The methods work in place.  ``lengths`` stop at
     the table's room; ``over`` has how many of a row's newest tokens lie beyond,
-    which no page holds and no token sees."""
+    which no page holds and no token sees.  ``missing`` counts the pages that
+    any ``advance`` could not give."""
 
     def __init__(self, layers, pages, kv_heads, head_dim, rows, columns, page=64, dtype=torch.bfloat16, device="cuda"):
         self.page = page
@@ -366,6 +370,7 @@ class PagedCache:
         self.refs = torch.zeros(pages, dtype=torch.int32, device=dev)
         self.over = torch.zeros(rows, dtype=torch.int32, device=dev)
         self.short = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.missing = torch.zeros(1, dtype=torch.int32, device=dev)
 
     def keys(self, layer):
         return self.kv[layer, 0]
@@ -374,9 +379,16 @@ class PagedCache:
         return self.kv[layer, 1]
 
     def advance(self, tokens=1, parents=None):
-        """``advance_pages``; ``self.short`` gets the pages that were missing."""
+        """``advance_pages``; ``self.short`` gets the pages that were missing, ``self.missing`` their sum so far."""
         advance_pages(self.kv, self.table, self.lengths, self.refs, tokens, parents,
-                      out=(self.table, self.lengths, self.refs, self.short), over=self.over)
+                      out=(self.table, self.lengths, self.refs, self.short), over=self.over, missing=self.missing)
+
+    def check(self):
+        """Raise if an ``advance`` so far, captured ones that were replayed among them, had not all the pages that it
+        wanted: tokens have been left out since.  Waits for the GPU; ``missing.zero_()`` starts anew."""
+        missing = self.missing.item()
+        if missing:
+            raise RuntimeError(f"the cache was short of {missing} pages: tokens were left out")
 
     def free(self, keep=None, window=0, sinks=0):
         free_pages(self.table, self.lengths, self.refs, page=self.page, keep=keep, window=window, sinks=sinks,

@@ -201,3 +201,30 @@ def test_append_rope_stores_no_half_of_a_position(dev):
     for pool, old in zip(pools, before):
         pool[7, :, 3] = old[7, :, 3]
         assert torch.equal(pool, old)
+
+
+@pytest.mark.parametrize("rows", [4, 64])
+def test_the_sum_of_missing_pages(dev, rows):
+    """It adds up over the steps, also over replayed ones, and stays at the largest int32."""
+    from quipsharp_amd.pages import PagedCache
+    cache = PagedCache(1, 4, 1, 64, rows, 2, page=16, device=dev)
+    want = 0
+    for tokens in (1, 16, 0, 40, 1):
+        cache.advance(tokens)
+        want += cache.short.item()
+        assert cache.missing.item() == want
+    assert want > 0
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cache.advance(1)
+    for _ in range(3):
+        graph.replay()
+        want += cache.short.item()
+        assert cache.short.item() == rows and cache.missing.item() == want
+    cache.advance(1 << 30)
+    cache.advance(1 << 30)
+    assert cache.missing.item() == min(want + 2 * rows * 2 ** 26, 2 ** 31 - 1)
+    with pytest.raises(RuntimeError, match="left out"):
+        cache.check()
+    cache.missing.zero_()
+    cache.check()

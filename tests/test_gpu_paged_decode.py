@@ -135,3 +135,41 @@ def test_the_last_page_of_a_row_is_whole(model, dev):
     assert dec.cache.short.item() == 0 and dec.cache.lengths.tolist() == [32, 24]
     dec.step(ids_of(2, 300, dev))
     assert dec.cache.short.item() == 1
+
+
+def test_a_short_cache_is_told(model, dev):
+    """A prompt that gets no room raises; a step that gets none is told by the next check or prompt, also where later
+    steps had all that they asked for."""
+    from quipsharp_amd.decode import PagedDecoder
+    with pytest.raises(RuntimeError, match="short of 2 pages"):
+        PagedDecoder(model, 2, 64, page=16, pages=3).prompt(ids_of(50, 15, dev), [33, 17])
+    with pytest.raises(RuntimeError, match="short of 1 pages"):
+        PagedDecoder(model, 2, 32, page=16).prompt(ids_of(50, 15, dev), [33, 17])
+    dec = PagedDecoder(model, 2, 64, page=16, pages=3)
+    dec.prompt(ids_of(31, 16, dev), [16, 15])
+    dec.cache.check()
+    for step in range(2):  # row 1 fills its page, then wants one that row 0 took
+        dec.step(ids_of(2, 400 + step, dev))
+    dec.cache.free(torch.tensor([True, False], device=dev))
+    dec.cache.advance(0)
+    assert dec.cache.short.item() == 0 and dec.cache.missing.item() == 1
+    with pytest.raises(RuntimeError, match="short of 1 pages"):
+        dec.cache.check()
+    with pytest.raises(RuntimeError, match="short of 1 pages"):
+        dec.prompt(ids_of(3, 17, dev), [0, 3])
+    dec.cache.missing.zero_()
+    dec.prompt(ids_of(3, 17, dev), [0, 3])
+
+
+@pytest.mark.parametrize("use_graph", [False, True])
+def test_beam_search_tells_a_shortage_of_any_step(model, dev, use_graph, monkeypatch):
+    """The first step has no page for the second beam's copy; the others ask for none."""
+    from quipsharp_amd import decode
+
+    class Fewer(decode.PagedDecoder):
+        def __init__(self, model, rows, max_len, page, pages):
+            super().__init__(model, rows, max_len, page, 2)
+
+    monkeypatch.setattr(decode, "PagedDecoder", Fewer)
+    with pytest.raises(RuntimeError, match="short of"):
+        decode.beam_decode(model, [ids_of(19, 18, dev)], 2, 8, use_graph=use_graph, page=16)

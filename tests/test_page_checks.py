@@ -267,3 +267,11 @@ def test_tokens_over_the_table_refuse(over, message):
                  lambda: advance_pages(*books(), over=over)):
         with pytest.raises(ValueError, match=message):
             call()
+
+
+def test_the_count_of_missing_pages_refuses():
+    for missing in (torch.zeros(2, dtype=I32), torch.zeros(1, dtype=torch.int64)):
+        with pytest.raises(ValueError, match="missing must be"):
+            advance_pages(*books(), missing=missing)
+    with pytest.raises(ValueError, match="missing is on"):
+        advance_pages(*books(), missing=torch.zeros(1, dtype=I32, device="meta"))
