@@ -6,6 +6,13 @@
 // needs (the running maximum and sum) and each slice's best `keep`; the
 // second launch adds the slices' sums and chooses among the slices' bests by
 // the score in fp64.
+//
+// Exponentials are fp32, sixteen of them are added by pairs in fp32, and all
+// else is fp64.  With units of 2^-24: a term D below the largest logit is off
+// by 2 D + 4 (twice a difference, a product with log2(e) and an exponential:
+// to its slice's largest and from there to the beam's), which over a softmax
+// of `vocab` terms, whose mean D is ln(vocab) at most, makes 2 ln(vocab) + 4,
+// and the pairs 4: a log sum is right to 32 units (2e-6) for 151936 tokens.
 #include <type_traits>
 
 #include "qs_chunk_dev.h"
@@ -37,12 +44,18 @@ __device__ __forceinline__ double order_double(uint64_t u) {
   return __builtin_bit_cast(double, u >> 63 ? u & ~(1ull << 63) : ~u);
 }
 
+// Of a slice: its largest logit, and the sum of the exponentials below it.
+struct Stat {
+  double sum;
+  float top;
+};
+
 struct SelectArgs {
   const void* logits;
   int64_t ld;
   const float* scores;
   const uint8_t* finished;
-  float *stats;    // [rows][slices][2]: maximum, sum
+  Stat* stats;     // [rows][slices]
   uint64_t* best;  // [rows][slices][keep]: order bits << 32 | ~token, in descending order; 0 for none
   float* scores_out;
   int32_t *parents_out, *tokens_out;
@@ -55,6 +68,21 @@ struct SelectArgs {
 __device__ __forceinline__ float exp_below(float x, float m) {
   const float d = x - (m == -INFINITY ? 0.f : m);
   return __builtin_amdgcn_exp2f(__builtin_fmaf(d, 1.44269502f, d * 1.92596299e-8f));
+}
+
+__device__ __forceinline__ double wave_sum64(double v, LaneX lx) {
+  auto add = [&](auto other) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __float_as_uint(other(__uint_as_float((uint32_t)u))), hi = __float_as_uint(other(__uint_as_float((uint32_t)(u >> 32))));
+    v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+  };
+  add([&](float x) { return lane_xor<32>(x, lx); });
+  add([&](float x) { return lane_xor<16>(x, lx); });
+  add([&](float x) { return lane_xor<8>(x, lx); });
+  add([&](float x) { return lane_xor<4>(x, lx); });
+  add([&](float x) { return lane_xor<2>(x, lx); });
+  add([&](float x) { return lane_xor<1>(x, lx); });
+  return v;
 }
 
 // The largest u such that at least n lanes (1 .. 64) have a key of u or more.
@@ -127,7 +155,8 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
   typedef Slice<T, WIDE, E> S;
   __shared__ uint64_t room[kRoom];
   __shared__ float tops[kThreads];
-  __shared__ float red[4][4];
+  __shared__ float red[3][4];
+  __shared__ double sums[4];
   __shared__ float line;
   __shared__ int count;
   const LaneX lx = lane_x_init();
@@ -150,12 +179,12 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
   const float edge_w = keep <= 32 ? order_float(nth_key(order_bits(m), keep)) : -INFINITY;
   const float part_w = keep <= 32 && keep > 8 ? order_float(nth_key(order_bits(m), (keep + 3) / 4)) : -INFINITY;
   tops[tid] = m;
-  if (lane == 0) red[0][w] = top, red[1][w] = edge_w, red[3][w] = part_w;
+  if (lane == 0) red[0][w] = top, red[1][w] = edge_w, red[2][w] = part_w;
   if (tid == 0) count = 0;
   __syncthreads();
   const float all = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
   float edge = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
-  edge = fmaxf(edge, fminf(fminf(red[3][0], red[3][1]), fminf(red[3][2], red[3][3])));
+  edge = fmaxf(edge, fminf(fminf(red[2][0], red[2][1]), fminf(red[2][2], red[2][3])));
   auto threads_edge = [&]() {
     int above = 0, same = 0;
     for (int i = 0; i < kThreads; ++i) above += tops[i] > m, same += tops[i] == m;
@@ -164,18 +193,22 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
     return line;
   };
   if (keep > 32) edge = threads_edge();
-  float sum = 0.f;
+  double sum = 0.0;
   if (all < INFINITY) {
 #pragma unroll
     for (int p = 0; p < E; p += 16) {
-      float part = 0.f;
+      float part[16];
 #pragma unroll
-      for (int i = p; i < p + 16; ++i) part += exp_below(s.x[i], all);
-      sum += part;
+      for (int i = 0; i < 16; ++i) part[i] = exp_below(s.x[p + i], all);
+#pragma unroll
+      for (int n = 8; n > 0; n /= 2)
+#pragma unroll
+        for (int i = 0; i < n; ++i) part[i] += part[i + n];
+      sum += part[0];
     }
   }
-  sum = wave_sum(sum, lx);
-  if (lane == 0) red[2][w] = sum;
+  sum = wave_sum64(sum, lx);
+  if (lane == 0) sums[w] = sum;
   auto add = [&](int i) {
     const int at = atomicAdd(&count, 1);
     if (at < kRoom) room[at] = (uint64_t)order_bits(s.x[i]) << 32 | (uint32_t)~S::token(t0, i);
@@ -218,8 +251,7 @@ __global__ __launch_bounds__(kThreads) void beam_slice_kernel(SelectArgs a) {
   }
   for (int c = n + tid; c < keep; c += kThreads) best[c] = 0;
   if (tid == 0) {
-    float* st = a.stats + 2 * (row * a.slices + slice);
-    st[0] = all, st[1] = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+    a.stats[row * a.slices + slice] = Stat{(sums[0] + sums[1]) + (sums[2] + sums[3]), all};
   }
 }
 
@@ -234,8 +266,8 @@ __device__ __forceinline__ bool over(const Candidate& x, const Candidate& y) {
 // One work-group per request.
 __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidate* spill) {
   constexpr int kList = 512, kAhead = 4, kMore = 4;
-  __shared__ double base[1024];  // the sum; then score - log sum, of a beam without continuations -inf
-  __shared__ float largest[1024];
+  __shared__ double base[1024];    // the sum; then the log sum, of a finished beam its score
+  __shared__ float largest[1024];  // the largest logit; then the score
   __shared__ uint8_t state[1024];
   __shared__ Candidate list[kList];
   __shared__ Candidate tops[kJoin], line;
@@ -265,23 +297,23 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidat
   }
   for (int j = w; j < a.beams; j += kJoin / 64) {
     // lane i: slices i, i + 64 ..
-    const float2* st = reinterpret_cast<const float2*>(a.stats) + (b * a.beams + j) * a.slices;
-    float m = -INFINITY, l = 0.f;
-    for (int i = lane; i < a.slices; i += 64) {
-      const float2 x = st[i];
-      const float up = fmaxf(m, x.x);
-      l = l * exp_below(m, up) + x.y * exp_below(x.x, up);
-      m = up;
-    }
-    float top = m;
+    const Stat* st = a.stats + (b * a.beams + j) * a.slices;
+    const Stat own = lane < a.slices ? st[lane] : Stat{0.0, -INFINITY};
+    float top = own.top;
+    for (int i = lane + 64; i < a.slices; i += 64) top = fmaxf(top, st[i].top);
     top = fmaxf(top, lane_xor<32>(top, lx));
     top = fmaxf(top, lane_xor<16>(top, lx));
     top = fmaxf(top, lane_xor<8>(top, lx));
     top = fmaxf(top, lane_xor<4>(top, lx));
     top = fmaxf(top, lane_xor<2>(top, lx));
     top = fmaxf(top, lane_xor<1>(top, lx));
-    const float sum = wave_sum(fabsf(top) < INFINITY ? l * exp_below(m, top) : 0.f, lx);
-    if (lane == 0) base[j] = sum, largest[j] = top;
+    double l = 0.0;
+    if (fabsf(top) < INFINITY) {
+      l = own.sum * exp_below(own.top, top);
+      for (int i = lane + 64; i < a.slices; i += 64) l += st[i].sum * exp_below(st[i].top, top);
+    }
+    l = wave_sum64(l, lx);
+    if (lane == 0) base[j] = l, largest[j] = top;
   }
   if (tid == 0) count = 0, edge = 0;
   __syncthreads();
@@ -289,10 +321,9 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidat
     const int64_t row = b * a.beams + j;
     const bool done = a.finished && a.finished[row];
     const float s = a.scores[row], top = largest[j];
-    double c = -INFINITY;
-    if (fabsf(s) < INFINITY && done) c = s;
-    else if (fabsf(s) < INFINITY && fabsf(top) < INFINITY) c = (double)s - ((double)top + log(base[j]));
-    base[j] = c, state[j] = done ? 1 : c == -INFINITY ? 2 : 0;
+    const bool fine = fabsf(s) < INFINITY, runs = !done && fine && fabsf(top) < INFINITY;
+    base[j] = runs ? (double)top + log(base[j]) : fine ? s : -INFINITY;
+    largest[j] = s, state[j] = runs ? 0 : done ? 1 : 2;
   }
   __syncthreads();
   // a beam offers slices * keep candidates; one that is finished or has none keep + 1: eos and the first tokens
@@ -302,7 +333,7 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidat
     if (state[j] == 0) {
       if (!k) return Candidate{0, 0};
       t = (uint32_t)~k;
-      v = base[j] + (double)order_float((uint32_t)(k >> 32));
+      v = largest[j] + ((double)order_float((uint32_t)(k >> 32)) - base[j]);  // in this order: equal continuations tie
     } else {
       const bool has = state[j] == 1 && a.eos >= 0 && a.eos < a.vocab;
       if (i > a.keep || (i == a.keep && !has)) return Candidate{0, 0};
@@ -467,7 +498,7 @@ Layout layout_of(int64_t batch, int beams, int64_t vocab, int keep) {
   const int64_t per = (int64_t)l.slices * keep > keep + 1 ? (int64_t)l.slices * keep : keep + 1;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   l.stats = 0;
-  l.best = up((size_t)rows * l.slices * 2 * sizeof(float));
+  l.best = up((size_t)rows * l.slices * sizeof(Stat));
   l.spill = l.best + up((size_t)rows * l.slices * keep * sizeof(uint64_t));
   l.bytes = l.spill + up((size_t)rows * per * sizeof(Candidate));
   return l;
@@ -540,7 +571,7 @@ extern "C" int qs_beam_select(const void* logits, int dtype, int64_t ld, int64_t
   QS_REQUIRE(workspace && workspace_bytes >= l.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
              "qs_beam_select: workspace of %zu bytes (16-byte aligned), %zu needed", workspace_bytes, l.bytes);
   char* ws = static_cast<char*>(workspace);
-  const SelectArgs a{logits, ld, scores, finished, reinterpret_cast<float*>(ws + l.stats),
+  const SelectArgs a{logits, ld, scores, finished, reinterpret_cast<Stat*>(ws + l.stats),
                      reinterpret_cast<uint64_t*>(ws + l.best), scores_out, parents_out, tokens_out, eos, beams,
                      (int)vocab, keep, l.slices, dtype};
   const size_t size = dtype == QS_DTYPE_F32 ? 4 : 2;

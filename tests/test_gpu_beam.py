@@ -221,3 +221,36 @@ def test_far_more_above_the_edge_than_room(dev, kind, keep, dtype):
     logits = x.repeat(rows, 1)
     logits[1::2, 100] = 9.5
     check(dev, logits.to(dtype), -(torch.arange(rows) % 5).float().view(100, 3), keep)
+
+
+def small_beside_one(at, vocab=12288, small=4096):
+    """A logit of 0 at `at` and others whose exponentials are 0.95 of half an fp32 step of its, at the other tokens below
+    `small`; the rest are nothing beside them."""
+    x = torch.full((vocab,), -1e4)
+    x[:small] = math.log(0.95 * 2.0 ** -24)
+    x[at] = 0
+    return x
+
+
+def test_terms_below_half_a_step_of_the_largest_count(dev):
+    """4095 of them make 3890 units (2^-24) of the sum.  A sum of 16 exponentials by pairs is off by 4 units at most
+    (4 additions), the sums of those are 64-bit, and a relative error of 40 units in 4095 terms of 2^-24 is nothing:
+    5 units for the logarithm and the rounding of a score near 0."""
+    from quipsharp_amd.beam import beam_select
+    for at in (0, 1, 700, 3075, 4095):
+        logits = torch.stack([small_beside_one(at)] * 2)
+        scores = torch.zeros(1, 2)
+        want = select(logits, scores, 2, None, -1)
+        got = beam_select(logits.to(dev), scores.to(dev), 2)
+        assert torch.equal(got[1].cpu().long(), want[1]) and torch.equal(got[2].cpu().long(), want[2])
+        assert ((got[0].cpu().double() - want[0]).abs() <= 5 * 2.0 ** -24).all(), at
+
+
+def test_beams_with_the_same_logits_in_another_order(dev):
+    """Two beams of one sum, the second 12 units ahead by its score: more than twice what a sum is off by, so it comes
+    first, wherever the beams have their largest logit."""
+    from quipsharp_amd.beam import beam_select
+    for first, second in ((0, 3075), (3075, 0), (4095, 1), (1, 2048)):
+        logits = torch.stack([small_beside_one(first), small_beside_one(second)]).to(dev)
+        _, parents, tokens = beam_select(logits, torch.tensor([[0.0, 12 * 2.0 ** -24]], device=dev), 2)
+        assert parents.tolist() == [[1, 0]] and tokens.tolist() == [[second, first]]
