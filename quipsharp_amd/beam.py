@@ -1,6 +1,7 @@
 """Beam search over a quantized decoder's logits: the best continuations over
-beams and vocabulary, and the states that follow them.  No counterpart in the
-reference.  The computation runs in libquipsharp_hip.so (csrc/qs_beam.hip)."""
+beams and vocabulary, and the states that follow them.  Neither has a gradient:
+inputs that require one are refused where gradients are recorded.  No
+counterpart in the reference.  The computation runs in libquipsharp_hip.so (csrc/qs_beam.hip)."""
 import ctypes
 import math
 
@@ -59,6 +60,7 @@ def beam_select(logits: Tensor, scores: Tensor, keep: int = None, finished: Tens
     if keep < 1:
         raise ValueError(f"keep {keep} must be 1 or more")
     code = _lib.dtype_code(logits.dtype)
+    _lib.no_gradient(logits, scores, what="beam_select")
     _lib.require_gpu(logits, what="beam_select")
     best = scores.new_empty((batch, keep))
     parents, tokens = torch.empty_like(best, dtype=torch.int32), torch.empty_like(best, dtype=torch.int32)
@@ -91,6 +93,7 @@ def reorder_states(states, parents: Tensor):
         each = s.element_size()
         size.append((s.numel() // rows if rows else math.prod(shape[1:])) * each)
         stride.append(s.stride()[0] * each if rows > 1 else size[-1])
+    _lib.no_gradient(*states, what="reorder_states")
     _lib.require_gpu(*states, what="reorder_states")
     for s in states:
         out.append(torch.empty_like(s, memory_format=torch.contiguous_format) if n == rows

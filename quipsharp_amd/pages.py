@@ -18,7 +18,8 @@ table's room, and ``over`` has how many of the row's newest tokens lie beyond.
 
 The functions return new tables and leave their arguments as they are, unless
 ``out`` names the tensors to write, which may be the arguments themselves;
-the pool is changed in place.  ``PagedCache`` keeps the tensors together and
+the pool is changed in place.  None of them has a gradient: inputs that
+require one are refused where gradients are recorded.  ``PagedCache`` keeps the tensors together and
 works in place.
 """
 import ctypes
@@ -150,6 +151,7 @@ def append_pages(k_pages: Tensor, v_pages: Tensor, k: Tensor, v: Tensor, table: 
         _int32("starts", starts, (rows + 1,), dev)
     if over is not None:
         _int32("over", over, (rows,), dev)
+    _lib.no_gradient(k, v, k_pages, v_pages, what="append_pages")
     _lib.require_gpu(k_pages, what="append_pages")
     _lib.check(_lib.lib().qs_page_append_over(k.data_ptr(), v.data_ptr(), k.shape[0], rows, k.shape[1], dim, ks[0],
                                               ks[1], vs[0], vs[1], _lib.ptr(starts), pool, _lib.ptr(over),
@@ -189,6 +191,7 @@ def attend_token(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     if over is not None:
         _int32("over", over, (rows,), dev)
     out = _output(out, q)
+    _lib.no_gradient(q, k_pages, v_pages, what="attend_token")
     _lib.require_gpu(k_pages, what="attend_token")
     L, heads = _lib.lib(), q.shape[1]
     need = L.qs_attend_token_workspace_bytes(rows, heads, kv_heads, dim, cols, page, window, sinks)
@@ -218,6 +221,7 @@ def attend_chunk(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     if over is not None:
         _int32("over", over, (rows,), dev)
     out = _output(out, q)
+    _lib.no_gradient(q, k_pages, v_pages, what="attend_chunk")
     _lib.require_gpu(k_pages, what="attend_chunk")
     L, (tokens, heads, _) = _lib.lib(), q.shape
     need = L.qs_attend_chunk_workspace_bytes(tokens, rows, heads, kv_heads, dim, cols, page, window, sinks)

@@ -275,3 +275,24 @@ def test_the_count_of_missing_pages_refuses():
             advance_pages(*books(), missing=missing)
     with pytest.raises(ValueError, match="missing is on"):
         advance_pages(*books(), missing=torch.zeros(1, dtype=I32, device="meta"))
+
+
+def test_gradients_are_refused():
+    """An input that requires a gradient is refused where one would be recorded, and taken where none is."""
+    one = torch.tensor([0, 1, 2], dtype=I32)
+    grad = lambda *shape, dtype=BF: torch.zeros(*shape, dtype=dtype, requires_grad=True)  # noqa: E731
+    a, new = attention(), torch.zeros(2, 2, 128, dtype=BF)
+    calls = [lambda: attend_token(**attention(q=grad(2, 8, 128))),
+             lambda: attend_chunk(starts=one, **attention(q=grad(2, 8, 128))),
+             lambda: attend_token(**attention(v_pages=grad(5, 2, 32, 128))),
+             lambda: attend_chunk(starts=one, **attention(k_pages=grad(5, 2, 32, 128))),
+             lambda: append_pages(a["k_pages"], a["v_pages"], grad(2, 2, 128), new, a["table"], a["lengths"]),
+             lambda: append_pages(a["k_pages"], a["v_pages"], new, grad(2, 2, 128), a["table"], a["lengths"]),
+             lambda: beam_select(grad(6, 50, dtype=torch.float32), torch.zeros(2, 3)),
+             lambda: beam_select(torch.zeros(6, 50), grad(2, 3, dtype=torch.float32)),
+             lambda: reorder_states([torch.zeros(4, 6), grad(4, 6)], torch.zeros(3, dtype=I32))]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="has no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(RuntimeError, match="runs on the GPU"):
+            call()
