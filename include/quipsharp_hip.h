@@ -441,7 +441,8 @@ int qs_page_append_rope_over(const void *q, const void *k, const void *v, const 
  * row's pages: out[r][h * head_dim + d] = sum_p softmax_p(scale q_h . k_p)
  * v_p with kv head h / (heads / kv_heads), over the positions p <= lengths[r]
  * - 1 that are within the last `window` (0: all) or among the first `sinks`.
- * A row that sees nothing gets zeros.  scale: finite, not 0.  bf16 or fp16, head_dim 64, 128 or 256;
+ * A row that sees nothing gets zeros.  scale: not 0, finite times log2(e) in
+ * fp32.  bf16 or fp16, head_dim 64, 128 or 256;
  * scores, softmax and sums in fp32, weights in the cache's type.  q: strides
  * q_row, q_head; 16-byte aligned like out, whose rows are out_row apart. */
 size_t qs_attend_token_workspace_bytes(int64_t rows, int heads, int kv_heads, int head_dim, int64_t cols, int page,

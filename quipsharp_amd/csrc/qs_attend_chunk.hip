@@ -616,7 +616,7 @@ int launch_chunk(const PagePool& pp, const ChunkArgs& a, hipStream_t stream) {
 
 int page_pool_checks(const char* fn, const qs_page_pool* p, int dtype, int64_t rows, int heads, int kv_heads,
                      int head_dim, float scale, int window, int sinks, const int32_t* over, PagePool& out) {
-  QS_REQUIRE(std::isfinite(scale) && scale != 0.f, "%s: scale %g", fn, (double)scale);
+  QS_REQUIRE(std::isfinite(scale * kLog2E) && scale != 0.f, "%s: scale %g", fn, (double)scale);
   QS_SUPPORTED(dtype == QS_DTYPE_BF16 || dtype == QS_DTYPE_F16, "%s: dtype %d (bf16 and fp16 only)", fn, dtype);
   QS_SUPPORTED(head_dim == 64 || head_dim == 128 || head_dim == 256, "%s: head_dim %d (64, 128 or 256)", fn, head_dim);
   QS_REQUIRE(p && p->k && p->v && p->table && p->lengths, "%s: null pointer", fn);
@@ -693,7 +693,7 @@ extern "C" int qs_attend_chunk_over(const void* q, int dtype, int64_t tokens, in
              "qs_attend_chunk: workspace of %zu bytes (16-byte aligned), %zu needed", workspace_bytes, need);
   const int splits = workspace && need ? chunk_splits(tokens, rows, heads, kv_heads, pool->cols, pool->page, window, sinks) : 1;
   ChunkArgs a{static_cast<const uint16_t*>(q), q_token, q_head, static_cast<uint16_t*>(out), out_token, starts, (int)tokens,
-              (int)rows, heads, kv_heads, window, sinks, static_cast<float*>(workspace), splits, fabsf(scale) * 1.44269504088896340736f, scale < 0 ? 0x80008000u : 0u};
+              (int)rows, heads, kv_heads, window, sinks, static_cast<float*>(workspace), splits, fabsf(scale) * kLog2E, scale < 0 ? 0x80008000u : 0u};
   const bool bf = dtype == QS_DTYPE_BF16;
   const hipStream_t st = as_stream(stream);
   if (head_dim == 64) return bf ? launch_chunk<true, 64>(pp, a, st) : launch_chunk<false, 64>(pp, a, st);

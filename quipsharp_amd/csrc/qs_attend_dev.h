@@ -92,6 +92,8 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   }
 }
 
+constexpr float kLog2E = 1.44269504088896340736f;
+
 // The weight of a score that lies `below` the maximum; scale holds log2(e).
 // The difference is taken before the product, which could leave the range of
 // fp32 for scores near its end.

@@ -280,7 +280,7 @@ extern "C" int qs_attend_token_over(const void* q, int dtype, int64_t rows, int 
   const Shares sh = token_shares(rows, heads, kv_heads, pool->cols, pool->page, window, sinks);
   TokenArgs a{static_cast<const uint16_t*>(q), q_row, q_head, static_cast<uint16_t*>(out), out_row,
               static_cast<float*>(workspace), heads, kv_heads, sh.splits, window, sinks,
-              fabsf(scale) * 1.44269504088896340736f, scale < 0 ? 0x80008000u : 0u};
+              fabsf(scale) * kLog2E, scale < 0 ? 0x80008000u : 0u};
   // A layer's pages that exceed the chip's 256 MB cache are not found in it by
   // the next call, and values that go past it leave it to the keys: 311 us
   // with, 287 us without over 1.6 GB; where they fit, 26.4 and 27.4 us over

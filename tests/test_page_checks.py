@@ -296,3 +296,9 @@ def test_gradients_are_refused():
             call()
         with torch.no_grad(), pytest.raises(RuntimeError, match="runs on the GPU"):
             call()
+
+
+@pytest.mark.parametrize("scale", [2.5e38, -3.4e38])
+def test_scales_whose_product_with_log2_e_is_none(scale):
+    L = _lib.lib()
+    assert token(L, scale=scale) == 1 and b"scale" in L.qs_last_error()
