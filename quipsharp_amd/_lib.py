@@ -187,9 +187,9 @@ def require_gpu(*tensors, what="quipsharp_amd"):
             raise RuntimeError(f"{what} runs on the GPU (MI355X / gfx950); got a tensor on {t.device}")
 
 
-def no_gradient(*tensors, what):
-    """A call that records nothing for autograd refuses tensors whose gradients it would lose."""
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+def no_gradient(what):
+    """A call that records nothing for autograd, and was given a tensor that requires a gradient, would lose it."""
+    if torch.is_grad_enabled():
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or detach its inputs")
 
 

@@ -60,7 +60,8 @@ def beam_select(logits: Tensor, scores: Tensor, keep: int = None, finished: Tens
     if keep < 1:
         raise ValueError(f"keep {keep} must be 1 or more")
     code = _lib.dtype_code(logits.dtype)
-    _lib.no_gradient(logits, scores, what="beam_select")
+    if logits.requires_grad or scores.requires_grad:
+        _lib.no_gradient("beam_select")
     _lib.require_gpu(logits, what="beam_select")
     best = scores.new_empty((batch, keep))
     parents, tokens = torch.empty_like(best, dtype=torch.int32), torch.empty_like(best, dtype=torch.int32)
@@ -90,10 +91,11 @@ def reorder_states(states, parents: Tensor):
             raise ValueError(f"every state must have {rows} rows on {dev}, got {tuple(shape)} on {s.device}")
         if not s.is_contiguous() and rows and not s[0].is_contiguous():
             raise ValueError("the elements of a state's row must lie together")
+        if s.requires_grad:
+            _lib.no_gradient("reorder_states")
         each = s.element_size()
         size.append((s.numel() // rows if rows else math.prod(shape[1:])) * each)
         stride.append(s.stride()[0] * each if rows > 1 else size[-1])
-    _lib.no_gradient(*states, what="reorder_states")
     _lib.require_gpu(*states, what="reorder_states")
     for s in states:
         out.append(torch.empty_like(s, memory_format=torch.contiguous_format) if n == rows

@@ -151,7 +151,8 @@ def append_pages(k_pages: Tensor, v_pages: Tensor, k: Tensor, v: Tensor, table: 
         _int32("starts", starts, (rows + 1,), dev)
     if over is not None:
         _int32("over", over, (rows,), dev)
-    _lib.no_gradient(k, v, k_pages, v_pages, what="append_pages")
+    if k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _lib.no_gradient("append_pages")
     _lib.require_gpu(k_pages, what="append_pages")
     _lib.check(_lib.lib().qs_page_append_over(k.data_ptr(), v.data_ptr(), k.shape[0], rows, k.shape[1], dim, ks[0],
                                               ks[1], vs[0], vs[1], _lib.ptr(starts), pool, _lib.ptr(over),
@@ -191,14 +192,16 @@ def attend_token(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     if over is not None:
         _int32("over", over, (rows,), dev)
     out = _output(out, q)
-    _lib.no_gradient(q, k_pages, v_pages, what="attend_token")
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _lib.no_gradient("attend_token")
     _lib.require_gpu(k_pages, what="attend_token")
     L, heads = _lib.lib(), q.shape[1]
     need = L.qs_attend_token_workspace_bytes(rows, heads, kv_heads, dim, cols, page, window, sinks)
     workspace = _workspace(workspace, need, dev)
     _lib.check(L.qs_attend_token_over(q.data_ptr(), _lib.dtype_code(dtype), rows, heads, kv_heads, dim, st[0], st[1],
-                                      pool, _lib.ptr(over), dim ** -0.5 if scale is None else scale, window, sinks,
-                                      out.data_ptr(), out.stride(0), *_room(workspace), _lib.stream_of(q)))
+                                      pool, None if over is None else over.data_ptr(),
+                                      dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+                                      out.stride(0), *_room(workspace), _lib.stream_of(q)))
     return out
 
 
@@ -221,7 +224,8 @@ def attend_chunk(q: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, len
     if over is not None:
         _int32("over", over, (rows,), dev)
     out = _output(out, q)
-    _lib.no_gradient(q, k_pages, v_pages, what="attend_chunk")
+    if q.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+        _lib.no_gradient("attend_chunk")
     _lib.require_gpu(k_pages, what="attend_chunk")
     L, (tokens, heads, _) = _lib.lib(), q.shape
     need = L.qs_attend_chunk_workspace_bytes(tokens, rows, heads, kv_heads, dim, cols, page, window, sinks)
