@@ -508,7 +508,7 @@ int qs_page_advance(const qs_page_store *store, const int32_t *table, const int3
                     int32_t *lengths_out, int32_t *refs_out, int32_t *short_pages, void *workspace,
                     size_t workspace_bytes, qs_stream_t stream);
 /* The same with a number of tokens for every row: row_tokens [rows] (below 0
- * counts as 0; NULL: `tokens` for all). */
+ * counts as 0, above 2^30 as 2^30; NULL: `tokens` for all). */
 int qs_page_advance_rows(const qs_page_store *store, const int32_t *table, const int32_t *lengths, const int32_t *refs,
                          const int32_t *parents, int64_t rows, int64_t cols, int tokens, const int32_t *row_tokens,
                          int32_t *table_out, int32_t *lengths_out, int32_t *refs_out, int32_t *short_pages,

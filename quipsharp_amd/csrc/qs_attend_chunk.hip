@@ -170,9 +170,10 @@ __device__ __forceinline__ bool find_block(const ChunkArgs& a, const PagePool& p
 // One work-group per kv head and 128 columns of a row, column c being head c %
 // group of the row's token c / group; one wave per 32 of them, whose sums stay
 // in its registers.  Tiles of kT positions go through LDS, which all four
-// waves read (straight from the L1 every wave would load every tile: 616 us
-// for 8192 tokens under a window of 1024 instead of 192), past the registers
-// (through them 242 us); the next tile is on its way while one is worked on.
+// waves read, past the registers; the next tile is on its way while one is
+// worked on.  8192 tokens under a window of 1024 took 616 us with every wave
+// loading every tile from the L1, 242 through the registers, 208 past them,
+// and take 169 now.
 // Two work-groups share a CU, so that one's softmax runs beside the other's
 // products.  Both products are transposed, so that a column stays the lane's
 // own (lane & 31): a 32x32 result of K Q^T leaves lane (hf = lane / 32) with
@@ -182,12 +183,17 @@ __device__ __forceinline__ bool find_block(const ChunkArgs& a, const PagePool& p
 // The weights refer to a base that follows the running maximum only where it
 // has fallen 2^8 behind, so that most tiles rescale nothing; in fp16 they
 // carry a factor of 2^7 too, which keeps 2^-21 of the largest from being
-// subnormal and the largest below 2^15.
+// subnormal and the largest below 2^15.  They are rounded to the cache's type
+// for the second product, and their sum is that of the unrounded ones: an
+// output is off by 0.20 to 0.22 % in the 2-norm in bf16 (fp16: an eighth),
+// where its own rounding alone is 0.165 %.
 //
-// Bound by the matrix and vector instructions together, at the clock that
-// their power leaves: 129 GFLOP in 192 us (8192 tokens, window 1024) and 237
-// in 286 (six rows), 670 and 830 TFLOP/s, where the products alone would run
-// at 1750.
+// Bound by the matrix and vector instructions, which run nearly one after the
+// other (of 365 k cycles matrix units are busy 138 k and vector units 167 k),
+// at the clock that their power leaves: 129 GFLOP in 169 us (8192 tokens,
+// window 1024) and 237 in 276 (six rows), 760 and 860 TFLOP/s, where the
+// products alone would run at 1750.  Heads of 256 (one wave a SIMD, tiles of
+// 32): 4096 tokens of 16 heads 236 us, 583 TFLOP/s.
 //
 // GR = 2: eight waves, of which the second four take every other tile; their
 // results meet in LDS at the end.  For calls whose work-groups do not fill
@@ -576,7 +582,7 @@ int64_t likely_blocks(int64_t tokens, int64_t rows, int heads, int kv_heads) {
 // than half the chip's CUs, and shares of less than 8 tiles do not repay the
 // second launch and the parts that it joins (16 tokens of 8 kv heads behind
 // 6000 positions: 136 us whole, 26 us in shares; a prompt of 512 with 64 heads:
-// 21 us whole, 36 us in two).  Blocks that are not full leave few parts to
+// 21 us whole, 36 us in two, and 18 whole since it runs in eight waves).  Blocks that are not full leave few parts to
 // join, so that twice the shares pay (16 rows of up to 8 tokens behind up to
 // 4000 positions: 38.5 us instead of 45; full ones, 100 tokens behind 6000
 // positions: 59 us instead of 41).

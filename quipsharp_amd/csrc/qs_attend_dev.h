@@ -152,7 +152,7 @@ __device__ __forceinline__ unsigned lds_address(const void* p) {
 // The loads are the whole cost, so each of them takes whole rows: keys go
 // straight to the wave's own part of LDS (a lane's operand is 16 bytes of each
 // of 16 rows, and loads in that shape took 288 us instead of 281 over 1.6 GB,
-// 10.3 instead of 7.2 us over 577 positions), values lie as they are used, 16
+// 10.3 instead of 8.0 us over 577 positions), values lie as they are used, 16
 // lanes to a row: the operand wants 8 positions of one dimension, so the lane
 // takes rows 4 qd + j and 16 + 4 qd + j and puts halves together, and the
 // dimension of operand row m of tile j is DPL m + j.
@@ -268,7 +268,8 @@ struct WaveAttend {
         t8 += pr[t][j];
       }
     sum = sum * f + t8;
-    // the weights in the cache's type, as the matrix instructions take them: half a step of at most 1
+    // the weights in the cache's type, as the matrix instructions take them (half a step of each, in their sum none):
+    // an output is off by 0.20 % in the 2-norm in bf16, its own rounding alone is 0.165 %
     const uint4 pb = make_uint4(pack16<BF>(pr[0][0], pr[0][1]), pack16<BF>(pr[0][2], pr[0][3]),
                                 pack16<BF>(pr[1][0], pr[1][1]), pack16<BF>(pr[1][2], pr[1][3]));
 #pragma unroll

@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kJoin) void beam_join_kernel(SelectArgs a, Candidat
   const int some = a.slices * a.keep, per = some > a.keep + 1 ? some : a.keep + 1, all = a.beams * per;
   // More candidates than the threads have at hand at first, and lists enough for
   // a close edge: by lists (the request above 22 us, 300 beams of 20000 tokens,
-  // keep 128, 91 instead of 540, 32 x 8 beams, keep 8, 35.4 instead of 37.8;
+  // keep 128, 97 instead of 540, 32 x 8 beams, keep 8, 35.4 instead of 37.8;
   // 4 beams of 151936, keep 4, of 592 candidates, 11.0 by lists, 10.7 without).
   const bool lists = all > kAhead * kJoin && a.beams * a.slices >= 64 && a.beams * a.slices >= 2 * a.keep;
   // a thread's first candidates are on their way while the sums are made
