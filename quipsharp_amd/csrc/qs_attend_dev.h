@@ -35,7 +35,7 @@ struct PagePool {
 // further.
 __device__ __forceinline__ int end_of(const int32_t* lengths, const int32_t* over, int most, int64_t row) {
   const int n = lengths[row] < 0 ? 0 : lengths[row];
-  if (!over || n < most) return n;
+  if (!over || n != most) return n;
   const int o = over[row] < 0 ? 0 : over[row];
   return o < INT32_MAX - n ? n + o : INT32_MAX;
 }

@@ -490,7 +490,7 @@ __global__ __launch_bounds__(256) void page_remap_kernel(const int32_t* table, i
 // Where a row's tokens end, as the attention has it.
 __device__ __forceinline__ int64_t row_end(const qs_page_pool& pool, const int32_t* over, int64_t row) {
   const int64_t n = pool.lengths[row];
-  return over && n >= pool.cols * pool.page && over[row] > 0 ? n + over[row] : n;
+  return over && n == pool.cols * pool.page && over[row] > 0 ? n + over[row] : n;
 }
 
 struct AppendArgs {
