@@ -2,6 +2,8 @@
 csrc/qs_attend_token.hip, csrc/qs_attend_chunk.hip): what is cached stays as it
 is, tokens without a place are left out, and they are counted.  Pools are
 compared bit by bit, attention to the tolerance of test_gpu_attend.py."""
+import random
+
 import pytest
 import torch
 
@@ -228,3 +230,65 @@ def test_the_sum_of_missing_pages(dev, rows):
         cache.check()
     cache.missing.zero_()
     cache.check()
+
+
+@pytest.mark.parametrize("rows,cols,pages", [(5, 4, 14), (12, 3, 60), (3, 6, 9), (20, 5, 9000)])
+def test_what_rows_hold_is_their_own(dev, rows, cols, pages):
+    """A long run of forks, prompts, waiting rows, frees, windows and compactions over tables and pools that run out:
+    wherever a row has a page, it holds that row's tokens, those of the rows it came from among them."""
+    from quipsharp_amd.pages import PagedCache
+    cache = PagedCache(1, pages, 1, 8, rows, cols, page=PAGE, device=dev)
+    r = random.Random(rows)
+    told, room, own = 0, cols * PAGE, [{} for _ in range(rows)]  # position -> number of the token stored there
+    missing = lost = 0
+    for step in range(70):
+        op = r.choice(["step", "step", "fork", "counts", "counts", "free", "window", "compact"])
+        if op in ("step", "fork", "counts"):
+            parents = [r.choice([i, r.randrange(rows), r.randrange(-1, rows)]) for i in range(rows)] if op == "fork" else None
+            counts = [r.choice([0, 1, 3, 2 * PAGE + 1]) if op == "counts" else 1 for _ in range(rows)]
+            old = cache.lengths.tolist()
+            cache.advance(ints(counts, dev) if op == "counts" else 1, None if parents is None else ints(parents, dev))
+            start = old if parents is None else [old[p] if p >= 0 else 0 for p in parents]
+            if parents is not None:
+                own = [dict(own[p]) if p >= 0 else {} for p in parents]
+            table, left = cache.table.tolist(), 0
+            x = []
+            for i in range(rows):
+                for p in range(start[i], start[i] + counts[i]):
+                    told += 1
+                    x.append(told)
+                    if p < room and table[i][p // PAGE] >= 0:
+                        own[i][p] = told
+                    else:
+                        left += 1
+            assert cache.lengths.tolist() == [min(s + n, room) for s, n in zip(start, counts)]
+            assert cache.over.tolist() == [max(s + n - room, 0) for s, n in zip(start, counts)]
+            assert (cache.short.item() > 0) == (left > 0)
+            missing += cache.short.item()
+            lost += left
+            # a number in three elements, exact in bf16
+            if x:
+                k = torch.tensor([[[n % 128, n // 128 % 128, n // 16384] + [0] * 5] for n in x]).to(BF).to(dev)
+                cache.append(0, k, -k, ints([sum(counts[:i]) for i in range(rows + 1)], dev))
+        elif op == "free":
+            keep = [r.random() < 0.8 for _ in range(rows)]
+            cache.free(torch.tensor(keep, device=dev))
+            own = [o if k else {} for o, k in zip(own, keep)]
+        elif op == "window":
+            cache.free(window=r.randint(1, room), sinks=r.choice([0, 3, PAGE]))
+        else:
+            cache.compact()
+        assert cache.missing.item() == missing
+        kv, table, lengths = cache.kv[0, :, :, 0].float().cpu(), cache.table.tolist(), cache.lengths.tolist()
+        refs = [0] * pages
+        for i in range(rows):
+            for c, page in enumerate(table[i]):
+                if page < 0:
+                    continue
+                refs[page] += 1
+                for p in range(c * PAGE, min((c + 1) * PAGE, lengths[i])):
+                    n = own[i][p]
+                    want = torch.tensor([n % 128, n // 128 % 128, n // 16384], dtype=torch.float32)
+                    assert torch.equal(kv[0, page, p % PAGE, :3], want) and torch.equal(kv[1, page, p % PAGE, :3], -want)
+        assert cache.refs.tolist() == refs
+    assert (lost > 0) == (missing > 0) and lost > 0
