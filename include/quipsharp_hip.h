@@ -578,6 +578,70 @@ int qs_reorder_states(int count, const void *const *src, void *const *dst, const
                       const int64_t *src_stride, const int32_t *parents, int64_t rows_out, int64_t rows_in,
                       qs_stream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Around the quantized linears of a served step.  No counterpart in the
+ * reference.
+ * --------------------------------------------------------------------------- */
+
+/* Rotary positions with the cache write: of every new token the first 2 pairs
+ * elements of each query and key head are turned, pair i by the angle position
+ * * frequencies[i] (radians, fp64 device memory, [pairs]; the product is taken
+ * in fp64), times factor; the rest of a head stays.  A pair is elements i and
+ * i + pairs, or 2 i and 2 i + 1 (interleaved).  Queries go to q_out
+ * [tokens][heads][head_dim] (tokens out_token apart; may be q itself), keys and
+ * values to the token's place in the pages.  Tokens, rows, starts, pool and
+ * over as in qs_page_append_over; heads need not divide.  A token whose
+ * position is below 0 gets zero queries and is stored nowhere, one that has no
+ * page or lies beyond the table is turned but stored nowhere, one of no row is
+ * left out.  bf16 or fp16; strides multiples of 8 elements, 16-byte aligned;
+ * head_dim a multiple of 8, pairs <= 256. */
+int qs_page_append_rotated(const void *q, const void *k, const void *v, int dtype, int64_t tokens, int64_t rows,
+                           int heads, int kv_heads, int head_dim, int64_t q_token, int64_t q_head, int64_t k_token,
+                           int64_t k_head, int64_t v_token, int64_t v_head, const int32_t *starts,
+                           const qs_page_pool *pool, const int32_t *over, const double *frequencies, int pairs,
+                           int interleaved, float factor, void *q_out, int64_t out_token, qs_stream_t stream);
+
+/* One linear's adapters: down [adapters][rank][n], up [adapters][m][rank] (the
+ * dtype of x; strides in elements, multiples of 8), scale [adapters] (fp32).
+ * rank: a multiple of 8 up to 128 (zeros beyond an adapter's own). */
+typedef struct qs_adapter_job {
+  const void *down, *up;
+  const float *scale;
+  int64_t down_adapter, down_row, up_adapter, up_row;
+  int rank;
+  int64_t m;
+  const void *y; /* [tokens][m], ldy apart */
+  int64_t ldy;
+  void *out; /* [tokens][m], ldo apart: y itself, or apart from it */
+  int64_t ldo;
+} qs_adapter_job;
+
+/* out_g[t] = y_g[t] + scale_g[a] up_g[a] (down_g[a] x[t]) with a = which[t] for
+ * up to QS_MAX_GROUP linears g that read the same x [tokens][n] (bf16 or fp16,
+ * n a multiple of 8).  Tokens whose which is not in 0 .. adapters - 1 have
+ * out = y.  fp32 sums, one rounding.  workspace: qs_adapters_workspace_bytes. */
+size_t qs_adapters_workspace_bytes(int64_t tokens, int64_t n, int64_t adapters, int count, const int *ranks);
+int qs_adapters_add(const void *x, int dtype, int64_t ldx, int64_t tokens, int64_t n, const int32_t *which,
+                    int64_t adapters, int count, const qs_adapter_job *jobs, void *workspace, size_t workspace_bytes,
+                    qs_stream_t stream);
+
+/* Log probabilities of given tokens: for each of `rows` rows of logits (fp32,
+ * fp16 or bf16, ld apart) and its token t (int32 or int64, token_bytes 4 or 8),
+ * with m the row's largest logit and S = sum exp(x - m):
+ *   logprobs  x_t - m - log S                 (0 where t is no token)
+ *   entropy   log S - sum exp(x - m) (x - m) / S
+ *   ranks     how many tokens are ahead: a larger logit, or an equal one and a
+ *             lower token                     (-1 where t is no token)
+ *   top_logprobs, top_tokens [rows][top]: the best tokens' log probabilities,
+ *             ties to the lower token; -inf and -1 where there are none left
+ * A NaN logit counts as -inf, and a token at -inf is no alternative.  A row
+ * whose largest logit is not finite has log probabilities -inf, entropy 0 and
+ * no alternatives.  top <= 64, vocab <= 2^30. */
+size_t qs_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int top);
+int qs_token_logprobs(const void *logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const void *tokens,
+                      int token_bytes, int top, float *logprobs, float *entropy, int32_t *ranks, float *top_logprobs,
+                      int32_t *top_tokens, void *workspace, size_t workspace_bytes, qs_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

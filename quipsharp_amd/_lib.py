@@ -4,6 +4,7 @@ The library is mandatory: every compute entry point of quipsharp_amd goes
 through it, and there is no CPU or pure-PyTorch substitute.  A missing or
 unloadable library raises immediately.
 """
+import contextlib
 import ctypes
 import os
 
@@ -58,6 +59,14 @@ class PageStore(ctypes.Structure):
     """qs_page_store (include/quipsharp_hip.h)."""
     _fields_ = [("data", ctypes.c_void_p), ("planes", ctypes.c_int64), ("pages", ctypes.c_int64),
                 ("kv_heads", ctypes.c_int), ("page", ctypes.c_int), ("row_bytes", ctypes.c_int64)]
+
+
+class AdapterJob(ctypes.Structure):
+    """qs_adapter_job (include/quipsharp_hip.h)."""
+    _fields_ = [("down", ctypes.c_void_p), ("up", ctypes.c_void_p), ("scale", ctypes.c_void_p),
+                ("down_adapter", ctypes.c_int64), ("down_row", ctypes.c_int64), ("up_adapter", ctypes.c_int64),
+                ("up_row", ctypes.c_int64), ("rank", ctypes.c_int), ("m", ctypes.c_int64), ("y", ctypes.c_void_p),
+                ("ldy", ctypes.c_int64), ("out", ctypes.c_void_p), ("ldo", ctypes.c_int64)]
 
 
 _i64 = ctypes.c_int64
@@ -139,6 +148,14 @@ _SIGNATURES = {
                         ctypes.c_size_t, _vp], _int),
     "qs_reorder_states": ([_int, ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_i64),
                            ctypes.POINTER(_i64), _vp, _i64, _i64, _vp], _int),
+    "qs_page_append_rotated": ([_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64,
+                                _vp, _pool_p, _vp, _vp, _int, _int, _f32, _vp, _i64, _vp], _int),
+    "qs_adapters_workspace_bytes": ([_i64, _i64, _i64, _int, _int_p], ctypes.c_size_t),
+    "qs_adapters_add": ([_vp, _int, _i64, _i64, _i64, _vp, _i64, _int, ctypes.POINTER(AdapterJob), _vp,
+                         ctypes.c_size_t, _vp], _int),
+    "qs_token_logprobs_workspace_bytes": ([_i64, _i64, _int, _int], ctypes.c_size_t),
+    "qs_token_logprobs": ([_vp, _int, _i64, _i64, _i64, _vp, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp,
+                           ctypes.c_size_t, _vp], _int),
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -178,6 +195,14 @@ def ptr(t):
 
 def stream_of(t):
     return _vp(torch._C._cuda_getCurrentRawStream(t.get_device()))  # torch.cuda.current_stream's handle alone
+
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def device_of(t):
+    """A context in which kernels go to t's device, at no cost where that is the current one."""
+    return _HERE_ALREADY if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
 
 
 def require_gpu(*tensors, what="quipsharp_amd"):

@@ -1,0 +1,441 @@
+// Log probabilities of given tokens with entropy, rank and the best
+// alternatives (qs_token_logprobs).  With m the row's largest logit and S = sum
+// exp(x - m):
+//
+//   log p_t = x_t - m - log S
+//   H       = log S - sum exp(x - m) (x - m) / S
+//   rank    = #{j : x_j > x_t, or x_j = x_t and j < t}
+//
+// in one pass over the logits.  A thread keeps a level near the maximum of what
+// it has seen, and both sums below it; they are turned to a new level when the
+// maximum rises more than 1 above the old one, and joined at the end.
+// Alternatives go by the logits alone, which no arithmetic touches.
+//
+// Exponentials are fp32, eight of a kind are added in fp32, and all else is
+// fp64.  With units of 2^-24: a term D below its level is off by 2.25 D + 2 (the
+// difference, log2(e), the product and the exponential), a turn adds D + 2, of
+// which those after the first count for little (a sum is a third or less of
+// itself after each), and there are two joins; eight added make 7.  The mean of
+// D over a softmax is at most ln(vocab), so that a log sum is off by
+// 3 ln(vocab) + 20 units (3.3e-6 for 151936 tokens) at most.
+#include <type_traits>
+
+#include "qs_order_dev.h"
+
+namespace qs {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kMaxTop = 64;
+constexpr int kMaxParts = 128;  // of a row: its lists fit the join's room
+constexpr int kHold = 128;      // candidates that may wait for the next slice
+// Candidates at a time: those that wait, and of a slice those above its edge
+// (63 threads' 32), or fewer than 64 of them and one row of equal ones.
+constexpr int kRoom = 2304;
+static_assert(kRoom >= kHold + (kMaxTop - 1) * 32 && kRoom >= kHold + kMaxTop - 1 + kThreads * 8, "candidates of a slice");
+static_assert(kRoom >= kMaxTop * (kMaxParts * kMaxTop / kThreads), "candidates of the join");
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Of a part of a row: its level, both sums below it and how many are ahead of the token.
+struct Stat {
+  double sum, weighted;
+  float top;
+  int ahead;
+};
+
+struct ScoreArgs {
+  const void* logits;
+  int64_t ld, vocab;
+  const void* tokens;
+  int wide_tokens;  // int64
+  int top, parts, slices, per;  // per: slices of a part
+  Stat* stats;      // [rows][parts]
+  uint64_t* lists;  // [rows][parts][top]: order bits << 32 | ~token, in descending order; 0 for none
+  float *logp, *entropy, *top_logp;
+  int32_t *ranks, *top_tokens;
+};
+
+// exp(d)
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * 1.44269504f); }
+
+// Sums below the level `from` turned to the larger `to`.
+__device__ __forceinline__ void turn(double& sum, double& weighted, float from, float to) {
+  if (from == -INFINITY || !(from < to)) return;
+  const double d = (double)from - (double)to;
+  const double r = d < -200.0 ? 0.0 : (double)__builtin_amdgcn_exp2f((float)(d * 1.4426950408889634));
+  weighted = r == 0.0 ? 0.0 : r * (weighted + d * sum);
+  sum *= r;
+}
+
+__device__ __forceinline__ float wave_max(float v, LaneX lx) {
+  v = fmaxf(v, lane_xor<32>(v, lx));
+  v = fmaxf(v, lane_xor<16>(v, lx));
+  v = fmaxf(v, lane_xor<8>(v, lx));
+  v = fmaxf(v, lane_xor<4>(v, lx));
+  v = fmaxf(v, lane_xor<2>(v, lx));
+  v = fmaxf(v, lane_xor<1>(v, lx));
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ float value_of(const T* row, int64_t t) {
+  float f;
+  if constexpr (sizeof(T) == 4) f = row[t];
+  else if constexpr (std::is_same<T, _Float16>::value) f = (float)row[t];
+  else f = __uint_as_float((uint32_t)row[t] << 16);
+  return fmaxf(f, -INFINITY);  // NaN counts as -inf
+}
+
+__device__ __forceinline__ int64_t token_of(const ScoreArgs& a, int64_t row) {
+  const int64_t t = a.wide_tokens ? static_cast<const int64_t*>(a.tokens)[row] : static_cast<const int32_t*>(a.tokens)[row];
+  return t >= 0 && t < a.vocab ? t : -1;
+}
+
+// What is written for a row, from its level and sums: one thread.
+__device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t row, int64_t t, float xt, const Stat& s, double log_sum) {
+  const bool runs = fabsf(s.top) < INFINITY;
+  a.logp[row] = t < 0 ? 0.f : runs ? (float)(((double)xt - s.top) - log_sum) : -INFINITY;
+  a.entropy[row] = runs ? (float)fmax(0.0, log_sum - s.weighted / s.sum) : 0.f;
+  a.ranks[row] = t < 0 ? -1 : s.ahead;
+}
+__device__ __forceinline__ void write_alternative(const ScoreArgs& a, int64_t row, int i, uint64_t key, float top, double log_sum) {
+  const bool has = key && fabsf(top) < INFINITY;
+  a.top_logp[row * a.top + i] = has ? (float)(((double)order_float((uint32_t)(key >> 32)) - top) - log_sum) : -INFINITY;
+  a.top_tokens[row * a.top + i] = has ? (int32_t)~(uint32_t)key : -1;
+}
+
+// The best `top` of the first n candidates, in order, in best; zeros behind them.
+__device__ __forceinline__ void rank_all(const uint64_t* room, int n, uint64_t* best, int top) {
+  for (int c = threadIdx.x; c < n; c += kThreads) {
+    const uint64_t me = room[c];
+    int place = 0;
+    for (int i = 0; i < n; ++i) place += room[i] > me;
+    if (place < top) best[place] = me;
+  }
+  for (int c = n + threadIdx.x; c < top; c += kThreads) best[c] = 0;
+}
+
+// One work-group per part of a row.  A row is read in 16-byte pieces that
+// begin at or before its first logit, so rows at odd places load as widely as
+// others: piece i * 256 + tid of a slice is the thread's i-th.
+template <typename T, int E, bool SELECT>
+__global__ __launch_bounds__(kThreads) void score_kernel(ScoreArgs a) {
+  constexpr int W = 16 / sizeof(T), P = E / W;
+  __shared__ uint64_t room[SELECT ? kRoom : 1];
+  __shared__ uint64_t best[kMaxTop];
+  __shared__ float tops[kThreads];
+  __shared__ float red[3][4];
+  __shared__ Stat stat[4];
+  __shared__ float line;
+  __shared__ int count;
+  const LaneX lx = lane_x_init();
+  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, part = blockIdx.y, top = a.top;
+  const int64_t row = blockIdx.x;
+  const T* from = static_cast<const T*>(a.logits) + row * a.ld;
+  const int lead = (int)((reinterpret_cast<uintptr_t>(from) & 15) / sizeof(T));
+  const u32x4* pieces = reinterpret_cast<const u32x4*>(from - lead);
+  const int64_t end = lead + a.vocab;                // elements from the first piece on
+  const int64_t t = token_of(a, row);
+  const float xt = t < 0 ? INFINITY : value_of(from, t);
+  const int first = part * a.per, last = first + a.per < a.slices ? first + a.per : a.slices;
+
+  auto fetch = [&](int slice, u32x4 (&raw)[P]) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const int64_t at = ((int64_t)slice * P + i) * kThreads + tid;
+      raw[i] = at * W < end ? __builtin_nontemporal_load(pieces + at) : u32x4{};
+    }
+  };
+  float m = -INFINITY, edge = -INFINITY;
+  double sum = 0.0, weighted = 0.0;
+  int ahead = 0, held = 0;
+  if (SELECT && tid == 0) count = 0;
+  if (SELECT) __syncthreads();
+  u32x4 raw[P];
+  if (first < last) fetch(first, raw);
+  for (int slice = first; slice < last; ++slice) {
+    const int64_t e0 = (int64_t)slice * (P * kThreads * W);  // the slice's first element
+    auto token = [&](int i) { return e0 + ((int64_t)(i / W) * kThreads + tid) * W + i % W - lead; };
+    float x[E];
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      const u32x4 u = raw[i];
+#pragma unroll
+      for (int e = 0; e < W; ++e) {
+        if constexpr (sizeof(T) == 4) x[i * W + e] = __uint_as_float(u[e]);
+        else if constexpr (std::is_same<T, _Float16>::value) x[i * W + e] = (float)__builtin_bit_cast(_Float16, (uint16_t)(u[e / 2] >> 16 * (e & 1)));
+        else x[i * W + e] = __uint_as_float(e & 1 ? u[e / 2] & 0xFFFF0000u : u[e / 2] << 16);
+      }
+    }
+    if (e0 < lead || e0 + E * kThreads > end) {
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (token(i) < 0 || token(i) >= a.vocab) x[i] = -INFINITY;
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i) x[i] = fmaxf(x[i], -INFINITY);  // NaN counts as -inf
+    if (slice + 1 < last) fetch(slice + 1, raw);
+    float ms = x[0];
+#pragma unroll
+    for (int i = 1; i < E; ++i) ms = fmaxf(ms, x[i]);
+    if (ms > m + 1.f) turn(sum, weighted, m, ms), m = ms;
+    if (m > -INFINITY) {
+#pragma unroll
+      for (int i = 0; i < E; i += 8) {
+        float s = 0.f, v = 0.f;
+#pragma unroll
+        for (int e = i; e < i + 8; ++e) {
+          const float d = fmaxf(x[e] - m, -200.f), p = exp_of(d);
+          s += p, v = __builtin_fmaf(p, d, v);
+        }
+        sum += s, weighted += v;
+      }
+    }
+    // how many are ahead of the token: at or above it before its place, above it behind
+    if (t >= 0) {
+      const int64_t t0 = e0 - lead, t1 = t0 + E * kThreads;
+      if (t1 <= t && xt > -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) ahead += __popcll(__ballot(x[i] >= xt));
+      } else if (t0 > t) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) ahead += __popcll(__ballot(x[i] > xt));
+      } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          ahead += __popcll(__ballot(x[i] > xt || (x[i] == xt && token(i) >= 0 && token(i) < t)));
+      }
+    }
+    if constexpr (SELECT) {
+      // Only what is above the edge can be among the best: the top-th of what
+      // came before (an equal one behind it is not), or in the first slice
+      // the largest of the waves' top-th largest maxima of threads and the
+      // least of their top / 4-th.
+      const bool fresh = slice == first;
+      auto threads_edge = [&]() {  // top-th largest of the threads' maxima, at all threads
+        tops[tid] = ms;
+        if (tid == 0) line = -INFINITY;
+        __syncthreads();
+        int above = 0, same = 0;
+        for (int i = 0; i < kThreads; ++i) above += tops[i] > ms, same += tops[i] == ms;
+        if (above < top && top <= above + same) line = ms;  // all that write it write the same
+        __syncthreads();
+        return line;
+      };
+      if (fresh) {
+        if (top > 32) {
+          edge = threads_edge();
+        } else {
+          const float edge_w = order_float(nth_key(order_bits(ms), top));
+          const float part_w = top > 8 ? order_float(nth_key(order_bits(ms), (top + 3) / 4)) : -INFINITY;
+          if (lane == 0) red[1][w] = edge_w, red[2][w] = part_w;
+          __syncthreads();
+          edge = fmaxf(fmaxf(red[1][0], red[1][1]), fmaxf(red[1][2], red[1][3]));
+          edge = fmaxf(edge, fminf(fminf(red[2][0], red[2][1]), fminf(red[2][2], red[2][3])));
+        }
+      }
+      auto add = [&](int i) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kRoom) room[at] = (uint64_t)order_bits(x[i]) << 32 | (uint32_t)~(uint32_t)token(i);
+      };
+      if (__any(fresh ? ms >= edge : ms > edge)) {
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if ((fresh ? x[i] >= edge : x[i] > edge) && x[i] > -INFINITY) add(i);
+      }
+      __syncthreads();
+      int n = count;
+      __syncthreads();
+      if (n > kRoom) {
+        // Too many: of this slice those above its threads' edge, then the
+        // equal ones by rising tokens until there are enough.
+        const float low = threads_edge();
+        if (tid == 0) count = held;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < E; ++i)
+          if (x[i] > low) add(i);
+        __syncthreads();
+        if (low > -INFINITY) {
+#pragma unroll
+          for (int i = 0; i < E; i += W) {
+            const bool enough = count - held >= top;
+            __syncthreads();
+            if (enough) continue;
+#pragma unroll
+            for (int e = i; e < i + W; ++e)
+              if (x[e] == low) add(e);
+            __syncthreads();
+          }
+        }
+        n = count;
+        __syncthreads();
+      }
+      if (n > kHold || slice + 1 == last || (n >= top && fresh)) {
+        rank_all(room, n, best, top);
+        __syncthreads();
+        if (tid < top) room[tid] = best[tid];
+        n = n < top ? n : top;
+        if (n == top) edge = order_float((uint32_t)(best[top - 1] >> 32));
+        else edge = -INFINITY;
+        if (tid == 0) count = n;
+        __syncthreads();
+      }
+      held = n;
+    }
+  }
+  // the threads' sums below the highest level
+  float all = wave_max(m, lx);
+  if (lane == 0) red[0][w] = all;
+  __syncthreads();
+  all = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  if (all < INFINITY) turn(sum, weighted, m, all);
+  sum = wave_sum64(sum, lx), weighted = wave_sum64(weighted, lx);
+  if (lane == 0) stat[w] = Stat{sum, weighted, all, ahead};
+  __syncthreads();
+  const Stat s{(stat[0].sum + stat[1].sum) + (stat[2].sum + stat[3].sum),
+               (stat[0].weighted + stat[1].weighted) + (stat[2].weighted + stat[3].weighted), all,
+               (stat[0].ahead + stat[1].ahead) + (stat[2].ahead + stat[3].ahead)};
+  if (a.parts > 1) {
+    if (tid == 0) a.stats[row * a.parts + part] = s;
+    if (SELECT && tid < top) a.lists[(row * a.parts + part) * top + tid] = best[tid];
+    return;
+  }
+  const double log_sum = log(s.sum);
+  if (tid == 0) write_row(a, row, t, xt, s, log_sum);
+  if (SELECT && tid < top) write_alternative(a, row, tid, best[tid], all, log_sum);
+}
+
+// The parts of a row together: one work-group per row.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
+  __shared__ uint64_t room[kRoom];
+  __shared__ uint64_t best[kMaxTop], tops[kThreads], line;
+  __shared__ Stat stat;
+  __shared__ int count;
+  const LaneX lx = lane_x_init();
+  const int tid = threadIdx.x, top = a.top;
+  const int64_t row = blockIdx.x;
+  const int n = a.parts * top;
+  const uint64_t* lists = a.lists + row * n;
+  uint64_t mine[kMaxParts * kMaxTop / kThreads];
+  uint64_t high = 0;
+#pragma unroll
+  for (int i = 0; i < kMaxParts * kMaxTop / kThreads; ++i) {
+    const int c = i * kThreads + tid;
+    mine[i] = c < n ? lists[c] : 0;
+    high = mine[i] > high ? mine[i] : high;
+  }
+  tops[tid] = high;
+  if (tid == 0) count = 0, line = 0;
+  if (tid < 64) {
+    const Stat* st = a.stats + row * a.parts;
+    const Stat none{0.0, 0.0, -INFINITY, 0};
+    Stat s = tid < a.parts ? st[tid] : none, s2 = tid + 64 < a.parts ? st[tid + 64] : none;
+    const float all = wave_max(fmaxf(s.top, s2.top), lx);
+    if (all < INFINITY) turn(s.sum, s.weighted, s.top, all), turn(s2.sum, s2.weighted, s2.top, all);
+    const double sum = wave_sum64(s.sum + s2.sum, lx), weighted = wave_sum64(s.weighted + s2.weighted, lx);
+    const double ahead = wave_sum64((double)s.ahead + s2.ahead, lx);
+    if (tid == 0) stat = Stat{sum, weighted, all, (int)ahead};
+  }
+  __syncthreads();
+  // no two candidates are alike, so that at most `top` threads have one at or above the edge
+  if (top > 0) {
+    int above = 0;
+    for (int i = 0; i < kThreads; ++i) above += tops[i] > high;
+    if (above == top - 1 && high) line = high;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kMaxParts * kMaxTop / kThreads; ++i)
+      if (mine[i] && mine[i] >= line) room[atomicAdd(&count, 1)] = mine[i];
+    __syncthreads();
+    rank_all(room, count, best, top);
+    __syncthreads();
+  }
+  const double log_sum = log(stat.sum);
+  if (tid == 0) {
+    const int64_t t = token_of(a, row);
+    write_row(a, row, t, t < 0 ? 0.f : value_of(static_cast<const T*>(a.logits) + row * a.ld, t), stat, log_sum);
+  }
+  if (tid < top) write_alternative(a, row, tid, best[tid], stat.top, log_sum);
+}
+
+struct Layout {
+  int each, slices, per, parts;
+  size_t lists, bytes;
+};
+
+Layout layout_of(int64_t rows, int64_t vocab, int top, int size) {
+  Layout l;
+  l.each = rows * ((vocab + 8191) / 8192) >= 512 ? 32 : 8;
+  const int64_t slice = (int64_t)kThreads * l.each;
+  l.slices = (int)((vocab + 16 / size - 1 + slice - 1) / slice);  // wherever the row begins in its first piece
+  int64_t parts = (1024 + rows - 1) / rows;
+  parts = parts < l.slices ? parts : l.slices;
+  parts = parts < kMaxParts ? parts : kMaxParts;
+  l.per = (int)((l.slices + parts - 1) / parts);
+  l.parts = (l.slices + l.per - 1) / l.per;
+  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+  l.lists = l.parts > 1 ? up((size_t)rows * l.parts * sizeof(Stat)) : 0;
+  l.bytes = l.parts > 1 ? l.lists + up((size_t)rows * l.parts * top * sizeof(uint64_t)) : 0;
+  return l;
+}
+
+template <typename T>
+auto score_kernel_of(int each, bool select) {
+  if (select) return each == 32 ? score_kernel<T, 32, true> : score_kernel<T, 8, true>;
+  return each == 32 ? score_kernel<T, 32, false> : score_kernel<T, 8, false>;
+}
+
+bool sizes_fit(int64_t rows, int64_t vocab, int top) {
+  return rows >= 1 && rows <= INT32_MAX && vocab >= 1 && vocab <= (1 << 30) && top >= 0 && top <= kMaxTop && top <= vocab;
+}
+
+}  // namespace
+}  // namespace qs
+
+using namespace qs;
+
+extern "C" size_t qs_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int top) {
+  if (!sizes_fit(rows, vocab, top)) return 0;
+  return layout_of(rows, vocab, top, dtype == QS_DTYPE_F32 ? 4 : 2).bytes;
+}
+
+extern "C" int qs_token_logprobs(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const void* tokens,
+                                 int token_bytes, int top, float* logprobs, float* entropy, int32_t* ranks,
+                                 float* top_logprobs, int32_t* top_tokens, void* workspace, size_t workspace_bytes,
+                                 qs_stream_t stream) {
+  const char* fn = "qs_token_logprobs";
+  if (rows == 0) return QS_OK;
+  QS_REQUIRE(logits && tokens && logprobs && entropy && ranks && (top == 0 || (top_logprobs && top_tokens)), "%s: null pointer", fn);
+  QS_REQUIRE(dtype == QS_DTYPE_F32 || dtype == QS_DTYPE_F16 || dtype == QS_DTYPE_BF16, "%s: dtype %d", fn, dtype);
+  QS_REQUIRE(token_bytes == 4 || token_bytes == 8, "%s: tokens of %d bytes", fn, token_bytes);
+  QS_REQUIRE(rows >= 1 && vocab >= 1 && (rows == 1 || ld >= vocab), "%s: %lld rows of %lld tokens, %lld apart", fn,
+             (long long)rows, (long long)vocab, (long long)ld);
+  QS_REQUIRE(top >= 0 && top <= vocab, "%s: %d alternatives of %lld tokens", fn, top, (long long)vocab);
+  QS_SUPPORTED(sizes_fit(rows, vocab, top), "%s: %lld rows of %lld tokens, %d alternatives (at most %d, of 2^30 tokens)", fn,
+               (long long)rows, (long long)vocab, top, kMaxTop);
+  const int size = dtype_bytes(dtype);
+  QS_REQUIRE(reinterpret_cast<uintptr_t>(logits) % size == 0 && reinterpret_cast<uintptr_t>(tokens) % token_bytes == 0,
+             "%s: logits and tokens must be aligned to their elements", fn);
+  const Layout l = layout_of(rows, vocab, top, size);
+  QS_REQUIRE(l.bytes == 0 || (workspace && workspace_bytes >= l.bytes && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0),
+             "%s: workspace of %zu bytes (16-byte aligned), %zu needed", fn, workspace_bytes, l.bytes);
+  char* ws = static_cast<char*>(workspace);
+  const ScoreArgs a{logits, rows == 1 ? vocab : ld, vocab, tokens, token_bytes == 8, top, l.parts, l.slices, l.per,
+                    reinterpret_cast<Stat*>(ws), reinterpret_cast<uint64_t*>(ws + l.lists), logprobs, entropy,
+                    top_logprobs, ranks, top_tokens};
+  const auto kernel = dtype == QS_DTYPE_F32   ? score_kernel_of<float>(l.each, top > 0)
+                      : dtype == QS_DTYPE_F16 ? score_kernel_of<_Float16>(l.each, top > 0)
+                                              : score_kernel_of<uint16_t>(l.each, top > 0);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)rows, (unsigned)l.parts), dim3(kThreads), 0, as_stream(stream), a);
+  QS_LAUNCHED("score_kernel");
+  if (l.parts > 1) {
+    const auto join = dtype == QS_DTYPE_F32   ? score_join_kernel<float>
+                      : dtype == QS_DTYPE_F16 ? score_join_kernel<_Float16>
+                                              : score_join_kernel<uint16_t>;
+    hipLaunchKernelGGL(join, dim3((unsigned)rows), dim3(kThreads), 0, as_stream(stream), a);
+    QS_LAUNCHED("score_join_kernel");
+  }
+  return QS_OK;
+}
