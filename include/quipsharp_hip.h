@@ -636,7 +636,7 @@ int qs_adapters_add(const void *x, int dtype, int64_t ldx, int64_t tokens, int64
  *             ties to the lower token; -inf and -1 where there are none left
  * A NaN logit counts as -inf, and a token at -inf is no alternative.  A row
  * whose largest logit is not finite has log probabilities -inf, entropy 0 and
- * no alternatives.  top <= 64, vocab <= 2^30. */
+ * no alternatives.  top <= 64, vocab <= 2^24. */
 size_t qs_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int top);
 int qs_token_logprobs(const void *logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const void *tokens,
                       int token_bytes, int top, float *logprobs, float *entropy, int32_t *ranks, float *top_logprobs,

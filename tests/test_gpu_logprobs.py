@@ -73,12 +73,13 @@ def test_scores(dev, rows, vocab, top, dtype):
 
 @pytest.mark.parametrize("rows", [1, 40, 700])
 @pytest.mark.parametrize("top", [0, 1, 20, 64])
-@pytest.mark.parametrize("order", ["ascending", "descending", "equal", "two values", "steps"])
+@pytest.mark.parametrize("order", ["ascending", "descending", "equal", "two values", "steps", "rare", "few"])
 def test_orders(dev, order, top, rows):
     """Every slice brings better ones, none does, and all are alike: the lower tokens win."""
     V = 20011
     x = {"ascending": torch.arange(V) / 997.0, "descending": -torch.arange(V) / 997.0, "equal": torch.full((V,), 1.5),
-         "two values": (torch.arange(V) % 7 == 3).float(), "steps": (torch.arange(V) // 40).float() / 8}[order]
+         "two values": (torch.arange(V) % 7 == 3).float(), "steps": (torch.arange(V) // 40).float() / 8,
+         "rare": (torch.arange(V) % 61 == 60).float(), "few": torch.arange(V) % 500 // 499 + (torch.arange(V) % 33 == 7) / 2}[order]
     x = x.float()[None].repeat(rows, 1)
     tokens = torch.tensor([(7 * i + 3) % V for i in range(rows)])
     tokens[-1] = V - 1
@@ -136,6 +137,19 @@ def test_rows_at_odd_places(dev):
             tokens = torch.randint(0, V, (9,), generator=g)
             on_gpu = torch.as_strided(whole.to(dev), (9, V), (ld, 1), first)
             check(dev, rows, tokens, 6, on_gpu)
+
+
+def test_the_longest_vocabulary(dev):
+    """Parts of as many slices as their threads have room to note, and a vocabulary one short of a part's more."""
+    for V, rows in ((1 << 24, 1), (20 * 8192 - 1, 600), (20 * 8192 + 1, 2)):
+        g = torch.Generator().manual_seed(V)
+        x = (torch.randn(1, V, generator=g) * 2).bfloat16().repeat(rows, 1)
+        tokens = torch.randint(0, V, (1,), generator=g).repeat(rows)
+        got = check(dev, x[:1], tokens[:1], 64, None if rows < 3 else x.to(dev)[:1])
+        from quipsharp_amd.logprobs import token_logprobs
+        for a, b in zip(token_logprobs(x.to(dev), tokens.to(dev), 64), got):
+            a = a.cpu()
+            assert (a == a[:1]).all() and (torch.equal(a[:1], b) if b.dtype is torch.int32 else torch.allclose(a[:1], b, rtol=0, atol=2e-5))
 
 
 def test_sharp_and_flat_distributions(dev):

@@ -272,7 +272,7 @@ def scores_c(L, **over):
     (dict(logits=None), 1, "null"), (dict(tokens=None), 1, "null"), (dict(best=None), 1, "null"), (dict(dtype=3), 1, "dtype 3"),
     (dict(token_bytes=2), 1, "2 bytes"), (dict(ld=49), 1, "49 apart"), (dict(top=51), 1, "51 alternatives"),
     (dict(top=-1), 1, "-1 alternatives"), (dict(vocab=0, ld=0), 1, "of 0 tokens"), (dict(top=65, vocab=100, ld=100), 3, "at most 64"),
-    (dict(vocab=(1 << 30) + 1, ld=1 << 31), 3, "2^30"), (dict(logits=ctypes.c_void_p(4098)), 1, "aligned"),
+    (dict(vocab=(1 << 24) + 1, ld=1 << 25), 3, "2^24"), (dict(logits=ctypes.c_void_p(4098)), 1, "aligned"),
     (dict(tokens=ctypes.c_void_p(4100)), 1, "aligned"), (dict(vocab=50000, ld=50000, bytes=64), 1, "workspace of 64"),
     (dict(vocab=50000, ld=50000, ws=None), 1, "workspace"),
 ])
