@@ -37,11 +37,13 @@ constexpr int kRoom = (kMaxTop - 1) * kGroup + kMaxTop;
 static_assert(kRoom >= kMaxTop * (kMaxParts * kMaxTop / kThreads), "candidates of the join");
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// Of a part of a row: its level, both sums below it and how many are ahead of the token.
+// Of a part of a row: its level, both sums below it and how many are ahead of
+// the token; the token's logit (+inf where it is none), the same in all parts.
 struct Stat {
   double sum, weighted;
   float top;
   int ahead;
+  float xt;
 };
 
 struct ScoreArgs {
@@ -93,11 +95,11 @@ __device__ __forceinline__ int64_t token_of(const ScoreArgs& a, int64_t row) {
 }
 
 // What is written for a row, from its level and sums: one thread.
-__device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t row, int64_t t, float xt, const Stat& s, double log_sum) {
+__device__ __forceinline__ void write_row(const ScoreArgs& a, int64_t row, bool none, const Stat& s, double log_sum) {
   const bool runs = fabsf(s.top) < INFINITY;
-  a.logp[row] = t < 0 ? 0.f : runs ? (float)(((double)xt - s.top) - log_sum) : -INFINITY;
+  a.logp[row] = none ? 0.f : runs ? (float)(((double)s.xt - s.top) - log_sum) : -INFINITY;
   a.entropy[row] = runs ? (float)fmax(0.0, log_sum - s.weighted / s.sum) : 0.f;
-  a.ranks[row] = t < 0 ? -1 : s.ahead;
+  a.ranks[row] = none ? -1 : s.ahead;
 }
 __device__ __forceinline__ void write_alternative(const ScoreArgs& a, int64_t row, int i, uint64_t key, float top, double log_sum) {
   const bool has = key && fabsf(top) < INFINITY;
@@ -110,6 +112,7 @@ __device__ __forceinline__ void rank_all(const uint64_t* room, int n, uint64_t* 
   for (int c = threadIdx.x; c < n; c += kThreads) {
     const uint64_t me = room[c];
     int place = 0;
+#pragma unroll 8
     for (int i = 0; i < n; ++i) place += room[i] > me;
     if (place < top) best[place] = me;
   }
@@ -185,12 +188,15 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t token) { return (ui
 // the edge are too many, it is the top-th largest maximum of the groups: the
 // logits above it lie in fewer than `top` groups, and of those at it the lowest
 // tokens are taken.
-template <typename T, int P>
-__device__ void select_best(const Groups<T, P>& g, float largest, int top, Room& r, LaneX lx) {
+//
+// `own`: the part is one slice, which the threads still have: held(use) calls
+// use(logit, token) for the thread's.
+template <typename T, int P, typename Held>
+__device__ __forceinline__ void select_best(const Groups<T, P>& g, float largest, int top, Room& r, bool own, Held held) {
   typedef Note<T> N;
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const uint32_t bits = order_bits(largest);
-  const float edge_w = order_float(nth_key(bits, top)), part_w = order_float(nth_key(bits, (top + 3) / 4));
+  const float edge_w = order_float(nth_key(bits, top)), part_w = top > 8 ? order_float(nth_key(bits, (top + 3) / 4)) : -INFINITY;
   if (lane == 0) r.red[0][w] = edge_w, r.red[1][w] = part_w;
   if (tid == 0) r.groups = 0, r.count = 0;
   __syncthreads();
@@ -217,30 +223,48 @@ __device__ void select_best(const Groups<T, P>& g, float largest, int top, Room&
       });
     }
   };
-  if (largest >= edge) list([&](float m) { return m >= edge; });
-  __syncthreads();
-  const int groups = r.groups;
-  if (groups <= kListed) read(groups, [&](float x) { return x >= edge; });
+  int groups = 0;
+  if (own) {
+    if (__any(largest >= edge)) {
+      held([&](float x, uint32_t token) {
+        if (x >= edge && x > -INFINITY) add(x, token);
+      });
+    }
+  } else {
+    if (largest >= edge) list([&](float m) { return m >= edge; });
+    __syncthreads();
+    groups = r.groups;
+    if (groups <= kListed) read(groups, [&](float x) { return x >= edge; });
+  }
   __syncthreads();
   int n = r.count;
   if (groups > kListed || n > kRoom) {
-    if (tid < 32) r.above[tid] = 0;
     __syncthreads();
-    uint32_t u = 0;
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint32_t v = u | 1u << bit;
-      int many = 0;
-      for (int s = 0; s < g.runs; ++s) many += __popcll(__ballot(order_bits(N::value(g.notes[s * kThreads + tid])) >= v));
-      if (lane == 0) atomicAdd(&r.above[bit], many);
-      __syncthreads();
-      if (r.above[bit] >= top) u = v;
-    }
-    edge = order_float(u);
+    if (tid < 32) r.above[tid] = 0;
     if (tid == 0) r.groups = 0, r.count = 0;
     __syncthreads();
     list([&](float m) { return m > edge; });
     __syncthreads();
-    read(r.groups, [&](float x) { return x > edge; });
+    groups = r.groups;
+    if (groups >= top) {
+      // the edge is too low
+      uint32_t u = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t v = u | 1u << bit;
+        int many = 0;
+        for (int s = 0; s < g.runs; ++s) many += __popcll(__ballot(order_bits(N::value(g.notes[s * kThreads + tid])) >= v));
+        if (lane == 0) atomicAdd(&r.above[bit], many);
+        __syncthreads();
+        if (r.above[bit] >= top) u = v;
+      }
+      edge = order_float(u);
+      if (tid == 0) r.groups = 0;
+      __syncthreads();
+      list([&](float m) { return m > edge; });
+      __syncthreads();
+      groups = r.groups;
+    }
+    read(groups, [&](float x) { return x > edge; });
     __syncthreads();
     n = r.count;
     __syncthreads();
@@ -308,13 +332,12 @@ __global__ __launch_bounds__(kThreads) void score_kernel(ScoreArgs a) {
   fetch(first, raw);
   const int64_t t = token_of(a, row);
   const float xt = t < 0 ? INFINITY : value_of(from, t);
-  float m = -INFINITY, largest = -INFINITY, noted = -INFINITY;
+  float x[E], m = -INFINITY, largest = -INFINITY, noted = -INFINITY;
   double sum = 0.0, weighted = 0.0;
   int ahead = 0;
   for (int slice = first; slice < last; ++slice) {
     const int64_t e0 = (int64_t)slice * (P * kThreads * W);  // the slice's first element
     auto token = [&](int i) { return e0 + ((int64_t)(i / W) * kThreads + tid) * W + i % W - lead; };
-    float x[E];
 #pragma unroll
     for (int i = 0; i < P; ++i) unpack<T>(raw[i], x + i * W);
     if (e0 < lead || e0 + E * kThreads > end) {
@@ -368,16 +391,19 @@ __global__ __launch_bounds__(kThreads) void score_kernel(ScoreArgs a) {
   all = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   if (all < INFINITY) turn(sum, weighted, m, all);
   sum = wave_sum64(sum, lx), weighted = wave_sum64(weighted, lx);
-  if (lane == 0) stat[w] = Stat{sum, weighted, all, ahead};
+  if (lane == 0) stat[w] = Stat{sum, weighted, all, ahead, xt};
   if constexpr (SELECT) {
     const Groups<T, kGroup / W> g{pieces, (int64_t)first * P * kThreads, end, a.vocab, lead, (last - first + H - 1) / H, (last - first) * P, notes};
-    select_best(g, largest, top, room, lx);
+    select_best(g, largest, top, room, last - first == 1, [&](auto use) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) use(x[i], (uint32_t)(((int64_t)first * P + i / W) * (kThreads * W) + tid * W + i % W - lead));
+    });
   } else {
     __syncthreads();
   }
   const Stat s{(stat[0].sum + stat[1].sum) + (stat[2].sum + stat[3].sum),
                (stat[0].weighted + stat[1].weighted) + (stat[2].weighted + stat[3].weighted), all,
-               (stat[0].ahead + stat[1].ahead) + (stat[2].ahead + stat[3].ahead)};
+               t < 0 ? -1 : (stat[0].ahead + stat[1].ahead) + (stat[2].ahead + stat[3].ahead), xt};
   if (a.parts > 1) {
     if (tid == 0) a.stats[row * a.parts + part] = s;
     if constexpr (SELECT)
@@ -385,16 +411,16 @@ __global__ __launch_bounds__(kThreads) void score_kernel(ScoreArgs a) {
     return;
   }
   const double log_sum = log(s.sum);
-  if (tid == 0) write_row(a, row, t, xt, s, log_sum);
+  if (tid == 0) write_row(a, row, t < 0, s, log_sum);
   if constexpr (SELECT)
     if (tid < top) write_alternative(a, row, tid, room.best[tid], all, log_sum);
 }
 
 // The parts of a row together: one work-group per row.
-template <typename T>
 __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   __shared__ uint64_t room[kRoom];
   __shared__ uint64_t best[kMaxTop], tops[kThreads], line;
+  __shared__ uint32_t edge[4];
   __shared__ Stat stat;
   __shared__ int count;
   const LaneX lx = lane_x_init();
@@ -402,8 +428,6 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   const int64_t row = blockIdx.x;
   const int n = a.parts * top;
   const uint64_t* lists = a.lists + row * n;
-  const int64_t t = token_of(a, row);
-  const float xt = t < 0 ? 0.f : value_of(static_cast<const T*>(a.logits) + row * a.ld, t);
   uint64_t mine[kMaxParts * kMaxTop / kThreads];
   uint64_t high = 0;
 #pragma unroll
@@ -414,32 +438,54 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   }
   tops[tid] = high;
   if (tid == 0) count = 0, line = 0;
+  if (top > 0) {
+    const uint32_t e = nth_key((uint32_t)(high >> 32), top);
+    if ((tid & 63) == 0) edge[tid >> 6] = e;
+  }
   if (tid < 64) {
     const Stat* st = a.stats + row * a.parts;
-    const Stat none{0.0, 0.0, -INFINITY, 0};
+    const Stat none{0.0, 0.0, -INFINITY, 0, 0.f};
     Stat s = tid < a.parts ? st[tid] : none, s2 = tid + 64 < a.parts ? st[tid + 64] : none;
+    // a part counts -1 where the token is none
     const float all = wave_max(fmaxf(s.top, s2.top), lx);
     if (all < INFINITY) turn(s.sum, s.weighted, s.top, all), turn(s2.sum, s2.weighted, s2.top, all);
     const double sum = wave_sum64(s.sum + s2.sum, lx), weighted = wave_sum64(s.weighted + s2.weighted, lx);
     const double ahead = wave_sum64((double)s.ahead + s2.ahead, lx);
-    if (tid == 0) stat = Stat{sum, weighted, all, (int)ahead};
+    if (tid == 0) stat = Stat{sum, weighted, all, s.ahead < 0 ? -1 : (int)ahead, s.xt};
   }
   __syncthreads();
-  // no two candidates are alike, so that at most `top` threads have one at or above the edge
   if (top > 0) {
-    int above = 0;
-    for (int i = 0; i < kThreads; ++i) above += tops[i] > high;
-    if (above == top - 1 && high) line = high;
-    __syncthreads();
+    // at least `top` threads of a wave have a candidate whose logit is not below the edge
+    auto take = [&](uint64_t least) {
 #pragma unroll
-    for (int i = 0; i < kMaxParts * kMaxTop / kThreads; ++i)
-      if (mine[i] && mine[i] >= line) room[atomicAdd(&count, 1)] = mine[i];
+      for (int i = 0; i < kMaxParts * kMaxTop / kThreads; ++i)
+        if (mine[i] && mine[i] >= least) {
+          const int at = atomicAdd(&count, 1);
+          if (at < kRoom) room[at] = mine[i];
+        }
+    };
+    const uint64_t least = (uint64_t)(edge[0] > edge[1] ? edge[0] : edge[1]) << 32, others = (uint64_t)(edge[2] > edge[3] ? edge[2] : edge[3]) << 32;
+    if (high) take(least > others ? least : others);
     __syncthreads();
-    rank_all(room, count, best, top);
+    int many = count;
+    if (many > kRoom) {
+      // equal logits: no two candidates are alike, so that at most `top` threads have one at or above this edge
+      __syncthreads();
+      if (tid == 0) count = 0;
+      int above = 0;
+#pragma unroll 8
+      for (int i = 0; i < kThreads; ++i) above += tops[i] > high;
+      if (above == top - 1) line = high;
+      __syncthreads();
+      take(line);
+      __syncthreads();
+      many = count;
+    }
+    rank_all(room, many, best, top);
     __syncthreads();
   }
   const double log_sum = log(stat.sum);
-  if (tid == 0) write_row(a, row, t, xt, stat, log_sum);
+  if (tid == 0) write_row(a, row, stat.ahead < 0, stat, log_sum);
   if (tid < top) write_alternative(a, row, tid, best[tid], stat.top, log_sum);
 }
 
@@ -523,10 +569,7 @@ extern "C" int qs_token_logprobs(const void* logits, int dtype, int64_t ld, int6
   hipLaunchKernelGGL(kernel, dim3((unsigned)rows, (unsigned)l.parts), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("score_kernel");
   if (l.parts > 1) {
-    const auto join = dtype == QS_DTYPE_F32   ? score_join_kernel<float>
-                      : dtype == QS_DTYPE_F16 ? score_join_kernel<_Float16>
-                                              : score_join_kernel<uint16_t>;
-    hipLaunchKernelGGL(join, dim3((unsigned)rows), dim3(kThreads), 0, as_stream(stream), a);
+    hipLaunchKernelGGL(score_join_kernel, dim3((unsigned)rows), dim3(kThreads), 0, as_stream(stream), a);
     QS_LAUNCHED("score_join_kernel");
   }
   return QS_OK;
