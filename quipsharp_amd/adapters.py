@@ -40,52 +40,42 @@ def add_adapters(ys, x: Tensor, which: Tensor, downs, ups, scales, *, outs=None,
     or ``outs``, each of which is the y at its place itself or apart from all
     the call reads.  Sums are float32, rounded once at the end; the inner
     products go on with 16 significant bits or more."""
-    ys, downs, ups, scales = list(ys), list(downs), list(ups), list(scales)
     count = len(ys)
     if not 1 <= count <= _lib.QS_MAX_GROUP or not len(downs) == len(ups) == len(scales) == count:
         raise ValueError(f"{count} outputs for {len(downs)} / {len(ups)} / {len(scales)} adapters (1 to {_lib.QS_MAX_GROUP} linears)")
-    if x.dim() != 2:
-        raise ValueError(f"x must be (tokens, n), got {tuple(x.shape)}")
-    if x.dtype not in _HALF:
-        raise TypeError(f"unsupported dtype {x.dtype} (bfloat16 or float16)")
-    dev, dtype, (tokens, n) = x.device, x.dtype, x.shape
-    ldx = _rows("x", x, tokens, n, dtype, dev)
+    shape, st, dev, dtype = x.shape, x.stride(), x.device, x.dtype
+    if len(shape) != 2:
+        raise ValueError(f"x must be (tokens, n), got {tuple(shape)}")
+    if dtype not in _HALF:
+        raise TypeError(f"unsupported dtype {dtype} (bfloat16 or float16)")
+    tokens, n = shape
+    ldx = st[0] if st[1] == 1 and tokens > 1 else _rows("x", x, tokens, n, dtype, dev)
     _int32("which", which, (tokens,), dev)
+    adapters = downs[0].shape[0] if downs[0].dim() else 0
     if outs is None:
         outs = [torch.empty(tokens, y.shape[-1], dtype=dtype, device=dev) for y in ys]
-    else:
-        outs = list(outs)
-        if len(outs) != count:
-            raise ValueError(f"{len(outs)} outs for {count} linears")
-    if len({o.data_ptr() for o in outs}) < count and tokens:
+    elif len(outs) != count:
+        raise ValueError(f"{len(outs)} outs for {count} linears")
+    elif len({o.data_ptr() for o in outs}) < count and tokens:
         raise ValueError("every linear must have an output of its own")
-    adapters = None
-    jobs = (_lib.AdapterJob * count)()
-    ranks = (ctypes.c_int * count)()
-    for g, (y, o, down, up, scale) in enumerate(zip(ys, outs, downs, ups, scales)):
-        ldy, m = _rows(f"ys[{g}]", y, tokens, None, dtype, dev), y.shape[1]
-        ldo = ldy if o is y else _rows(f"outs[{g}]", o, tokens, m, dtype, dev)
-        if down.dim() != 3 or up.dim() != 3 or down.shape[2] != n or up.shape != (down.shape[0], m, down.shape[1]):
-            raise ValueError(f"adapters {g}: {tuple(down.shape)} and {tuple(up.shape)} for {n} inputs and {m} outputs")
-        adapters = down.shape[0] if adapters is None else adapters
-        rank = ranks[g] = down.shape[1]
-        if down.shape[0] != adapters:
-            raise ValueError(f"{down.shape[0]} adapters beside {adapters}")
-        if down.dtype is not dtype or up.dtype is not dtype:
-            raise TypeError(f"adapters {g} are {down.dtype} and {up.dtype}, x {dtype}")
-        if scale.dtype is not torch.float32 or scale.shape != (adapters,) or not scale.is_contiguous():
-            raise ValueError(f"scales[{g}] must be {adapters} contiguous float32 values, got {tuple(scale.shape)} x {scale.dtype}")
-        if down.device != dev or up.device != dev or scale.device != dev:
-            raise ValueError(f"adapters {g} are on {down.device}, {up.device} and {scale.device}, x on {dev}")
-        ds, us = down.stride(), up.stride()
-        if ds[2] != 1 or us[2] != 1:
-            raise ValueError("the elements of a row of an adapter must lie together (stride 1)")
-        if y.requires_grad or down.requires_grad or up.requires_grad or scale.requires_grad:
-            _lib.no_gradient("add_adapters")
+    jobs, ranks, grads = (_lib.AdapterJob * count)(), (ctypes.c_int * count)(), x.requires_grad
+    for g in range(count):
+        y, o, down, up, scale = ys[g], outs[g], downs[g], ups[g], scales[g]
+        ysh, yst, ost, dsh, ds, us = y.shape, y.stride(), o.stride(), down.shape, down.stride(), up.stride()
+        m = ysh[-1] if ysh else 0
+        # a decode step of one layer takes microseconds: what is refused is looked into only where something is
+        if not (len(ysh) == 2 and ysh[0] == tokens and o.shape == ysh and y.dtype is dtype and o.dtype is dtype and y.device == dev
+                and o.device == dev and yst[1] == 1 and ost[1] == 1 and len(dsh) == 3 and dsh[0] == adapters and dsh[2] == n
+                and up.shape == (adapters, m, dsh[1]) and down.dtype is dtype and up.dtype is dtype and ds[2] == 1 and us[2] == 1
+                and scale.dtype is torch.float32 and scale.shape == (adapters,) and scale.is_contiguous() and down.device == dev
+                and up.device == dev and scale.device == dev):
+            _refuse(g, y, o, down, up, scale, tokens, n, adapters, dtype, dev)
+        rank = ranks[g] = dsh[1]
+        grads = grads or y.requires_grad or down.requires_grad or up.requires_grad or scale.requires_grad
         jobs[g] = _lib.AdapterJob(down.data_ptr(), up.data_ptr(), scale.data_ptr(), ds[0] if adapters > 1 else 0, ds[1],
-                                  us[0] if adapters > 1 else 0, us[1] if m > 1 else rank, rank, m, y.data_ptr(), ldy,
-                                  o.data_ptr(), ldo)
-    if x.requires_grad:
+                                  us[0] if adapters > 1 else 0, us[1] if m > 1 else rank, rank, m, y.data_ptr(),
+                                  yst[0] if tokens > 1 else m, o.data_ptr(), ost[0] if tokens > 1 else m)
+    if grads:
         _lib.no_gradient("add_adapters")
     if adapters < 1:
         raise ValueError("no adapters")
@@ -96,6 +86,25 @@ def add_adapters(ys, x: Tensor, which: Tensor, downs, ups, scales, *, outs=None,
         _lib.check(L.qs_adapters_add(x.data_ptr(), _lib.dtype_code(dtype), ldx, tokens, n, which.data_ptr(), adapters,
                                      count, jobs, *_room(workspace), _lib.stream_of(x)))
     return outs
+
+
+def _refuse(g, y, o, down, up, scale, tokens, n, adapters, dtype, dev):
+    """Raises for linear g, in words; passes strides of a single column, which do not matter."""
+    _rows(f"ys[{g}]", y, tokens, None, dtype, dev)
+    m = y.shape[1]
+    _rows(f"outs[{g}]", o, tokens, m, dtype, dev)
+    if down.dim() != 3 or up.dim() != 3 or down.shape[2] != n or up.shape != (down.shape[0], m, down.shape[1]):
+        raise ValueError(f"adapters {g}: {tuple(down.shape)} and {tuple(up.shape)} for {n} inputs and {m} outputs")
+    if down.dtype is not dtype or up.dtype is not dtype:
+        raise TypeError(f"adapters {g} are {down.dtype} and {up.dtype}, x {dtype}")
+    if down.device != dev or up.device != dev or scale.device != dev:
+        raise ValueError(f"adapters {g} are on {down.device}, {up.device} and {scale.device}, x on {dev}")
+    if down.stride(2) != 1 or up.stride(2) != 1:
+        raise ValueError("the elements of a row of an adapter must lie together (stride 1)")
+    if down.shape[0] != adapters:
+        raise ValueError(f"{down.shape[0]} adapters beside {adapters}")
+    if scale.dtype is not torch.float32 or scale.shape != (adapters,) or not scale.is_contiguous():
+        raise ValueError(f"scales[{g}] must be {adapters} contiguous float32 values, got {tuple(scale.shape)} x {scale.dtype}")
 
 
 class Adapters:

@@ -18,6 +18,8 @@
 // the first, after an exact scaling of each token's by a power of two: what is
 // dropped lies 2^-16 (bf16) or 2^-22 (fp16) below the largest, and products
 // beyond fp16's range work.  All sums are fp32; the output is rounded once.
+#include <type_traits>
+
 #include "qs_attend_dev.h"
 
 namespace qs {
@@ -35,8 +37,7 @@ struct Linear {
   uint16_t* out;
   int64_t down_adapter, down_row, up_adapter, up_row, ldy, ldo, m;
   int rank, offset;  // offset: of its ranks among those of all linears
-  int first;         // its first work-group column of the second launch
-  int wide;          // y and out take 16-byte accesses
+  int first_run, first;  // its first work-group column of the first and the second launch
 };
 
 struct AdapterArgs {
@@ -45,7 +46,7 @@ struct AdapterArgs {
   const int32_t* which;
   int adapters, count, ranks;  // ranks: of all linears together
   int splits, steps;           // steps of 256 inputs of a split
-  int slots, chunks;           // work-groups that share a tile's groups; runs of kColumns of a work-group
+  int slots, chunks;           // work-groups that share a tile's groups, a power of two; runs of kColumns of a work-group
   float* part;                 // [splits][tokens][ranks]
   Linear linear[QS_MAX_GROUP];
 };
@@ -71,7 +72,7 @@ __device__ __forceinline__ void each_group(const AdapterArgs& a, int64_t t0, int
     const int adapter = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
     const uint64_t mine = __ballot(id == adapter);
     todo &= ~mine;
-    if (nth % a.slots != slot) continue;
+    if ((nth & (a.slots - 1)) != slot) continue;
     // a permutation of the lanes: the group's first, in order
     const uint64_t below = (1ull << lane) - 1;
     const int size = __popcll(mine);
@@ -86,69 +87,180 @@ __device__ __forceinline__ int place_in_tile(const Group& g, int c) {
   return __builtin_amdgcn_ds_bpermute(c * 4, g.inverse);
 }
 
-// One group of the first launch: NB blocks of 16 tokens, RB of 16 ranks.
+// One group of the first launch: NB blocks of 16 tokens, RB of 16 ranks from
+// rank0 on.  All that changes along the inputs is a scalar; a lane's places in
+// the rows are 32-bit offsets.
 template <bool BF, int RB, int NB>
-__device__ __forceinline__ void down_group(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, int split,
+__device__ __forceinline__ void down_group(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, int split, int rank0,
                                            f32x4 (*sums)[NB][64]) {
-  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, q = lane >> 4, r = lane & 15;
-  const uint16_t* rows[NB];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, q = lane >> 4, r = lane & 15;
+  const char* x = reinterpret_cast<const char*>(a.x + t0 * a.ldx);
+  const char* down = reinterpret_cast<const char*>(l.down + g.adapter * l.down_adapter);
+  uint32_t x_at[NB], down_at[RB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) rows[b] = a.x + (t0 + place_in_tile(g, 16 * b + r)) * a.ldx;
-  const uint16_t* down = l.down + g.adapter * l.down_adapter;
+  for (int b = 0; b < NB; ++b) x_at[b] = 2u * ((uint32_t)place_in_tile(g, 16 * b + r) * (uint32_t)a.ldx + 8 * q);
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    const int rank = rank0 + 16 * i + r;  // the sums of rows beyond go nowhere
+    down_at[i] = 2u * ((uint32_t)(rank < l.rank ? rank : l.rank - 1) * (uint32_t)l.down_row + 8 * q);
+  }
   f32x4 acc[RB][NB];
 #pragma unroll
   for (int i = 0; i < RB; ++i)
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[i][b] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int64_t k0 = (int64_t)split * a.steps * 256, k1 = k0 + a.steps * 256 < a.n ? k0 + a.steps * 256 : a.n;
-  // 64 inputs at a time: a lane's 16 lie together, 8 for each of two products
-  for (int64_t k = k0 + 64 * w; k < k1; k += 256) {
-    uint4 av[RB][2], xv[NB][2];
+  const int n = (int)a.n, k0 = split * a.steps * 256, k1 = k0 + a.steps * 256 < n ? k0 + a.steps * 256 : n;
+  // 64 inputs at a time, 32 for each of two products
+  uint4 xv[NB][2], av[RB][2];
+  auto load = [&](int k) {
+    const char *xk = x + 2 * (int64_t)k, *dk = down + 2 * (int64_t)k;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int64_t at = k + 16 * q + 8 * j;
-      const bool in = at < k1;
 #pragma unroll
-      for (int i = 0; i < RB; ++i)
-        av[i][j] = in && 16 * i + r < l.rank ? *reinterpret_cast<const uint4*>(down + (16 * i + r) * l.down_row + at) : uint4{};
+      for (int b = 0; b < NB; ++b) xv[b][j] = *reinterpret_cast<const uint4*>(xk + x_at[b] + 64 * j);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) xv[b][j] = in ? *reinterpret_cast<const uint4*>(rows[b] + at) : uint4{};
+      for (int i = 0; i < RB; ++i) av[i][j] = *reinterpret_cast<const uint4*>(dk + down_at[i] + 64 * j);
     }
+  };
+  auto multiply = [&]() {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < RB; ++i)
 #pragma unroll
         for (int b = 0; b < NB; ++b) acc[i][b] = mma_16x16x32<BF>(av[i][j], xv[b][j], acc[i][b]);
+  };
+  int k = k0 + 64 * w;
+  for (; k + 64 <= k1; k += 256) load(k), multiply();
+  if (k < k1) {
+    // fewer than 64 are left: zeros behind them
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const bool in = k + 32 * j + 8 * q < k1;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) xv[b][j] = in ? *reinterpret_cast<const uint4*>(x + 2 * (int64_t)k + x_at[b] + 64 * j) : uint4{};
+#pragma unroll
+      for (int i = 0; i < RB; ++i) av[i][j] = in ? *reinterpret_cast<const uint4*>(down + 2 * (int64_t)k + down_at[i] + 64 * j) : uint4{};
+    }
+    multiply();
   }
+  // the waves' sums together, a block of ranks at a time
+  float* part = a.part + ((int64_t)split * a.tokens + t0) * a.ranks + l.offset;
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) sums[w][b][lane] = acc[i][b];
     __syncthreads();
-    for (int e = tid; e < NB * 64; e += kThreads) {
-      const int b = e >> 6, c = 16 * b + (e & 15), rank = 16 * i + 4 * (e >> 4 & 3);
-      const f32x4 s = (sums[0][b][e & 63] + sums[1][b][e & 63]) + (sums[2][b][e & 63] + sums[3][b][e & 63]);
-      // all lanes take part in the exchange; e is a multiple of 64 and the lane
-      const int place = place_in_tile(g, c);
-      if (c < g.size && rank < l.rank)
-        *reinterpret_cast<f32x4*>(a.part + ((int64_t)split * a.tokens + t0 + place) * a.ranks + l.offset + rank) = s;
+    if (NB == 4 || w < NB) {
+      const int c = 16 * w + r, rank = rank0 + 16 * i + 4 * q;
+      const f32x4 s = (sums[0][w][lane] + sums[1][w][lane]) + (sums[2][w][lane] + sums[3][w][lane]);
+      const int place = place_in_tile(g, c);  // an exchange of all lanes
+      if (c < g.size && rank < l.rank) *reinterpret_cast<f32x4*>(part + place * a.ranks + rank) = s;
     }
     __syncthreads();
   }
 }
 
-template <bool BF, int RB, int NB>
-__global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
-  __shared__ f32x4 sums[4][NB][64];
-  const Linear& l = a.linear[blockIdx.x / a.splits];
-  const int split = blockIdx.x % a.splits;
-  const int64_t t0 = (int64_t)(blockIdx.y / a.slots) * kTile;
-  each_group(a, t0, blockIdx.y % a.slots, false, [&](const Group& g) {
-    if constexpr (NB > 1) {
-      if (g.size <= 16) return down_group<BF, RB, 1>(a, l, g, t0, split, reinterpret_cast<f32x4(*)[1][64]>(&sums[0][0][0]));
+// The same for more than 16 tokens: 64 tokens and 16 RB ranks by 64 inputs at a
+// time go straight to LDS, kAhead such stages ahead of their use, and each wave
+// multiplies its 16 tokens.  A row of a stage is eight pieces of 16 bytes, of
+// which piece p lies at place p ^ (row & 7), so that a wave's operands (one
+// piece of each of 16 rows) come from all banks.
+constexpr int kStageRow = 128, kAhead = 3;
+template <int RB>
+constexpr int stage_bytes() {
+  return (kTile + 16 * RB) * kStageRow;
+}
+
+template <bool BF, int RB>
+__device__ __forceinline__ void down_tile(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, int split, int rank0, char* stages) {
+  constexpr int NX = kTile / 32, NW = RB / 2, NL = NX + NW;  // loads of a wave in a stage, of 8 rows each
+  static_assert(RB % 2 == 0, "every wave brings as many rows");
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, q = lane >> 4, r = lane & 15;
+  const int n = (int)a.n, k0 = split * a.steps * 256, k1 = k0 + a.steps * 256 < n ? k0 + a.steps * 256 : n;
+  const int count = (k1 - k0 + 63) / 64, left = k1 - k0 - 64 * (count - 1);  // stages, inputs of the last
+  const int row8 = lane >> 3;  // of a load; every load begins at a multiple of 8 rows
+  const unsigned piece = 16 * ((lane & 7) ^ row8);
+  unsigned x_row[NX], down_row[NW], x_at[NX], down_at[NW];
+#pragma unroll
+  for (int j = 0; j < NX; ++j) x_row[j] = 2u * (uint32_t)place_in_tile(g, 8 * (NX * w + j) + row8) * (uint32_t)a.ldx, x_at[j] = x_row[j] + piece;
+#pragma unroll
+  for (int j = 0; j < NW; ++j) {
+    const int rank = rank0 + 8 * (NW * w + j) + row8;  // the sums of rows beyond go nowhere
+    down_row[j] = 2u * (uint32_t)(rank < l.rank ? rank : l.rank - 1) * (uint32_t)l.down_row, down_at[j] = down_row[j] + piece;
+  }
+  const char* x = reinterpret_cast<const char*>(a.x + t0 * a.ldx + k0);
+  const char* down = reinterpret_cast<const char*>(l.down + g.adapter * l.down_adapter + k0);
+  const unsigned lds = __builtin_amdgcn_readfirstlane(lds_address(stages));
+  auto fetch = [&](int s) {
+    const unsigned to = lds + (unsigned)(s % (kAhead + 1)) * stage_bytes<RB>();
+    if (s == count - 1 && left < 64) {
+      // pieces behind the last input: the last one again, which is not used
+      const unsigned end = 2u * (left - 8), p = piece < end ? piece : end;
+#pragma unroll
+      for (int j = 0; j < NX; ++j) x_at[j] = x_row[j] + p;
+#pragma unroll
+      for (int j = 0; j < NW; ++j) down_at[j] = down_row[j] + p;
     }
-    down_group<BF, RB, NB>(a, l, g, t0, split, sums);
+    load_rows(x + 128 * (int64_t)s, x_at, to + w * (NX * 1024));
+    load_rows(down + 128 * (int64_t)s, down_at, to + kTile * kStageRow + w * (NW * 1024));
+  };
+  f32x4 acc[RB];
+#pragma unroll
+  for (int i = 0; i < RB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const bool busy = 16 * w < g.size;
+#pragma unroll
+  for (int s = 0; s < kAhead; ++s)
+    if (s < count) fetch(s);
+  for (int s = 0; s < count; ++s) {
+    if (s + kAhead <= count) wait_loads<(kAhead - 1) * NL>();
+    else wait_loads<0>();
+    __syncthreads();
+    if (s + kAhead < count) fetch(s + kAhead);
+    if (busy) {
+      const char* at = stages + (s % (kAhead + 1)) * stage_bytes<RB>();
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const int p = 16 * ((4 * j + q) ^ (r & 7));
+        uint4 xv = *reinterpret_cast<const uint4*>(at + (16 * w + r) * kStageRow + p), av[RB];
+#pragma unroll
+        for (int i = 0; i < RB; ++i) av[i] = *reinterpret_cast<const uint4*>(at + (kTile + 16 * i + r) * kStageRow + p);
+        if (s == count - 1 && left < 64 && 32 * j + 8 * q >= left) {
+          xv = uint4{};
+#pragma unroll
+          for (int i = 0; i < RB; ++i) av[i] = uint4{};
+        }
+#pragma unroll
+        for (int i = 0; i < RB; ++i) acc[i] = mma_16x16x32<BF>(av[i], xv, acc[i]);
+      }
+    }
+  }
+  const int c = 16 * w + r, place = place_in_tile(g, c);
+  float* part = a.part + ((int64_t)split * a.tokens + t0 + place) * a.ranks + l.offset;
+#pragma unroll
+  for (int i = 0; i < RB; ++i) {
+    const int rank = rank0 + 16 * i + 4 * q;
+    if (c < g.size && rank < l.rank) *reinterpret_cast<f32x4*>(part + rank) = acc[i];
+  }
+  __syncthreads();  // the next group's stages lie where these did
+}
+
+// blockIdx.x: (linear, its run of 16 RB ranks, split), the split fastest.
+template <bool BF, int RB, bool MANY>
+__global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
+  constexpr int kSums = 4 * 64 * sizeof(f32x4), kStages = MANY ? (kAhead + 1) * stage_bytes<RB>() : 0;
+  __shared__ __align__(16) char room[kStages > kSums ? kStages : kSums];
+  const int split = blockIdx.x % a.splits, run = blockIdx.x / a.splits;
+  int gi = 0;
+  while (gi + 1 < a.count && run >= a.linear[gi + 1].first_run) ++gi;
+  const Linear& l = a.linear[gi];
+  const int rank0 = (run - l.first_run) * (16 * RB);
+  const int64_t t0 = (int64_t)(blockIdx.y / a.slots) * kTile;
+  each_group(a, t0, blockIdx.y & (a.slots - 1), false, [&](const Group& g) {
+    if constexpr (MANY) {
+      if (g.size > 16) return down_tile<BF, RB>(a, l, g, t0, split, rank0, room);
+    }
+    down_group<BF, RB, 1>(a, l, g, t0, split, rank0, reinterpret_cast<f32x4(*)[1][64]>(room));
   });
 }
 
@@ -172,14 +284,173 @@ __device__ __forceinline__ uint4 add_8(uint4 y, const f32x4& d0, const f32x4& d1
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// The second launch: a group's tokens against 64 columns a wave at a time.
-template <bool BF, int KB>
-__global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
-  constexpr int R = 32 * KB, kRow = R + 8;  // 16-bit elements of a token's row, 16 bytes further than the products need
-  __shared__ uint4 high[kTile * kRow / 8], low[kTile * kRow / 8];
-  __shared__ float factor[kTile];
-  __shared__ int token[kTile];
-  const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63, q = lane >> 4, r = lane & 15;
+// The inner products of N tokens of a group, summed over the splits, as two
+// 16-bit numbers: four ranks a thread, a token's R / 4 threads in one wave.
+template <bool BF, int R, int kRow, int N>
+__device__ __forceinline__ void inner_products(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, uint4* high,
+                                               uint4* low, float* factor) {
+  constexpr int T = R / 4, I = N * T / kThreads > 0 ? N * T / kThreads : 1, U = I < 2 ? 1 : 2;
+  const int tid = threadIdx.x;
+  if (N * T < kThreads && tid >= N * T) return;  // whole waves: N T is a multiple of 64
+  const float* base = a.part + t0 * a.ranks + l.offset;
+  const int64_t next = a.tokens * a.ranks;
+  const int rank = tid % T * 4;
+  const float scale = l.scale[g.adapter];
+#pragma unroll
+  for (int i0 = 0; i0 < I; i0 += U) {
+    f32x4 s[U];
+    uint32_t from[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      from[i] = (uint32_t)place_in_tile(g, (i0 + i) * (kThreads / T) + tid / T) * (uint32_t)a.ranks + (rank < l.rank ? rank : 0);
+      s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll 4
+    for (int p = 0; p < a.splits; ++p)
+#pragma unroll
+      for (int i = 0; i < U; ++i) s[i] += *reinterpret_cast<const f32x4*>(base + p * next + from[i]);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int c = (i0 + i) * (kThreads / T) + tid / T;
+      if (rank >= l.rank) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+      float most = fmaxf(fmaxf(fabsf(s[i][0]), fabsf(s[i][1])), fmaxf(fabsf(s[i][2]), fabsf(s[i][3])));
+#pragma unroll
+      for (int x = 1; x < T; x *= 2) most = fmaxf(most, __shfl_xor(most, x));
+      int e = (int)(__float_as_uint(most) >> 23);
+      e = e < 2 ? 2 : e > 252 ? 252 : e;
+      const float shrink = __uint_as_float((uint32_t)(254 - e) << 23);
+      uint32_t hi[2], lo[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float f0 = s[i][2 * x] * shrink, f1 = s[i][2 * x + 1] * shrink;
+        hi[x] = pack16<BF>(f0, f1);
+        const float h0 = float_of<BF>(hi[x] & 0xFFFF), h1 = float_of<BF>(hi[x] >> 16);
+        // an infinite product has no remainder
+        lo[x] = pack16<BF>(fabsf(h0) < INFINITY ? f0 - h0 : 0.f, fabsf(h1) < INFINITY ? f1 - h1 : 0.f);
+      }
+      const int at = (c * kRow + rank) / 4;
+      reinterpret_cast<uint2*>(high)[at] = make_uint2(hi[0], hi[1]), reinterpret_cast<uint2*>(low)[at] = make_uint2(lo[0], lo[1]);
+      if (rank == 0) factor[c] = __uint_as_float((uint32_t)e << 23) * scale;
+    }
+    __builtin_amdgcn_sched_barrier(0);  // more at a time would take more registers than the products
+  }
+}
+
+// The second launch: a group's tokens, NB blocks of 16, against 64 columns a
+// wave at a time.
+template <bool BF, int KB, int NB, bool WIDE>
+__device__ __forceinline__ void up_group(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, int64_t m_begin,
+                                         int64_t m_end, uint4* high, uint4* low, float* factor) {
+  constexpr int R = 32 * KB, kRow = R + 8;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, q = lane >> 4, r = lane & 15;
+  const char* up = reinterpret_cast<const char*>(l.up + g.adapter * l.up_adapter);
+  auto row_of = [&](int j) { return 32 * (j >> 1) + 8 * (r >> 2) + 4 * (j & 1) + (r & 3); };
+  uint32_t w_at[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w_at[j] = 2u * ((uint32_t)row_of(j) * (uint32_t)l.up_row + 8 * q);
+  auto weights = [&](int64_t m0, uint4 (&wv)[4][KB]) {
+    const char* from = up + 2 * m0 * l.up_row;
+    const int last = m0 + 64 <= l.m ? 63 : (int)(l.m - m0) - 1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t at = row_of(j) <= last ? w_at[j] : 2u * ((uint32_t)last * (uint32_t)l.up_row + 8 * q);
+#pragma unroll
+      for (int k = 0; k < KB; ++k)
+        wv[j][k] = 32 * k + 8 * q < l.rank ? *reinterpret_cast<const uint4*>(from + at + 64 * k) : uint4{};
+    }
+  };
+  // A lane's results of a token are columns m0 + 8 q .. + 7 and m0 + 32 + 8 q .. + 7, so that an access of the wave
+  // takes 64 bytes together of 16 rows.
+  const char* y0 = reinterpret_cast<const char*>(l.y + t0 * l.ldy);
+  char* out0 = reinterpret_cast<char*>(l.out + t0 * l.ldo);
+  uint32_t y_at[NB], out_at[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+    const uint32_t place = place_in_tile(g, 16 * b + r);
+    y_at[b] = 2u * (place * (uint32_t)l.ldy + 8 * q), out_at[b] = 2u * (place * (uint32_t)l.ldo + 8 * q);
+  }
+  uint4 wv[4][KB], y[NB][2];
+  auto load_y = [&](int b, int64_t m0) {
+    if constexpr (WIDE) {
+      const char* from = y0 + 2 * m0;
+      const int left = (int)(l.m - m0 < 64 ? l.m - m0 : 64) - 8 * q;
+      if (left > 0) y[b][0] = *reinterpret_cast<const uint4*>(from + y_at[b]);
+      if (left > 32) y[b][1] = *reinterpret_cast<const uint4*>(from + y_at[b] + 64);
+    }
+  };
+  int64_t m0 = m_begin + 64 * w;
+  if (m0 < m_end) {
+    weights(m0, wv);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) load_y(b, m0);
+  }
+  __syncthreads();  // the group before is done with the tables
+  inner_products<BF, R, kRow, 16 * NB>(a, l, g, t0, high, low, factor);
+  __syncthreads();
+  for (; m0 < m_end; m0 += kColumns) {
+    const bool more = m0 + kColumns < m_end;
+    const int left = (int)(l.m - m0 < 64 ? l.m - m0 : 64) - 8 * q;  // columns from the lane's first on
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int c = 16 * b + r;
+      f32x4 acc[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const uint4 h = high[(c * kRow + 32 * k + 8 * q) / 8], o = low[(c * kRow + 32 * k + 8 * q) / 8];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] = mma_16x16x32<BF>(wv[j][k], o, mma_16x16x32<BF>(wv[j][k], h, acc[j]));
+      }
+      if (b == NB - 1 && more) weights(m0 + kColumns, wv);
+      if (c < g.size) {
+        const float scale = factor[c];
+        char* to = out0 + 2 * m0;
+        if constexpr (WIDE) {
+          if (left > 0) *reinterpret_cast<uint4*>(to + out_at[b]) = add_8<BF>(y[b][0], acc[0], acc[1], scale);
+          if (left > 32) *reinterpret_cast<uint4*>(to + out_at[b] + 64) = add_8<BF>(y[b][1], acc[2], acc[3], scale);
+        } else {
+          const uint16_t* from = reinterpret_cast<const uint16_t*>(y0 + 2 * m0 + y_at[b]);
+          uint16_t* into = reinterpret_cast<uint16_t*>(to + out_at[b]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int at = 32 * (i >> 3) + (i & 7);  // behind the lane's first column
+            if (at < left) into[at] = (uint16_t)pack16<BF>(__builtin_fmaf(acc[i >> 2][i & 3], scale, float_of<BF>(from[at])), 0.f);
+          }
+        }
+      }
+      if (more) load_y(b, m0 + kColumns);
+      __builtin_amdgcn_sched_barrier(0);  // blocks that overlap would take twice the registers
+    }
+  }
+}
+
+// y of the tokens without an adapter goes on as it is, eight tokens of a wave at a time.
+template <bool WIDE>
+__device__ __forceinline__ void copy_group(const Linear& l, const Group& g, int64_t t0, int64_t m_begin, int64_t m_end) {
+  typedef typename std::conditional<WIDE, u32x4, uint16_t>::type Piece;
+  constexpr int W = sizeof(Piece) / 2, U = 8;
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  for (int c0 = w; c0 < g.size; c0 += 4 * U) {
+    int64_t t[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) t[i] = t0 + place_in_tile(g, c0 + 4 * i);  // the last token again behind it
+    for (int64_t m = m_begin + W * lane; m < m_end; m += 64 * W) {
+      Piece v[U];
+#pragma unroll
+      for (int i = 0; i < U; ++i) v[i] = *reinterpret_cast<const Piece*>(l.y + t[i] * l.ldy + m);
+#pragma unroll
+      for (int i = 0; i < U; ++i)
+        if (c0 + 4 * i < g.size) *reinterpret_cast<Piece*>(l.out + t[i] * l.ldo + m) = v[i];
+    }
+  }
+}
+
+template <bool BF, int KB, int NB, bool WIDE>
+__global__ __launch_bounds__(kThreads, NB == 1 ? 1 : KB == 4 ? 2 : 3) void adapter_up_kernel(AdapterArgs a) {
+  constexpr int kRow = 32 * KB + 8;  // 16-bit elements of a token's row, 16 bytes more than the products need
+  __shared__ uint4 high[16 * NB * kRow / 8], low[16 * NB * kRow / 8];
+  __shared__ float factor[16 * NB];
   int gi = 0;
   while (gi + 1 < a.count && (int)blockIdx.x >= a.linear[gi + 1].first) ++gi;
   const Linear& l = a.linear[gi];
@@ -187,119 +458,51 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
   const int64_t m_end = m_begin + a.chunks * kColumns < l.m ? m_begin + a.chunks * kColumns : l.m;
   const int64_t t0 = (int64_t)(blockIdx.y / a.slots) * kTile;
   each_group(a, t0, blockIdx.y % a.slots, l.out != l.y, [&](const Group& g) {
-    if (g.adapter < 0) {
-      for (int c = w; c < g.size; c += 4) {
-        const int64_t t = t0 + place_in_tile(g, c);
-        for (int64_t m = m_begin + lane; m < m_end; m += 64) l.out[t * l.ldo + m] = l.y[t * l.ldy + m];
-      }
-      return;
+    if (g.adapter < 0) return copy_group<WIDE>(l, g, t0, m_begin, m_end);
+    if constexpr (NB > 1) {
+      if (g.size <= 16) return up_group<BF, KB, 1, WIDE>(a, l, g, t0, m_begin, m_end, high, low, factor);
     }
-    __syncthreads();  // the group before is done with the tables
-    {
-      // four threads a token: its products, summed over the splits, each its quarter of the ranks
-      const int c = tid >> 2, j = tid & 3;
-      const int place = place_in_tile(g, c);
-      float v[R / 4], most = 0.f;
-#pragma unroll
-      for (int i = 0; i < R / 4; i += 4) {
-        f32x4 s{0.f, 0.f, 0.f, 0.f};
-        const int rank = j * (R / 4) + i;
-        if (c < g.size && rank < l.rank)
-          for (int p = 0; p < a.splits; ++p)
-            s += *reinterpret_cast<const f32x4*>(a.part + ((int64_t)p * a.tokens + t0 + place) * a.ranks + l.offset + rank);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[i + e] = s[e], most = fmaxf(most, fabsf(s[e]));
-      }
-      most = fmaxf(most, __shfl_xor(most, 1));
-      most = fmaxf(most, __shfl_xor(most, 2));
-      int e = (int)(__float_as_uint(most) >> 23);
-      e = e < 2 ? 2 : e > 252 ? 252 : e;
-      const float shrink = __uint_as_float((uint32_t)(254 - e) << 23);
-#pragma unroll
-      for (int i = 0; i < R / 4; i += 8) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float f0 = v[i + 2 * x] * shrink, f1 = v[i + 2 * x + 1] * shrink;
-          hi[x] = pack16<BF>(f0, f1);
-          const float h0 = float_of<BF>(hi[x] & 0xFFFF), h1 = float_of<BF>(hi[x] >> 16);
-          // an infinite product has no remainder
-          lo[x] = pack16<BF>(fabsf(h0) < INFINITY ? f0 - h0 : 0.f, fabsf(h1) < INFINITY ? f1 - h1 : 0.f);
-        }
-        const int at = (c * kRow + j * (R / 4) + i) / 8;
-        high[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]), low[at] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
-      if (j == 0) factor[c] = __uint_as_float((uint32_t)e << 23) * l.scale[g.adapter], token[c] = place;
-    }
-    __syncthreads();
-    const uint16_t* up = l.up + g.adapter * l.up_adapter;
-    const int blocks = (g.size + 15) / 16;
-    for (int64_t m0 = m_begin + 64 * w; m0 < m_end; m0 += kColumns) {
-      uint4 wv[4][KB];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        int64_t m = m0 + 16 * (r >> 2) + 4 * j + (r & 3);
-        m = m < l.m ? m : l.m - 1;
-#pragma unroll
-        for (int k = 0; k < KB; ++k)
-          wv[j][k] = 32 * k + 8 * q < l.rank ? *reinterpret_cast<const uint4*>(up + m * l.up_row + 32 * k + 8 * q) : uint4{};
-      }
-      const int64_t m = m0 + 16 * q;
-      for (int b = 0; b < blocks; ++b) {
-        const int c = 16 * b + r;
-        f32x4 acc[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < KB; ++k) {
-          const uint4 h = high[(c * kRow + 32 * k + 8 * q) / 8], o = low[(c * kRow + 32 * k + 8 * q) / 8];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[j] = mma_16x16x32<BF>(wv[j][k], o, mma_16x16x32<BF>(wv[j][k], h, acc[j]));
-        }
-        if (c < g.size && m < l.m) {
-          const int64_t t = t0 + token[c];
-          const float scale = factor[c];
-          const uint16_t* from = l.y + t * l.ldy + m;
-          uint16_t* to = l.out + t * l.ldo + m;
-          if (l.wide && m + 16 <= l.m) {
-            const uint4 y0 = *reinterpret_cast<const uint4*>(from), y1 = *reinterpret_cast<const uint4*>(from + 8);
-            *reinterpret_cast<uint4*>(to) = add_8<BF>(y0, acc[0], acc[1], scale);
-            *reinterpret_cast<uint4*>(to + 8) = add_8<BF>(y1, acc[2], acc[3], scale);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (m + i < l.m) to[i] = (uint16_t)pack16<BF>(__builtin_fmaf(acc[i >> 2][i & 3], scale, float_of<BF>(from[i])), 0.f);
-          }
-        }
-      }
-    }
+    up_group<BF, KB, NB, WIDE>(a, l, g, t0, m_begin, m_end, high, low, factor);
   });
 }
 
-template <bool BF, int NB>
-auto down_kernel(int rank) {
-  return rank <= 16 ? adapter_down_kernel<BF, 1, NB> : rank <= 32 ? adapter_down_kernel<BF, 2, NB>
-         : rank <= 64 ? adapter_down_kernel<BF, 4, NB> : adapter_down_kernel<BF, 8, NB>;
+template <bool BF>
+auto down_kernel(int blocks, bool many) {
+  if (many) return blocks <= 2 ? adapter_down_kernel<BF, 2, true> : adapter_down_kernel<BF, 4, true>;
+  return blocks == 1 ? adapter_down_kernel<BF, 1, false> : blocks == 2 ? adapter_down_kernel<BF, 2, false> : adapter_down_kernel<BF, 4, false>;
+}
+template <bool BF, int NB, bool WIDE>
+auto up_kernel(int rank) {
+  return rank <= 32 ? adapter_up_kernel<BF, 1, NB, WIDE> : rank <= 64 ? adapter_up_kernel<BF, 2, NB, WIDE> : adapter_up_kernel<BF, 4, NB, WIDE>;
 }
 template <bool BF>
-auto up_kernel(int rank) {
-  return rank <= 32 ? adapter_up_kernel<BF, 1> : rank <= 64 ? adapter_up_kernel<BF, 2> : adapter_up_kernel<BF, 4>;
+auto up_kernel(int rank, bool many, bool wide) {
+  if (many) return wide ? up_kernel<BF, 4, true>(rank) : up_kernel<BF, 4, false>(rank);
+  return wide ? up_kernel<BF, 1, true>(rank) : up_kernel<BF, 1, false>(rank);
 }
 
 struct Plan {
   int64_t tiles;
-  int slots, splits, steps;
+  int slots, blocks, runs;  // blocks of 16 ranks of a work-group, and work-groups for all of them
+  int splits, steps;
 };
 
-Plan plan_of(int64_t tokens, int64_t n, int64_t adapters, int count) {
+Plan plan_of(int64_t tokens, int64_t n, int64_t adapters, int count, const int* ranks) {
   Plan p;
   p.tiles = (tokens + kTile - 1) / kTile;
-  const int64_t most = tokens < kTile ? tokens : kTile, share = 64 / p.tiles > 4 ? 64 / p.tiles : 4;
-  int64_t slots = most < share ? most : share;
-  slots = slots < adapters + 1 ? slots : adapters + 1;
-  p.slots = (int)slots;
-  const int64_t steps = (n + 255) / 256, groups = p.tiles * (p.slots < 8 ? 1 : p.slots / 2) * count;
-  int64_t splits = (1024 + groups - 1) / groups;
+  const int64_t most = tokens < kTile ? tokens : kTile, share = p.tiles < 128 ? 128 / p.tiles : 1;
+  const int64_t slots = most < share ? most : share;
+  p.slots = 1;
+  while (p.slots < slots && p.slots < adapters + 1) p.slots *= 2;
+  int high = 0;
+  for (int g = 0; g < count; ++g) high = ranks[g] > high ? ranks[g] : high;
+  p.blocks = high > 32 ? 4 : high > 16 || tokens > 16 ? 2 : 1;
+  p.runs = 0;
+  for (int g = 0; g < count; ++g) p.runs += (ranks[g] + 16 * p.blocks - 1) / (16 * p.blocks);
+  const int64_t steps = (n + 255) / 256, groups = p.tiles * (p.slots < 8 ? 1 : p.slots / 2) * p.runs;
+  int64_t splits = 1;
+  if (p.tiles == 1) splits = (1024 + groups - 1) / groups;
+  else while (splits < 8 && groups * splits < (n <= 8192 ? 512 : 256)) splits *= 2;
   splits = splits < steps ? splits : steps;
   splits = splits < 16 ? splits : 16;
   p.steps = (int)((steps + splits - 1) / splits);
@@ -319,7 +522,7 @@ extern "C" size_t qs_adapters_workspace_bytes(int64_t tokens, int64_t n, int64_t
     if (ranks[g] < 1 || ranks[g] > kMaxRank) return 0;
     all += ranks[g];
   }
-  return (size_t)plan_of(tokens, n, adapters, count).splits * tokens * all * sizeof(float);
+  return (size_t)plan_of(tokens, n, adapters, count, ranks).splits * tokens * all * sizeof(float);
 }
 
 extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t tokens, int64_t n, const int32_t* which,
@@ -334,11 +537,12 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
                  (reinterpret_cast<uintptr_t>(x) & 15) == 0,
              "%s: %lld rows of %lld (a multiple of 8), %lld apart, %lld adapters; rows must be 16-byte aligned", fn,
              (long long)tokens, (long long)n, (long long)ldx, (long long)adapters);
-  QS_SUPPORTED(tokens <= (1 << 19) && n <= (1 << 24), "%s: %lld rows of %lld", fn, (long long)tokens, (long long)n);
+  QS_SUPPORTED(tokens <= (1 << 19) && ldx <= (1 << 24), "%s: %lld rows of %lld, %lld apart", fn, (long long)tokens, (long long)n, (long long)ldx);
   AdapterArgs a{};
   a.x = static_cast<const uint16_t*>(x), a.ldx = tokens == 1 ? 0 : ldx, a.tokens = tokens, a.n = n, a.which = which;
   a.adapters = (int)adapters, a.count = count;
-  int most = 0;
+  int most = 0, ranks[QS_MAX_GROUP];
+  bool wide = true;  // every y and out takes 16-byte accesses
   int64_t columns = 0;
   for (int g = 0; g < count; ++g) {
     const qs_adapter_job& j = jobs[g];
@@ -350,19 +554,22 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
                    (j.down_row | j.up_row | j.down_adapter | j.up_adapter) % 8 == 0 &&
                    ((reinterpret_cast<uintptr_t>(j.down) | reinterpret_cast<uintptr_t>(j.up)) & 15) == 0,
                "%s: linear %d: weights must be 16-byte aligned, rows %lld and %lld apart", fn, g, (long long)j.down_row, (long long)j.up_row);
+    QS_SUPPORTED(j.down_row <= (1 << 24) && j.up_row <= (1 << 24) && (tokens == 1 || (j.ldy <= (1 << 24) && j.ldo <= (1 << 24))),
+                 "%s: linear %d: weights' rows %lld and %lld apart, y and out %lld and %lld", fn, g, (long long)j.down_row, (long long)j.up_row, (long long)j.ldy, (long long)j.ldo);
     QS_REQUIRE(((reinterpret_cast<uintptr_t>(j.y) | reinterpret_cast<uintptr_t>(j.out)) & 1) == 0 && (reinterpret_cast<uintptr_t>(j.scale) & 3) == 0,
                "%s: linear %d: tensors must be aligned to their elements", fn, g);
     QS_REQUIRE(j.y != j.out || tokens == 1 || j.ldy == j.ldo, "%s: linear %d: y and out share memory with rows %lld and %lld apart", fn, g,
                (long long)j.ldy, (long long)j.ldo);
-    const bool wide = ((reinterpret_cast<uintptr_t>(j.y) | reinterpret_cast<uintptr_t>(j.out)) & 15) == 0 && (j.ldy | j.ldo) % 8 == 0;
+    wide = wide && ((reinterpret_cast<uintptr_t>(j.y) | reinterpret_cast<uintptr_t>(j.out)) & 15) == 0 && j.m % 8 == 0 &&
+           (tokens == 1 || (j.ldy | j.ldo) % 8 == 0);
     a.linear[g] = Linear{static_cast<const uint16_t*>(j.down), static_cast<const uint16_t*>(j.up), j.scale,
                          static_cast<const uint16_t*>(j.y), static_cast<uint16_t*>(j.out), j.down_adapter, j.down_row,
-                         j.up_adapter, j.up_row, tokens == 1 ? 0 : j.ldy, tokens == 1 ? 0 : j.ldo, j.m, j.rank, a.ranks, 0, wide};
-    a.ranks += j.rank;
+                         j.up_adapter, j.up_row, tokens == 1 ? 0 : j.ldy, tokens == 1 ? 0 : j.ldo, j.m, j.rank, a.ranks, 0, 0};
+    a.ranks += j.rank, ranks[g] = j.rank;
     most = j.rank > most ? j.rank : most;
     columns += (j.m + kColumns - 1) / kColumns;
   }
-  const Plan p = plan_of(tokens, n, adapters, count);
+  const Plan p = plan_of(tokens, n, adapters, count, ranks);
   a.slots = p.slots, a.splits = p.splits, a.steps = p.steps;
   const size_t need = (size_t)p.splits * tokens * a.ranks * sizeof(float);
   QS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
@@ -370,19 +577,21 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
   a.part = static_cast<float*>(workspace);
   // a work-group takes several runs of columns where there are tiles enough
   a.chunks = 1;
-  while (a.chunks < 8 && p.tiles * columns / (2 * a.chunks) >= 2048) a.chunks *= 2;
-  int grid = 0;
+  const int64_t groups = p.tiles * (p.slots < 8 ? 1 : p.slots / 2);
+  while (a.chunks < 8 && groups * columns / (2 * a.chunks) >= 512) a.chunks *= 2;
+  int grid = 0, run = 0;
   for (int g = 0; g < count; ++g) {
+    a.linear[g].first_run = run;
+    run += (ranks[g] + 16 * p.blocks - 1) / (16 * p.blocks);
     a.linear[g].first = grid;
     grid += (int)((a.linear[g].m + (int64_t)a.chunks * kColumns - 1) / ((int64_t)a.chunks * kColumns));
   }
   const bool bf = dtype == QS_DTYPE_BF16;
-  const auto down = tokens <= 16 ? (bf ? down_kernel<true, 1>(most) : down_kernel<false, 1>(most))
-                                 : (bf ? down_kernel<true, 4>(most) : down_kernel<false, 4>(most));
+  const auto down = bf ? down_kernel<true>(p.blocks, tokens > 16) : down_kernel<false>(p.blocks, tokens > 16);
   const unsigned rows = (unsigned)(p.tiles * p.slots);
-  hipLaunchKernelGGL(down, dim3((unsigned)(count * p.splits), rows), dim3(kThreads), 0, as_stream(stream), a);
+  hipLaunchKernelGGL(down, dim3((unsigned)(p.runs * p.splits), rows), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("adapter_down_kernel");
-  const auto up = bf ? up_kernel<true>(most) : up_kernel<false>(most);
+  const auto up = bf ? up_kernel<true>(most, tokens > 16, wide) : up_kernel<false>(most, tokens > 16, wide);
   hipLaunchKernelGGL(up, dim3((unsigned)grid, rows), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("adapter_up_kernel");
   return QS_OK;

@@ -104,7 +104,7 @@ def adapters_c(L, **over):
     (dict(x=None), 1, "null"), (dict(which=None), 1, "null"), (dict(dtype=0), 1, "dtype 0"), (dict(count=5), 1, "5 linears"),
     (dict(count=0), 1, "0 linears"), (dict(n=60), 1, "rows of 60"), (dict(ldx=56), 1, "56 apart"), (dict(ldx=68), 1, "68 apart"),
     (dict(adapters=0), 1, "0 adapters"), (dict(x=ctypes.c_void_p(4104)), 1, "16-byte aligned"),
-    (dict(tokens=(1 << 19) + 1), 3, "524289 rows"), (dict(down=None), 1, "linear 0: null"), (dict(scale=None), 1, "linear 0: null"),
+    (dict(tokens=(1 << 19) + 1), 3, "524289 rows"), (dict(ldx=(1 << 24) + 8), 3, "16777224 apart"), (dict(down_row=(1 << 24) + 8), 3, "rows 16777224 and 8 apart"), (dict(down=None), 1, "linear 0: null"), (dict(scale=None), 1, "linear 0: null"),
     (dict(rank=12), 1, "rank 12"), (dict(rank=136), 1, "rank 136"), (dict(rank=0), 1, "rank 0"), (dict(m=0), 1, "0 outputs"),
     (dict(ldy=39), 1, "39 and 40 apart"), (dict(ldo=39), 1, "40 and 39 apart"), (dict(down_row=56), 1, "rows 56"),
     (dict(up_row=12), 1, "and 12 apart"), (dict(down=4104), 1, "weights must be"), (dict(y=4097), 1, "aligned to their"),
