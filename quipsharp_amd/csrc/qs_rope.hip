@@ -17,6 +17,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kMaxPairs = 256;
 constexpr int kTable = 1024;  // sines and cosines of a work-group: tokens x pairs
+constexpr int kTokens = 64;   // of a work-group, at most
 
 struct RotateArgs {
   const uint16_t *q, *k, *v;
@@ -25,7 +26,8 @@ struct RotateArgs {
   const int32_t *starts, *over;
   const double* frequencies;
   float factor;
-  int rows, heads, kv_heads, head_dim, pairs, block;  // block: tokens of a work-group
+  int rows, heads, kv_heads, head_dim, pairs;
+  int block, lanes;  // tokens of a work-group; log2 of the threads of a head
 };
 
 // Where a token stands: its position (below 0: no row has it or it has none),
@@ -63,64 +65,65 @@ __device__ __forceinline__ Place place_of(const qs_page_pool& pool, const Rotate
 }
 
 template <bool BF>
-__device__ __forceinline__ float wide_of(uint16_t u) {
-  if constexpr (BF) return __uint_as_float((uint32_t)u << 16);
-  else return (float)__builtin_bit_cast(_Float16, u);
+__device__ __forceinline__ float wide_of(uint32_t u) {
+  if constexpr (BF) return __uint_as_float(u << 16);
+  else return (float)__builtin_bit_cast(_Float16, (uint16_t)u);
 }
 
-// W elements from one place (W 16-bit words, aligned to their size where that is a power of two).
+// W elements, in one access.
 template <int W>
-struct Words {
-  uint16_t w[W];
-  __device__ __forceinline__ void load(const uint16_t* p) {
-    if constexpr (W == 8) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
-    else if constexpr (W == 4) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
-    else
-#pragma unroll
-      for (int i = 0; i < W; ++i) w[i] = p[i];
-  }
-  __device__ __forceinline__ void store(uint16_t* p) const {
-    if constexpr (W == 8) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(w);
-    else if constexpr (W == 4) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(w);
-    else
-#pragma unroll
-      for (int i = 0; i < W; ++i) p[i] = w[i];
-  }
+struct Piece {
+  typedef uint32_t type __attribute__((ext_vector_type(W / 2)));
 };
+template <>
+struct Piece<1> {
+  typedef uint16_t type;
+};
+template <int W>
+using piece_t = typename Piece<W>::type;
+template <int W>
+__device__ __forceinline__ piece_t<W> get(const uint16_t* p) {
+  return *reinterpret_cast<const piece_t<W>*>(p);
+}
+template <int W>
+__device__ __forceinline__ void put(uint16_t* p, piece_t<W> v) {
+  *reinterpret_cast<piece_t<W>*>(p) = v;
+}
 
-// One unit of a head: W pairs turned, or W elements copied.  A thread reads all
-// of a unit before it writes it, so queries may be turned in place.
+// a and b of a pair at the angle whose cosine and sine are r.x and r.y, in 16 bits each.
+template <bool BF>
+__device__ __forceinline__ uint32_t turned(float a, float b, float2 r) {
+  return pack16<BF>(__builtin_fmaf(a, r.x, -b * r.y), __builtin_fmaf(b, r.x, a * r.y));
+}
+
+// W pairs, of which x and y are the 2 W elements in order: the first elements
+// of the pairs and the second ones, or pair by pair.
 template <bool BF, bool INTER, int W>
-__device__ __forceinline__ void turn_unit(const uint16_t* from, uint16_t* to, int u, int pairs, const float2* cs) {
-  Words<W> x, y;
-  const int n = pairs / W;
-  if (u >= n) {
-    const int at = 2 * pairs + (u - n) * W;
-    x.load(from + at);
-    x.store(to + at);
-    return;
-  }
-  const int i = u * W;
-  const int p0 = INTER ? 2 * i : i, p1 = INTER ? 2 * i + W : i + pairs;
-  x.load(from + p0), y.load(from + p1);
+__device__ __forceinline__ void turn(piece_t<W>& x, piece_t<W>& y, const float2* cs) {
+  if constexpr (W == 1) {
+    const uint32_t o = turned<BF>(wide_of<BF>(x), wide_of<BF>(y), cs[0]);
+    x = (uint16_t)o, y = (uint16_t)(o >> 16);
+  } else if constexpr (INTER) {
 #pragma unroll
-  for (int e = 0; e < W; ++e) {
-    // interleaved: pair e is elements 2 e and 2 e + 1 of the 2 W
-    uint16_t* pa = INTER ? (2 * e < W ? &x.w[2 * e] : &y.w[2 * e - W]) : &x.w[e];
-    uint16_t* pb = INTER ? (2 * e + 1 < W ? &x.w[2 * e + 1] : &y.w[2 * e + 1 - W]) : &y.w[e];
-    const float a = wide_of<BF>(*pa), b = wide_of<BF>(*pb);
-    const float2 r = cs[i + e];
-    const uint32_t o = pack16<BF>(__builtin_fmaf(a, r.x, -b * r.y), __builtin_fmaf(b, r.x, a * r.y));
-    *pa = (uint16_t)o, *pb = (uint16_t)(o >> 16);
+    for (int i = 0; i < W / 2; ++i) {
+      x[i] = turned<BF>(wide_of<BF>(x[i] & 0xFFFF), wide_of<BF>(x[i] >> 16), cs[i]);
+      y[i] = turned<BF>(wide_of<BF>(y[i] & 0xFFFF), wide_of<BF>(y[i] >> 16), cs[W / 2 + i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < W / 2; ++i) {
+      const uint32_t o0 = turned<BF>(wide_of<BF>(x[i] & 0xFFFF), wide_of<BF>(y[i] & 0xFFFF), cs[2 * i]);
+      const uint32_t o1 = turned<BF>(wide_of<BF>(x[i] >> 16), wide_of<BF>(y[i] >> 16), cs[2 * i + 1]);
+      x[i] = (o0 & 0xFFFF) | o1 << 16, y[i] = o0 >> 16 | (o1 & 0xFFFF0000u);
+    }
   }
-  x.store(to + p0), y.store(to + p1);
 }
 
 template <bool BF, bool INTER, int W>
 __global__ __launch_bounds__(kThreads) void append_rotated_kernel(qs_page_pool pool, RotateArgs a) {
   __shared__ float2 table[kTable];
-  __shared__ Place places[kTable];
-  __shared__ bool ours[kTable];
+  __shared__ Place places[kTokens];
+  __shared__ bool ours[kTokens];
   const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * a.block;
   const int n = a.tokens - t0 < a.block ? (int)(a.tokens - t0) : a.block;
@@ -139,45 +142,39 @@ __global__ __launch_bounds__(kThreads) void append_rotated_kernel(qs_page_pool p
   __syncthreads();
   const int per = (a.head_dim - a.pairs * 2) / W + a.pairs / W;  // units of a turned head
   const int all = a.heads + 2 * a.kv_heads;
-  // heads of this work-group: every gridDim.y-th
+  // heads of this work-group: every gridDim.y-th, 2^lanes threads a head
   const int mine = (all - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;
-  const int units = n * mine * per;
-  for (int i = tid; i < units; i += kThreads) {
-    const int u = i % per, h = i / per % mine * (int)gridDim.y + (int)blockIdx.y, b = i / per / mine;
+  const int step = kThreads >> a.lanes, pieces = a.pairs / W;
+  int b = 0, i = tid >> a.lanes;
+  for (;; i += step) {
+    while (i >= mine) i -= mine, ++b;
+    if (b >= n) break;
     if (!ours[b]) continue;
+    const int h = i * (int)gridDim.y + (int)blockIdx.y;
     const Place p = places[b];
     const int64_t t = t0 + b;
-    if (h < a.heads) {
-      uint16_t* to = a.q_out + t * a.out_token + (int64_t)h * a.head_dim;
-      if (p.pos >= 0) {
-        turn_unit<BF, INTER, W>(a.q + t * a.q_token + h * a.q_head, to, u, a.pairs, table + b * a.pairs);
+    // the head's source and destination, and what is done on the way
+    const bool query = h < a.heads, key = !query && h < a.heads + a.kv_heads;
+    if (!query && p.page < 0) continue;
+    const int g = query ? h : key ? h - a.heads : h - a.heads - a.kv_heads;
+    const uint16_t* from = query ? a.q + t * a.q_token + g * a.q_head : key ? a.k + t * a.k_token + g * a.k_head : a.v + t * a.v_token + g * a.v_head;
+    uint16_t* to = query ? a.q_out + t * a.out_token + (int64_t)g * a.head_dim
+                   : key ? static_cast<uint16_t*>(pool.k) + p.page * pool.k_page + g * pool.k_head + p.at * pool.k_pos
+                         : static_cast<uint16_t*>(pool.v) + p.page * pool.v_page + g * pool.v_head + p.at * pool.v_pos;
+    const bool nothing = p.pos < 0;  // zero queries
+    for (int u = tid & ((1 << a.lanes) - 1); u < per; u += 1 << a.lanes) {
+      if (u < pieces) {
+        // both are read before either is written, so queries may be turned in place
+        const int at0 = INTER ? 2 * u * W : u * W, at1 = INTER ? 2 * u * W + W : u * W + a.pairs;
+        piece_t<W> x = get<W>(from + at0), y = get<W>(from + at1);
+        if (query || key) turn<BF, INTER, W>(x, y, table + b * a.pairs + u * W);
+        if (nothing) x = piece_t<W>{}, y = piece_t<W>{};
+        put<W>(to + at0, x), put<W>(to + at1, y);
       } else {
-        const Words<W> zero{};
-        const int m = a.pairs / W;
-        if (u >= m) {
-          zero.store(to + 2 * a.pairs + (u - m) * W);
-        } else {
-          zero.store(to + (INTER ? 2 * u * W : u * W));
-          zero.store(to + (INTER ? 2 * u * W + W : u * W + a.pairs));
-        }
-      }
-    } else if (p.page >= 0) {
-      const int g = h - a.heads;
-      if (g < a.kv_heads) {
-        uint16_t* to = static_cast<uint16_t*>(pool.k) + p.page * pool.k_page + g * pool.k_head + p.at * pool.k_pos;
-        turn_unit<BF, INTER, W>(a.k + t * a.k_token + g * a.k_head, to, u, a.pairs, table + b * a.pairs);
-      } else {
-        const int gv = g - a.kv_heads;
-        uint16_t* to = static_cast<uint16_t*>(pool.v) + p.page * pool.v_page + gv * pool.v_head + p.at * pool.v_pos;
-        const uint16_t* from = a.v + t * a.v_token + gv * a.v_head;
-        const int m = a.pairs / W;
-        Words<W> x;
-        if (u >= m) {
-          x.load(from + 2 * a.pairs + (u - m) * W), x.store(to + 2 * a.pairs + (u - m) * W);
-        } else {
-          x.load(from + 2 * u * W), x.store(to + 2 * u * W);
-          x.load(from + 2 * u * W + W), x.store(to + 2 * u * W + W);
-        }
+        const int at = 2 * a.pairs + (u - pieces) * W;
+        piece_t<W> x = get<W>(from + at);
+        if (nothing) x = piece_t<W>{};
+        put<W>(to + at, x);
       }
     }
   }
@@ -219,16 +216,19 @@ extern "C" int qs_page_append_rotated(const void* q, const void* k, const void* 
   QS_REQUIRE((reinterpret_cast<uintptr_t>(frequencies) & 7) == 0, "%s: frequencies must be 8-byte aligned", fn);
   const int all = heads + 2 * kv_heads;
   QS_SUPPORTED((int64_t)all * head_dim <= (1 << 24), "%s: %d heads of %d", fn, all, head_dim);
-  int block = kTable / pairs;
+  int block = kTable / pairs < kTokens ? kTable / pairs : kTokens;
   while (block > 1 && (tokens < 512 * (int64_t)block || (int64_t)block * all * head_dim > (1 << 30))) block /= 2;
   const int64_t blocks = (tokens + block - 1) / block;
   int split = 1;
   while (split * 4 <= all && blocks * split < 512) split *= 2;
   const int rest = head_dim - 2 * pairs;
   const int w = pairs % 8 == 0 && rest % 8 == 0 ? 8 : pairs % 4 == 0 && rest % 4 == 0 ? 4 : 1;
+  const int per = rest / w + pairs / w;
+  int lanes = 0;
+  while (lanes < 8 && 1 << lanes < per) ++lanes;
   const RotateArgs a{static_cast<const uint16_t*>(q), static_cast<const uint16_t*>(k), static_cast<const uint16_t*>(v),
                      static_cast<uint16_t*>(q_out), q_token, q_head, k_token, k_head, v_token, v_head, out_token, tokens,
-                     starts, over, frequencies, factor, (int)rows, heads, kv_heads, head_dim, pairs, block};
+                     starts, over, frequencies, factor, (int)rows, heads, kv_heads, head_dim, pairs, block, lanes};
   const auto kernel = dtype == QS_DTYPE_BF16 ? (interleaved ? rotated_kernel<true, true>(w) : rotated_kernel<true, false>(w))
                                              : (interleaved ? rotated_kernel<false, true>(w) : rotated_kernel<false, false>(w));
   hipLaunchKernelGGL(kernel, dim3((unsigned)blocks, (unsigned)split), dim3(kThreads), 0, as_stream(stream), *pool, a);
