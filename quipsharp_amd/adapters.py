@@ -153,3 +153,16 @@ def beside(x: Tensor, linears, ys, which: Tensor):
         add_adapters(own, x, which, [a.down for _, a in with_some], [a.up for _, a in with_some],
                      [a.scale for _, a in with_some], outs=own)
     return ys
+
+
+def attach_adapters(model, count, rank, names=("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj"),
+                    dtype=torch.bfloat16):
+    """Gives every ``QuantizedLinear`` of ``model`` whose last name is among
+    ``names`` room for ``count`` adapters of rank ``rank``, empty at first, in
+    its attribute ``adapters``.  Returns them by the linears' names."""
+    from .checkpoint import QuantizedLinear
+    out = {}
+    for name, lin in model.named_modules():
+        if isinstance(lin, QuantizedLinear) and name.rpartition(".")[2] in names:
+            lin.adapters = out[name] = Adapters(count, rank, lin.in_features, lin.out_features, dtype, lin.codes.device)
+    return out

@@ -20,7 +20,7 @@ from torch import nn
 
 from .architectures import get_decoder_layers, get_linear_groups
 from .checkpoint import (QuantizedLinear, build_codebook, grouped_forward, grouped_forward_pre,
-                         link_sibling_linears)
+                         link_sibling_linears, run_preop)
 from .hadamard import is_pow2, kron_factor, rademacher
 
 QWEN3_32B = dict(hidden_size=5120, intermediate_size=25600, num_hidden_layers=64, num_attention_heads=64,
@@ -136,7 +136,8 @@ class StaticDecoder:
         self.model = model
         self.layers = get_decoder_layers(model)
         self.B, self.max_len = batch, max_len
-        self.nh, self.nkv, self.hd = cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        self.nh, self.nkv = cfg.num_attention_heads, cfg.num_key_value_heads
+        self.hd = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.nh
         self.hidden = cfg.hidden_size
         self.eps = float(cfg.rms_norm_eps)
         self.scale = self.hd ** -0.5
@@ -219,25 +220,31 @@ class StaticDecoder:
             a = Ly.self_attn
             # residual add + input norm inside the q/k/v launch (one row; on
             # their own launch otherwise)
-            qo, ko, vo = grouped_forward_pre(h, [a.q_proj, a.k_proj, a.v_proj],
-                                             {"kind": "rmsnorm", "delta": delta, "h_out": h_alt, "eps": self.eps,
-                                              "weight": self._weight(Ly.input_layernorm)})
+            qo, ko, vo = self._normed_linears(h, [a.q_proj, a.k_proj, a.v_proj],
+                                              {"kind": "rmsnorm", "delta": delta, "h_out": h_alt, "eps": self.eps,
+                                               "weight": self._weight(Ly.input_layernorm)})
             h, h_alt = h_alt, h
-            self._attend(i, qo.contiguous(), ko.contiguous(), vo.contiguous(),
-                         (self._weight(a.q_norm), self._weight(a.k_norm)), pos, attn, stream)
-            o = a.o_proj(attn).contiguous()
-            go, uo = grouped_forward_pre(h, [Ly.mlp.gate_proj, Ly.mlp.up_proj],
-                                         {"kind": "rmsnorm", "delta": o, "h_out": h_alt, "eps": self.eps,
-                                          "weight": self._weight(Ly.post_attention_layernorm)})
+            norms = (self._weight(a.q_norm), self._weight(a.k_norm)) if hasattr(a, "q_norm") else None
+            self._attend(i, qo.contiguous(), ko.contiguous(), vo.contiguous(), norms, pos, attn, stream)
+            o = self._linear(attn, a.o_proj).contiguous()
+            go, uo = self._normed_linears(h, [Ly.mlp.gate_proj, Ly.mlp.up_proj],
+                                          {"kind": "rmsnorm", "delta": o, "h_out": h_alt, "eps": self.eps,
+                                           "weight": self._weight(Ly.post_attention_layernorm)})
             h, h_alt = h_alt, h
             go, uo = go.contiguous(), uo.contiguous()
             act = torch.empty_like(go)
             inter = go.shape[-1]
             lib.check(L.qs_dec_silu_mul(vp(go), vp(uo), vp(act), B, inter, inter, inter, inter, stream))
-            delta = Ly.mlp.down_proj(act).contiguous()
+            delta = self._linear(act, Ly.mlp.down_proj).contiguous()
         x = torch.empty_like(h)
         lib.check(L.qs_dec_rmsnorm(vp(h), vp(delta), vp(h), vp(self._weight(m.norm)), vp(x), B, H, H, self.eps, stream))
         return self.model.lm_head(x)
+
+    def _normed_linears(self, h, linears, pre):
+        return grouped_forward_pre(h, linears, pre)
+
+    def _linear(self, x, linear):
+        return linear(x)
 
     def _attend(self, i, qo, ko, vo, norms, pos, out, stream):
         """q/k norm, rotary and the cache write inside the attention's launches."""
@@ -299,6 +306,13 @@ class PagedDecoder(StaticDecoder):
     fell out are given back).  Everything that a step needs to know of its rows
     lies on the GPU, so a step can be captured once and replayed.
 
+    Layers with q/k norms (Qwen3) have heads of 128; of those without (Llama,
+    Qwen2: model types ``llama`` and ``qwen2``) heads of 64, 128 or 256 turn by
+    ``rope.append_rotated`` with the config's frequencies, stretched contexts
+    included.  Where linears have adapters (``adapters.attach_adapters``),
+    ``which`` (int32 on the GPU, one for every row, -1 for none) says which of
+    them a row takes; a captured step follows it, and rows that fork keep it.
+
     Rows of at most ``max_len`` positions (rounded up to whole pages).  A step
     that runs out of pages or of positions leaves tokens out; it does not wait
     to say so, ``cache.check()`` and the next ``prompt`` raise for it."""
@@ -307,55 +321,123 @@ class PagedDecoder(StaticDecoder):
         from .pages import PagedCache
         columns = -(-max_len // page)
         super().__init__(model, rows, columns * page, cache=False)  # rotary tables to the last page's end
-        if not self.fused_ok:
-            raise ValueError("the paged decode step takes head_dim 128 and at most 16 query heads per kv head")
+        self.normed = all(hasattr(L.self_attn, "q_norm") for L in self.layers)
+        if self.normed:
+            if not self.fused_ok:
+                raise ValueError("the paged decode step takes head_dim 128 and at most 16 query heads per kv head")
+        else:
+            from .rope import model_frequencies
+            cfg = model.config
+            if cfg.model_type not in ("llama", "qwen2") or any(hasattr(L.self_attn, "q_norm") for L in self.layers) \
+                    or any(t != "full_attention" for t in getattr(cfg, "layer_types", None) or ()):
+                raise ValueError(f"the paged decoder takes models of type qwen3, llama and qwen2 whose layers see all of a "
+                                 f"row, not {cfg.model_type}")
+            if self.hd not in (64, 128, 256) or self.nh % self.nkv or self.nh // self.nkv > 16 or self.hidden % 8:
+                raise ValueError(f"the paged decode step takes heads of 64, 128 or 256, at most 16 of them per kv head, got "
+                                 f"{self.nh} and {self.nkv} of {self.hd}")
+            self.frequencies, self.turn_factor = model_frequencies(cfg, self.dev)
         self.window, self.sinks = window, sinks
         self.cache = PagedCache(len(self.layers), rows * columns if pages is None else pages, self.nkv, self.hd, rows,
                                 columns, page, torch.bfloat16, self.dev)
         self.spans = {"window": window, "sinks": sinks}
+        self.which = torch.full((rows,), -1, dtype=torch.int32, device=self.dev)
+        self._tokens_which = self.which  # of the tokens at hand: the rows', or a prompt's
 
-    @torch.no_grad()
-    def prompt(self, ids, counts):
-        """``counts[r]`` new tokens of row r (0: the row waits), their ids one
-        row after the other in ``ids``.  Logits of every row's last token, for
-        the rows with tokens."""
-        from transformers.models.qwen3.modeling_qwen3 import apply_rotary_pos_emb
+    def _adapted(self):
+        return any(getattr(mod, "adapters", None) is not None for L in self.layers for mod in
+                   [*L.self_attn.children(), *L.mlp.children()])
+
+    def _beside(self, x, linears, outs):
+        """The outputs of ``linears`` for x, with the adapters of the tokens' rows."""
+        if all(getattr(l, "adapters", None) is None for l in linears):
+            return outs
+        from .adapters import beside
+        flat = [y.reshape(-1, y.shape[-1]) for y in outs]
+        return [f.view(y.shape) for f, y in
+                zip(beside(x.reshape(-1, x.shape[-1]), linears, flat, self._tokens_which), outs)]
+
+    def _normed_linears(self, h, linears, pre):
+        if all(getattr(l, "adapters", None) is None for l in linears):
+            return grouped_forward_pre(h, linears, pre)
+        x = run_preop(h, pre)  # the adapters read the normed rows too
+        return self._beside(x, linears, grouped_forward(x, linears))
+
+    def _linear(self, x, linear):
+        return self._beside(x, [linear], [linear(x)])[0]
+
+    def _prompt_hidden(self, ids, counts):
+        """The last layer's normed output for all tokens of a prompt call, and the rows' first tokens and counts."""
         m, cache = self.model.model, self.cache
         T = int(sum(counts))
         if ids.shape != (T,) or len(counts) != self.B:
             raise ValueError(f"ids {tuple(ids.shape)} for {T} tokens in {len(counts)} of {self.B} rows")
         count = torch.tensor(counts, dtype=torch.int32)
         starts = torch.cat([torch.zeros(1, dtype=torch.int32), count.cumsum(0, dtype=torch.int32)]).to(self.dev)
-        last = (count.cumsum(0) - 1)[count > 0].to(self.dev)
         row = torch.repeat_interleave(torch.arange(self.B), count).to(self.dev)
         cache.advance(count.to(self.dev))
         cache.check()
-        pos = (cache.lengths + cache.over)[row] - starts[row + 1] + torch.arange(T, device=self.dev)
         h = m.embed_tokens(ids)[None]
-        cos, sin = m.rotary_emb(h, pos[None])
+        if self.normed:
+            from transformers.models.qwen3.modeling_qwen3 import apply_rotary_pos_emb
+            pos = (cache.lengths + cache.over)[row] - starts[row + 1] + torch.arange(T, device=self.dev)
+            cos, sin = m.rotary_emb(h, pos[None])
+        self._tokens_which = self.which[row]
+        bf = torch.bfloat16
         for i, L in enumerate(self.layers):
             a = L.self_attn
             x = L.input_layernorm(h)
-            qo, ko, vo = grouped_forward(x, [a.q_proj, a.k_proj, a.v_proj])
-            q = a.q_norm(qo.view(1, T, self.nh, self.hd)).transpose(1, 2)
-            k = a.k_norm(ko.view(1, T, self.nkv, self.hd)).transpose(1, 2)
-            q, k = apply_rotary_pos_emb(q, k, cos, sin)
-            bf = torch.bfloat16
-            cache.append(i, k[0].transpose(0, 1).to(bf).contiguous(), vo.view(T, self.nkv, self.hd).to(bf), starts)
-            o = cache.attend_chunk(i, q[0].transpose(0, 1).to(bf).contiguous(), starts, scale=self.scale, **self.spans)
-            h = h + a.o_proj(o.view(1, T, self.nh * self.hd).to(h.dtype))
+            qo, ko, vo = self._beside(x, [a.q_proj, a.k_proj, a.v_proj], grouped_forward(x, [a.q_proj, a.k_proj, a.v_proj]))
+            if self.normed:
+                q = a.q_norm(qo.view(1, T, self.nh, self.hd)).transpose(1, 2)
+                k = a.k_norm(ko.view(1, T, self.nkv, self.hd)).transpose(1, 2)
+                q, k = apply_rotary_pos_emb(q, k, cos, sin)
+                q = q[0].transpose(0, 1).to(bf).contiguous()
+                cache.append(i, k[0].transpose(0, 1).to(bf).contiguous(), vo.view(T, self.nkv, self.hd).to(bf), starts)
+            else:
+                q, k, v = (t.view(T, heads, self.hd).to(bf) for t, heads in ((qo, self.nh), (ko, self.nkv), (vo, self.nkv)))
+                q = cache.append_rotated(i, q, k, v, self.frequencies, starts, factor=self.turn_factor, out=q)
+            o = cache.attend_chunk(i, q, starts, scale=self.scale, **self.spans)
+            h = h + self._linear(o.view(1, T, self.nh * self.hd).to(h.dtype), a.o_proj)
             x = L.post_attention_layernorm(h)
-            go, uo = grouped_forward(x, [L.mlp.gate_proj, L.mlp.up_proj])
-            h = h + L.mlp.down_proj(L.mlp.act_fn(go) * uo)
+            go, uo = self._beside(x, [L.mlp.gate_proj, L.mlp.up_proj], grouped_forward(x, [L.mlp.gate_proj, L.mlp.up_proj]))
+            h = h + self._linear(L.mlp.act_fn(go) * uo, L.mlp.down_proj)
+        self._tokens_which = self.which
         if self.window:
             cache.free(window=self.window, sinks=self.sinks)
-        return self.model.lm_head(m.norm(h[0, last]))
+        return h[0], count
+
+    @torch.no_grad()
+    def prompt(self, ids, counts):
+        """``counts[r]`` new tokens of row r (0: the row waits), their ids one
+        row after the other in ``ids``.  Logits of every row's last token, for
+        the rows with tokens."""
+        h, count = self._prompt_hidden(ids, counts)
+        last = (count.cumsum(0) - 1)[count > 0].to(self.dev)
+        return self.model.lm_head(self.model.model.norm(h[last]))
+
+    @torch.no_grad()
+    def score(self, ids, counts, top=0, rows=1024):
+        """``prompt`` with scores in place of logits (``logprobs.token_logprobs``): entry t is about the token behind
+        ids[t] in its row, of which the row's last has none (log probability 0, rank -1; its entropy and alternatives
+        are those of the token to come).  The logits of ``rows`` tokens are there at a time."""
+        from .logprobs import token_logprobs
+        h, count = self._prompt_hidden(ids, counts)
+        behind = torch.full_like(ids, -100)
+        behind[:-1] = ids[1:]
+        behind[(count.cumsum(0) - 1)[count > 0].to(self.dev)] = -100
+        norm, head = self.model.model.norm, self.model.lm_head
+        parts = [token_logprobs(head(norm(x)), t.contiguous(), top) for x, t in zip(h.split(rows), behind.split(rows))]
+        return tuple(torch.cat(p) for p in zip(*parts))
 
     @torch.no_grad()
     def step(self, ids, parents=None):
         """One new token for every row, ids (rows,) or (rows, 1): row i goes on
-        from row ``parents[i]`` (int32; None: its own).  Logits (rows, vocab)."""
+        from row ``parents[i]`` (int32; None: its own), with that row's
+        adapters.  Logits (rows, vocab)."""
         self.cache.advance(1, parents)
+        if parents is not None and self._adapted():
+            named = (parents >= 0) & (parents < self.B)
+            self.which.copy_(torch.where(named, self.which[parents.clamp(0, self.B - 1).long()], -1))
         logits = self._decode_step(ids.reshape(-1, 1), None)
         if self.window:
             self.cache.free(window=self.window, sinks=self.sinks)
@@ -364,20 +446,90 @@ class PagedDecoder(StaticDecoder):
     def _attend(self, i, qo, ko, vo, norms, pos, out, stream):
         from .pages import _pool
         c, vp = self.cache, self._lib.ptr
-        q = torch.empty_like(out)
-        self._lib.check(self._L.qs_page_append_rope_over(
-            vp(qo), vp(ko), vp(vo), vp(norms[0]), vp(norms[1]), vp(self.cos), vp(self.sin), self.cos.shape[0], vp(q),
-            self.B, self.nh, self.nkv, self.hd, _pool(c.keys(i), c.values(i), c.table, c.lengths), vp(c.over), self.eps,
-            stream))
         heads = (self.B, self.nh, self.hd)
-        c.attend_token(i, q.view(heads), scale=self.scale, out=out.view(heads), **self.spans)
+        if norms is None:
+            kv = (self.B, self.nkv, self.hd)
+            q = c.append_rotated(i, qo.view(heads), ko.view(kv), vo.view(kv), self.frequencies, factor=self.turn_factor,
+                                 out=qo.view(heads))
+        else:
+            q = torch.empty_like(out)
+            self._lib.check(self._L.qs_page_append_rope_over(
+                vp(qo), vp(ko), vp(vo), vp(norms[0]), vp(norms[1]), vp(self.cos), vp(self.sin), self.cos.shape[0], vp(q),
+                self.B, self.nh, self.nkv, self.hd, _pool(c.keys(i), c.values(i), c.table, c.lengths), vp(c.over),
+                self.eps, stream))
+            q = q.view(heads)
+        c.attend_token(i, q, scale=self.scale, out=out.view(heads), **self.spans)
 
 
 @torch.no_grad()
-def beam_decode(model, prompts, beams, new_tokens, eos=-1, use_graph=True, page=64):
+def greedy_decode_paged(model, prompts, new_tokens, which=None, top=0, use_graph=True, page=64):
+    """Greedy decode of prompts of any lengths (a list of 1-D id tensors), each with the adapters that ``which`` (a
+    number for every prompt, -1 for none) names, and the log probabilities of what they take.  Steps are replays of one
+    HIP graph unless use_graph=False.  Returns (tokens (prompts, new_tokens), their scores: log probabilities, entropies
+    (prompts, new_tokens), the ``top`` best tokens' log probabilities and ids (prompts, new_tokens, top))."""
+    from .logprobs import token_logprobs
+    R, dev = len(prompts), prompts[0].device
+    dec = PagedDecoder(model, R, max(len(p) for p in prompts) + new_tokens, page)
+    if which is not None:
+        dec.which.copy_(torch.as_tensor(which, dtype=torch.int32))
+    logits = dec.prompt(torch.cat(list(prompts)), [len(p) for p in prompts])
+    shapes = (((), torch.int32), ((), torch.float32), ((), torch.float32), ((top,), torch.float32), ((top,), torch.int32))
+    out = [torch.zeros(R, new_tokens, *more, dtype=kind, device=dev) for more, kind in shapes]
+    last = torch.zeros(R, dtype=torch.int32, device=dev)
+    at = torch.zeros(1, dtype=torch.long, device=dev)
+
+    def take(logits):
+        last.copy_(logits.argmax(-1))
+        logp, entropy, _, best, tokens = token_logprobs(logits, last, top)
+        for o, new in zip(out, (last, logp, entropy, best, tokens)):
+            o.index_copy_(1, at, new.unsqueeze(1))
+        at.add_(1)
+
+    def step():
+        take(dec.step(last.long()))
+
+    take(logits)
+    todo, go = new_tokens - 1, step
+    if use_graph and todo > 1:
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            step()
+        torch.cuda.current_stream().wait_stream(s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        todo, go = todo - 1, graph.replay
+    for _ in range(todo):
+        go()
+    dec.cache.check()
+    return (out[0].long(), *out[1:])
+
+
+@torch.no_grad()
+def perplexity(model, ids, window=2048):
+    """The perplexity of a text's ids (n,) under any causal LM, over windows of ``window`` tokens that do not overlap,
+    each token given those before it in its window (as scripts/eval_ppl.py:41-65 takes it)."""
+    from .logprobs import token_logprobs
+    total, count = 0.0, 0
+    for part in ids.split(window):
+        if len(part) < 2:
+            continue
+        logits = model(input_ids=part[None], use_cache=False).logits[0, :-1]
+        total = total - token_logprobs(logits, part[1:].contiguous())[0].double().sum()
+        count += len(part) - 1
+    if not count:
+        raise ValueError(f"{len(ids)} ids in windows of {window}: no token has one before it")
+    return float(torch.exp(total / count))
+
+
+@torch.no_grad()
+def beam_decode(model, prompts, beams, new_tokens, eos=-1, use_graph=True, page=64, which=None):
     """Beam search: the ``beams`` best continuations of each prompt (a list of
     1-D id tensors, of any lengths) by ``new_tokens`` tokens, a beam that took
-    ``eos`` going on with it at its score.  Steps are replays of one HIP graph
+    ``eos`` going on with it at its score; ``which``: the adapters of each
+    prompt (PagedDecoder).  Steps are replays of one HIP graph
     unless use_graph=False.  Returns (tokens (prompts, beams, new_tokens) in
     descending order of scores (prompts, beams), prompt s, decode s)."""
     from .beam import beam_select, reorder_states
@@ -387,6 +539,8 @@ def beam_decode(model, prompts, beams, new_tokens, eos=-1, use_graph=True, page=
     # every beam may come to hold all its pages after the prompt's last full one, and a copy of what it goes on from
     pages = sum(len(p) // page + 1 for p in prompts) + R * beams * (-(-new_tokens // page) + 2)
     dec = PagedDecoder(model, R * beams, columns * page, page, pages)
+    if which is not None:
+        dec.which.copy_(torch.as_tensor(which, dtype=torch.int32).repeat_interleave(beams))
     counts = [0] * (R * beams)
     counts[::beams] = [len(p) for p in prompts]
     torch.cuda.synchronize()

@@ -408,6 +408,11 @@ class PagedCache:
     def append(self, layer, k, v, starts=None):
         append_pages(self.kv[layer, 0], self.kv[layer, 1], k, v, self.table, self.lengths, starts, self.over)
 
+    def append_rotated(self, layer, q, k, v, frequencies, starts=None, **options):
+        from .rope import append_rotated
+        return append_rotated(q, k, v, self.kv[layer, 0], self.kv[layer, 1], self.table, self.lengths, frequencies,
+                              starts=starts, over=self.over, **options)
+
     def attend_token(self, layer, q, **options):
         return attend_token(q, self.kv[layer, 0], self.kv[layer, 1], self.table, self.lengths, over=self.over, **options)
 

@@ -78,6 +78,16 @@ def rope_frequencies(dim: int, base: float = 10000.0, scaling: dict = None, devi
     return (slowed * w / factor + (1 - slowed) * w).to(device), float(attention)
 
 
+def model_frequencies(config, device="cuda"):
+    """``rope_frequencies`` of a transformers config: of its head's width, the
+    part of it that turns, its base and scaling."""
+    given = dict(getattr(config, "rope_parameters", None) or getattr(config, "rope_scaling", None) or {})
+    base = given.pop("rope_theta", None) or getattr(config, "rope_theta", 10000.0)
+    part = given.pop("partial_rotary_factor", None) or getattr(config, "partial_rotary_factor", None) or 1.0
+    head = getattr(config, "head_dim", None) or config.hidden_size // config.num_attention_heads
+    return rope_frequencies(int(head * part), base, given, device)
+
+
 def append_rotated(q: Tensor, k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Tensor, table: Tensor, lengths: Tensor,
                    frequencies: Tensor, *, starts: Tensor = None, over: Tensor = None, layout: str = "half",
                    factor: float = 1.0, out: Tensor = None) -> Tensor:
