@@ -18,8 +18,6 @@
 // the first, after an exact scaling of each token's by a power of two: what is
 // dropped lies 2^-16 (bf16) or 2^-22 (fp16) below the largest, and products
 // beyond fp16's range work.  All sums are fp32; the output is rounded once.
-#include <type_traits>
-
 #include "qs_attend_dev.h"
 
 namespace qs {
@@ -270,7 +268,27 @@ __device__ __forceinline__ float float_of(uint32_t u) {
   else return (float)__builtin_bit_cast(_Float16, (uint16_t)u);
 }
 
-// 16 columns of a token: y + scale * d in 16-byte pieces.
+// Rows of y and out may begin anywhere: 16 bytes from a place that is aligned to
+// an element only, which a global access takes on this target.
+typedef u32x4 Loose __attribute__((aligned(2)));
+__device__ __forceinline__ uint4 get_loose(const char* p) { return __builtin_bit_cast(uint4, (u32x4)*reinterpret_cast<const Loose*>(p)); }
+__device__ __forceinline__ void put_loose(char* p, const uint4& v) { *reinterpret_cast<Loose*>(p) = __builtin_bit_cast(u32x4, v); }
+// The first n of 8 elements, 0 < n < 8.
+__device__ __forceinline__ uint4 get_some(const char* p, int n) {
+  uint32_t v[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < n) v[i / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << 16 * (i & 1);
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void put_some(char* p, const uint4& x, int n) {
+  const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 7; ++i)
+    if (i < n) reinterpret_cast<uint16_t*>(p)[i] = (uint16_t)(v[i / 2] >> 16 * (i & 1));
+}
+
+// 8 columns of a token: y + scale * d.
 template <bool BF>
 __device__ __forceinline__ uint4 add_8(uint4 y, const f32x4& d0, const f32x4& d1, float scale) {
   const uint32_t in[4] = {y.x, y.y, y.z, y.w};
@@ -338,7 +356,7 @@ __device__ __forceinline__ void inner_products(const AdapterArgs& a, const Linea
 
 // The second launch: a group's tokens, NB blocks of 16, against 64 columns a
 // wave at a time.
-template <bool BF, int KB, int NB, bool WIDE>
+template <bool BF, int KB, int NB>
 __device__ __forceinline__ void up_group(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, int64_t m_begin,
                                          int64_t m_end, uint4* high, uint4* low, float* factor) {
   constexpr int R = 32 * KB, kRow = R + 8;
@@ -371,11 +389,13 @@ __device__ __forceinline__ void up_group(const AdapterArgs& a, const Linear& l, 
   }
   uint4 wv[4][KB], y[NB][2];
   auto load_y = [&](int b, int64_t m0) {
-    if constexpr (WIDE) {
-      const char* from = y0 + 2 * m0;
-      const int left = (int)(l.m - m0 < 64 ? l.m - m0 : 64) - 8 * q;
-      if (left > 0) y[b][0] = *reinterpret_cast<const uint4*>(from + y_at[b]);
-      if (left > 32) y[b][1] = *reinterpret_cast<const uint4*>(from + y_at[b] + 64);
+    const char* from = y0 + 2 * m0;
+    if (m0 + 64 <= l.m) {
+      y[b][0] = get_loose(from + y_at[b]), y[b][1] = get_loose(from + y_at[b] + 64);
+    } else {
+      const int left = (int)(l.m - m0) - 8 * q;  // columns from the lane's first on
+      if (left > 0) y[b][0] = left < 8 ? get_some(from + y_at[b], left) : get_loose(from + y_at[b]);
+      if (left > 32) y[b][1] = left < 40 ? get_some(from + y_at[b] + 64, left - 32) : get_loose(from + y_at[b] + 64);
     }
   };
   int64_t m0 = m_begin + 64 * w;
@@ -389,7 +409,6 @@ __device__ __forceinline__ void up_group(const AdapterArgs& a, const Linear& l, 
   __syncthreads();
   for (; m0 < m_end; m0 += kColumns) {
     const bool more = m0 + kColumns < m_end;
-    const int left = (int)(l.m - m0 < 64 ? l.m - m0 : 64) - 8 * q;  // columns from the lane's first on
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int c = 16 * b + r;
@@ -405,18 +424,16 @@ __device__ __forceinline__ void up_group(const AdapterArgs& a, const Linear& l, 
       if (b == NB - 1 && more) weights(m0 + kColumns, wv);
       if (c < g.size) {
         const float scale = factor[c];
-        char* to = out0 + 2 * m0;
-        if constexpr (WIDE) {
-          if (left > 0) *reinterpret_cast<uint4*>(to + out_at[b]) = add_8<BF>(y[b][0], acc[0], acc[1], scale);
-          if (left > 32) *reinterpret_cast<uint4*>(to + out_at[b] + 64) = add_8<BF>(y[b][1], acc[2], acc[3], scale);
+        char* to = out0 + 2 * m0 + out_at[b];
+        const uint4 o0 = add_8<BF>(y[b][0], acc[0], acc[1], scale), o1 = add_8<BF>(y[b][1], acc[2], acc[3], scale);
+        if (m0 + 64 <= l.m) {
+          put_loose(to, o0), put_loose(to + 64, o1);
         } else {
-          const uint16_t* from = reinterpret_cast<const uint16_t*>(y0 + 2 * m0 + y_at[b]);
-          uint16_t* into = reinterpret_cast<uint16_t*>(to + out_at[b]);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int at = 32 * (i >> 3) + (i & 7);  // behind the lane's first column
-            if (at < left) into[at] = (uint16_t)pack16<BF>(__builtin_fmaf(acc[i >> 2][i & 3], scale, float_of<BF>(from[at])), 0.f);
-          }
+          const int left = (int)(l.m - m0) - 8 * q;
+          if (left >= 8) put_loose(to, o0);
+          else if (left > 0) put_some(to, o0, left);
+          if (left >= 40) put_loose(to + 64, o1);
+          else if (left > 32) put_some(to + 64, o1, left - 32);
         }
       }
       if (more) load_y(b, m0 + kColumns);
@@ -426,27 +443,32 @@ __device__ __forceinline__ void up_group(const AdapterArgs& a, const Linear& l, 
 }
 
 // y of the tokens without an adapter goes on as it is, eight tokens of a wave at a time.
-template <bool WIDE>
 __device__ __forceinline__ void copy_group(const Linear& l, const Group& g, int64_t t0, int64_t m_begin, int64_t m_end) {
-  typedef typename std::conditional<WIDE, u32x4, uint16_t>::type Piece;
-  constexpr int W = sizeof(Piece) / 2, U = 8;
+  constexpr int U = 8;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (int c0 = w; c0 < g.size; c0 += 4 * U) {
     int64_t t[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) t[i] = t0 + place_in_tile(g, c0 + 4 * i);  // the last token again behind it
-    for (int64_t m = m_begin + W * lane; m < m_end; m += 64 * W) {
-      Piece v[U];
+    for (int64_t m = m_begin + 8 * lane; m < m_end; m += 512) {
+      if (m + 8 <= m_end) {
+        u32x4 v[U];
 #pragma unroll
-      for (int i = 0; i < U; ++i) v[i] = *reinterpret_cast<const Piece*>(l.y + t[i] * l.ldy + m);
+        for (int i = 0; i < U; ++i) v[i] = *reinterpret_cast<const Loose*>(l.y + t[i] * l.ldy + m);
 #pragma unroll
-      for (int i = 0; i < U; ++i)
-        if (c0 + 4 * i < g.size) *reinterpret_cast<Piece*>(l.out + t[i] * l.ldo + m) = v[i];
+        for (int i = 0; i < U; ++i)
+          if (c0 + 4 * i < g.size) *reinterpret_cast<Loose*>(l.out + t[i] * l.ldo + m) = v[i];
+      } else {
+        for (int64_t e = m; e < m_end; ++e)
+#pragma unroll
+          for (int i = 0; i < U; ++i)
+            if (c0 + 4 * i < g.size) l.out[t[i] * l.ldo + e] = l.y[t[i] * l.ldy + e];
+      }
     }
   }
 }
 
-template <bool BF, int KB, int NB, bool WIDE>
+template <bool BF, int KB, int NB>
 __global__ __launch_bounds__(kThreads, NB == 1 ? 1 : KB == 4 ? 2 : 3) void adapter_up_kernel(AdapterArgs a) {
   constexpr int kRow = 32 * KB + 8;  // 16-bit elements of a token's row, 16 bytes more than the products need
   __shared__ uint4 high[16 * NB * kRow / 8], low[16 * NB * kRow / 8];
@@ -458,11 +480,11 @@ __global__ __launch_bounds__(kThreads, NB == 1 ? 1 : KB == 4 ? 2 : 3) void adapt
   const int64_t m_end = m_begin + a.chunks * kColumns < l.m ? m_begin + a.chunks * kColumns : l.m;
   const int64_t t0 = (int64_t)(blockIdx.y / a.slots) * kTile;
   each_group(a, t0, blockIdx.y % a.slots, l.out != l.y, [&](const Group& g) {
-    if (g.adapter < 0) return copy_group<WIDE>(l, g, t0, m_begin, m_end);
+    if (g.adapter < 0) return copy_group(l, g, t0, m_begin, m_end);
     if constexpr (NB > 1) {
-      if (g.size <= 16) return up_group<BF, KB, 1, WIDE>(a, l, g, t0, m_begin, m_end, high, low, factor);
+      if (g.size <= 16) return up_group<BF, KB, 1>(a, l, g, t0, m_begin, m_end, high, low, factor);
     }
-    up_group<BF, KB, NB, WIDE>(a, l, g, t0, m_begin, m_end, high, low, factor);
+    up_group<BF, KB, NB>(a, l, g, t0, m_begin, m_end, high, low, factor);
   });
 }
 
@@ -471,14 +493,9 @@ auto down_kernel(int blocks, bool many) {
   if (many) return blocks <= 2 ? adapter_down_kernel<BF, 2, true> : adapter_down_kernel<BF, 4, true>;
   return blocks == 1 ? adapter_down_kernel<BF, 1, false> : blocks == 2 ? adapter_down_kernel<BF, 2, false> : adapter_down_kernel<BF, 4, false>;
 }
-template <bool BF, int NB, bool WIDE>
+template <bool BF, int NB>
 auto up_kernel(int rank) {
-  return rank <= 32 ? adapter_up_kernel<BF, 1, NB, WIDE> : rank <= 64 ? adapter_up_kernel<BF, 2, NB, WIDE> : adapter_up_kernel<BF, 4, NB, WIDE>;
-}
-template <bool BF>
-auto up_kernel(int rank, bool many, bool wide) {
-  if (many) return wide ? up_kernel<BF, 4, true>(rank) : up_kernel<BF, 4, false>(rank);
-  return wide ? up_kernel<BF, 1, true>(rank) : up_kernel<BF, 1, false>(rank);
+  return rank <= 32 ? adapter_up_kernel<BF, 1, NB> : rank <= 64 ? adapter_up_kernel<BF, 2, NB> : adapter_up_kernel<BF, 4, NB>;
 }
 
 struct Plan {
@@ -542,7 +559,6 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
   a.x = static_cast<const uint16_t*>(x), a.ldx = tokens == 1 ? 0 : ldx, a.tokens = tokens, a.n = n, a.which = which;
   a.adapters = (int)adapters, a.count = count;
   int most = 0, ranks[QS_MAX_GROUP];
-  bool wide = true;  // every y and out takes 16-byte accesses
   int64_t columns = 0;
   for (int g = 0; g < count; ++g) {
     const qs_adapter_job& j = jobs[g];
@@ -560,8 +576,6 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
                "%s: linear %d: tensors must be aligned to their elements", fn, g);
     QS_REQUIRE(j.y != j.out || tokens == 1 || j.ldy == j.ldo, "%s: linear %d: y and out share memory with rows %lld and %lld apart", fn, g,
                (long long)j.ldy, (long long)j.ldo);
-    wide = wide && ((reinterpret_cast<uintptr_t>(j.y) | reinterpret_cast<uintptr_t>(j.out)) & 15) == 0 && j.m % 8 == 0 &&
-           (tokens == 1 || (j.ldy | j.ldo) % 8 == 0);
     a.linear[g] = Linear{static_cast<const uint16_t*>(j.down), static_cast<const uint16_t*>(j.up), j.scale,
                          static_cast<const uint16_t*>(j.y), static_cast<uint16_t*>(j.out), j.down_adapter, j.down_row,
                          j.up_adapter, j.up_row, tokens == 1 ? 0 : j.ldy, tokens == 1 ? 0 : j.ldo, j.m, j.rank, a.ranks, 0, 0};
@@ -591,7 +605,8 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
   const unsigned rows = (unsigned)(p.tiles * p.slots);
   hipLaunchKernelGGL(down, dim3((unsigned)(p.runs * p.splits), rows), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("adapter_down_kernel");
-  const auto up = bf ? up_kernel<true>(most, tokens > 16, wide) : up_kernel<false>(most, tokens > 16, wide);
+  const auto up = tokens <= 16 ? (bf ? up_kernel<true, 1>(most) : up_kernel<false, 1>(most))
+                               : (bf ? up_kernel<true, 4>(most) : up_kernel<false, 4>(most));
   hipLaunchKernelGGL(up, dim3((unsigned)grid, rows), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("adapter_up_kernel");
   return QS_OK;

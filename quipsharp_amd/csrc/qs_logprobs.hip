@@ -107,8 +107,38 @@ __device__ __forceinline__ void write_alternative(const ScoreArgs& a, int64_t ro
   a.top_tokens[row * a.top + i] = has ? (int32_t)~(uint32_t)key : -1;
 }
 
-// The best `top` of the first n candidates, in order, in best; zeros behind them.
-__device__ __forceinline__ void rank_all(const uint64_t* room, int n, uint64_t* best, int top) {
+// Leaves the best `top` of n > top candidates, no two of which are alike, at
+// the front of room: their least is found bit by bit.
+__device__ void narrow(uint64_t* room, int n, int top, int* above) {
+  constexpr int kEach = (kRoom + kThreads - 1) / kThreads;
+  const int tid = threadIdx.x;
+  uint64_t mine[kEach];
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) mine[i] = i * kThreads + tid < n ? room[i * kThreads + tid] : 0;
+  if (tid < 65) above[tid] = 0;
+  __syncthreads();
+  uint64_t least = 0;
+  for (int bit = 63; bit >= 0; --bit) {
+    const uint64_t v = least | 1ull << bit;
+    int many = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) many += __popcll(__ballot(mine[i] >= v));
+    if ((tid & 63) == 0) atomicAdd(&above[bit], many);
+    __syncthreads();
+    if (above[bit] >= top) least = v;
+  }
+#pragma unroll
+  for (int i = 0; i < kEach; ++i)
+    if (mine[i] >= least) room[atomicAdd(&above[64], 1)] = mine[i];
+  __syncthreads();
+}
+
+// The best `top` of the first n candidates, in order, in best; zeros behind
+// them.  More than kFew are narrowed first (2048 equal logits of a slice, 64
+// wanted: 100 us by their ranks alone, 6 so).
+constexpr int kFew = 192;
+__device__ __forceinline__ void rank_all(uint64_t* room, int n, uint64_t* best, int top, int* above) {
+  if (n > kFew) narrow(room, n, top, above), n = top;
   for (int c = threadIdx.x; c < n; c += kThreads) {
     const uint64_t me = room[c];
     int place = 0;
@@ -174,7 +204,7 @@ struct Room {
   uint64_t keys[kRoom], best[kMaxTop];
   uint16_t listed[kListed];
   float red[2][4];
-  int above[32];  // of the search for the exact edge, a count for each bit
+  int above[65];  // of a search bit by bit, a count for each
   int groups, count, sums[4];
 };
 
@@ -296,7 +326,7 @@ __device__ __forceinline__ void select_best(const Groups<T, P>& g, float largest
       __syncthreads();
     }
   }
-  rank_all(r.keys, n, r.best, top);
+  rank_all(r.keys, n, r.best, top, r.above);
   __syncthreads();
 }
 
@@ -422,7 +452,7 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   __shared__ uint64_t best[kMaxTop], tops[kThreads], line;
   __shared__ uint32_t edge[4];
   __shared__ Stat stat;
-  __shared__ int count;
+  __shared__ int count, above[65];
   const LaneX lx = lane_x_init();
   const int tid = threadIdx.x, top = a.top;
   const int64_t row = blockIdx.x;
@@ -472,16 +502,16 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
       // equal logits: no two candidates are alike, so that at most `top` threads have one at or above this edge
       __syncthreads();
       if (tid == 0) count = 0;
-      int above = 0;
+      int higher = 0;
 #pragma unroll 8
-      for (int i = 0; i < kThreads; ++i) above += tops[i] > high;
-      if (above == top - 1) line = high;
+      for (int i = 0; i < kThreads; ++i) higher += tops[i] > high;
+      if (higher == top - 1) line = high;
       __syncthreads();
       take(line);
       __syncthreads();
       many = count;
     }
-    rank_all(room, many, best, top);
+    rank_all(room, many, best, top, above);
     __syncthreads();
   }
   const double log_sum = log(stat.sum);
