@@ -6,7 +6,15 @@
 // with rows that have no adapter left as they are.  Two launches: the inner
 // products with `down` (K = n is long, so it is split over work-groups, each
 // split leaving its fp32 sums), then the ones with `up` (K = rank), in whose
-// first step the splits are added.
+// first step the splits are added.  The rows of `down` of all linears count as
+// one matrix, so that x is read once for 128 of them.
+//
+// Both are bound by memory: single tokens by the weights of the adapters that
+// they name, prompts by x, y and out.  Measured: 48 tokens of 24 adapters of rank
+// 64, 5120 inputs to two linears of 25600, 10 and 33 us for 177 MB (4.1 TB/s; a
+// large copy reaches 5.06); 3 prompts of 4096, 25600 inputs to 5120 at rank 64, 94
+// and 63 us for 756 MB (4.8 TB/s); 6 of 900, 3584 inputs to 3584 + 512 + 512 at rank
+// 24, 15 and 25 us for 114 MB; one token of the smallest sizes 4 and 5 us.
 //
 // Tokens are taken 64 at a time.  In each 64 those of one adapter form a group
 // (found by ballots: prompts come in runs, single tokens in any order), which
@@ -35,7 +43,7 @@ struct Linear {
   uint16_t* out;
   int64_t down_adapter, down_row, up_adapter, up_row, ldy, ldo, m;
   int rank, offset;  // offset: of its ranks among those of all linears
-  int first_run, first;  // its first work-group column of the first and the second launch
+  int first;         // its first work-group column of the second launch
 };
 
 struct AdapterArgs {
@@ -43,7 +51,7 @@ struct AdapterArgs {
   int64_t ldx, tokens, n;
   const int32_t* which;
   int adapters, count, ranks;  // ranks: of all linears together
-  int splits, steps;           // steps of 256 inputs of a split
+  int tiles, splits, steps;    // steps of 256 inputs of a split
   int slots, chunks;           // work-groups that share a tile's groups, a power of two; runs of kColumns of a work-group
   float* part;                 // [splits][tokens][ranks]
   Linear linear[QS_MAX_GROUP];
@@ -85,75 +93,72 @@ __device__ __forceinline__ int place_in_tile(const Group& g, int c) {
   return __builtin_amdgcn_ds_bpermute(c * 4, g.inverse);
 }
 
-// One group of the first launch: NB blocks of 16 tokens, RB of 16 ranks from
-// rank0 on.  All that changes along the inputs is a scalar; a lane's places in
-// the rows are 32-bit offsets.
-template <bool BF, int RB, int NB>
-__device__ __forceinline__ void down_group(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, int split, int rank0,
-                                           f32x4 (*sums)[NB][64]) {
+// Row `rank` of an adapter's `down`, those of all linears one after the other;
+// rows beyond repeat the last.
+__device__ __forceinline__ const char* down_row(const AdapterArgs& a, int adapter, int rank) {
+  rank = rank < a.ranks ? rank : a.ranks - 1;
+  const char* row = nullptr;
+#pragma unroll
+  for (int g = 0; g < QS_MAX_GROUP; ++g)
+    if (g < a.count && rank >= a.linear[g].offset) {
+      const Linear& l = a.linear[g];
+      row = reinterpret_cast<const char*>(l.down + adapter * l.down_adapter) + (uint64_t)(uint32_t)(rank - l.offset) * (2u * (uint32_t)l.down_row);
+    }
+  return row;
+}
+
+// One group of the first launch, of up to 16 tokens: RB blocks of 16 ranks from
+// rank0 on, the inputs shared out over the waves.
+template <bool BF, int RB>
+__device__ __forceinline__ void down_group(const AdapterArgs& a, const Group& g, int64_t t0, int split, int rank0, f32x4 (*sums)[64]) {
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, q = lane >> 4, r = lane & 15;
-  const char* x = reinterpret_cast<const char*>(a.x + t0 * a.ldx);
-  const char* down = reinterpret_cast<const char*>(l.down + g.adapter * l.down_adapter);
-  uint32_t x_at[NB], down_at[RB];
+  const char *x = reinterpret_cast<const char*>(a.x + (t0 + place_in_tile(g, r)) * a.ldx + 8 * q), *down[RB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) x_at[b] = 2u * ((uint32_t)place_in_tile(g, 16 * b + r) * (uint32_t)a.ldx + 8 * q);
+  for (int i = 0; i < RB; ++i) down[i] = down_row(a, g.adapter, rank0 + 16 * i + r) + 16 * q;
+  f32x4 acc[RB];
 #pragma unroll
-  for (int i = 0; i < RB; ++i) {
-    const int rank = rank0 + 16 * i + r;  // the sums of rows beyond go nowhere
-    down_at[i] = 2u * ((uint32_t)(rank < l.rank ? rank : l.rank - 1) * (uint32_t)l.down_row + 8 * q);
-  }
-  f32x4 acc[RB][NB];
-#pragma unroll
-  for (int i = 0; i < RB; ++i)
-#pragma unroll
-    for (int b = 0; b < NB; ++b) acc[i][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < RB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const int n = (int)a.n, k0 = split * a.steps * 256, k1 = k0 + a.steps * 256 < n ? k0 + a.steps * 256 : n;
   // 64 inputs at a time, 32 for each of two products
-  uint4 xv[NB][2], av[RB][2];
-  auto load = [&](int k) {
-    const char *xk = x + 2 * (int64_t)k, *dk = down + 2 * (int64_t)k;
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b) xv[b][j] = *reinterpret_cast<const uint4*>(xk + x_at[b] + 64 * j);
-#pragma unroll
-      for (int i = 0; i < RB; ++i) av[i][j] = *reinterpret_cast<const uint4*>(dk + down_at[i] + 64 * j);
-    }
-  };
+  uint4 xv[2], av[RB][2];
   auto multiply = [&]() {
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int i = 0; i < RB; ++i)
-#pragma unroll
-        for (int b = 0; b < NB; ++b) acc[i][b] = mma_16x16x32<BF>(av[i][j], xv[b][j], acc[i][b]);
+      for (int i = 0; i < RB; ++i) acc[i] = mma_16x16x32<BF>(av[i][j], xv[j], acc[i]);
   };
   int k = k0 + 64 * w;
-  for (; k + 64 <= k1; k += 256) load(k), multiply();
+  for (; k + 64 <= k1; k += 256) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      xv[j] = *reinterpret_cast<const uint4*>(x + 2 * (int64_t)k + 64 * j);
+#pragma unroll
+      for (int i = 0; i < RB; ++i) av[i][j] = *reinterpret_cast<const uint4*>(down[i] + 2 * (int64_t)k + 64 * j);
+    }
+    multiply();
+  }
   if (k < k1) {
     // fewer than 64 are left: zeros behind them
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       const bool in = k + 32 * j + 8 * q < k1;
+      xv[j] = in ? *reinterpret_cast<const uint4*>(x + 2 * (int64_t)k + 64 * j) : uint4{};
 #pragma unroll
-      for (int b = 0; b < NB; ++b) xv[b][j] = in ? *reinterpret_cast<const uint4*>(x + 2 * (int64_t)k + x_at[b] + 64 * j) : uint4{};
-#pragma unroll
-      for (int i = 0; i < RB; ++i) av[i][j] = in ? *reinterpret_cast<const uint4*>(down + 2 * (int64_t)k + down_at[i] + 64 * j) : uint4{};
+      for (int i = 0; i < RB; ++i) av[i][j] = in ? *reinterpret_cast<const uint4*>(down[i] + 2 * (int64_t)k + 64 * j) : uint4{};
     }
     multiply();
   }
   // the waves' sums together, a block of ranks at a time
-  float* part = a.part + ((int64_t)split * a.tokens + t0) * a.ranks + l.offset;
+  float* part = a.part + ((int64_t)split * a.tokens + t0) * a.ranks;
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
-#pragma unroll
-    for (int b = 0; b < NB; ++b) sums[w][b][lane] = acc[i][b];
+    sums[w][lane] = acc[i];
     __syncthreads();
-    if (NB == 4 || w < NB) {
-      const int c = 16 * w + r, rank = rank0 + 16 * i + 4 * q;
-      const f32x4 s = (sums[0][w][lane] + sums[1][w][lane]) + (sums[2][w][lane] + sums[3][w][lane]);
-      const int place = place_in_tile(g, c);  // an exchange of all lanes
-      if (c < g.size && rank < l.rank) *reinterpret_cast<f32x4*>(part + place * a.ranks + rank) = s;
+    if (w == 0) {
+      const int rank = rank0 + 16 * i + 4 * q;
+      const f32x4 s = (sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]);
+      const int place = place_in_tile(g, r);  // an exchange of all lanes
+      if (r < g.size && rank < a.ranks) *reinterpret_cast<f32x4*>(part + place * a.ranks + rank) = s;
     }
     __syncthreads();
   }
@@ -164,59 +169,66 @@ __device__ __forceinline__ void down_group(const AdapterArgs& a, const Linear& l
 // multiplies its 16 tokens.  A row of a stage is eight pieces of 16 bytes, of
 // which piece p lies at place p ^ (row & 7), so that a wave's operands (one
 // piece of each of 16 rows) come from all banks.
-constexpr int kStageRow = 128, kAhead = 3;
+constexpr int kStageRow = 128;
+template <int RB>
+constexpr int kAhead = RB > 4 ? 2 : 3;
 template <int RB>
 constexpr int stage_bytes() {
   return (kTile + 16 * RB) * kStageRow;
 }
 
 template <bool BF, int RB>
-__device__ __forceinline__ void down_tile(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, int split, int rank0, char* stages) {
-  constexpr int NX = kTile / 32, NW = RB / 2, NL = NX + NW;  // loads of a wave in a stage, of 8 rows each
+__device__ __forceinline__ void down_tile(const AdapterArgs& a, const Group& g, int64_t t0, int split, int rank0, char* stages) {
+  constexpr int NX = kTile / 32, NW = RB / 2, NL = NX + NW, A = kAhead<RB>;  // loads of a wave in a stage, of 8 rows each
   static_assert(RB % 2 == 0, "every wave brings as many rows");
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, q = lane >> 4, r = lane & 15;
   const int n = (int)a.n, k0 = split * a.steps * 256, k1 = k0 + a.steps * 256 < n ? k0 + a.steps * 256 : n;
   const int count = (k1 - k0 + 63) / 64, left = k1 - k0 - 64 * (count - 1);  // stages, inputs of the last
   const int row8 = lane >> 3;  // of a load; every load begins at a multiple of 8 rows
   const unsigned piece = 16 * ((lane & 7) ^ row8);
-  unsigned x_row[NX], down_row[NW], x_at[NX], down_at[NW];
+  unsigned x_row[NX], w_row[NW], x_at[NX], w_at[NW];
+  const char* down[NW];  // a load's rows are of one linear: ranks are multiples of 8
 #pragma unroll
   for (int j = 0; j < NX; ++j) x_row[j] = 2u * (uint32_t)place_in_tile(g, 8 * (NX * w + j) + row8) * (uint32_t)a.ldx, x_at[j] = x_row[j] + piece;
 #pragma unroll
   for (int j = 0; j < NW; ++j) {
-    const int rank = rank0 + 8 * (NW * w + j) + row8;  // the sums of rows beyond go nowhere
-    down_row[j] = 2u * (uint32_t)(rank < l.rank ? rank : l.rank - 1) * (uint32_t)l.down_row, down_at[j] = down_row[j] + piece;
+    int rank = rank0 + 8 * (NW * w + j), gi = 0;  // the sums of rows beyond go nowhere
+    rank = rank < a.ranks ? rank : a.ranks - 8;
+    while (gi + 1 < a.count && rank >= a.linear[gi + 1].offset) ++gi;
+    const Linear& l = a.linear[gi];
+    down[j] = reinterpret_cast<const char*>(l.down + g.adapter * l.down_adapter + (rank - l.offset) * l.down_row + k0);
+    w_row[j] = 2u * (uint32_t)row8 * (uint32_t)l.down_row, w_at[j] = w_row[j] + piece;
   }
   const char* x = reinterpret_cast<const char*>(a.x + t0 * a.ldx + k0);
-  const char* down = reinterpret_cast<const char*>(l.down + g.adapter * l.down_adapter + k0);
   const unsigned lds = __builtin_amdgcn_readfirstlane(lds_address(stages));
   auto fetch = [&](int s) {
-    const unsigned to = lds + (unsigned)(s % (kAhead + 1)) * stage_bytes<RB>();
+    const unsigned to = lds + (unsigned)(s % (A + 1)) * stage_bytes<RB>();
     if (s == count - 1 && left < 64) {
       // pieces behind the last input: the last one again, which is not used
       const unsigned end = 2u * (left - 8), p = piece < end ? piece : end;
 #pragma unroll
       for (int j = 0; j < NX; ++j) x_at[j] = x_row[j] + p;
 #pragma unroll
-      for (int j = 0; j < NW; ++j) down_at[j] = down_row[j] + p;
+      for (int j = 0; j < NW; ++j) w_at[j] = w_row[j] + p;
     }
     load_rows(x + 128 * (int64_t)s, x_at, to + w * (NX * 1024));
-    load_rows(down + 128 * (int64_t)s, down_at, to + kTile * kStageRow + w * (NW * 1024));
+#pragma unroll
+    for (int j = 0; j < NW; ++j) load_to_lds<0>(down[j] + 128 * (int64_t)s, w_at[j], to + kTile * kStageRow + (NW * w + j) * 1024);
   };
   f32x4 acc[RB];
 #pragma unroll
   for (int i = 0; i < RB; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   const bool busy = 16 * w < g.size;
 #pragma unroll
-  for (int s = 0; s < kAhead; ++s)
+  for (int s = 0; s < A; ++s)
     if (s < count) fetch(s);
   for (int s = 0; s < count; ++s) {
-    if (s + kAhead <= count) wait_loads<(kAhead - 1) * NL>();
+    if (s + A <= count) wait_loads<(A - 1) * NL>();
     else wait_loads<0>();
     __syncthreads();
-    if (s + kAhead < count) fetch(s + kAhead);
+    if (s + A < count) fetch(s + A);
     if (busy) {
-      const char* at = stages + (s % (kAhead + 1)) * stage_bytes<RB>();
+      const char* at = stages + (s % (A + 1)) * stage_bytes<RB>();
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int p = 16 * ((4 * j + q) ^ (r & 7));
@@ -234,31 +246,29 @@ __device__ __forceinline__ void down_tile(const AdapterArgs& a, const Linear& l,
     }
   }
   const int c = 16 * w + r, place = place_in_tile(g, c);
-  float* part = a.part + ((int64_t)split * a.tokens + t0 + place) * a.ranks + l.offset;
+  float* part = a.part + ((int64_t)split * a.tokens + t0 + place) * a.ranks;
 #pragma unroll
   for (int i = 0; i < RB; ++i) {
     const int rank = rank0 + 16 * i + 4 * q;
-    if (c < g.size && rank < l.rank) *reinterpret_cast<f32x4*>(part + rank) = acc[i];
+    if (c < g.size && rank < a.ranks) *reinterpret_cast<f32x4*>(part + rank) = acc[i];
   }
   __syncthreads();  // the next group's stages lie where these did
 }
 
-// blockIdx.x: (linear, its run of 16 RB ranks, split), the split fastest.
+// blockIdx.x: (run of 16 RB ranks, split), the split fastest.  blockIdx.y: (slot,
+// tile), the tile fastest, so that slots without a group do not fall to the same
+// XCDs (18 tiles in 4 slots: 18.3 us with the slot fastest, 13.9 so).
 template <bool BF, int RB, bool MANY>
 __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
-  constexpr int kSums = 4 * 64 * sizeof(f32x4), kStages = MANY ? (kAhead + 1) * stage_bytes<RB>() : 0;
+  constexpr int kSums = 4 * 64 * sizeof(f32x4), kStages = MANY ? (kAhead<RB> + 1) * stage_bytes<RB>() : 0;
   __shared__ __align__(16) char room[kStages > kSums ? kStages : kSums];
-  const int split = blockIdx.x % a.splits, run = blockIdx.x / a.splits;
-  int gi = 0;
-  while (gi + 1 < a.count && run >= a.linear[gi + 1].first_run) ++gi;
-  const Linear& l = a.linear[gi];
-  const int rank0 = (run - l.first_run) * (16 * RB);
-  const int64_t t0 = (int64_t)(blockIdx.y / a.slots) * kTile;
-  each_group(a, t0, blockIdx.y & (a.slots - 1), false, [&](const Group& g) {
+  const int split = blockIdx.x % a.splits, rank0 = blockIdx.x / a.splits * (16 * RB);
+  const int64_t t0 = (int64_t)(blockIdx.y % a.tiles) * kTile;
+  each_group(a, t0, blockIdx.y / a.tiles, false, [&](const Group& g) {
     if constexpr (MANY) {
-      if (g.size > 16) return down_tile<BF, RB>(a, l, g, t0, split, rank0, room);
+      if (g.size > 16) return down_tile<BF, RB>(a, g, t0, split, rank0, room);
     }
-    down_group<BF, RB, 1>(a, l, g, t0, split, rank0, reinterpret_cast<f32x4(*)[1][64]>(room));
+    down_group<BF, RB>(a, g, t0, split, rank0, reinterpret_cast<f32x4(*)[64]>(room));
   });
 }
 
@@ -302,149 +312,248 @@ __device__ __forceinline__ uint4 add_8(uint4 y, const f32x4& d0, const f32x4& d1
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
-// The inner products of N tokens of a group, summed over the splits, as two
+// An exact power of two that brings a largest size near 1, and its inverse.
+__device__ __forceinline__ float powers(float most, float& inverse) {
+  int e = (int)(__float_as_uint(most) >> 23);
+  e = e < 2 ? 2 : e > 252 ? 252 : e;
+  inverse = __uint_as_float((uint32_t)e << 23);
+  return __uint_as_float((uint32_t)(254 - e) << 23);
+}
+// Two numbers as 16 bits and the remainder in 16 more; an infinite one has none.
+template <bool BF>
+__device__ __forceinline__ void two_parts(float f0, float f1, uint32_t& hi, uint32_t& lo) {
+  hi = pack16<BF>(f0, f1);
+  const float h0 = float_of<BF>(hi & 0xFFFF), h1 = float_of<BF>(hi >> 16);
+  lo = pack16<BF>(fabsf(h0) < INFINITY ? f0 - h0 : 0.f, fabsf(h1) < INFINITY ? f1 - h1 : 0.f);
+}
+
+// The inner products of up to 16 tokens of a group, summed over the splits, as two
 // 16-bit numbers: four ranks a thread, a token's R / 4 threads in one wave.
-template <bool BF, int R, int kRow, int N>
+template <bool BF, int R, int kRow>
 __device__ __forceinline__ void inner_products(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, uint4* high,
                                                uint4* low, float* factor) {
-  constexpr int T = R / 4, I = N * T / kThreads > 0 ? N * T / kThreads : 1, U = I < 2 ? 1 : 2;
+  constexpr int T = R == 96 ? 32 : R / 4;  // a power of two
+  constexpr int U = T == 32 ? 2 : 1;       // tokens of a thread
   const int tid = threadIdx.x;
-  if (N * T < kThreads && tid >= N * T) return;  // whole waves: N T is a multiple of 64
+  if (16 * T < kThreads && tid >= 16 * T) return;  // whole waves: 16 T is a multiple of 64
   const float* base = a.part + t0 * a.ranks + l.offset;
   const int64_t next = a.tokens * a.ranks;
   const int rank = tid % T * 4;
   const float scale = l.scale[g.adapter];
+  f32x4 s[U];
+  uint32_t from[U];
 #pragma unroll
-  for (int i0 = 0; i0 < I; i0 += U) {
-    f32x4 s[U];
-    uint32_t from[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      from[i] = (uint32_t)place_in_tile(g, (i0 + i) * (kThreads / T) + tid / T) * (uint32_t)a.ranks + (rank < l.rank ? rank : 0);
-      s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    }
+  for (int i = 0; i < U; ++i) {
+    from[i] = (uint32_t)place_in_tile(g, i * (kThreads / T) + tid / T) * (uint32_t)a.ranks + (rank < l.rank ? rank : 0);
+    s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
 #pragma unroll 4
-    for (int p = 0; p < a.splits; ++p)
+  for (int p = 0; p < a.splits; ++p)
 #pragma unroll
-      for (int i = 0; i < U; ++i) s[i] += *reinterpret_cast<const f32x4*>(base + p * next + from[i]);
+    for (int i = 0; i < U; ++i) s[i] += *reinterpret_cast<const f32x4*>(base + p * next + from[i]);
 #pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int c = (i0 + i) * (kThreads / T) + tid / T;
-      if (rank >= l.rank) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      float most = fmaxf(fmaxf(fabsf(s[i][0]), fabsf(s[i][1])), fmaxf(fabsf(s[i][2]), fabsf(s[i][3])));
+  for (int i = 0; i < U; ++i) {
+    const int c = i * (kThreads / T) + tid / T;
+    if (rank >= l.rank) s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float most = fmaxf(fmaxf(fabsf(s[i][0]), fabsf(s[i][1])), fmaxf(fabsf(s[i][2]), fabsf(s[i][3])));
 #pragma unroll
-      for (int x = 1; x < T; x *= 2) most = fmaxf(most, __shfl_xor(most, x));
-      int e = (int)(__float_as_uint(most) >> 23);
-      e = e < 2 ? 2 : e > 252 ? 252 : e;
-      const float shrink = __uint_as_float((uint32_t)(254 - e) << 23);
-      uint32_t hi[2], lo[2];
+    for (int x = 1; x < T; x *= 2) most = fmaxf(most, __shfl_xor(most, x));
+    float grow;
+    const float shrink = powers(most, grow);
+    uint32_t hi[2], lo[2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const float f0 = s[i][2 * x] * shrink, f1 = s[i][2 * x + 1] * shrink;
-        hi[x] = pack16<BF>(f0, f1);
-        const float h0 = float_of<BF>(hi[x] & 0xFFFF), h1 = float_of<BF>(hi[x] >> 16);
-        // an infinite product has no remainder
-        lo[x] = pack16<BF>(fabsf(h0) < INFINITY ? f0 - h0 : 0.f, fabsf(h1) < INFINITY ? f1 - h1 : 0.f);
-      }
-      const int at = (c * kRow + rank) / 4;
-      reinterpret_cast<uint2*>(high)[at] = make_uint2(hi[0], hi[1]), reinterpret_cast<uint2*>(low)[at] = make_uint2(lo[0], lo[1]);
-      if (rank == 0) factor[c] = __uint_as_float((uint32_t)e << 23) * scale;
-    }
-    __builtin_amdgcn_sched_barrier(0);  // more at a time would take more registers than the products
+    for (int x = 0; x < 2; ++x) two_parts<BF>(s[i][2 * x] * shrink, s[i][2 * x + 1] * shrink, hi[x], lo[x]);
+    const int at = (c * kRow + rank) / 4;
+    if (R < 4 * T && rank >= R) continue;
+    reinterpret_cast<uint2*>(high)[at] = make_uint2(hi[0], hi[1]), reinterpret_cast<uint2*>(low)[at] = make_uint2(lo[0], lo[1]);
+    if (rank == 0) factor[c] = grow * scale;
   }
 }
 
-// The second launch: a group's tokens, NB blocks of 16, against 64 columns a
-// wave at a time.
-template <bool BF, int KB, int NB>
+// What a lane's part of the products reads and writes of y and out: columns m0
+// + 8 q .. + 7 and m0 + 32 + 8 q .. + 7 of a token, so that an access of the
+// wave takes 64 bytes together of 16 rows.  left: columns from m0 + 8 q on.
+__device__ __forceinline__ void load_y(const char* from, int left, uint4 (&y)[2]) {
+  if (left >= 40) {
+    y[0] = get_loose(from), y[1] = get_loose(from + 64);
+  } else {
+    if (left > 0) y[0] = left < 8 ? get_some(from, left) : get_loose(from);
+    if (left > 32) y[1] = get_some(from + 64, left - 32);
+  }
+}
+template <bool BF>
+__device__ __forceinline__ void store_out(char* to, int left, const uint4 (&y)[2], const f32x4 (&acc)[4], float scale) {
+  const uint4 o0 = add_8<BF>(y[0], acc[0], acc[1], scale), o1 = add_8<BF>(y[1], acc[2], acc[3], scale);
+  if (left >= 40) {
+    put_loose(to, o0), put_loose(to + 64, o1);
+  } else {
+    if (left >= 8) put_loose(to, o0);
+    else if (left > 0) put_some(to, o0, left);
+    if (left > 32) put_some(to + 64, o1, left - 32);
+  }
+}
+// The column of row r of the j-th of the four products over 64 columns.
+__device__ __forceinline__ int column_of(int j, int r) { return 32 * (j >> 1) + 8 * (r >> 2) + 4 * (j & 1) + (r & 3); }
+
+// The second launch for a group of up to 16 tokens: each wave takes 64 columns
+// at a time, whose weights go to its registers, the next ones on their way.
+template <bool BF, int KB>
 __device__ __forceinline__ void up_group(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, int64_t m_begin,
-                                         int64_t m_end, uint4* high, uint4* low, float* factor) {
-  constexpr int R = 32 * KB, kRow = R + 8;
+                                         int64_t m_end, char* room) {
+  constexpr int R = 32 * KB, kRow = R + 8;  // 16-bit elements of a token's row, 16 bytes more than the products need
+  uint4 *high = reinterpret_cast<uint4*>(room), *low = high + 16 * kRow / 8;
+  float* factor = reinterpret_cast<float*>(low + 16 * kRow / 8);
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, q = lane >> 4, r = lane & 15;
   const char* up = reinterpret_cast<const char*>(l.up + g.adapter * l.up_adapter);
-  auto row_of = [&](int j) { return 32 * (j >> 1) + 8 * (r >> 2) + 4 * (j & 1) + (r & 3); };
   uint32_t w_at[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w_at[j] = 2u * ((uint32_t)row_of(j) * (uint32_t)l.up_row + 8 * q);
+  for (int j = 0; j < 4; ++j) w_at[j] = 2u * ((uint32_t)column_of(j, r) * (uint32_t)l.up_row + 8 * q);
   auto weights = [&](int64_t m0, uint4 (&wv)[4][KB]) {
     const char* from = up + 2 * m0 * l.up_row;
     const int last = m0 + 64 <= l.m ? 63 : (int)(l.m - m0) - 1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t at = row_of(j) <= last ? w_at[j] : 2u * ((uint32_t)last * (uint32_t)l.up_row + 8 * q);
+      const uint32_t at = column_of(j, r) <= last ? w_at[j] : 2u * ((uint32_t)last * (uint32_t)l.up_row + 8 * q);
 #pragma unroll
       for (int k = 0; k < KB; ++k)
         wv[j][k] = 32 * k + 8 * q < l.rank ? *reinterpret_cast<const uint4*>(from + at + 64 * k) : uint4{};
     }
   };
-  // A lane's results of a token are columns m0 + 8 q .. + 7 and m0 + 32 + 8 q .. + 7, so that an access of the wave
-  // takes 64 bytes together of 16 rows.
-  const char* y0 = reinterpret_cast<const char*>(l.y + t0 * l.ldy);
-  char* out0 = reinterpret_cast<char*>(l.out + t0 * l.ldo);
-  uint32_t y_at[NB], out_at[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b) {
-    const uint32_t place = place_in_tile(g, 16 * b + r);
-    y_at[b] = 2u * (place * (uint32_t)l.ldy + 8 * q), out_at[b] = 2u * (place * (uint32_t)l.ldo + 8 * q);
-  }
-  uint4 wv[4][KB], y[NB][2];
-  auto load_y = [&](int b, int64_t m0) {
-    const char* from = y0 + 2 * m0;
-    if (m0 + 64 <= l.m) {
-      y[b][0] = get_loose(from + y_at[b]), y[b][1] = get_loose(from + y_at[b] + 64);
-    } else {
-      const int left = (int)(l.m - m0) - 8 * q;  // columns from the lane's first on
-      if (left > 0) y[b][0] = left < 8 ? get_some(from + y_at[b], left) : get_loose(from + y_at[b]);
-      if (left > 32) y[b][1] = left < 40 ? get_some(from + y_at[b] + 64, left - 32) : get_loose(from + y_at[b] + 64);
-    }
-  };
+  const uint32_t place = place_in_tile(g, r);
+  const char* y0 = reinterpret_cast<const char*>(l.y + t0 * l.ldy) + 2u * (place * (uint32_t)l.ldy + 8 * q);
+  char* out0 = reinterpret_cast<char*>(l.out + t0 * l.ldo) + 2u * (place * (uint32_t)l.ldo + 8 * q);
+  auto left_of = [&](int64_t m0) { return (int)(l.m - m0 < 64 ? l.m - m0 : 64) - 8 * q; };
+  uint4 wv[4][KB], y[2];
   int64_t m0 = m_begin + 64 * w;
-  if (m0 < m_end) {
-    weights(m0, wv);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) load_y(b, m0);
-  }
+  if (m0 < m_end) weights(m0, wv), load_y(y0 + 2 * m0, left_of(m0), y);
   __syncthreads();  // the group before is done with the tables
-  inner_products<BF, R, kRow, 16 * NB>(a, l, g, t0, high, low, factor);
+  inner_products<BF, R, kRow>(a, l, g, t0, high, low, factor);
   __syncthreads();
+  uint4 h[KB], o[KB];
+#pragma unroll
+  for (int k = 0; k < KB; ++k) h[k] = high[(r * kRow + 32 * k + 8 * q) / 8], o[k] = low[(r * kRow + 32 * k + 8 * q) / 8];
+  const float scale = factor[r];
   for (; m0 < m_end; m0 += kColumns) {
-    const bool more = m0 + kColumns < m_end;
+    f32x4 acc[4];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int c = 16 * b + r;
-      f32x4 acc[4];
+    for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < KB; ++k)
 #pragma unroll
-      for (int k = 0; k < KB; ++k) {
-        const uint4 h = high[(c * kRow + 32 * k + 8 * q) / 8], o = low[(c * kRow + 32 * k + 8 * q) / 8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j] = mma_16x16x32<BF>(wv[j][k], o, mma_16x16x32<BF>(wv[j][k], h, acc[j]));
-      }
-      if (b == NB - 1 && more) weights(m0 + kColumns, wv);
-      if (c < g.size) {
-        const float scale = factor[c];
-        char* to = out0 + 2 * m0 + out_at[b];
-        const uint4 o0 = add_8<BF>(y[b][0], acc[0], acc[1], scale), o1 = add_8<BF>(y[b][1], acc[2], acc[3], scale);
-        if (m0 + 64 <= l.m) {
-          put_loose(to, o0), put_loose(to + 64, o1);
-        } else {
-          const int left = (int)(l.m - m0) - 8 * q;
-          if (left >= 8) put_loose(to, o0);
-          else if (left > 0) put_some(to, o0, left);
-          if (left >= 40) put_loose(to + 64, o1);
-          else if (left > 32) put_some(to + 64, o1, left - 32);
-        }
-      }
-      if (more) load_y(b, m0 + kColumns);
-      __builtin_amdgcn_sched_barrier(0);  // blocks that overlap would take twice the registers
-    }
+      for (int j = 0; j < 4; ++j) acc[j] = mma_16x16x32<BF>(wv[j][k], o[k], mma_16x16x32<BF>(wv[j][k], h[k], acc[j]));
+    const uint4 y_now[2] = {y[0], y[1]};
+    if (m0 + kColumns < m_end) weights(m0 + kColumns, wv), load_y(y0 + 2 * (m0 + kColumns), left_of(m0 + kColumns), y);
+    if (r < g.size) store_out<BF>(out0 + 2 * m0, left_of(m0), y_now, acc, scale);
   }
 }
 
-// y of the tokens without an adapter goes on as it is, eight tokens of a wave at a time.
+// The same for more tokens: a wave has 16 of them, whose inner products stay in
+// its registers as the operand that they are, and the weights of 64 columns at
+// a time lie in LDS for all four, the next ones on their way.  (Through up_group's
+// way, with the inner products in LDS and the weights in registers, 142 tokens of
+// rank 72 took 23 us in place of 16, long prompts as much as here.)
+template <int KB>
+constexpr int tile_row() {
+  return 64 * KB + 16;  // bytes of a row of weights: an odd number of pieces, so that 8 rows' same pieces come from all banks
+}
+template <bool BF, int KB>
+__device__ __forceinline__ void up_tile(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, int64_t m_begin,
+                                        int64_t m_end, char* room) {
+  constexpr int kRow = tile_row<KB>(), kBuffer = 64 * kRow;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, q = lane >> 4, r = lane & 15;
+  // thread: row tid / 4 of 64, pieces tid % 4 + 4 k
+  const int row = tid >> 2, piece = tid & 3, column = column_of(row >> 4, row & 15);
+  const char* up = reinterpret_cast<const char*>(l.up + g.adapter * l.up_adapter) + 16 * piece;
+  uint4 wn[KB];
+  auto fetch = [&](int64_t m0) {
+    int64_t m = m0 + column;
+    m = m < l.m ? m : l.m - 1;  // the results of columns beyond go nowhere
+    const char* from = up + 2 * m * l.up_row;
+#pragma unroll
+    for (int k = 0; k < KB; ++k) wn[k] = 32 * k + 8 * piece < l.rank ? *reinterpret_cast<const uint4*>(from + 64 * k) : uint4{};
+  };
+  auto keep = [&](int buffer) {
+#pragma unroll
+    for (int k = 0; k < KB; ++k) *reinterpret_cast<uint4*>(room + buffer * kBuffer + row * kRow + 64 * k + 16 * piece) = wn[k];
+  };
+  fetch(m_begin);
+  const int c = 16 * w + r;
+  const uint32_t place = place_in_tile(g, c);
+  const char* y0 = reinterpret_cast<const char*>(l.y + t0 * l.ldy) + 2u * (place * (uint32_t)l.ldy + 8 * q);
+  char* out0 = reinterpret_cast<char*>(l.out + t0 * l.ldo) + 2u * (place * (uint32_t)l.ldo + 8 * q);
+  auto left_of = [&](int64_t m0) { return (int)(l.m - m0 < 64 ? l.m - m0 : 64) - 8 * q; };
+  const bool mine = c < g.size;
+  uint4 y[2], h[KB], o[KB];
+  if (mine) load_y(y0 + 2 * m_begin, left_of(m_begin), y);
+  float scale;
+  {
+    const float* from = a.part + (t0 + place) * a.ranks + l.offset;
+    f32x4 s[KB][2];
+#pragma unroll
+    for (int k = 0; k < KB; ++k) s[k][0] = s[k][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int64_t next = a.tokens * a.ranks;
+#pragma unroll 8
+    for (int p = 0; p < a.splits; ++p)
+#pragma unroll
+      for (int k = 0; k < KB; ++k) {
+        const int rank = 32 * k + 8 * q;
+        const float* at = from + p * next + (rank < l.rank ? rank : 0);
+        s[k][0] += *reinterpret_cast<const f32x4*>(at), s[k][1] += *reinterpret_cast<const f32x4*>(at + 4);
+      }
+    float most = 0.f;
+#pragma unroll
+    for (int k = 0; k < KB; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (32 * k + 8 * q >= l.rank) s[k][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(s[k][i][e]));
+      }
+    most = fmaxf(most, __shfl_xor(most, 16));
+    most = fmaxf(most, __shfl_xor(most, 32));
+    float grow;
+    const float shrink = powers(most, grow);
+    scale = grow * l.scale[g.adapter];
+#pragma unroll
+    for (int k = 0; k < KB; ++k) {
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) two_parts<BF>(s[k][x >> 1][2 * (x & 1)] * shrink, s[k][x >> 1][2 * (x & 1) + 1] * shrink, hi[x], lo[x]);
+      h[k] = make_uint4(hi[0], hi[1], hi[2], hi[3]), o[k] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    }
+  }
+  __syncthreads();  // the group before is done with the room
+  keep(0);
+  if (m_begin + 64 < m_end) fetch(m_begin + 64);
+  __syncthreads();
+  int buffer = 0;
+  for (int64_t m0 = m_begin; m0 < m_end; m0 += 64) {
+    const uint4 y_now[2] = {y[0], y[1]};
+    if (mine && m0 + 64 < m_end) load_y(y0 + 2 * (m0 + 64), left_of(m0 + 64), y);
+    if (16 * w < g.size) {
+      f32x4 acc[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const char* at = room + buffer * kBuffer + r * kRow + 16 * q;
+#pragma unroll
+      for (int k = 0; k < KB; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint4 wv = *reinterpret_cast<const uint4*>(at + 16 * j * kRow + 64 * k);
+          acc[j] = mma_16x16x32<BF>(wv, o[k], mma_16x16x32<BF>(wv, h[k], acc[j]));
+        }
+      if (mine) store_out<BF>(out0 + 2 * m0, left_of(m0), y_now, acc, scale);
+    }
+    buffer ^= 1;
+    if (m0 + 64 < m_end) keep(buffer);  // all are done with it since the last barrier
+    if (m0 + 128 < m_end) fetch(m0 + 128);
+    __syncthreads();
+  }
+}
+
+// y of the tokens without an adapter goes on as it is, four tokens of a wave at a time.
 __device__ __forceinline__ void copy_group(const Linear& l, const Group& g, int64_t t0, int64_t m_begin, int64_t m_end) {
-  constexpr int U = 8;
+  constexpr int U = 4;
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (int c0 = w; c0 < g.size; c0 += 4 * U) {
     int64_t t[U];
@@ -468,34 +577,35 @@ __device__ __forceinline__ void copy_group(const Linear& l, const Group& g, int6
   }
 }
 
-template <bool BF, int KB, int NB>
-__global__ __launch_bounds__(kThreads, NB == 1 ? 1 : KB == 4 ? 2 : 3) void adapter_up_kernel(AdapterArgs a) {
-  constexpr int kRow = 32 * KB + 8;  // 16-bit elements of a token's row, 16 bytes more than the products need
-  __shared__ uint4 high[16 * NB * kRow / 8], low[16 * NB * kRow / 8];
-  __shared__ float factor[16 * NB];
+template <bool BF, int KB, bool MANY>
+__global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
+  constexpr int kFew = 16 * (32 * KB + 8) * 4 + 64, kMany = MANY ? 2 * 64 * tile_row<KB>() : 0;
+  __shared__ __align__(16) char room[kMany > kFew ? kMany : kFew];
   int gi = 0;
   while (gi + 1 < a.count && (int)blockIdx.x >= a.linear[gi + 1].first) ++gi;
   const Linear& l = a.linear[gi];
   const int64_t m_begin = (int64_t)((int)blockIdx.x - l.first) * a.chunks * kColumns;
   const int64_t m_end = m_begin + a.chunks * kColumns < l.m ? m_begin + a.chunks * kColumns : l.m;
-  const int64_t t0 = (int64_t)(blockIdx.y / a.slots) * kTile;
-  each_group(a, t0, blockIdx.y % a.slots, l.out != l.y, [&](const Group& g) {
+  const int64_t t0 = (int64_t)(blockIdx.y % a.tiles) * kTile;
+  each_group(a, t0, blockIdx.y / a.tiles, l.out != l.y, [&](const Group& g) {
     if (g.adapter < 0) return copy_group(l, g, t0, m_begin, m_end);
-    if constexpr (NB > 1) {
-      if (g.size <= 16) return up_group<BF, KB, 1>(a, l, g, t0, m_begin, m_end, high, low, factor);
+    if constexpr (MANY) {
+      if (g.size > 16) return up_tile<BF, KB>(a, l, g, t0, m_begin, m_end, room);
     }
-    up_group<BF, KB, NB>(a, l, g, t0, m_begin, m_end, high, low, factor);
+    up_group<BF, KB>(a, l, g, t0, m_begin, m_end, room);
   });
 }
 
 template <bool BF>
 auto down_kernel(int blocks, bool many) {
-  if (many) return blocks <= 2 ? adapter_down_kernel<BF, 2, true> : adapter_down_kernel<BF, 4, true>;
+  if (many) return blocks == 2 ? adapter_down_kernel<BF, 2, true> : blocks == 4 ? adapter_down_kernel<BF, 4, true>
+                   : blocks == 6 ? adapter_down_kernel<BF, 6, true> : adapter_down_kernel<BF, 8, true>;
   return blocks == 1 ? adapter_down_kernel<BF, 1, false> : blocks == 2 ? adapter_down_kernel<BF, 2, false> : adapter_down_kernel<BF, 4, false>;
 }
-template <bool BF, int NB>
+template <bool BF, bool MANY>
 auto up_kernel(int rank) {
-  return rank <= 32 ? adapter_up_kernel<BF, 1, NB> : rank <= 64 ? adapter_up_kernel<BF, 2, NB> : adapter_up_kernel<BF, 4, NB>;
+  return rank <= 32 ? adapter_up_kernel<BF, 1, MANY> : rank <= 64 ? adapter_up_kernel<BF, 2, MANY>
+         : rank <= 96 ? adapter_up_kernel<BF, 3, MANY> : adapter_up_kernel<BF, 4, MANY>;
 }
 
 struct Plan {
@@ -511,15 +621,32 @@ Plan plan_of(int64_t tokens, int64_t n, int64_t adapters, int count, const int* 
   const int64_t slots = most < share ? most : share;
   p.slots = 1;
   while (p.slots < slots && p.slots < adapters + 1) p.slots *= 2;
-  int high = 0;
-  for (int g = 0; g < count; ++g) high = ranks[g] > high ? ranks[g] : high;
-  p.blocks = high > 32 ? 4 : high > 16 || tokens > 16 ? 2 : 1;
-  p.runs = 0;
-  for (int g = 0; g < count; ++g) p.runs += (ranks[g] + 16 * p.blocks - 1) / (16 * p.blocks);
-  const int64_t steps = (n + 255) / 256, groups = p.tiles * (p.slots < 8 ? 1 : p.slots / 2) * p.runs;
+  int all = 0;
+  for (int g = 0; g < count; ++g) all += ranks[g];
+  const int blocks = (all + 15) / 16;
+  const int64_t steps = (n + 255) / 256, groups = p.tiles * (p.slots < 8 ? 1 : p.slots / 2);
+  // Few tokens need many narrow work-groups, many tokens wide ones that read x
+  // once: one token's 48 ranks of 4096 inputs in blocks of 16 take 4.2 us, in one of
+  // 64 5.1; 48 tokens with 24 adapters of 128 ranks in blocks of 32 11.9, of 64 9.8;
+  // 300 tokens with 128 ranks in blocks of 32 6.6, of 64 7.6, of 128 10.4; 1136 with
+  // 240 ranks 16.2, 13.8 and 16.3; 8296 with 160 ranks of 24296 inputs in blocks of
+  // 64 254, of 96 194.
+  auto widest = [&](int width) { p.runs = (blocks + width - 1) / width, p.blocks = (blocks + p.runs - 1) / p.runs; };
+  if (p.tiles == 1) {
+    int width = tokens > 16 ? 2 : 1;
+    widest(width);
+    while (width < 4 && groups * p.runs * (steps < 16 ? steps : 16) > 512) widest(width *= 2);
+  } else {
+    widest(p.tiles < 16 ? 2 : p.tiles < 64 ? 4 : 8);
+  }
+  if (p.blocks > 1 || tokens > 16) p.blocks += p.blocks & 1;
+  // Splits fill the GPU, but each is read again by the second launch: 6 prompts
+  // of 900 with 4 splits of 3584 inputs (340 work-groups) take 15 + 25 us, with 8 18
+  // + 29, with 2 18 + 23.  Groups of single tokens have shorter loops and want four
+  // times as many.
   int64_t splits = 1;
-  if (p.tiles == 1) splits = (1024 + groups - 1) / groups;
-  else while (splits < 8 && groups * splits < (n <= 8192 ? 512 : 256)) splits *= 2;
+  if (p.tiles == 1) splits = (1024 + groups * p.runs - 1) / (groups * p.runs);
+  else while (splits < 8 && groups * p.runs * splits < 256) splits *= 2;
   splits = splits < steps ? splits : steps;
   splits = splits < 16 ? splits : 16;
   p.steps = (int)((steps + splits - 1) / splits);
@@ -578,36 +705,42 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
                (long long)j.ldy, (long long)j.ldo);
     a.linear[g] = Linear{static_cast<const uint16_t*>(j.down), static_cast<const uint16_t*>(j.up), j.scale,
                          static_cast<const uint16_t*>(j.y), static_cast<uint16_t*>(j.out), j.down_adapter, j.down_row,
-                         j.up_adapter, j.up_row, tokens == 1 ? 0 : j.ldy, tokens == 1 ? 0 : j.ldo, j.m, j.rank, a.ranks, 0, 0};
+                         j.up_adapter, j.up_row, tokens == 1 ? 0 : j.ldy, tokens == 1 ? 0 : j.ldo, j.m, j.rank, a.ranks, 0};
     a.ranks += j.rank, ranks[g] = j.rank;
     most = j.rank > most ? j.rank : most;
     columns += (j.m + kColumns - 1) / kColumns;
   }
   const Plan p = plan_of(tokens, n, adapters, count, ranks);
-  a.slots = p.slots, a.splits = p.splits, a.steps = p.steps;
+  a.tiles = (int)p.tiles, a.splits = p.splits, a.steps = p.steps;
   const size_t need = (size_t)p.splits * tokens * a.ranks * sizeof(float);
   QS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
              "%s: workspace of %zu bytes (16-byte aligned), %zu needed", fn, workspace_bytes, need);
   a.part = static_cast<float*>(workspace);
-  // a work-group takes several runs of columns where there are tiles enough
+  // A work-group takes several runs of columns where there are groups enough: it
+  // splits up the inner products once for all of them.  Groups of single tokens
+  // are short, 512 of them fill the GPU (48 tokens to 2 x 25600: 33 us, with 2048
+  // 48); tiles of prompts want more (8296 tokens to 12659 columns: 126 us, with 512
+  // 210).
   a.chunks = 1;
   const int64_t groups = p.tiles * (p.slots < 8 ? 1 : p.slots / 2);
-  while (a.chunks < 8 && groups * columns / (2 * a.chunks) >= 512) a.chunks *= 2;
-  int grid = 0, run = 0;
+  while (a.chunks < 8 && groups * columns / (2 * a.chunks) >= (p.tiles == 1 ? 512 : 2048)) a.chunks *= 2;
+  int grid = 0;
   for (int g = 0; g < count; ++g) {
-    a.linear[g].first_run = run;
-    run += (ranks[g] + 16 * p.blocks - 1) / (16 * p.blocks);
     a.linear[g].first = grid;
     grid += (int)((a.linear[g].m + (int64_t)a.chunks * kColumns - 1) / ((int64_t)a.chunks * kColumns));
   }
   const bool bf = dtype == QS_DTYPE_BF16;
   const auto down = bf ? down_kernel<true>(p.blocks, tokens > 16) : down_kernel<false>(p.blocks, tokens > 16);
-  const unsigned rows = (unsigned)(p.tiles * p.slots);
-  hipLaunchKernelGGL(down, dim3((unsigned)(p.runs * p.splits), rows), dim3(kThreads), 0, as_stream(stream), a);
+  // at a boundary of two prompts the second one's tokens go to work-groups of
+  // their own: 15 us in place of 21 where 6 prompts of 900 have 72 ranks of 3584
+  // inputs.  (The second launch has many more, of which half would be empty.)
+  a.slots = p.tiles > 1 && p.slots < 2 ? 2 : p.slots;
+  hipLaunchKernelGGL(down, dim3((unsigned)(p.runs * p.splits), (unsigned)(p.tiles * a.slots)), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("adapter_down_kernel");
-  const auto up = tokens <= 16 ? (bf ? up_kernel<true, 1>(most) : up_kernel<false, 1>(most))
-                               : (bf ? up_kernel<true, 4>(most) : up_kernel<false, 4>(most));
-  hipLaunchKernelGGL(up, dim3((unsigned)grid, rows), dim3(kThreads), 0, as_stream(stream), a);
+  const auto up = tokens > 16 ? (bf ? up_kernel<true, true>(most) : up_kernel<false, true>(most))
+                              : (bf ? up_kernel<true, false>(most) : up_kernel<false, false>(most));
+  a.slots = p.slots;
+  hipLaunchKernelGGL(up, dim3((unsigned)grid, (unsigned)(p.tiles * p.slots)), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("adapter_up_kernel");
   return QS_OK;
 }

@@ -99,6 +99,16 @@ def test_long_prompts(dev):
     run(dev, which, 1024, [640], 64, dtype=HF, inplace=True)
 
 
+@pytest.mark.parametrize("ranks", [[8, 24, 8], [72], [88, 8], [96, 40, 104], [128, 128, 128, 128]])
+@pytest.mark.parametrize("tokens", [100, 1100, 4200])
+def test_ranks_that_differ_for_prompts(dev, tokens, ranks):
+    """Blocks of ranks that belong to two linears, whole runs of them and the last one's end; groups of more and of
+    fewer than 16 tokens; widths that end inside an access."""
+    cuts = [tokens // 3 + 5, 9, tokens // 2, tokens]
+    which = [a for a, c in zip((2, 1, -1, 0), cuts) for _ in range(c)][:tokens]
+    run(dev, which, 200, [131, 64, 33, 7][:len(ranks)], 0, ranks=ranks, adapters=3, dtype=HF if tokens == 100 else BF)
+
+
 def test_every_token_its_own_adapter(dev):
     run(dev, torch.randperm(64, generator=gen(1)), 256, [256], 16, adapters=64)
     run(dev, torch.randperm(300, generator=gen(1)), 256, [64], 8, adapters=300)
