@@ -13,6 +13,7 @@ from . import _lib
 from .pages import _HALF, _int32, _room, _workspace
 
 MAX_RANK = 128
+NAMES = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
 
 
 def _rows(name, t, tokens, width, dtype, device):
@@ -132,6 +133,8 @@ class Adapters:
                              f"{self.down.shape[2]} inputs and {self.up.shape[1]} outputs")
         if not 0 <= i < len(self.scale):
             raise IndexError(f"adapter {i} of {len(self.scale)}")
+        # its own values may be given, so nothing is cleared before they are read
+        down, up = down.to(self.down, copy=True), up.to(self.up, copy=True)
         self.clear(i)
         self.down[i, :r] = down
         self.up[i, :, :r] = up
@@ -155,12 +158,13 @@ def beside(x: Tensor, linears, ys, which: Tensor):
     return ys
 
 
-def attach_adapters(model, count, rank, names=("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj"),
-                    dtype=torch.bfloat16):
+def attach_adapters(model, count, rank, names=NAMES, dtype=torch.bfloat16):
     """Gives every ``QuantizedLinear`` of ``model`` whose last name is among
-    ``names`` room for ``count`` adapters of rank ``rank``, empty at first, in
-    its attribute ``adapters``.  Returns them by the linears' names."""
+    ``names`` (of ``NAMES``) room for ``count`` adapters of rank ``rank``, empty
+    at first, in its attribute ``adapters``.  Returns them by the linears' names."""
     from .checkpoint import QuantizedLinear
+    if not set(names) <= set(NAMES):
+        raise ValueError(f"no decoder takes adapters beside {sorted(set(names) - set(NAMES))} (only {', '.join(NAMES)})")
     out = {}
     for name, lin in model.named_modules():
         if isinstance(lin, QuantizedLinear) and name.rpartition(".")[2] in names:

@@ -703,6 +703,9 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
                "%s: linear %d: tensors must be aligned to their elements", fn, g);
     QS_REQUIRE(j.y != j.out || tokens == 1 || j.ldy == j.ldo, "%s: linear %d: y and out share memory with rows %lld and %lld apart", fn, g,
                (long long)j.ldy, (long long)j.ldo);
+    for (int h = 0; h < count; ++h)
+      QS_REQUIRE(h == g || (j.out != jobs[h].y && j.out != jobs[h].out), "%s: the output of linear %d is linear %d's y or output", fn, g, h);
+    QS_REQUIRE(j.out != x, "%s: the output of linear %d is x", fn, g);
     a.linear[g] = Linear{static_cast<const uint16_t*>(j.down), static_cast<const uint16_t*>(j.up), j.scale,
                          static_cast<const uint16_t*>(j.y), static_cast<uint16_t*>(j.out), j.down_adapter, j.down_row,
                          j.up_adapter, j.up_row, tokens == 1 ? 0 : j.ldy, tokens == 1 ? 0 : j.ldo, j.m, j.rank, a.ranks, 0};

@@ -341,7 +341,7 @@ class PagedDecoder(StaticDecoder):
                                 columns, page, torch.bfloat16, self.dev)
         self.spans = {"window": window, "sinks": sinks}
         self.which = torch.full((rows,), -1, dtype=torch.int32, device=self.dev)
-        self._tokens_which = self.which  # of the tokens at hand: the rows', or a prompt's
+        self._prompt_which = None  # of a prompt's tokens, while it runs
 
     def _adapted(self):
         return any(getattr(mod, "adapters", None) is not None for L in self.layers for mod in
@@ -353,8 +353,8 @@ class PagedDecoder(StaticDecoder):
             return outs
         from .adapters import beside
         flat = [y.reshape(-1, y.shape[-1]) for y in outs]
-        return [f.view(y.shape) for f, y in
-                zip(beside(x.reshape(-1, x.shape[-1]), linears, flat, self._tokens_which), outs)]
+        which = self.which if self._prompt_which is None else self._prompt_which
+        return [f.view(y.shape) for f, y in zip(beside(x.reshape(-1, x.shape[-1]), linears, flat, which), outs)]
 
     def _normed_linears(self, h, linears, pre):
         if all(getattr(l, "adapters", None) is None for l in linears):
@@ -366,7 +366,7 @@ class PagedDecoder(StaticDecoder):
         return self._beside(x, [linear], [linear(x)])[0]
 
     def _prompt_hidden(self, ids, counts):
-        """The last layer's normed output for all tokens of a prompt call, and the rows' first tokens and counts."""
+        """The last layer's output for all tokens of a prompt call, and the rows' counts."""
         m, cache = self.model.model, self.cache
         T = int(sum(counts))
         if ids.shape != (T,) or len(counts) != self.B:
@@ -378,11 +378,21 @@ class PagedDecoder(StaticDecoder):
         cache.check()
         h = m.embed_tokens(ids)[None]
         if self.normed:
-            from transformers.models.qwen3.modeling_qwen3 import apply_rotary_pos_emb
             pos = (cache.lengths + cache.over)[row] - starts[row + 1] + torch.arange(T, device=self.dev)
             cos, sin = m.rotary_emb(h, pos[None])
-        self._tokens_which = self.which[row]
-        bf = torch.bfloat16
+        self._prompt_which = self.which[row]
+        try:
+            h = self._prompt_layers(h, starts, (cos, sin) if self.normed else None)
+        finally:
+            self._prompt_which = None
+        if self.window:
+            cache.free(window=self.window, sinks=self.sinks)
+        return h[0], count
+
+    def _prompt_layers(self, h, starts, turns):
+        if self.normed:
+            from transformers.models.qwen3.modeling_qwen3 import apply_rotary_pos_emb
+        cache, T, bf = self.cache, h.shape[1], torch.bfloat16
         for i, L in enumerate(self.layers):
             a = L.self_attn
             x = L.input_layernorm(h)
@@ -390,7 +400,7 @@ class PagedDecoder(StaticDecoder):
             if self.normed:
                 q = a.q_norm(qo.view(1, T, self.nh, self.hd)).transpose(1, 2)
                 k = a.k_norm(ko.view(1, T, self.nkv, self.hd)).transpose(1, 2)
-                q, k = apply_rotary_pos_emb(q, k, cos, sin)
+                q, k = apply_rotary_pos_emb(q, k, *turns)
                 q = q[0].transpose(0, 1).to(bf).contiguous()
                 cache.append(i, k[0].transpose(0, 1).to(bf).contiguous(), vo.view(T, self.nkv, self.hd).to(bf), starts)
             else:
@@ -401,10 +411,7 @@ class PagedDecoder(StaticDecoder):
             x = L.post_attention_layernorm(h)
             go, uo = self._beside(x, [L.mlp.gate_proj, L.mlp.up_proj], grouped_forward(x, [L.mlp.gate_proj, L.mlp.up_proj]))
             h = h + self._linear(L.mlp.act_fn(go) * uo, L.mlp.down_proj)
-        self._tokens_which = self.which
-        if self.window:
-            cache.free(window=self.window, sinks=self.sinks)
-        return h[0], count
+        return h
 
     @torch.no_grad()
     def prompt(self, ids, counts):
@@ -468,6 +475,8 @@ def greedy_decode_paged(model, prompts, new_tokens, which=None, top=0, use_graph
     HIP graph unless use_graph=False.  Returns (tokens (prompts, new_tokens), their scores: log probabilities, entropies
     (prompts, new_tokens), the ``top`` best tokens' log probabilities and ids (prompts, new_tokens, top))."""
     from .logprobs import token_logprobs
+    if not prompts or any(len(p) < 1 for p in prompts) or new_tokens < 1:
+        raise ValueError(f"{new_tokens} new tokens behind prompts of {[len(p) for p in prompts]}: every prompt has a token or more")
     R, dev = len(prompts), prompts[0].device
     dec = PagedDecoder(model, R, max(len(p) for p in prompts) + new_tokens, page)
     if which is not None:
@@ -479,9 +488,9 @@ def greedy_decode_paged(model, prompts, new_tokens, which=None, top=0, use_graph
     at = torch.zeros(1, dtype=torch.long, device=dev)
 
     def take(logits):
-        last.copy_(logits.argmax(-1))
-        logp, entropy, _, best, tokens = token_logprobs(logits, last, top)
-        for o, new in zip(out, (last, logp, entropy, best, tokens)):
+        _, entropy, _, best, tokens = token_logprobs(logits, last, max(top, 1))
+        last.copy_(tokens[:, 0].clamp_min(0))  # a row without a finite logit takes token 0
+        for o, new in zip(out, (last, best[:, 0], entropy, best[:, :top], tokens[:, :top])):
             o.index_copy_(1, at, new.unsqueeze(1))
         at.add_(1)
 

@@ -41,9 +41,11 @@ def rope_frequencies(dim: int, base: float = 10000.0, scaling: dict = None, devi
     kind = scaling.get("rope_type", scaling.get("type", "default"))
     if kind not in _SCALINGS:
         raise NotImplementedError(f"rope_type {kind!r} ({', '.join(_SCALINGS)})")
-    if any(scaling.get(name) is None for name in _SCALINGS[kind]) or not scaling.get("factor", 1.0) > 0:
-        raise ValueError(f"{kind} scaling takes {', '.join(_SCALINGS[kind])}, the factor above 0; got {scaling}")
-    base, factor = float(base), float(scaling.get("factor", 1.0))
+    if any(not (scaling.get(name) or 0) > 0 for name in _SCALINGS[kind]):
+        raise ValueError(f"{kind} scaling takes {', '.join(_SCALINGS[kind])}, all above 0; got {scaling}")
+    base, factor = float(base), float(scaling.get("factor") or 1.0)
+    if not base > 1:
+        raise ValueError(f"a base of {base}: a number above 1")
     if kind == "ntk":
         if dim == 2:
             raise ValueError("ntk scaling takes more than one pair")
@@ -56,6 +58,8 @@ def rope_frequencies(dim: int, base: float = 10000.0, scaling: dict = None, devi
     trained = scaling["original_max_position_embeddings"]
     if kind == "llama3":
         low, high = float(scaling["low_freq_factor"]), float(scaling["high_freq_factor"])
+        if not low < high:
+            raise ValueError(f"llama3 scaling blends from {low} to {high} turns: the first must be the lower")
         kept = ((trained * w / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
         return (kept * w + (1 - kept) * w / factor).to(device), 1.0
 

@@ -164,6 +164,24 @@ def test_greedy_decode_with_scores(model, dev):
         assert ((logp[r] - want).abs() <= 2 * 0.02 * logits.norm(dim=1)).all()
 
 
+def test_rows_adapters_given_as_a_new_tensor(model, dev):
+    """A step takes the ``which`` that the decoder has then, a tensor of its own among them, and a refused prompt leaves
+    nothing behind."""
+    from quipsharp_amd.decode import PagedDecoder
+    one, two = (PagedDecoder(model, 2, 64, 16) for _ in range(2))
+    ids, counts = ids_of(12, 20, dev), [7, 5]
+    one.prompt(ids, counts), two.prompt(ids, counts)
+    one.which.copy_(torch.tensor([1, 0], dtype=torch.int32))
+    two.which = torch.tensor([1, 0], dtype=torch.int32, device=dev)
+    assert torch.equal(one.step(ids[:2]), two.step(ids[:2]))
+    two.which = two.which.long()
+    with pytest.raises(ValueError, match="which must be"):
+        two.prompt(ids[:3], [2, 1])
+    two.which = one.which
+    two.cache.lengths.copy_(one.cache.lengths)
+    assert torch.equal(one.step(ids[2:4]), two.step(ids[2:4]))
+
+
 def test_beam_search_with_adapters(model, dev):
     """Beams of one request keep its adapters; one beam is greedy decode."""
     from quipsharp_amd.decode import beam_decode, greedy_decode_paged

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from quipsharp_amd import _lib
-from quipsharp_amd.adapters import Adapters, add_adapters
+from quipsharp_amd.adapters import Adapters, add_adapters, attach_adapters
 from quipsharp_amd.logprobs import token_logprobs
 from quipsharp_amd.rope import append_rotated, rope_frequencies
 
@@ -87,6 +87,34 @@ def test_bank_refuses():
     assert bank.down[1].sum() == 192 and bank.up[1].sum() == 120 and bank.scale.tolist() == [0.0, 2.0]
     bank.clear(1)
     assert not bank.down.any() and not bank.up.any() and not bank.scale.any()
+
+
+def test_bank_takes_its_own_values():
+    bank = Adapters(2, 8, 64, 40, device="cpu")
+    bank.load(0, torch.randn(8, 64), torch.randn(40, 8))
+    down, up = bank.down[0].clone(), bank.up[0].clone()
+    bank.load(0, bank.down[0, 2:5], bank.up[0, :, 2:5], 3.0)
+    assert torch.equal(bank.down[0, :3], down[2:5]) and torch.equal(bank.up[0, :, :3], up[:, 2:5])
+    assert not bank.down[0, 3:].any() and not bank.up[0, :, 3:].any() and bank.scale[0] == 3.0
+
+
+def test_adapters_beside_other_linears_are_refused():
+    with pytest.raises(ValueError, match="lm_head"):
+        attach_adapters(torch.nn.Module(), 2, 8, names=("q_proj", "lm_head"))
+
+
+@pytest.mark.parametrize("y,out,message", [
+    ((4096, 12288), (12288, 8192), "the output of linear 0 is linear 1's y or output"),
+    ((4096, 12288), (8192, 4096), "the output of linear 1 is linear 0's y"),
+    ((4096, 12288), (8192, 8192), "the output of linear 0 is linear 1's y or output"),
+    ((8192, 12288), (4096, 16384), "the output of linear 0 is x"),
+])
+def test_adapters_c_refuse_outputs_that_are_read(y, out, message):
+    L = _lib.lib()
+    jobs = (_lib.AdapterJob * 2)(*[_lib.AdapterJob(down=4096, up=4096, scale=4096, down_adapter=512, down_row=64, up_adapter=320,
+                                                   up_row=8, rank=8, m=40, y=a, ldy=40, out=b, ldo=40) for a, b in zip(y, out)])
+    assert L.qs_adapters_add(P, 2, 64, 3, 64, P, 2, 2, jobs, P, 1 << 20, None) == 1
+    assert message in L.qs_last_error().decode()
 
 
 def adapters_c(L, **over):
@@ -236,6 +264,20 @@ def test_frequencies_refuse():
                     dict(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192, low_freq_factor=1.0)):
         with pytest.raises(ValueError, match="scaling takes"):
             rope_frequencies(64, scaling=scaling, device="cpu")
+    with pytest.raises(ValueError, match="must be the lower"):
+        rope_frequencies(64, scaling=dict(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192,
+                                          low_freq_factor=4.0, high_freq_factor=4.0), device="cpu")
+    for base in (0.0, 1.0):
+        with pytest.raises(ValueError, match="above 1"):
+            rope_frequencies(64, base, device="cpu")
+    assert rope_frequencies(64, scaling=dict(rope_type="default", factor=None), device="cpu")[1] == 1.0
+
+
+def test_greedy_decode_refuses():
+    from quipsharp_amd.decode import greedy_decode_paged
+    for prompts, new in (([], 3), ([torch.zeros(2), torch.zeros(0)], 3), ([torch.zeros(2)], 0)):
+        with pytest.raises(ValueError, match="every prompt has a token"):
+            greedy_decode_paged(None, prompts, new)
 
 
 # ---------------------------------------------------------------------------
