@@ -34,7 +34,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTile = 64;     // tokens at a time
 constexpr int kMaxRank = 128;
-constexpr int kColumns = 256;  // output columns of a work-group at a time, 64 a wave
+constexpr int kColumns = 256;  // output columns of a work-group of single tokens at a time, 64 a wave
 
 struct Linear {
   const uint16_t *down, *up;
@@ -52,7 +52,7 @@ struct AdapterArgs {
   const int32_t* which;
   int adapters, count, ranks;  // ranks: of all linears together
   int tiles, splits, steps;    // steps of 256 inputs of a split
-  int slots, chunks;           // work-groups that share a tile's groups, a power of two; runs of kColumns of a work-group
+  int slots, span;             // work-groups that share a tile's groups, a power of two; columns of one of the second launch
   float* part;                 // [splits][tokens][ranks]
   Linear linear[QS_MAX_GROUP];
 };
@@ -584,8 +584,8 @@ __global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
   int gi = 0;
   while (gi + 1 < a.count && (int)blockIdx.x >= a.linear[gi + 1].first) ++gi;
   const Linear& l = a.linear[gi];
-  const int64_t m_begin = (int64_t)((int)blockIdx.x - l.first) * a.chunks * kColumns;
-  const int64_t m_end = m_begin + a.chunks * kColumns < l.m ? m_begin + a.chunks * kColumns : l.m;
+  const int64_t m_begin = (int64_t)((int)blockIdx.x - l.first) * a.span;
+  const int64_t m_end = m_begin + a.span < l.m ? m_begin + a.span : l.m;
   const int64_t t0 = (int64_t)(blockIdx.y % a.tiles) * kTile;
   each_group(a, t0, blockIdx.y / a.tiles, l.out != l.y, [&](const Group& g) {
     if (g.adapter < 0) return copy_group(l, g, t0, m_begin, m_end);
@@ -711,7 +711,7 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
                          j.up_adapter, j.up_row, tokens == 1 ? 0 : j.ldy, tokens == 1 ? 0 : j.ldo, j.m, j.rank, a.ranks, 0};
     a.ranks += j.rank, ranks[g] = j.rank;
     most = j.rank > most ? j.rank : most;
-    columns += (j.m + kColumns - 1) / kColumns;
+    columns += j.m;
   }
   const Plan p = plan_of(tokens, n, adapters, count, ranks);
   a.tiles = (int)p.tiles, a.splits = p.splits, a.steps = p.steps;
@@ -719,18 +719,26 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
   QS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
              "%s: workspace of %zu bytes (16-byte aligned), %zu needed", fn, workspace_bytes, need);
   a.part = static_cast<float*>(workspace);
-  // A work-group takes several runs of columns where there are groups enough: it
-  // splits up the inner products once for all of them.  Groups of single tokens
-  // are short, 512 of them fill the GPU (48 tokens to 2 x 25600: 33 us, with 2048
-  // 48); tiles of prompts want more (8296 tokens to 12659 columns: 126 us, with 512
-  // 210).
-  a.chunks = 1;
-  const int64_t groups = p.tiles * (p.slots < 8 ? 1 : p.slots / 2);
-  while (a.chunks < 8 && groups * columns / (2 * a.chunks) >= (p.tiles == 1 ? 512 : 2048)) a.chunks *= 2;
+  // Columns of a work-group, which splits up the inner products once for all of
+  // them.  Groups of single tokens take 256 at a time, 64 a wave, and 512
+  // work-groups of them fill the GPU (48 tokens to 2 x 25600: 33 us with 1024 columns,
+  // 48 with 256).  Prompts take 64 at a time and are cut finer where there are few
+  // (142 tokens to 1315 columns: 8.5 us with 64, 12 with 256) and coarser where there
+  // are many (10358 to 5120: 58 us with 512, 62 with 256, 80 with 128; but 8296 to
+  // 12659 151 us with 1024, 128 with 512); work-groups of slots without a group cost
+  // their launch (232 tokens in 16 slots to 20507 columns: 20 us with 64, 9 with 256).
+  if (p.tiles == 1) {
+    const int64_t groups = p.slots < 8 ? 1 : p.slots / 2;
+    a.span = kColumns;
+    while (a.span < 8 * kColumns && groups * columns / (2 * a.span) >= 512) a.span *= 2;
+  } else {
+    a.span = 64;
+    while (a.span < (p.slots > 1 ? 256 : 512) && p.tiles * p.slots * columns / (2 * a.span) >= 640) a.span *= 2;
+  }
   int grid = 0;
   for (int g = 0; g < count; ++g) {
     a.linear[g].first = grid;
-    grid += (int)((a.linear[g].m + (int64_t)a.chunks * kColumns - 1) / ((int64_t)a.chunks * kColumns));
+    grid += (int)((a.linear[g].m + a.span - 1) / a.span);
   }
   const bool bf = dtype == QS_DTYPE_BF16;
   const auto down = bf ? down_kernel<true>(p.blocks, tokens > 16) : down_kernel<false>(p.blocks, tokens > 16);
