@@ -619,7 +619,10 @@ typedef struct qs_adapter_job {
 /* out_g[t] = y_g[t] + scale_g[a] up_g[a] (down_g[a] x[t]) with a = which[t] for
  * up to QS_MAX_GROUP linears g that read the same x [tokens][n] (bf16 or fp16,
  * n a multiple of 8).  Tokens whose which is not in 0 .. adapters - 1 have
- * out = y.  fp32 sums, one rounding.  workspace: qs_adapters_workspace_bytes. */
+ * out = y.  fp32 sums, one rounding.  No out may be x, another linear's y or its
+ * out.  workspace: qs_adapters_workspace_bytes, for this call alone while it
+ * runs.  At most 2^19 tokens; rows of x, y, out and weights at most 2^24 elements
+ * apart. */
 size_t qs_adapters_workspace_bytes(int64_t tokens, int64_t n, int64_t adapters, int count, const int *ranks);
 int qs_adapters_add(const void *x, int dtype, int64_t ldx, int64_t tokens, int64_t n, const int32_t *which,
                     int64_t adapters, int count, const qs_adapter_job *jobs, void *workspace, size_t workspace_bytes,

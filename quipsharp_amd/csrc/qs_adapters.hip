@@ -12,9 +12,10 @@
 // Both are bound by memory: single tokens by the weights of the adapters that
 // they name, prompts by x, y and out.  Measured: 48 tokens of 24 adapters of rank
 // 64, 5120 inputs to two linears of 25600, 10 and 33 us for 177 MB (4.1 TB/s; a
-// large copy reaches 5.06); 3 prompts of 4096, 25600 inputs to 5120 at rank 64, 94
-// and 63 us for 756 MB (4.8 TB/s); 6 of 900, 3584 inputs to 3584 + 512 + 512 at rank
-// 24, 15 and 25 us for 114 MB; one token of the smallest sizes 4 and 5 us.
+// large copy reaches 5.06); 10358 tokens of 3 prompts, 25600 inputs to 5120 at rank
+// 64, 95 and 58 us for 747 MB (4.9 TB/s); 4247 of 6, 3584 inputs to 3584 + 512 + 512
+// at rank 24, 15 and 25 us for 114 MB (2.8 TB/s: short loops behind each
+// work-group's start); one token, 4096 inputs to 4096 + 1024 + 1024, 4 and 5 us.
 //
 // Tokens are taken 64 at a time.  In each 64 those of one adapter form a group
 // (found by ballots: prompts come in runs, single tokens in any order), which
