@@ -108,34 +108,57 @@ __device__ __forceinline__ void write_alternative(const ScoreArgs& a, int64_t ro
 }
 
 // Leaves the best `top` of n > top candidates, no two of which are alike, at
-// the front of room: their least is found bit by bit.
+// the front of room: their least is found two at a time of the bits in which
+// candidates differ, and no further than it takes to tell it from the next.
+constexpr int kCounts = 97;  // three for every two bits, and one
 __device__ void narrow(uint64_t* room, int n, int top, int* above) {
   constexpr int kEach = (kRoom + kThreads - 1) / kThreads;
-  const int tid = threadIdx.x;
-  uint64_t mine[kEach];
+  __shared__ uint64_t some[4], all[4];
+  const int tid = threadIdx.x, w = tid >> 6;
+  uint64_t mine[kEach], any = 0, every = ~0ull;
 #pragma unroll
-  for (int i = 0; i < kEach; ++i) mine[i] = i * kThreads + tid < n ? room[i * kThreads + tid] : 0;
-  if (tid < 65) above[tid] = 0;
+  for (int i = 0; i < kEach; ++i) {
+    const bool is = i * kThreads + tid < n;
+    mine[i] = is ? room[i * kThreads + tid] : 0;
+    any |= mine[i], every &= is ? mine[i] : ~0ull;
+  }
+#pragma unroll
+  for (int x = 1; x < 64; x *= 2) any |= __shfl_xor(any, x), every &= __shfl_xor(every, x);
+  if ((tid & 63) == 0) some[w] = any, all[w] = every;
+  if (tid < kCounts) above[tid] = 0;
   __syncthreads();
-  uint64_t least = 0;
-  for (int bit = 63; bit >= 0; --bit) {
-    const uint64_t v = least | 1ull << bit;
-    int many = 0;
+  uint64_t least = all[0] & all[1] & all[2] & all[3], open = (some[0] | some[1] | some[2] | some[3]) & ~least;
+  for (int* counts = above; open; counts += 3) {
+    const uint64_t one = 1ull << (63 - __builtin_clzll(open));
+    open &= ~one;
+    const uint64_t two = open ? 1ull << (63 - __builtin_clzll(open)) : 0;
+    open &= ~two;
+    const uint64_t at[3] = {least | two, least | one, least | one | two};
+    int many[3] = {0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) many += __popcll(__ballot(mine[i] >= v));
-    if ((tid & 63) == 0) atomicAdd(&above[bit], many);
+    for (int i = 0; i < kEach; ++i)
+      if (i * kThreads < n)
+#pragma unroll
+        for (int k = 0; k < 3; ++k) many[k] += __popcll(__ballot(mine[i] >= at[k]));
+    if ((tid & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) atomicAdd(&counts[k], many[k]);
     __syncthreads();
-    if (above[bit] >= top) least = v;
+    int have = 0;
+#pragma unroll
+    for (int k = 2; k >= 0; --k)
+      if (!have && counts[k] >= top) have = counts[k], least = at[k];
+    if (have == top) break;
   }
 #pragma unroll
   for (int i = 0; i < kEach; ++i)
-    if (mine[i] >= least) room[atomicAdd(&above[64], 1)] = mine[i];
+    if (i * kThreads + tid < n && mine[i] >= least) room[atomicAdd(&above[kCounts - 1], 1)] = mine[i];
   __syncthreads();
 }
 
 // The best `top` of the first n candidates, in order, in best; zeros behind
-// them.  More than kFew are narrowed first (2048 equal logits of a slice, 64
-// wanted: 100 us by their ranks alone, 6 so).
+// them.  More than kFew are narrowed first (2040 equal logits, 64 wanted: 12
+// us in all, by their ranks alone 100).
 constexpr int kFew = 192;
 __device__ __forceinline__ void rank_all(uint64_t* room, int n, uint64_t* best, int top, int* above) {
   if (n > kFew) narrow(room, n, top, above), n = top;
@@ -203,8 +226,8 @@ struct Groups {
 struct Room {
   uint64_t keys[kRoom], best[kMaxTop];
   uint16_t listed[kListed];
-  float red[2][4];
-  int above[65];  // of a search bit by bit, a count for each
+  float red[4][4];
+  int above[kCounts];  // of a search bit by bit
   int groups, count, sums[4];
 };
 
@@ -214,7 +237,9 @@ __device__ __forceinline__ uint64_t key_of(float x, uint32_t token) { return (ui
 // thread's largest logit is `largest`.  At least `top` groups have a maximum
 // that is not below the edge, the largest of the waves' top-th largest
 // maxima of threads or the least of their top / 4-th, and the best lie in groups
-// of which that is so: those are read again.  Where they or their logits at
+// of which that is so: those are read again.  (In a part of fewer pieces than
+// threads, of which waves have nothing: the second of their top / 2-th or the third
+// of their top / 3-th; 64 alternatives of 8 rows of 21818 24 us without, 9 so.)  Where they or their logits at
 // the edge are too many, it is the top-th largest maximum of the groups: the
 // logits above it lie in fewer than `top` groups, and of those at it the lowest
 // tokens are taken.
@@ -227,11 +252,25 @@ __device__ __forceinline__ void select_best(const Groups<T, P>& g, float largest
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const uint32_t bits = order_bits(largest);
   const float edge_w = order_float(nth_key(bits, top)), part_w = top > 8 ? order_float(nth_key(bits, (top + 3) / 4)) : -INFINITY;
+  const bool sparse = top > 8 && g.end - g.first * Groups<T, P>::W < kThreads * Groups<T, P>::W;
   if (lane == 0) r.red[0][w] = edge_w, r.red[1][w] = part_w;
+  if (sparse) {
+    const float half = order_float(nth_key(bits, (top + 1) / 2)), third = order_float(nth_key(bits, (top + 2) / 3));
+    if (lane == 0) r.red[2][w] = half, r.red[3][w] = third;
+  }
   if (tid == 0) r.groups = 0, r.count = 0;
   __syncthreads();
   float edge = fmaxf(fmaxf(r.red[0][0], r.red[0][1]), fmaxf(r.red[0][2], r.red[0][3]));
   edge = fmaxf(edge, fminf(fminf(r.red[1][0], r.red[1][1]), fminf(r.red[1][2], r.red[1][3])));
+  if (sparse) {
+    auto inner = [&](const float (&v)[4], float& second, float& third) {
+      const float h0 = fmaxf(v[0], v[1]), l0 = fminf(v[0], v[1]), h1 = fmaxf(v[2], v[3]), l1 = fminf(v[2], v[3]);
+      second = fmaxf(fminf(h0, h1), fmaxf(l0, l1)), third = fminf(fmaxf(l0, l1), fminf(h0, h1));
+    };
+    float half, third, other;
+    inner(r.red[2], half, other), inner(r.red[3], other, third);
+    edge = fmaxf(edge, fmaxf(half, third));
+  }
   auto add = [&](float x, uint32_t token) {
     const int at = atomicAdd(&r.count, 1);
     if (at < kRoom) r.keys[at] = key_of(x, token);
@@ -454,13 +493,16 @@ __global__ __launch_bounds__(kThreads) void score_kernel(ScoreArgs a) {
     if (tid < top) write_alternative(a, row, tid, room.best[tid], all, log_sum);
 }
 
-// The parts of a row together: one work-group per row.
+// The parts of a row together: one work-group per row.  LONG: lists of more than
+// 32 (64 alternatives of 48 rows in 19 parts: 8 us, 21 without it; 20
+// alternatives 6.9, with it 7.4).
+template <bool LONG>
 __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   __shared__ uint64_t room[kRoom];
   __shared__ uint64_t best[kMaxTop], tops[kThreads], line;
-  __shared__ uint32_t edge[4];
+  __shared__ uint32_t edge[4], share[4];
   __shared__ Stat stat;
-  __shared__ int count, above[65];
+  __shared__ int count, above[kCounts];
   const LaneX lx = lane_x_init();
   const int tid = threadIdx.x, top = a.top;
   const int64_t row = blockIdx.x;
@@ -468,17 +510,29 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   const uint64_t* lists = a.lists + row * n;
   uint64_t mine[kMaxParts * kMaxTop / kThreads];
   uint64_t high = 0;
+  // Long lists: their first entries, then their second ones, and so on, dealt to
+  // the waves in turn, or the threads' maxima would tell little.
+  int part = 0, place = 0;
+  if (LONG) {
+    const int c = 4 * (tid & 63) + (tid >> 6);
+    part = c % a.parts, place = c / a.parts;
+  }
 #pragma unroll
   for (int i = 0; i < kMaxParts * kMaxTop / kThreads; ++i) {
-    const int c = i * kThreads + tid;
+    int c = i * kThreads + tid;
+    if (LONG) {
+      c = place < top ? part * top + place : n;
+      part += kThreads % a.parts, place += kThreads / a.parts;
+      if (part >= a.parts) part -= a.parts, ++place;
+    }
     mine[i] = c < n ? lists[c] : 0;
     high = mine[i] > high ? mine[i] : high;
   }
   tops[tid] = high;
   if (tid == 0) count = 0, line = 0;
   if (top > 0) {
-    const uint32_t e = nth_key((uint32_t)(high >> 32), top);
-    if ((tid & 63) == 0) edge[tid >> 6] = e;
+    const uint32_t bits = (uint32_t)(high >> 32), e = nth_key(bits, top), s = LONG ? nth_key(bits, (top + 3) / 4) : 0;
+    if ((tid & 63) == 0) edge[tid >> 6] = e, share[tid >> 6] = s;
   }
   if (tid < 64) {
     const Stat* st = a.stats + row * a.parts;
@@ -493,7 +547,8 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
   }
   __syncthreads();
   if (top > 0) {
-    // at least `top` threads of a wave have a candidate whose logit is not below the edge
+    // at least `top` threads of a wave, or a fourth of that in every wave, have a
+    // candidate whose logit is not below the edge
     auto take = [&](uint64_t least) {
 #pragma unroll
       for (int i = 0; i < kMaxParts * kMaxTop / kThreads; ++i)
@@ -502,8 +557,8 @@ __global__ __launch_bounds__(kThreads) void score_join_kernel(ScoreArgs a) {
           if (at < kRoom) room[at] = mine[i];
         }
     };
-    const uint64_t least = (uint64_t)(edge[0] > edge[1] ? edge[0] : edge[1]) << 32, others = (uint64_t)(edge[2] > edge[3] ? edge[2] : edge[3]) << 32;
-    if (high) take(least > others ? least : others);
+    const uint32_t whole = max(max(edge[0], edge[1]), max(edge[2], edge[3])), fourths = min(min(share[0], share[1]), min(share[2], share[3]));
+    if (high) take((uint64_t)max(whole, fourths) << 32);
     __syncthreads();
     int many = count;
     if (many > kRoom) {
@@ -607,7 +662,8 @@ extern "C" int qs_token_logprobs(const void* logits, int dtype, int64_t ld, int6
   hipLaunchKernelGGL(kernel, dim3((unsigned)rows, (unsigned)l.parts), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("score_kernel");
   if (l.parts > 1) {
-    hipLaunchKernelGGL(score_join_kernel, dim3((unsigned)rows), dim3(kThreads), 0, as_stream(stream), a);
+    const auto join = top > 32 ? score_join_kernel<true> : score_join_kernel<false>;
+    hipLaunchKernelGGL(join, dim3((unsigned)rows), dim3(kThreads), 0, as_stream(stream), a);
     QS_LAUNCHED("score_join_kernel");
   }
   return QS_OK;
