@@ -183,6 +183,26 @@ def test_strides(dev):
     assert (out[:, :5] == 0).all() and (out[:, 5 + m:] == 0).all()
 
 
+@pytest.mark.parametrize("tokens", [9, 70, 300])
+def test_rows_as_far_apart_as_they_may_be(dev, tokens):
+    """x, y, out and weights with rows 2^24 elements apart: 2^32 bytes are in 128 of them, a tile's last token lies 2^31
+    behind its first."""
+    from quipsharp_amd.adapters import add_adapters
+    g = gen(10)
+    far, n, m, rank = 2 ** 24, 72, 75, 16
+    space = torch.empty(tokens * far, dtype=BF, device=dev).view(tokens, far)
+    x, y, out = space[:, :n], space[:, 1001:1001 + m], space[:, 2003:2003 + m]
+    weights = torch.empty(2 * m * far, dtype=BF, device=dev).view(2, m, far)
+    down, up = weights[:, :rank, 128:128 + n], weights[:, :, :rank]
+    for t, scale in ((x, 1.0), (y, 1.0), (down, 0.1), (up, 1.0)):
+        t.copy_(torch.randn(t.shape, generator=g) * scale)
+    out.zero_()
+    which = (torch.arange(tokens) // 40 % 3 - 1).int()
+    got, = add_adapters([y], x, which.to(dev), [down], [up], [torch.ones(2, device=dev)], outs=[out])
+    want, err = expected(y.cpu(), x.cpu(), which, down.cpu(), up.cpu(), torch.ones(2))
+    near(got, want, err, BF)
+
+
 def test_a_call_repeats_itself(dev):
     g = gen(6)
     which = torch.randint(-1, 5, (200,), generator=g)

@@ -139,6 +139,15 @@ def test_rows_at_odd_places(dev):
             check(dev, rows, tokens, 6, on_gpu)
 
 
+def test_rows_beyond_32_bits(dev):
+    """Rows 2^24 elements apart, 300 of them: the last begins 10 GB behind the first."""
+    g = torch.Generator().manual_seed(12)
+    x = (torch.randn(300, 5000, generator=g) * 3).bfloat16()
+    rows = torch.empty(300 << 24, dtype=torch.bfloat16, device=dev).view(300, -1)[:, 3:5003]
+    rows.copy_(x)
+    check(dev, x, torch.randint(0, 5000, (300,), generator=g), 4, rows)
+
+
 def test_the_longest_vocabulary(dev):
     """Parts of as many slices as their threads have room to note, and a vocabulary one short of a part's more."""
     for V, rows in ((1 << 24, 1), (20 * 8192 - 1, 600), (20 * 8192 + 1, 2)):

@@ -1,7 +1,7 @@
 """Rotary positions with the cache write (csrc/qs_rope.hip) against the
 definition in 64 bits, a pair as one complex number.  What is allowed per
-element: half a step of its type for the one rounding (2^-8 / 2 of a bf16 value,
-2^-11 / 2 of an fp16 value, 2^-25 below fp16's normal ones), and of the sizes of
+element: half a step of its type for the one rounding (2^-8 of a bf16 value,
+2^-11 of an fp16 value, 2^-25 below fp16's normal ones), and of the sizes of
 its pair 2^-21 for the sine and cosine (a fraction of a turn in 32 bits, 2 steps
 of the functions, products) and 2^-50 of the angle for the 64-bit product."""
 import itertools
@@ -132,6 +132,26 @@ def test_strides_and_in_place(dev, layout):
 def test_tokens_of_no_row(dev):
     run(dev, [5, 9], [3, 20], tokens=40)
     run(dev, [5, 9], [3, 20], tokens=15, inplace=True)
+
+
+def test_pages_beyond_32_bits(dev):
+    """Pages that lie 9 GB into a pool, and rows of q 2^28 elements apart."""
+    from quipsharp_amd.rope import append_rotated
+    g = gen(9)
+    pages, page, dim = 1_150_000, 16, 128
+    kv = torch.empty(2, pages, 2, page, dim, dtype=BF, device=dev)
+    wide = torch.empty(9 * 2 ** 28, dtype=BF, device=dev)
+    q = torch.as_strided(wide, (9, 4, dim), (2 ** 28, dim, 1))
+    q.copy_(torch.randn(9, 4, dim, generator=g))
+    k, v = torch.randn(2, 9, 2, dim, generator=g).to(BF)
+    table = torch.arange(pages - 9, pages, dtype=I32)[:, None]
+    lengths = torch.arange(1, 10, dtype=I32)
+    w = 1e4 ** (-torch.arange(64, dtype=torch.float64) / 64)
+    got = append_rotated(q, k.to(dev), v.to(dev), kv[0], kv[1], table.to(dev), lengths.to(dev), w.to(dev))
+    pos = lengths.long() - 1
+    near(got.cpu(), *turned(q.cpu(), pos, w, "half", 1.0), BF)
+    near(kv[0, pages - 9:].cpu()[torch.arange(9), :, pos], *turned(k, pos, w, "half", 1.0), BF)
+    assert torch.equal(kv[1, pages - 9:].cpu()[torch.arange(9), :, pos], v)
 
 
 def test_no_page_no_row_no_position(dev):
