@@ -13,8 +13,8 @@
 // they name, prompts by x, y and out.  Measured: 48 tokens of 24 adapters of rank
 // 64, 5120 inputs to two linears of 25600, 10 and 33 us for 177 MB (4.1 TB/s; a
 // large copy reaches 5.06); 10358 tokens of 3 prompts, 25600 inputs to 5120 at rank
-// 64, 95 and 58 us for 747 MB (4.9 TB/s); 4247 of 6, 3584 inputs to 3584 + 512 + 512
-// at rank 24, 15 and 25 us for 114 MB (2.8 TB/s: short loops behind each
+// 64, 95 and 55 us for 747 MB (5.0 TB/s); 4247 of 6, 3584 inputs to 3584 + 512 + 512
+// at rank 24, 15 and 24 us for 114 MB (2.9 TB/s: short loops behind each
 // work-group's start); one token, 4096 inputs to 4096 + 1024 + 1024, 4 and 5 us.
 //
 // Tokens are taken 64 at a time.  In each 64 those of one adapter form a group
@@ -382,15 +382,13 @@ __device__ __forceinline__ void load_y(const char* from, int left, uint4 (&y)[2]
     if (left > 32) y[1] = get_some(from + 64, left - 32);
   }
 }
-template <bool BF>
-__device__ __forceinline__ void store_out(char* to, int left, const uint4 (&y)[2], const f32x4 (&acc)[4], float scale) {
-  const uint4 o0 = add_8<BF>(y[0], acc[0], acc[1], scale), o1 = add_8<BF>(y[1], acc[2], acc[3], scale);
+__device__ __forceinline__ void store_out(char* to, int left, const uint4 (&o)[2]) {
   if (left >= 40) {
-    put_loose(to, o0), put_loose(to + 64, o1);
+    put_loose(to, o[0]), put_loose(to + 64, o[1]);
   } else {
-    if (left >= 8) put_loose(to, o0);
-    else if (left > 0) put_some(to, o0, left);
-    if (left > 32) put_some(to + 64, o1, left - 32);
+    if (left >= 8) put_loose(to, o[0]);
+    else if (left > 0) put_some(to, o[0], left);
+    if (left > 32) put_some(to + 64, o[1], left - 32);
   }
 }
 // The column of row r of the j-th of the four products over 64 columns.
@@ -442,15 +440,18 @@ __device__ __forceinline__ void up_group(const AdapterArgs& a, const Linear& l, 
     for (int k = 0; k < KB; ++k)
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[j] = mma_16x16x32<BF>(wv[j][k], o[k], mma_16x16x32<BF>(wv[j][k], h[k], acc[j]));
-    const uint4 y_now[2] = {y[0], y[1]};
+    const uint4 o8[2] = {add_8<BF>(y[0], acc[0], acc[1], scale), add_8<BF>(y[1], acc[2], acc[3], scale)};
     if (m0 + kColumns < m_end) weights(m0 + kColumns, wv), load_y(y0 + 2 * (m0 + kColumns), left_of(m0 + kColumns), y);
-    if (r < g.size) store_out<BF>(out0 + 2 * m0, left_of(m0), y_now, acc, scale);
+    if (r < g.size) store_out(out0 + 2 * m0, left_of(m0), o8);
   }
 }
 
 // The same for more tokens: a wave has 16 of them, whose inner products stay in
 // its registers as the operand that they are, and the weights of 64 columns at
-// a time lie in LDS for all four, the next ones on their way.  (Through up_group's
+// a time lie in LDS for all four, the next ones on their way.  y is on its way two
+// steps ahead, asked for before the step's results are stored, since a wait for
+// it is one for the stores before it too (one step ahead: 10358 tokens to 5120
+// at rank 64 58 us, so 55; 31144 to 5664 169 and 158).  (Through up_group's
 // way, with the inner products in LDS and the weights in registers, 142 tokens of
 // rank 72 took 23 us in place of 16, long prompts as much as here.)
 template <int KB>
@@ -484,8 +485,9 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, const Linear& l, c
   char* out0 = reinterpret_cast<char*>(l.out + t0 * l.ldo) + 2u * (place * (uint32_t)l.ldo + 8 * q);
   auto left_of = [&](int64_t m0) { return (int)(l.m - m0 < 64 ? l.m - m0 : 64) - 8 * q; };
   const bool mine = c < g.size;
-  uint4 y[2], h[KB], o[KB];
-  if (mine) load_y(y0 + 2 * m_begin, left_of(m_begin), y);
+  uint4 y[2][2], h[KB], o[KB];
+  if (mine) load_y(y0 + 2 * m_begin, left_of(m_begin), y[0]);
+  if (mine && m_begin + 64 < m_end) load_y(y0 + 2 * (m_begin + 64), left_of(m_begin + 64), y[1]);
   float scale;
   {
     const float* from = a.part + (t0 + place) * a.ranks + l.offset;
@@ -527,10 +529,7 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, const Linear& l, c
   keep(0);
   if (m_begin + 64 < m_end) fetch(m_begin + 64);
   __syncthreads();
-  int buffer = 0;
-  for (int64_t m0 = m_begin; m0 < m_end; m0 += 64) {
-    const uint4 y_now[2] = {y[0], y[1]};
-    if (mine && m0 + 64 < m_end) load_y(y0 + 2 * (m0 + 64), left_of(m0 + 64), y);
+  auto step = [&](int64_t m0, int buffer, uint4 (&yb)[2]) {
     if (16 * w < g.size) {
       f32x4 acc[4];
 #pragma unroll
@@ -543,12 +542,19 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, const Linear& l, c
           const uint4 wv = *reinterpret_cast<const uint4*>(at + 16 * j * kRow + 64 * k);
           acc[j] = mma_16x16x32<BF>(wv, o[k], mma_16x16x32<BF>(wv, h[k], acc[j]));
         }
-      if (mine) store_out<BF>(out0 + 2 * m0, left_of(m0), y_now, acc, scale);
+      const uint4 o8[2] = {add_8<BF>(yb[0], acc[0], acc[1], scale), add_8<BF>(yb[1], acc[2], acc[3], scale)};
+      if (mine) {
+        if (m0 + 128 < m_end) load_y(y0 + 2 * (m0 + 128), left_of(m0 + 128), yb);
+        store_out(out0 + 2 * m0, left_of(m0), o8);
+      }
     }
-    buffer ^= 1;
-    if (m0 + 64 < m_end) keep(buffer);  // all are done with it since the last barrier
+    if (m0 + 64 < m_end) keep(buffer ^ 1);  // all are done with it since the last barrier
     if (m0 + 128 < m_end) fetch(m0 + 128);
     __syncthreads();
+  };
+  for (int64_t m0 = m_begin; m0 < m_end; m0 += 128) {
+    step(m0, 0, y[0]);
+    if (m0 + 64 < m_end) step(m0 + 64, 1, y[1]);
   }
 }
 
@@ -578,8 +584,10 @@ __device__ __forceinline__ void copy_group(const Linear& l, const Group& g, int6
   }
 }
 
+// (For ranks up to 96 the compiler would take more than 256 registers by itself,
+// and one wave a SIMD: 31144 tokens of rank 88 313 us, with two 222.)
 template <bool BF, int KB, bool MANY>
-__global__ __launch_bounds__(kThreads) void adapter_up_kernel(AdapterArgs a) {
+__global__ __launch_bounds__(kThreads, MANY && KB == 3 ? 2 : 1) void adapter_up_kernel(AdapterArgs a) {
   constexpr int kFew = 16 * (32 * KB + 8) * 4 + 64, kMany = MANY ? 2 * 64 * tile_row<KB>() : 0;
   __shared__ __align__(16) char room[kMany > kFew ? kMany : kFew];
   int gi = 0;
