@@ -182,6 +182,38 @@ def test_rows_adapters_given_as_a_new_tensor(model, dev):
     assert torch.equal(one.step(ids[2:4]), two.step(ids[2:4]))
 
 
+@pytest.mark.parametrize("window", [0, 24])
+def test_a_captured_step_follows_the_rows_adapters(model, dev, window):
+    """Replays, with other adapters and parents from one to the next and eager work between, give what an eager
+    decoder's steps give."""
+    from quipsharp_amd.decode import PagedDecoder
+    captured, eager = (PagedDecoder(model, 3, 96, page=16, window=window, sinks=4 if window else 0) for _ in range(2))
+    prompts = [ids_of(n, 80 + n, dev) for n in (30, 17, 5)]
+    ids, parents = torch.zeros(3, dtype=torch.long, device=dev), torch.arange(3, dtype=torch.int32, device=dev)
+    for dec in (captured, eager):
+        dec.which.copy_(torch.tensor([0, -1, 1], dtype=torch.int32))
+        dec.prompt(torch.cat(prompts), [len(p) for p in prompts])
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            dec.step(ids, parents)  # loads what the first call loads
+        torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = captured.step(ids, parents)
+    for step, (which, order) in enumerate((([0, -1, 1], [0, 1, 2]), ([1, 1, -1], [2, 1, 0]), ([2, 0, 0], [0, 0, 1]), (None, [0, 1, 2]))):
+        ids.copy_(ids_of(3, 90 + step, dev))
+        parents.copy_(torch.tensor(order, dtype=torch.int32))
+        if which is not None:
+            for dec in (captured, eager):
+                dec.which.copy_(torch.tensor(which, dtype=torch.int32))
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, eager.step(ids, parents))
+        assert torch.equal(captured.which, eager.which)
+
+
 def test_beam_search_with_adapters(model, dev):
     """Beams of one request keep its adapters; one beam is greedy decode."""
     from quipsharp_amd.decode import beam_decode, greedy_decode_paged
