@@ -52,7 +52,7 @@ struct AdapterArgs {
   int64_t ldx, tokens, n;
   const int32_t* which;
   int adapters, count, ranks;  // ranks: of all linears together
-  int tiles, splits, steps;    // steps of 256 inputs of a split
+  int tiles, runs, splits, steps;  // runs: work-groups for all ranks; steps of 256 inputs of a split
   int slots, span;             // work-groups that share a tile's groups, a power of two; columns of one of the second launch
   float* part;                 // [splits][tokens][ranks]
   Linear linear[QS_MAX_GROUP];
@@ -256,16 +256,24 @@ __device__ __forceinline__ void down_tile(const AdapterArgs& a, const Group& g, 
   __syncthreads();  // the next group's stages lie where these did
 }
 
-// blockIdx.x: (run of 16 RB ranks, split), the split fastest.  blockIdx.y: (slot,
-// tile), the tile fastest, so that slots without a group do not fall to the same
-// XCDs (18 tiles in 4 slots: 18.3 us with the slot fastest, 13.9 so).
+// A work-group: (slot, tile, split, run of 16 RB ranks).  Work-groups go to the
+// eight XCDs in turn.  The runs of a tile's split, which read the same x, go to
+// one XCD, one after the other (5768 tokens, 5120 inputs, three runs of 128: 74 us
+// with the runs on XCDs beside each other, 67 so), and the slot is slowest, so that
+// slots without a group do not fall to the same XCDs (18 tiles in 4 slots: 18.3 us
+// with the slot fastest, 13.9 so).  One tile has its work-groups in plain order.
 template <bool BF, int RB, bool MANY>
 __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
   constexpr int kSums = 4 * 64 * sizeof(f32x4), kStages = MANY ? (kAhead<RB> + 1) * stage_bytes<RB>() : 0;
   __shared__ __align__(16) char room[kStages > kSums ? kStages : kSums];
-  const int split = blockIdx.x % a.splits, rank0 = blockIdx.x / a.splits * (16 * RB);
-  const int64_t t0 = (int64_t)(blockIdx.y % a.tiles) * kTile;
-  each_group(a, t0, blockIdx.y / a.tiles, false, [&](const Group& g) {
+  int unit = blockIdx.x / a.runs, run = blockIdx.x % a.runs;
+  if (a.tiles > 1) {
+    unit = (int)(blockIdx.x / 8) / a.runs * 8 + (int)(blockIdx.x % 8), run = (int)(blockIdx.x / 8) % a.runs;
+    if (unit >= a.slots * a.tiles * a.splits) return;
+  }
+  const int split = unit % a.splits, rank0 = run * (16 * RB);
+  const int64_t t0 = (int64_t)(unit / a.splits % a.tiles) * kTile;
+  each_group(a, t0, unit / a.splits / a.tiles, false, [&](const Group& g) {
     if constexpr (MANY) {
       if (g.size > 16) return down_tile<BF, RB>(a, g, t0, split, rank0, room);
     }
@@ -723,7 +731,7 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
     columns += j.m;
   }
   const Plan p = plan_of(tokens, n, adapters, count, ranks);
-  a.tiles = (int)p.tiles, a.splits = p.splits, a.steps = p.steps;
+  a.tiles = (int)p.tiles, a.runs = p.runs, a.splits = p.splits, a.steps = p.steps;
   const size_t need = (size_t)p.splits * tokens * a.ranks * sizeof(float);
   QS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
              "%s: workspace of %zu bytes (16-byte aligned), %zu needed", fn, workspace_bytes, need);
@@ -755,7 +763,8 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
   // their own: 15 us in place of 21 where 6 prompts of 900 have 72 ranks of 3584
   // inputs.  (The second launch has many more, of which half would be empty.)
   a.slots = p.tiles > 1 && p.slots < 2 ? 2 : p.slots;
-  hipLaunchKernelGGL(down, dim3((unsigned)(p.runs * p.splits), (unsigned)(p.tiles * a.slots)), dim3(kThreads), 0, as_stream(stream), a);
+  const int64_t units = p.tiles > 1 ? (p.tiles * a.slots * p.splits + 7) / 8 * 8 : a.slots * p.splits;
+  hipLaunchKernelGGL(down, dim3((unsigned)units * p.runs), dim3(kThreads), 0, as_stream(stream), a);
   QS_LAUNCHED("adapter_down_kernel");
   const auto up = tokens > 16 ? (bf ? up_kernel<true, true>(most) : up_kernel<false, true>(most))
                               : (bf ? up_kernel<true, false>(most) : up_kernel<false, false>(most));
