@@ -12,8 +12,8 @@
 // Both are bound by memory: single tokens by the weights of the adapters that
 // they name, prompts by x, y and out.  Measured: 48 tokens of 24 adapters of rank
 // 64, 5120 inputs to two linears of 25600, 10 and 33 us for 177 MB (4.1 TB/s; a
-// large copy reaches 5.06); 10358 tokens of 3 prompts, 25600 inputs to 5120 at rank
-// 64, 95 and 55 us for 747 MB (5.0 TB/s); 4247 of 6, 3584 inputs to 3584 + 512 + 512
+// large copy reaches 5.06); 10313 tokens of 3 prompts, 25600 inputs to 5120 at rank
+// 64, 95 and 55 us for 747 MB (5.0 TB/s); 4260 of 6, 3584 inputs to 3584 + 512 + 512
 // at rank 24, 15 and 24 us for 114 MB (2.9 TB/s: short loops behind each
 // work-group's start); one token, 4096 inputs to 4096 + 1024 + 1024, 4 and 5 us.
 //
@@ -260,7 +260,7 @@ __device__ __forceinline__ void down_tile(const AdapterArgs& a, const Group& g, 
 // eight XCDs in turn.  The runs of a tile's split, which read the same x, go to
 // one XCD, one after the other (5768 tokens, 5120 inputs, three runs of 128: 74 us
 // with the runs on XCDs beside each other, 67 so), and the slot is slowest, so that
-// slots without a group do not fall to the same XCDs (18 tiles in 4 slots: 18.3 us
+// slots without a group do not fall to the same XCDs (14 tiles in 4 slots: 18.3 us
 // with the slot fastest, 13.9 so).  One tile has its work-groups in plain order.
 template <bool BF, int RB, bool MANY>
 __global__ __launch_bounds__(kThreads) void adapter_down_kernel(AdapterArgs a) {
@@ -458,8 +458,8 @@ __device__ __forceinline__ void up_group(const AdapterArgs& a, const Linear& l, 
 // its registers as the operand that they are, and the weights of 64 columns at
 // a time lie in LDS for all four, the next ones on their way.  y is on its way two
 // steps ahead, asked for before the step's results are stored, since a wait for
-// it is one for the stores before it too (one step ahead: 10358 tokens to 5120
-// at rank 64 58 us, so 55; 31144 to 5664 169 and 158).  (Through up_group's
+// it is one for the stores before it too (one step ahead: 10313 tokens to 5120
+// at rank 64 58 us, so 55; 24287 to 5664 169 and 158).  (Through up_group's
 // way, with the inner products in LDS and the weights in registers, 142 tokens of
 // rank 72 took 23 us in place of 16, long prompts as much as here.)
 template <int KB>
@@ -593,7 +593,7 @@ __device__ __forceinline__ void copy_group(const Linear& l, const Group& g, int6
 }
 
 // (For ranks up to 96 the compiler would take more than 256 registers by itself,
-// and one wave a SIMD: 31144 tokens of rank 88 313 us, with two 222.)
+// and one wave a SIMD: 20719 tokens of rank 88 313 us, with two 222.)
 template <bool BF, int KB, bool MANY>
 __global__ __launch_bounds__(kThreads, MANY && KB == 3 ? 2 : 1) void adapter_up_kernel(AdapterArgs a) {
   constexpr int kFew = 16 * (32 * KB + 8) * 4 + 64, kMany = MANY ? 2 * 64 * tile_row<KB>() : 0;
@@ -645,8 +645,8 @@ Plan plan_of(int64_t tokens, int64_t n, int64_t adapters, int count, const int* 
   // Few tokens need many narrow work-groups, many tokens wide ones that read x
   // once: one token's 48 ranks of 4096 inputs in blocks of 16 take 4.2 us, in one of
   // 64 5.1; 48 tokens with 24 adapters of 128 ranks in blocks of 32 11.9, of 64 9.8;
-  // 300 tokens with 128 ranks in blocks of 32 6.6, of 64 7.6, of 128 10.4; 1136 with
-  // 240 ranks 16.2, 13.8 and 16.3; 8296 with 160 ranks of 24296 inputs in blocks of
+  // 229 tokens with 128 ranks in blocks of 32 6.6, of 64 7.6, of 128 10.4; 848 with
+  // 240 ranks 16.2, 13.8 and 16.3; 5641 with 160 ranks of 24296 inputs in blocks of
   // 64 254, of 96 194.
   auto widest = [&](int width) { p.runs = (blocks + width - 1) / width, p.blocks = (blocks + p.runs - 1) / p.runs; };
   if (p.tiles == 1) {
@@ -657,8 +657,8 @@ Plan plan_of(int64_t tokens, int64_t n, int64_t adapters, int count, const int* 
     widest(p.tiles < 16 ? 2 : p.tiles < 64 ? 4 : 8);
   }
   if (p.blocks > 1 || tokens > 16) p.blocks += p.blocks & 1;
-  // Splits fill the GPU, but each is read again by the second launch: 6 prompts
-  // of 900 with 4 splits of 3584 inputs (340 work-groups) take 15 + 25 us, with 8 18
+  // Splits fill the GPU, but each is read again by the second launch: 4260 tokens
+  // of 6 prompts with 4 splits of 3584 inputs (268 work-groups) take 15 + 25 us, with 8 18
   // + 29, with 2 18 + 23.  Groups of single tokens have shorter loops and want four
   // times as many.
   int64_t splits = 1;
@@ -741,9 +741,9 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
   // work-groups of them fill the GPU (48 tokens to 2 x 25600: 33 us with 1024 columns,
   // 48 with 256).  Prompts take 64 at a time and are cut finer where there are few
   // (142 tokens to 1315 columns: 8.5 us with 64, 12 with 256) and coarser where there
-  // are many (10358 to 5120: 58 us with 512, 62 with 256, 80 with 128; but 8296 to
+  // are many (10313 to 5120: 58 us with 512, 62 with 256, 80 with 128; but 5641 to
   // 12659 151 us with 1024, 128 with 512); work-groups of slots without a group cost
-  // their launch (232 tokens in 16 slots to 20507 columns: 20 us with 64, 9 with 256).
+  // their launch (74 tokens in 32 slots to 20507 columns: 20 us with 64, 9 with 256).
   if (p.tiles == 1) {
     const int64_t groups = p.slots < 8 ? 1 : p.slots / 2;
     a.span = kColumns;
@@ -760,8 +760,8 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
   const bool bf = dtype == QS_DTYPE_BF16;
   const auto down = bf ? down_kernel<true>(p.blocks, tokens > 16) : down_kernel<false>(p.blocks, tokens > 16);
   // at a boundary of two prompts the second one's tokens go to work-groups of
-  // their own: 15 us in place of 21 where 6 prompts of 900 have 72 ranks of 3584
-  // inputs.  (The second launch has many more, of which half would be empty.)
+  // their own: 15 us in place of 21 where 4260 tokens of 6 prompts have 72 ranks of
+  // 3584 inputs.  (The second launch has many more, of which half would be empty.)
   a.slots = p.tiles > 1 && p.slots < 2 ? 2 : p.slots;
   const int64_t units = p.tiles > 1 ? (p.tiles * a.slots * p.splits + 7) / 8 * 8 : a.slots * p.splits;
   hipLaunchKernelGGL(down, dim3((unsigned)units * p.runs), dim3(kThreads), 0, as_stream(stream), a);
