@@ -11,7 +11,7 @@
 //
 // Both are bound by memory: single tokens by the weights of the adapters that
 // they name, prompts by x, y and out.  Measured: 48 tokens of 24 adapters of rank
-// 64, 5120 inputs to two linears of 25600, 10 and 33 us for 177 MB (4.1 TB/s; a
+// 64, 5120 inputs to two linears of 25600, 10 and 32 us for 175 MB (4.2 TB/s; a
 // large copy reaches 5.06); 10313 tokens of 3 prompts, 25600 inputs to 5120 at rank
 // 64, 95 and 55 us for 747 MB (5.0 TB/s); 4260 of 6, 3584 inputs to 3584 + 512 + 512
 // at rank 24, 15 and 24 us for 114 MB (2.9 TB/s: short loops behind each
@@ -338,11 +338,15 @@ __device__ __forceinline__ void two_parts(float f0, float f1, uint32_t& hi, uint
 
 // The inner products of up to 16 tokens of a group, summed over the splits, as two
 // 16-bit numbers: four ranks a thread, a token's R / 4 threads in one wave.
+// Splits on their way together: 9 tokens of rank 112 take 10.8 us with a loop
+// that the compiler unrolls by four, 7.0 with eight at a time; 48 tokens of rank 64
+// to 2 x 25600 34 and 32, with sixteen 37.  Ranks up to 32 keep the loop: few
+// splits of prompts 24 us with it, 29 without.
 template <bool BF, int R, int kRow>
 __device__ __forceinline__ void inner_products(const AdapterArgs& a, const Linear& l, const Group& g, int64_t t0, uint4* high,
                                                uint4* low, float* factor) {
   constexpr int T = R == 96 ? 32 : R / 4;  // a power of two
-  constexpr int U = T == 32 ? 2 : 1;       // tokens of a thread
+  constexpr int U = T == 32 ? 2 : 1, P = 8 / U;  // tokens of a thread, splits at a time
   const int tid = threadIdx.x;
   if (16 * T < kThreads && tid >= 16 * T) return;  // whole waves: 16 T is a multiple of 64
   const float* base = a.part + t0 * a.ranks + l.offset;
@@ -356,10 +360,23 @@ __device__ __forceinline__ void inner_products(const AdapterArgs& a, const Linea
     from[i] = (uint32_t)place_in_tile(g, i * (kThreads / T) + tid / T) * (uint32_t)a.ranks + (rank < l.rank ? rank : 0);
     s[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
+  if constexpr (R == 32) {
 #pragma unroll 4
-  for (int p = 0; p < a.splits; ++p)
+    for (int p = 0; p < a.splits; ++p) s[0] += *reinterpret_cast<const f32x4*>(base + p * next + from[0]);
+  } else {
+    for (int p0 = 0; p0 < a.splits; p0 += P) {
+      f32x4 v[P][U];  // on their way together
 #pragma unroll
-    for (int i = 0; i < U; ++i) s[i] += *reinterpret_cast<const f32x4*>(base + p * next + from[i]);
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+          v[p][i] = p0 + p < a.splits ? *reinterpret_cast<const f32x4*>(base + (p0 + p) * next + from[i]) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int i = 0; i < U; ++i) s[i] += v[p][i];
+    }
+  }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
     const int c = i * (kThreads / T) + tid / T;
