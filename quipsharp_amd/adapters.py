@@ -13,6 +13,7 @@ from . import _lib
 from .pages import _HALF, _int32, _room, _workspace
 
 MAX_RANK = 128
+MAX_TOKENS = 1 << 19
 NAMES = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
 
 
@@ -156,6 +157,36 @@ def beside(x: Tensor, linears, ys, which: Tensor):
         add_adapters(own, x, which, [a.down for _, a in with_some], [a.up for _, a in with_some],
                      [a.scale for _, a in with_some], outs=own)
     return ys
+
+
+def check_beside(linears, which: Tensor, rows: int, tokens: int, dtype, device):
+    """Raises where ``beside`` would refuse the adapters of ``linears``, which read the same rows of this type, for
+    ``tokens`` tokens of ``rows`` rows whose adapters ``which`` names: for callers that must know before they run."""
+    banks = [(lin, lin.adapters) for lin in linears if getattr(lin, "adapters", None) is not None]
+    if not banks:
+        return
+    _int32("which", which, (rows,), device)
+    if tokens > MAX_TOKENS:
+        raise ValueError(f"{tokens} tokens at a time with adapters (at most {MAX_TOKENS})")
+    count, place = banks[0][1].scale.shape[0], which.get_device()
+    for g, (lin, bank) in enumerate(banks):
+        down, up, scale, n, m = bank.down, bank.up, bank.scale, lin.in_features, lin.out_features
+        shape = down.shape
+        rank = shape[1] if len(shape) == 3 else 0
+        # banks as they are made; what else there may be is looked into behind
+        if shape == (count, rank, n) and up.shape == (count, m, rank) and scale.shape == (count,) and down.is_contiguous() \
+                and up.is_contiguous() and scale.is_contiguous() and down.dtype is dtype and up.dtype is dtype \
+                and scale.dtype is torch.float32 and down.get_device() == up.get_device() == scale.get_device() == place \
+                and count and 8 <= rank <= MAX_RANK and not (rank | n) % 8 and not (down.data_ptr() | up.data_ptr()) & 15:
+            continue
+        y = torch.empty(0, m, dtype=dtype, device=device)
+        _refuse(g, y, y, down, up, scale, 0, n, count, dtype, device)
+        ds, us = down.stride(), up.stride()
+        apart = ds[1] | (us[1] if m > 1 else 0) | (ds[0] | us[0] if count > 1 else 0)
+        if not (count and 8 <= rank <= MAX_RANK and not (rank | n | apart) % 8 and ds[1] >= n and (us[1] >= rank or m == 1)
+                and not (down.data_ptr() | up.data_ptr()) & 15):
+            raise ValueError(f"adapters {g}: {tuple(shape)} and {tuple(up.shape)}: the rank must be a multiple of 8 up to "
+                             f"{MAX_RANK}, rows 16-byte aligned and apart")
 
 
 def attach_adapters(model, count, rank, names=NAMES, dtype=torch.bfloat16):

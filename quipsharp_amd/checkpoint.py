@@ -59,6 +59,8 @@ class QuantizedLinear(nn.Module):
     around the library's decode-matvec).
     """
 
+    adapters = None  # adapters.Adapters beside it, for a decode.PagedDecoder's rows
+
     def __init__(self, in_features: int, out_features: int, g: int, transform_kind: str, num_stages: int = 1,
                  has_bias: bool = False):
         super().__init__()

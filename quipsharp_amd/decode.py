@@ -347,6 +347,20 @@ class PagedDecoder(StaticDecoder):
         return any(getattr(mod, "adapters", None) is not None for L in self.layers for mod in
                    [*L.self_attn.children(), *L.mlp.children()])
 
+    def _check_beside(self, tokens):
+        """Refuses what the layers would refuse of ``which`` and the adapters: before the cache grows, since it keeps what
+        it was given room for."""
+        from .adapters import check_beside
+        dtype = self.model.model.embed_tokens.weight.dtype
+        for L in self.layers:
+            a, mlp = L.self_attn._modules, L.mlp._modules
+            for linears in ((a["q_proj"], a["k_proj"], a["v_proj"]), (a["o_proj"],), (mlp["gate_proj"], mlp["up_proj"]),
+                            (mlp["down_proj"],)):
+                for linear in linears:
+                    if getattr(linear, "adapters", None) is not None:
+                        check_beside(linears, self.which, self.B, tokens, dtype, self.dev)
+                        break
+
     def _beside(self, x, linears, outs):
         """The outputs of ``linears`` for x, with the adapters of the tokens' rows."""
         if all(getattr(l, "adapters", None) is None for l in linears):
@@ -374,6 +388,7 @@ class PagedDecoder(StaticDecoder):
         count = torch.tensor(counts, dtype=torch.int32)
         starts = torch.cat([torch.zeros(1, dtype=torch.int32), count.cumsum(0, dtype=torch.int32)]).to(self.dev)
         row = torch.repeat_interleave(torch.arange(self.B), count).to(self.dev)
+        self._check_beside(T)
         cache.advance(count.to(self.dev))
         cache.check()
         h = m.embed_tokens(ids)[None]
@@ -441,6 +456,11 @@ class PagedDecoder(StaticDecoder):
         """One new token for every row, ids (rows,) or (rows, 1): row i goes on
         from row ``parents[i]`` (int32; None: its own), with that row's
         adapters.  Logits (rows, vocab)."""
+        if ids.numel() != self.B:
+            raise ValueError(f"ids {tuple(ids.shape)} for {self.B} rows")
+        if self.model.model.embed_tokens.weight.dtype != torch.bfloat16:
+            raise TypeError("the decode step runs bf16 models")
+        self._check_beside(self.B)
         self.cache.advance(1, parents)
         if parents is not None and self._adapted():
             named = (parents >= 0) & (parents < self.B)

@@ -1,0 +1,93 @@
+"""What the paged decoder refuses, on the host: of its rows' adapters before the
+cache has room for tokens that no layer will write, and of models."""
+import pytest
+import torch
+
+from quipsharp_amd.adapters import attach_adapters
+from quipsharp_amd.checkpoint import QuantizedLinear
+from quipsharp_amd.decode import PagedDecoder
+
+BF, HF, I32 = torch.bfloat16, torch.float16, torch.int32
+SIZES = dict(hidden_size=256, intermediate_size=512, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+             vocab_size=100, max_position_embeddings=128)
+
+
+def llama(dtype=BF, kind="llama", **more):
+    from transformers import AutoModelForCausalLM, LlamaConfig, Qwen2Config, Qwen3Config
+    config = {"llama": LlamaConfig, "qwen2": Qwen2Config, "qwen3": Qwen3Config}[kind](**dict(SIZES, **more))
+    model = AutoModelForCausalLM.from_config(config, dtype=dtype)
+    for layer in model.model.layers:
+        for part in (layer.self_attn, layer.mlp):
+            for name, lin in list(part.named_children()):
+                if isinstance(lin, torch.nn.Linear):
+                    setattr(part, name, QuantizedLinear(lin.in_features, lin.out_features, 8, "rht"))
+    return model
+
+
+@pytest.fixture
+def decoder(monkeypatch):
+    """A decoder of two rows on the CPU whose cache notes that it was advanced."""
+    model = llama()
+    attach_adapters(model, 3, 8)
+    dec = PagedDecoder(model, 2, 64, 16)
+    dec.advanced = []
+    monkeypatch.setattr(dec.cache, "advance", lambda *a: dec.advanced.append(a))
+    return dec
+
+
+def last_bank(dec):
+    return dec.layers[-1].mlp.down_proj.adapters
+
+
+def strided(dec):
+    bank = last_bank(dec)
+    bank.down = torch.zeros(3, 8, 2 * bank.down.shape[2], dtype=BF)[:, :, ::2]
+
+
+SPOILED = [
+    (lambda d: setattr(d, "which", d.which.long()), ValueError, "which must be"),
+    (lambda d: setattr(d, "which", torch.zeros(3, dtype=I32)), ValueError, "which must be"),
+    (lambda d: setattr(d, "which", torch.zeros(2, dtype=I32, device="meta")), ValueError, "which is on"),
+    (lambda d: setattr(last_bank(d), "up", last_bank(d).up.half()), TypeError, "adapters 0 are"),
+    (lambda d: setattr(last_bank(d), "down", last_bank(d).down[:, :, :128]), ValueError, "512 inputs"),
+    (lambda d: setattr(last_bank(d), "scale", last_bank(d).scale[:2]), ValueError, "adapters"),
+    (lambda d: setattr(last_bank(d), "scale", last_bank(d).scale.double()), ValueError, r"scales\[0\] must be"),
+    (strided, ValueError, "stride 1"),
+    (lambda d: attach_adapters(d.model, 5, 8, names=("v_proj",)), ValueError, "5 adapters beside 3"),
+    (lambda d: attach_adapters(d.model, 3, 8, names=("gate_proj",), dtype=HF), TypeError, "adapters 0 are"),
+]
+
+
+@pytest.mark.parametrize("spoil,error,message", SPOILED)
+def test_adapters_are_refused_before_the_cache_grows(decoder, spoil, error, message):
+    spoil(decoder)
+    ids = torch.arange(4)
+    for call in (lambda: decoder.prompt(ids, [3, 1]), lambda: decoder.score(ids, [3, 1]), lambda: decoder.step(ids[:2])):
+        with pytest.raises(error, match=message):
+            call()
+    assert not decoder.advanced
+
+
+def test_ranks_and_alignment_are_refused_before_the_cache_grows(decoder):
+    bank = last_bank(decoder)
+    down, up = bank.down, bank.up
+    n = down.shape[2]
+    for bank.down, bank.up in ((down[:, :4].contiguous(), up[:, :, :4].contiguous()),
+                               (torch.zeros(3 * 8 * n + 4, dtype=BF)[4:].view(3, 8, n), up),
+                               (down[:, :1].expand(3, 8, n), up)):
+        with pytest.raises(ValueError, match="multiple of 8"):
+            decoder.step(torch.arange(2))
+    bank.down, bank.up = torch.zeros(3, 8, n + 8, dtype=BF)[:, :, :n], up  # rows of a wider tensor are fine
+    decoder._check_beside(2)
+    with pytest.raises(ValueError, match="524289 tokens"):
+        decoder._check_beside((1 << 19) + 1)
+    assert not decoder.advanced
+
+
+def test_other_ids_are_refused_before_the_cache_grows(decoder):
+    with pytest.raises(ValueError, match="for 2 rows"):
+        decoder.step(torch.arange(3))
+    decoder.model.half()
+    with pytest.raises(TypeError, match="bf16 models"):
+        decoder.step(torch.arange(2))
+    assert not decoder.advanced
