@@ -127,8 +127,9 @@ class StaticDecoder:
     does the residual add and the RMSNorm before it
     (checkpoint.grouped_forward_pre; at more rows the norm runs on its own
     launch first).  The prompt
-    (several tokens per row) runs transformers' modules with the same bf16
-    cache (attention in fp32)."""
+    (several tokens per row), and every step of a model whose activation is
+    not SiLU, runs transformers' modules with the same bf16 cache (attention
+    in fp32)."""
 
     def __init__(self, model, batch, max_len, cache=True):
         from . import _lib
@@ -158,8 +159,9 @@ class StaticDecoder:
         if cache:
             nbytes = L.qs_dec_attention_workspace_bytes(batch, self.nkv, max_len)
             self.attn_ws = torch.empty(max(int(nbytes), 256), dtype=torch.uint8, device=dev)
+        self.silu = getattr(cfg, "hidden_act", "silu") in ("silu", "swish")  # what the decode step computes
         self.fused_ok = self.hd == 128 and self.nh % self.nkv == 0 and self.nh // self.nkv <= 16 \
-            and self.hidden % 8 == 0
+            and self.hidden % 8 == 0 and self.silu
 
     def _weight(self, mod):
         w = mod.weight
@@ -309,7 +311,7 @@ class PagedDecoder(StaticDecoder):
     Layers with q/k norms (Qwen3) have heads of 128; of those without (Llama,
     Qwen2: model types ``llama`` and ``qwen2``) heads of 64, 128 or 256 turn by
     ``rope.append_rotated`` with the config's frequencies, stretched contexts
-    included.  Where linears have adapters (``adapters.attach_adapters``),
+    included.  Activations are SiLU.  Where linears have adapters (``adapters.attach_adapters``),
     ``which`` (int32 on the GPU, one for every row, -1 for none) says which of
     them a row takes; a captured step follows it, and rows that fork keep it.
 
@@ -321,6 +323,8 @@ class PagedDecoder(StaticDecoder):
         from .pages import PagedCache
         columns = -(-max_len // page)
         super().__init__(model, rows, columns * page, cache=False)  # rotary tables to the last page's end
+        if not self.silu:
+            raise ValueError(f"the paged decode step computes SiLU(gate) * up, the model has {model.config.hidden_act!r}")
         self.normed = all(hasattr(L.self_attn, "q_norm") for L in self.layers)
         if self.normed:
             if not self.fused_ok:

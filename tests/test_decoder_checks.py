@@ -91,3 +91,29 @@ def test_other_ids_are_refused_before_the_cache_grows(decoder):
     with pytest.raises(TypeError, match="bf16 models"):
         decoder.step(torch.arange(2))
     assert not decoder.advanced
+
+
+# ---------------------------------------------------------------------------
+# models
+# ---------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kind", ["llama", "qwen2", "qwen3"])
+def test_other_activations_are_refused(kind):
+    """The step's kernel computes SiLU, the prompt the model's own activation: one that differs would be right in the
+    prompt and wrong in every step."""
+    heads = dict(head_dim=128) if kind == "qwen3" else {}
+    with pytest.raises(ValueError, match="the model has 'relu'"):
+        PagedDecoder(llama(kind=kind, hidden_act="relu", **heads), 2, 64, 16)
+    for act in ("silu", "swish"):
+        assert PagedDecoder(llama(kind=kind, hidden_act=act, **heads), 2, 64, 16).fused_ok == (kind == "qwen3")
+
+
+def test_static_steps_of_other_activations_run_the_models_own():
+    from quipsharp_amd.decode import StaticDecoder
+    for act, fused in (("silu", True), ("relu", False)):
+        dec = StaticDecoder(llama(kind="qwen3", head_dim=128, hidden_act=act), 1, 32)
+        took = []
+        dec._decode_step = lambda *a: took.append("kernels")
+        dec._prompt_step = lambda *a: took.append("modules")
+        dec.step(torch.zeros(1, 1, dtype=torch.long), torch.zeros(1, dtype=torch.long))
+        assert took == ["kernels" if fused else "modules"]
