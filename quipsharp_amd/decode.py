@@ -340,6 +340,9 @@ class PagedDecoder(StaticDecoder):
                 raise ValueError(f"the paged decode step takes heads of 64, 128 or 256, at most 16 of them per kv head, got "
                                  f"{self.nh} and {self.nkv} of {self.hd}")
             self.frequencies, self.turn_factor = model_frequencies(cfg, self.dev)
+            if 2 * len(self.frequencies) != self.hd:  # their own modules turn whole heads, or fail
+                raise ValueError(f"the paged decoder turns whole heads of {cfg.model_type} models, the config has "
+                                 f"{2 * len(self.frequencies)} elements of {self.hd} turned")
         self.window, self.sinks = window, sinks
         self.cache = PagedCache(len(self.layers), rows * columns if pages is None else pages, self.nkv, self.hd, rows,
                                 columns, page, torch.bfloat16, self.dev)

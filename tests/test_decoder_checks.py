@@ -117,3 +117,13 @@ def test_static_steps_of_other_activations_run_the_models_own():
         dec._prompt_step = lambda *a: took.append("modules")
         dec.step(torch.zeros(1, 1, dtype=torch.long), torch.zeros(1, dtype=torch.long))
         assert took == ["kernels" if fused else "modules"]
+
+
+@pytest.mark.parametrize("kind", ["llama", "qwen2"])
+def test_heads_that_turn_in_part_are_refused(kind):
+    """transformers' modules of these models turn whole heads whatever partial_rotary_factor says (the default
+    frequencies) or fail (scaled ones)."""
+    whole = dict(rope_type="default", rope_theta=1e4)
+    assert len(PagedDecoder(llama(kind=kind, rope_parameters=whole), 2, 64, 16).frequencies) == 32
+    with pytest.raises(ValueError, match="32 elements of 64"):
+        PagedDecoder(llama(kind=kind, rope_parameters=dict(whole, partial_rotary_factor=0.5)), 2, 64, 16)
