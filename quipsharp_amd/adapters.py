@@ -192,7 +192,9 @@ def check_beside(linears, which: Tensor, rows: int, tokens: int, dtype, device):
 def attach_adapters(model, count, rank, names=NAMES, dtype=torch.bfloat16):
     """Gives every ``QuantizedLinear`` of ``model`` whose last name is among
     ``names`` (of ``NAMES``) room for ``count`` adapters of rank ``rank``, empty
-    at first, in its attribute ``adapters``.  Returns them by the linears' names."""
+    at first, in its attribute ``adapters``.  ``decode.PagedDecoder`` and what is built on it run them; the model's own
+    forward, and with it ``decode.greedy_decode`` and ``decode.perplexity``, stays the base model's.  Returns them by the
+    linears' names."""
     from .checkpoint import QuantizedLinear
     if not set(names) <= set(NAMES):
         raise ValueError(f"no decoder takes adapters beside {sorted(set(names) - set(NAMES))} (only {', '.join(NAMES)})")

@@ -92,7 +92,8 @@ def random_quantized_model(config, device="cuda", seed=0):
 @torch.no_grad()
 def greedy_decode(model, prompt_ids, new_tokens):
     """Prefill ``prompt_ids`` (B, P), then ``new_tokens`` greedy steps with a
-    KV cache.  Returns (tokens (B, new_tokens), prefill s, decode s)."""
+    KV cache, by the model's own forward (no adapters run there).  Returns
+    (tokens (B, new_tokens), prefill s, decode s)."""
     from transformers import DynamicCache
     cache = DynamicCache()
     torch.cuda.synchronize()
@@ -146,6 +147,9 @@ class StaticDecoder:
         self.dev = dev
         bf = torch.bfloat16
         if cache:
+            if not all(hasattr(L.self_attn, "q_norm") for L in self.layers):
+                raise ValueError(f"the static decoder takes layers with q/k norms (Qwen3), not {cfg.model_type}: PagedDecoder "
+                                 f"takes Llama and Qwen2 too")
             self.k = [torch.zeros(batch, self.nkv, max_len, self.hd, device=dev, dtype=bf) for _ in self.layers]
             self.v = [torch.zeros(batch, self.nkv, max_len, self.hd, device=dev, dtype=bf) for _ in self.layers]
         self.kpos = torch.arange(max_len, device=dev)
@@ -169,9 +173,15 @@ class StaticDecoder:
             raise TypeError("the decode step takes bf16 norm weights")
         return w
 
+    def _adapted(self):
+        return any(getattr(mod, "adapters", None) is not None for L in self.layers for part in (L.self_attn, L.mlp)
+                   for mod in part._modules.values())
+
     @torch.no_grad()
     def step(self, ids, pos):
         """Logits of the last position; ids (B, q), pos (q,) int64 positions."""
+        if self._adapted():
+            raise ValueError("the static decoder runs no adapters (PagedDecoder does): the model's linears have some")
         if ids.shape[1] == 1 and self.fused_ok:
             return self._decode_step(ids, pos)
         return self._prompt_step(ids, pos)
@@ -349,10 +359,6 @@ class PagedDecoder(StaticDecoder):
         self.spans = {"window": window, "sinks": sinks}
         self.which = torch.full((rows,), -1, dtype=torch.int32, device=self.dev)
         self._prompt_which = None  # of a prompt's tokens, while it runs
-
-    def _adapted(self):
-        return any(getattr(mod, "adapters", None) is not None for L in self.layers for mod in
-                   [*L.self_attn.children(), *L.mlp.children()])
 
     def _check_beside(self, tokens):
         """Refuses what the layers would refuse of ``which`` and the adapters: before the cache grows, since it keeps what
@@ -546,7 +552,8 @@ def greedy_decode_paged(model, prompts, new_tokens, which=None, top=0, use_graph
 @torch.no_grad()
 def perplexity(model, ids, window=2048):
     """The perplexity of a text's ids (n,) under any causal LM, over windows of ``window`` tokens that do not overlap,
-    each token given those before it in its window (as scripts/eval_ppl.py:41-65 takes it)."""
+    each token given those before it in its window (as scripts/eval_ppl.py:41-65 takes it).  By the model's own forward,
+    which runs no adapters: a fine-tune's tokens are scored by ``PagedDecoder.score``."""
     from .logprobs import token_logprobs
     total, count = 0.0, 0
     for part in ids.split(window):

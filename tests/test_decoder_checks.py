@@ -127,3 +127,21 @@ def test_heads_that_turn_in_part_are_refused(kind):
     assert len(PagedDecoder(llama(kind=kind, rope_parameters=whole), 2, 64, 16).frequencies) == 32
     with pytest.raises(ValueError, match="32 elements of 64"):
         PagedDecoder(llama(kind=kind, rope_parameters=dict(whole, partial_rotary_factor=0.5)), 2, 64, 16)
+
+
+def test_the_static_decoder_refuses_what_it_does_not_run():
+    """Layers without q/k norms, and adapters, which it would leave out, attached before or after it is made."""
+    from quipsharp_amd.decode import StaticDecoder
+    with pytest.raises(ValueError, match="not llama"):
+        StaticDecoder(llama(), 1, 32)
+    model = llama(kind="qwen3", head_dim=128)
+    dec, ids, pos = StaticDecoder(model, 1, 32), torch.zeros(1, 3, dtype=torch.long), torch.arange(3)
+    dec._decode_step = dec._prompt_step = lambda *a: "ran"
+    assert dec.step(ids, pos) == dec.step(ids[:, :1], pos[:1]) == "ran"
+    banks = attach_adapters(model, 2, 8, names=("down_proj",))
+    for n in (3, 1):
+        with pytest.raises(ValueError, match="runs no adapters"):
+            dec.step(ids[:, :n], pos[:n])
+    for layer in model.model.layers:
+        layer.mlp.down_proj.adapters = None
+    assert len(banks) == 2 and dec.step(ids, pos) == "ran"
