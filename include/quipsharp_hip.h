@@ -621,7 +621,8 @@ typedef struct qs_adapter_job {
  * n a multiple of 8).  Tokens whose which is not in 0 .. adapters - 1 have
  * out = y.  fp32 sums, one rounding.  No out may be x, another linear's y or its
  * out.  workspace: qs_adapters_workspace_bytes, for this call alone while it
- * runs.  At most 2^19 tokens; rows of x, y, out and weights at most 2^24 elements
+ * runs; a workspace of that size serves fewer tokens and any number of adapters
+ * too.  At most 2^19 tokens; rows of x, y, out and weights at most 2^24 elements
  * apart. */
 size_t qs_adapters_workspace_bytes(int64_t tokens, int64_t n, int64_t adapters, int count, const int *ranks);
 int qs_adapters_add(const void *x, int dtype, int64_t ldx, int64_t tokens, int64_t n, const int32_t *which,
@@ -639,8 +640,12 @@ int qs_adapters_add(const void *x, int dtype, int64_t ldx, int64_t tokens, int64
  *             ties to the lower token; -inf and -1 where there are none left
  * A NaN logit counts as -inf, and a token at -inf is no alternative.  A row
  * whose largest logit is not finite has log probabilities -inf, entropy 0 and
- * no alternatives.  top <= 64, vocab <= 2^24. */
+ * no alternatives.  top <= 64, vocab <= 2^24.  workspace:
+ * qs_token_logprobs_workspace_bytes, which falls as rows grow, to 0 from 1024
+ * rows on (up to 163833 tokens); one that serves any number of rows up to `rows`
+ * has qs_token_logprobs_workspace_most. */
 size_t qs_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab, int dtype, int top);
+size_t qs_token_logprobs_workspace_most(int64_t rows, int64_t vocab, int dtype, int top);
 int qs_token_logprobs(const void *logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const void *tokens,
                       int token_bytes, int top, float *logprobs, float *entropy, int32_t *ranks, float *top_logprobs,
                       int32_t *top_tokens, void *workspace, size_t workspace_bytes, qs_stream_t stream);

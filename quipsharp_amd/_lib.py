@@ -154,6 +154,7 @@ _SIGNATURES = {
     "qs_adapters_add": ([_vp, _int, _i64, _i64, _i64, _vp, _i64, _int, ctypes.POINTER(AdapterJob), _vp,
                          ctypes.c_size_t, _vp], _int),
     "qs_token_logprobs_workspace_bytes": ([_i64, _i64, _int, _int], ctypes.c_size_t),
+    "qs_token_logprobs_workspace_most": ([_i64, _i64, _int, _int], ctypes.c_size_t),
     "qs_token_logprobs": ([_vp, _int, _i64, _i64, _i64, _vp, _int, _int, _vp, _vp, _vp, _vp, _vp, _vp,
                            ctypes.c_size_t, _vp], _int),
 }

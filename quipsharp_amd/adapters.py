@@ -30,6 +30,12 @@ def _rows(name, t, tokens, width, dtype, device):
     return t.stride(0) if tokens > 1 else t.shape[1]
 
 
+def workspace_bytes(tokens, n, ranks) -> int:
+    """Bytes of workspace that serve ``add_adapters`` of up to ``tokens`` rows of n elements beside linears of these
+    ranks."""
+    return int(_lib.lib().qs_adapters_workspace_bytes(tokens, n, 1, len(ranks), _lib.int_array(ranks)))
+
+
 def add_adapters(ys, x: Tensor, which: Tensor, downs, ups, scales, *, outs=None, workspace: Tensor = None):
     """``ys[g][t] + scales[g][a] * ups[g][a] @ (downs[g][a] @ x[t])`` with ``a =
     which[t]``, for up to four linears g that read the same x.
@@ -41,7 +47,8 @@ def add_adapters(ys, x: Tensor, which: Tensor, downs, ups, scales, *, outs=None,
     (adapters,) float32; ys[g]: (tokens, m) in x's type.  Returns new tensors,
     or ``outs``, each of which is the y at its place itself or apart from all
     the call reads.  Sums are float32, rounded once at the end; the inner
-    products go on with 16 significant bits or more."""
+    products go on with 16 significant bits or more.  ``workspace``: uint8, of
+    ``workspace_bytes`` for the most tokens of any call that has it."""
     count = len(ys)
     if not 1 <= count <= _lib.QS_MAX_GROUP or not len(downs) == len(ups) == len(scales) == count:
         raise ValueError(f"{count} outputs for {len(downs)} / {len(ups)} / {len(scales)} adapters (1 to {_lib.QS_MAX_GROUP} linears)")

@@ -35,6 +35,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kTile = 64;     // tokens at a time
 constexpr int kMaxRank = 128;
+constexpr int64_t kMaxTokens = 1 << 19;
 constexpr int kColumns = 256;  // output columns of a work-group of single tokens at a time, 64 a wave
 
 struct Linear {
@@ -700,7 +701,19 @@ extern "C" size_t qs_adapters_workspace_bytes(int64_t tokens, int64_t n, int64_t
     if (ranks[g] < 1 || ranks[g] > kMaxRank) return 0;
     all += ranks[g];
   }
-  return (size_t)plan_of(tokens, n, adapters, count, ranks).splits * tokens * all * sizeof(float);
+  if (tokens > kMaxTokens) return 0;
+  // What any number of tokens up to this takes, of any number of adapters: fewer
+  // tokens may be cut into more splits.  One tile has up to 16, several up to 8, and
+  // fewer than 512 work-groups if more than one.
+  const int64_t steps = (n + 255) / 256, one = tokens < kTile ? tokens : kTile;
+  int64_t rows = one * (steps < 16 ? steps : 16);
+  if (tokens > kTile) {
+    int64_t more = tokens * (steps < 8 ? steps : 8);
+    more = more < 512 * kTile ? more : 512 * kTile;
+    more = more > tokens ? more : tokens;
+    rows = rows > more ? rows : more;
+  }
+  return (size_t)(rows * all) * sizeof(float);
 }
 
 extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t tokens, int64_t n, const int32_t* which,
@@ -715,7 +728,7 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
                  (reinterpret_cast<uintptr_t>(x) & 15) == 0,
              "%s: %lld rows of %lld (a multiple of 8), %lld apart, %lld adapters; rows must be 16-byte aligned", fn,
              (long long)tokens, (long long)n, (long long)ldx, (long long)adapters);
-  QS_SUPPORTED(tokens <= (1 << 19) && ldx <= (1 << 24), "%s: %lld rows of %lld, %lld apart", fn, (long long)tokens, (long long)n, (long long)ldx);
+  QS_SUPPORTED(tokens <= kMaxTokens && ldx <= (1 << 24), "%s: %lld rows of %lld, %lld apart", fn, (long long)tokens, (long long)n, (long long)ldx);
   AdapterArgs a{};
   a.x = static_cast<const uint16_t*>(x), a.ldx = tokens == 1 ? 0 : ldx, a.tokens = tokens, a.n = n, a.which = which;
   a.adapters = (int)adapters, a.count = count;

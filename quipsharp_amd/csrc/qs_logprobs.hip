@@ -632,6 +632,18 @@ extern "C" size_t qs_token_logprobs_workspace_bytes(int64_t rows, int64_t vocab,
   return layout_of(rows, vocab, top, dtype == QS_DTYPE_F32 ? 4 : 2).bytes;
 }
 
+extern "C" size_t qs_token_logprobs_workspace_most(int64_t rows, int64_t vocab, int dtype, int top) {
+  if (!sizes_fit(rows, vocab, top)) return 0;
+  // from 1024 rows on a row has as many parts whatever their number
+  const int size = dtype == QS_DTYPE_F32 ? 4 : 2;
+  size_t most = layout_of(rows, vocab, top, size).bytes;
+  for (int64_t r = 1; r < rows && r < 1024; ++r) {
+    const size_t bytes = layout_of(r, vocab, top, size).bytes;
+    most = bytes > most ? bytes : most;
+  }
+  return most;
+}
+
 extern "C" int qs_token_logprobs(const void* logits, int dtype, int64_t ld, int64_t rows, int64_t vocab, const void* tokens,
                                  int token_bytes, int top, float* logprobs, float* entropy, int32_t* ranks,
                                  float* top_logprobs, int32_t* top_tokens, void* workspace, size_t workspace_bytes,

@@ -13,6 +13,12 @@ from .pages import _room, _workspace
 MAX_TOP = 64
 
 
+def workspace_bytes(rows, vocab, dtype, top=0) -> int:
+    """Bytes of workspace that serve ``token_logprobs`` of any number of rows up to ``rows`` (few rows take more than
+    many)."""
+    return int(_lib.lib().qs_token_logprobs_workspace_most(rows, vocab, _lib.dtype_code(dtype), top))
+
+
 def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0, *, workspace: Tensor = None):
     """Scores of ``tokens`` (rows,) int32 or int64 under ``logits`` (rows,
     vocab) float32, float16 or bfloat16.
@@ -30,7 +36,8 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0, *, workspace: T
     alternative.  A row whose largest logit is not finite has log probabilities
     -inf, entropy 0 and no alternatives.  Exponentials are 32-bit, their sums
     and logarithms 64-bit: a log sum is off by ``(3 ln(vocab) + 20) 2 ** -24`` at
-    most (3.3e-6 for 151936 tokens)."""
+    most (3.3e-6 for 151936 tokens).  ``workspace``: uint8, of
+    ``workspace_bytes`` for the most rows of any call that has it."""
     if logits.dim() != 2:
         raise ValueError(f"logits must be (rows, vocab), got {tuple(logits.shape)}")
     rows, vocab = logits.shape
