@@ -80,7 +80,7 @@ def add_adapters(ys, x: Tensor, which: Tensor, downs, ups, scales, *, outs=None,
                 and up.device == dev and scale.device == dev):
             _refuse(g, y, o, down, up, scale, tokens, n, adapters, dtype, dev)
         rank = ranks[g] = dsh[1]
-        grads = grads or y.requires_grad or down.requires_grad or up.requires_grad or scale.requires_grad
+        grads = grads or y.requires_grad or o.requires_grad or down.requires_grad or up.requires_grad or scale.requires_grad
         jobs[g] = _lib.AdapterJob(down.data_ptr(), up.data_ptr(), scale.data_ptr(), ds[0] if adapters > 1 else 0, ds[1],
                                   us[0] if adapters > 1 else 0, us[1] if m > 1 else rank, rank, m, y.data_ptr(),
                                   yst[0] if tokens > 1 else m, o.data_ptr(), ost[0] if tokens > 1 else m)

@@ -132,7 +132,8 @@ def append_rotated(q: Tensor, k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Te
     if layout not in LAYOUTS:
         raise ValueError(f"layout {layout!r} (half or interleaved)")
     out = _output(out, q)
-    if q.requires_grad or k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad:
+    if q.requires_grad or k.requires_grad or v.requires_grad or k_pages.requires_grad or v_pages.requires_grad \
+            or frequencies.requires_grad or out.requires_grad:
         _lib.no_gradient("append_rotated")
     _lib.require_gpu(k_pages, what="append_rotated")
     with _lib.device_of(k_pages):
