@@ -588,12 +588,12 @@ int qs_reorder_states(int count, const void *const *src, void *const *dst, const
  * * frequencies[i] (radians, fp64 device memory, [pairs]; the product is taken
  * in fp64), times factor; the rest of a head stays.  A pair is elements i and
  * i + pairs, or 2 i and 2 i + 1 (interleaved).  Queries go to q_out
- * [tokens][heads][head_dim] (tokens out_token apart; may be q itself), keys and
- * values to the token's place in the pages.  Tokens, rows, starts, pool and
- * over as in qs_page_append_over; heads need not divide.  A token whose
- * position is below 0 gets zero queries and is stored nowhere, one that has no
- * page or lies beyond the table is turned but stored nowhere, one of no row is
- * left out.  bf16 or fp16; strides multiples of 8 elements, 16-byte aligned;
+ * [tokens][heads][head_dim] (tokens out_token apart; q itself, or apart from q,
+ * k and v), keys and values to the token's place in the pages.  Tokens, rows,
+ * starts, pool and over as in qs_page_append_over; heads need not divide.  A
+ * token whose position is below 0 gets zero queries and is stored nowhere, one
+ * that has no page or lies beyond the table is turned but stored nowhere, one of
+ * no row is left out.  bf16 or fp16; strides multiples of 8 elements, 16-byte aligned;
  * head_dim a multiple of 8, pairs <= 256. */
 int qs_page_append_rotated(const void *q, const void *k, const void *v, int dtype, int64_t tokens, int64_t rows,
                            int heads, int kv_heads, int head_dim, int64_t q_token, int64_t q_head, int64_t k_token,
@@ -619,11 +619,11 @@ typedef struct qs_adapter_job {
 /* out_g[t] = y_g[t] + scale_g[a] up_g[a] (down_g[a] x[t]) with a = which[t] for
  * up to QS_MAX_GROUP linears g that read the same x [tokens][n] (bf16 or fp16,
  * n a multiple of 8).  Tokens whose which is not in 0 .. adapters - 1 have
- * out = y.  fp32 sums, one rounding.  No out may be x, another linear's y or its
- * out.  workspace: qs_adapters_workspace_bytes, for this call alone while it
- * runs; a workspace of that size serves fewer tokens and any number of adapters
- * too.  At most 2^19 tokens; rows of x, y, out and weights at most 2^24 elements
- * apart. */
+ * out = y.  fp32 sums, one rounding.  An out that shares memory with what the
+ * call reads or writes, its own y at the same place aside, is refused.
+ * workspace: qs_adapters_workspace_bytes, for this call alone while it runs; a
+ * workspace of that size serves fewer tokens and any number of adapters too.  At
+ * most 2^19 tokens; rows of x, y, out and weights at most 2^24 elements apart. */
 size_t qs_adapters_workspace_bytes(int64_t tokens, int64_t n, int64_t adapters, int count, const int *ranks);
 int qs_adapters_add(const void *x, int dtype, int64_t ldx, int64_t tokens, int64_t n, const int32_t *which,
                     int64_t adapters, int count, const qs_adapter_job *jobs, void *workspace, size_t workspace_bytes,

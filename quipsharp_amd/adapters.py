@@ -46,7 +46,7 @@ def add_adapters(ys, x: Tensor, which: Tensor, downs, ups, scales, *, outs=None,
     multiple of 8 up to 128 (zeros beyond an adapter's own), scales[g]:
     (adapters,) float32; ys[g]: (tokens, m) in x's type.  Returns new tensors,
     or ``outs``, each of which is the y at its place itself or apart from all
-    the call reads.  Sums are float32, rounded once at the end; the inner
+    the call reads and writes (others are refused).  Sums are float32, rounded once at the end; the inner
     products go on with 16 significant bits or more.  ``workspace``: uint8, of
     ``workspace_bytes`` for the most tokens of any call that has it."""
     count = len(ys)

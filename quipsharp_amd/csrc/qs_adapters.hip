@@ -28,6 +28,7 @@
 // dropped lies 2^-16 (bf16) or 2^-22 (fp16) below the largest, and products
 // beyond fp16's range work.  All sums are fp32; the output is rounded once.
 #include "qs_attend_dev.h"
+#include "qs_overlap.h"
 
 namespace qs {
 namespace {
@@ -689,6 +690,32 @@ Plan plan_of(int64_t tokens, int64_t n, int64_t adapters, int count, const int* 
   return p;
 }
 
+// What linear g's output shares memory with of all that the call reads and
+// writes, its own y at the same place aside; nullptr: nothing.
+const char* meets(const AdapterArgs& a, const qs_adapter_job* jobs, int g) {
+  auto rows = [&](const void* p, int64_t ld, int64_t width) { return Rows{p, a.tokens, 2 * ld, 2 * width}; };
+  auto weights = [&](const void* p, int64_t adapter, int64_t rows, int64_t row, int64_t width, const Rows& out) {
+    const Rows all{p, 1, 0, 2 * ((a.adapters - 1) * adapter + (rows - 1) * row + width)};
+    if (!share_memory(all, out)) return false;
+    for (int64_t i = 0; i < a.adapters; ++i)
+      if (share_memory(Rows{static_cast<const uint16_t*>(p) + i * adapter, rows, 2 * row, 2 * width}, out)) return true;
+    return false;
+  };
+  const qs_adapter_job& j = jobs[g];
+  const Rows out = rows(j.out, j.ldo, j.m);
+  if (share_memory(out, rows(a.x, a.ldx, a.n))) return "x";
+  if (share_memory(out, Rows{a.which, 1, 0, 4 * a.tokens})) return "which";
+  for (int h = 0; h < a.count; ++h) {
+    const qs_adapter_job& k = jobs[h];
+    if (!(h == g && k.y == j.out) && share_memory(out, rows(k.y, k.ldy, k.m))) return "a y";
+    if (h != g && share_memory(out, rows(k.out, k.ldo, k.m))) return "another output";
+    if (weights(k.down, k.down_adapter, k.rank, k.down_row, a.n, out) || weights(k.up, k.up_adapter, k.m, k.up_row, k.rank, out) ||
+        share_memory(out, Rows{k.scale, 1, 0, 4 * (int64_t)a.adapters}))
+      return "weights";
+  }
+  return nullptr;
+}
+
 }  // namespace
 }  // namespace qs
 
@@ -759,6 +786,10 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
     a.ranks += j.rank, ranks[g] = j.rank;
     most = j.rank > most ? j.rank : most;
     columns += j.m;
+  }
+  for (int g = 0; g < count; ++g) {
+    const char* with = meets(a, jobs, g);
+    QS_REQUIRE(!with, "%s: the output of linear %d shares memory with %s", fn, g, with);
   }
   const Plan p = plan_of(tokens, n, adapters, count, ranks);
   a.tiles = (int)p.tiles, a.runs = p.runs, a.splits = p.splits, a.steps = p.steps;

@@ -10,6 +10,7 @@
 // rounded once, to the cache's type.
 #include "qs_rope_dev.h"
 #include "qs_attend_dev.h"
+#include "qs_overlap.h"
 
 namespace qs {
 namespace {
@@ -224,6 +225,17 @@ extern "C" int qs_page_append_rotated(const void* q, const void* k, const void* 
   QS_REQUIRE((reinterpret_cast<uintptr_t>(frequencies) & 7) == 0, "%s: frequencies must be 8-byte aligned", fn);
   const int all = heads + 2 * kv_heads;
   QS_SUPPORTED((int64_t)all * head_dim <= (1 << 24), "%s: %d heads of %d", fn, all, head_dim);
+  // Queries may be turned where they lie, each element by the thread that reads it.
+  const Rows to{q_out, tokens, 2 * out_token, 2 * (int64_t)heads * head_dim};
+  auto meets = [&](const void* p, int64_t token, int64_t head, int count) {
+    if (!share_memory(to, Rows{p, tokens, 2 * token, 2 * ((count - 1) * head + head_dim)})) return false;
+    for (int h = 0; h < count; ++h)
+      if (share_memory(to, Rows{static_cast<const uint16_t*>(p) + h * head, tokens, 2 * token, 2 * (int64_t)head_dim})) return true;
+    return false;
+  };
+  const bool in_place = q == q_out && (tokens == 1 || q_token == out_token) && (heads == 1 || q_head == head_dim);
+  QS_REQUIRE((in_place || !meets(q, q_token, q_head, heads)) && !meets(k, k_token, k_head, kv_heads) && !meets(v, v_token, v_head, kv_heads),
+             "%s: q_out shares memory with q, k or v, and is not q itself", fn);
   int block = kTable / pairs < kTokens ? kTable / pairs : kTokens;
   while (block > 1 && (tokens < 512 * (int64_t)block || (int64_t)block * all * head_dim > (1 << 30))) block /= 2;
   const int64_t blocks = (tokens + block - 1) / block;

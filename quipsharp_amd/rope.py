@@ -105,7 +105,7 @@ def append_rotated(q: Tensor, k: Tensor, v: Tensor, k_pages: Tensor, v_pages: Te
     ``rope_frequencies``; the product is taken in 64 bits) and multiplied by
     ``factor``; a pair is elements i and i + len(frequencies) (``half``) or 2 i
     and 2 i + 1 (``interleaved``).  Returns the queries, in ``out`` if given,
-    which may be q.
+    which may be q, and is refused where it shares memory with q, k or v otherwise.
 
     A token at a position below 0 gets zero queries and is stored nowhere, one
     without a page or beyond the table is turned all the same, and tokens of no

@@ -15,8 +15,8 @@ def needed(tokens, n, count, ranks):
     """The bytes that the entry point asks for when it is given none."""
     L = _lib.lib()
     jobs = (_lib.AdapterJob * 4)(*[_lib.AdapterJob(down=4096, up=4096, scale=4096, down_adapter=128 * n, down_row=n,
-                                                   up_adapter=8 * 128, up_row=128, rank=r, m=8, y=1 << 30, ldy=8,
-                                                   out=(2 + g) << 30, ldo=8) for g, r in enumerate(ranks)])
+                                                   up_adapter=8 * 128, up_row=128, rank=r, m=8, y=1 << 44, ldy=8,
+                                                   out=(2 + g) << 44, ldo=8) for g, r in enumerate(ranks)])
     assert L.qs_adapters_add(P, 2, n, tokens, n, P, count, len(ranks), jobs, P, 0, None) == 1
     message = L.qs_last_error().decode()
     assert "workspace of 0 bytes" in message
