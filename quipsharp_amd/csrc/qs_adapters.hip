@@ -324,9 +324,13 @@ __device__ __forceinline__ uint4 add_8(uint4 y, const f32x4& d0, const f32x4& d1
 }
 
 // An exact power of two that brings a largest size near 1, and its inverse.
+// Within 2^64 either way, so that the inverse times an adapter's scale neither
+// overflows nor loses bits: inner products of fp16 numbers are (products from
+// 2^-48 to 2^32, at most 2^24 of them added), and those of bf16 numbers go on as
+// bf16, which has fp32's exponents.
 __device__ __forceinline__ float powers(float most, float& inverse) {
   int e = (int)(__float_as_uint(most) >> 23);
-  e = e < 2 ? 2 : e > 252 ? 252 : e;
+  e = e < 127 - 64 ? 127 - 64 : e > 127 + 64 ? 127 + 64 : e;
   inverse = __uint_as_float((uint32_t)e << 23);
   return __uint_as_float((uint32_t)(254 - e) << 23);
 }
