@@ -640,7 +640,7 @@ int qs_adapters_add(const void *x, int dtype, int64_t ldx, int64_t tokens, int64
  *             ties to the lower token; -inf and -1 where there are none left
  * A NaN logit counts as -inf, and a token at -inf is no alternative.  A row
  * whose largest logit is not finite has log probabilities -inf, entropy 0 and
- * no alternatives.  top <= 64, vocab <= 2^24.  workspace:
+ * no alternatives.  top <= 64, vocab <= 2^24, rows < 2^24.  workspace:
  * qs_token_logprobs_workspace_bytes, which falls as rows grow, to 0 from 1024
  * rows on (up to 163833 tokens); one that serves any number of rows up to `rows`
  * has qs_token_logprobs_workspace_most. */

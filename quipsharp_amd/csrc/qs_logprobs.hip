@@ -618,8 +618,11 @@ auto score_kernel_of(int each, bool select) {
   return select ? score_kernel_of<T, true>(each) : score_kernel_of<T, false>(each);
 }
 
+// A grid has fewer than 2^32 threads along each side.
+constexpr int64_t kMaxRows = (1ll << 32) / kThreads - 1;
+
 bool sizes_fit(int64_t rows, int64_t vocab, int top) {
-  return rows >= 1 && rows <= INT32_MAX && vocab >= 1 && vocab <= (1 << 24) && top >= 0 && top <= kMaxTop && top <= vocab;
+  return rows >= 1 && rows <= kMaxRows && vocab >= 1 && vocab <= (1 << 24) && top >= 0 && top <= kMaxTop && top <= vocab;
 }
 
 }  // namespace
@@ -656,8 +659,8 @@ extern "C" int qs_token_logprobs(const void* logits, int dtype, int64_t ld, int6
   QS_REQUIRE(rows >= 1 && vocab >= 1 && (rows == 1 || ld >= vocab), "%s: %lld rows of %lld tokens, %lld apart", fn,
              (long long)rows, (long long)vocab, (long long)ld);
   QS_REQUIRE(top >= 0 && top <= vocab, "%s: %d alternatives of %lld tokens", fn, top, (long long)vocab);
-  QS_SUPPORTED(sizes_fit(rows, vocab, top), "%s: %lld rows of %lld tokens, %d alternatives (at most %d, of 2^24 tokens)", fn,
-               (long long)rows, (long long)vocab, top, kMaxTop);
+  QS_SUPPORTED(sizes_fit(rows, vocab, top), "%s: %lld rows of %lld tokens, %d alternatives (at most %d, of 2^24 tokens, of %lld rows)", fn,
+               (long long)rows, (long long)vocab, top, kMaxTop, (long long)kMaxRows);
   const int size = dtype_bytes(dtype);
   QS_REQUIRE(reinterpret_cast<uintptr_t>(logits) % size == 0 && reinterpret_cast<uintptr_t>(tokens) % token_bytes == 0,
              "%s: logits and tokens must be aligned to their elements", fn);

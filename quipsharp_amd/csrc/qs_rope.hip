@@ -239,6 +239,7 @@ extern "C" int qs_page_append_rotated(const void* q, const void* k, const void* 
   int block = kTable / pairs < kTokens ? kTable / pairs : kTokens;
   while (block > 1 && (tokens < 512 * (int64_t)block || (int64_t)block * all * head_dim > (1 << 30))) block /= 2;
   const int64_t blocks = (tokens + block - 1) / block;
+  QS_SUPPORTED(blocks < (1ll << 32) / kThreads, "%s: %lld tokens, %d of a work-group", fn, (long long)tokens, block);  // 2^32 threads
   int split = 1;
   while (split * 4 <= all && blocks * split < 512) split *= 2;
   const int rest = head_dim - 2 * pairs;

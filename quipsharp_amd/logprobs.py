@@ -36,7 +36,7 @@ def token_logprobs(logits: Tensor, tokens: Tensor, top: int = 0, *, workspace: T
     alternative.  A row whose largest logit is not finite has log probabilities
     -inf, entropy 0 and no alternatives.  Exponentials are 32-bit, their sums
     and logarithms 64-bit: a log sum is off by ``(3 ln(vocab) + 20) 2 ** -24`` at
-    most (3.3e-6 for 151936 tokens).  ``workspace``: uint8, of
+    most (3.3e-6 for 151936 tokens).  Fewer than 2 ** 24 rows.  ``workspace``: uint8, of
     ``workspace_bytes`` for the most rows of any call that has it."""
     if logits.dim() != 2:
         raise ValueError(f"logits must be (rows, vocab), got {tuple(logits.shape)}")

@@ -106,3 +106,19 @@ def test_rotation_refuses_queries_that_meet_what_is_read():
                                       None, pool, None, P, 4, 0, 1.0, out, out_token, None)
         assert rc == 1 and "q_out shares memory" in L.qs_last_error().decode()
     assert met > 500
+
+
+# ---------------------------------------------------------------------------
+# launches that would have 2^32 threads or more
+# ---------------------------------------------------------------------------
+
+def test_more_rows_than_a_grid_has_are_refused():
+    L = _lib.lib()
+    scores = lambda rows: L.qs_token_logprobs(P, 0, 4, rows, 4, P, 8, 1, P, P, P, P, P, None, 0, None)  # noqa: E731
+    assert scores(1 << 24) == 3 and "16777216 rows of 4 tokens" in L.qs_last_error().decode()
+    assert L.qs_token_logprobs_workspace_bytes(1 << 24, 4, 0, 1) == L.qs_token_logprobs_workspace_most(1 << 24, 4, 0, 1) == 0
+    pool = _lib.PagePool(k=1 << 40, v=1 << 41, k_page=4096, k_head=4096, k_pos=512, v_page=4096, v_head=4096, v_pos=512, pages=3,
+                         page=8, table=4096, table_ld=1, cols=1, lengths=4096)
+    turned = lambda tokens: L.qs_page_append_rotated(1 << 50, 1 << 51, 1 << 52, 2, tokens, 2, 1, 1, 512, 512, 512, 512, 512, 512, 512,  # noqa: E731
+                                                     P, pool, None, P, 256, 0, 1.0, 1 << 50, 512, None)
+    assert turned(1 << 26) == 3 and "67108864 tokens, 4 of a work-group" in L.qs_last_error().decode()
