@@ -625,6 +625,11 @@ typedef struct qs_adapter_job {
  * workspace of that size serves fewer tokens and any number of adapters too.  At
  * most 2^19 tokens; rows of x, y, out and weights at most 2^24 elements apart. */
 size_t qs_adapters_workspace_bytes(int64_t tokens, int64_t n, int64_t adapters, int count, const int *ranks);
+/* How such a call is cut, for tests and tuning; plan [5]: work-groups that share
+ * a tile of 64 tokens, blocks of 16 ranks of a work-group, work-groups for all
+ * ranks, splits of n, output columns of a work-group. */
+int qs_adapters_plan(int64_t tokens, int64_t n, int64_t adapters, int count, const int *ranks, const int64_t *ms,
+                     int *plan);
 int qs_adapters_add(const void *x, int dtype, int64_t ldx, int64_t tokens, int64_t n, const int32_t *which,
                     int64_t adapters, int count, const qs_adapter_job *jobs, void *workspace, size_t workspace_bytes,
                     qs_stream_t stream);

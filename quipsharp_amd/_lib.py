@@ -151,6 +151,7 @@ _SIGNATURES = {
     "qs_page_append_rotated": ([_vp, _vp, _vp, _int, _i64, _i64, _int, _int, _int, _i64, _i64, _i64, _i64, _i64, _i64,
                                 _vp, _pool_p, _vp, _vp, _int, _int, _f32, _vp, _i64, _vp], _int),
     "qs_adapters_workspace_bytes": ([_i64, _i64, _i64, _int, _int_p], ctypes.c_size_t),
+    "qs_adapters_plan": ([_i64, _i64, _i64, _int, _int_p, ctypes.POINTER(_i64), _int_p], _int),
     "qs_adapters_add": ([_vp, _int, _i64, _i64, _i64, _vp, _i64, _int, ctypes.POINTER(AdapterJob), _vp,
                          ctypes.c_size_t, _vp], _int),
     "qs_token_logprobs_workspace_bytes": ([_i64, _i64, _int, _int], ctypes.c_size_t),

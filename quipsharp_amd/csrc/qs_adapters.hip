@@ -694,6 +694,27 @@ Plan plan_of(int64_t tokens, int64_t n, int64_t adapters, int count, const int* 
   return p;
 }
 
+// Columns of a work-group of the second launch, which splits up the inner
+// products once for all of them.  Groups of single tokens take 256 at a time, 64 a
+// wave, and 512 work-groups of them fill the GPU (48 tokens to 2 x 25600: 33 us with
+// 1024 columns, 48 with 256).  Prompts take 64 at a time and are cut finer where
+// there are few (142 tokens to 1315 columns: 8.5 us with 64, 12 with 256) and coarser
+// where there are many (10313 to 5120: 58 us with 512, 62 with 256, 80 with 128; but
+// 5641 to 12659 151 us with 1024, 128 with 512); work-groups of slots without a group
+// cost their launch (74 tokens in 32 slots to 20507 columns: 20 us with 64, 9 with 256).
+int span_of(const Plan& p, int64_t columns) {
+  int span;
+  if (p.tiles == 1) {
+    const int64_t groups = p.slots < 8 ? 1 : p.slots / 2;
+    span = kColumns;
+    while (span < 8 * kColumns && groups * columns / (2 * span) >= 512) span *= 2;
+  } else {
+    span = 64;
+    while (span < (p.slots > 1 ? 256 : 512) && p.tiles * p.slots * columns / (2 * span) >= 640) span *= 2;
+  }
+  return span;
+}
+
 // What linear g's output shares memory with of all that the call reads and
 // writes, its own y at the same place aside; nullptr: nothing.
 const char* meets(const AdapterArgs& a, const qs_adapter_job* jobs, int g) {
@@ -745,6 +766,16 @@ extern "C" size_t qs_adapters_workspace_bytes(int64_t tokens, int64_t n, int64_t
     rows = rows > more ? rows : more;
   }
   return (size_t)(rows * all) * sizeof(float);
+}
+
+extern "C" int qs_adapters_plan(int64_t tokens, int64_t n, int64_t adapters, int count, const int* ranks, const int64_t* ms, int* plan) {
+  QS_REQUIRE(ranks && ms && plan, "qs_adapters_plan: null pointer");
+  QS_REQUIRE(qs_adapters_workspace_bytes(tokens, n, adapters, count, ranks) > 0, "qs_adapters_plan: no such call");
+  int64_t columns = 0;
+  for (int g = 0; g < count; ++g) columns += ms[g];
+  const Plan p = plan_of(tokens, n, adapters, count, ranks);
+  plan[0] = p.slots, plan[1] = p.blocks, plan[2] = p.runs, plan[3] = p.splits, plan[4] = span_of(p, columns);
+  return QS_OK;
 }
 
 extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t tokens, int64_t n, const int32_t* which,
@@ -801,22 +832,7 @@ extern "C" int qs_adapters_add(const void* x, int dtype, int64_t ldx, int64_t to
   QS_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
              "%s: workspace of %zu bytes (16-byte aligned), %zu needed", fn, workspace_bytes, need);
   a.part = static_cast<float*>(workspace);
-  // Columns of a work-group, which splits up the inner products once for all of
-  // them.  Groups of single tokens take 256 at a time, 64 a wave, and 512
-  // work-groups of them fill the GPU (48 tokens to 2 x 25600: 33 us with 1024 columns,
-  // 48 with 256).  Prompts take 64 at a time and are cut finer where there are few
-  // (142 tokens to 1315 columns: 8.5 us with 64, 12 with 256) and coarser where there
-  // are many (10313 to 5120: 58 us with 512, 62 with 256, 80 with 128; but 5641 to
-  // 12659 151 us with 1024, 128 with 512); work-groups of slots without a group cost
-  // their launch (74 tokens in 32 slots to 20507 columns: 20 us with 64, 9 with 256).
-  if (p.tiles == 1) {
-    const int64_t groups = p.slots < 8 ? 1 : p.slots / 2;
-    a.span = kColumns;
-    while (a.span < 8 * kColumns && groups * columns / (2 * a.span) >= 512) a.span *= 2;
-  } else {
-    a.span = 64;
-    while (a.span < (p.slots > 1 ? 256 : 512) && p.tiles * p.slots * columns / (2 * a.span) >= 640) a.span *= 2;
-  }
+  a.span = span_of(p, columns);
   int grid = 0;
   for (int g = 0; g < count; ++g) {
     a.linear[g].first = grid;
