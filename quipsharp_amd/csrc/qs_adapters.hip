@@ -10,12 +10,12 @@
 // one matrix, so that x is read once for 128 of them.
 //
 // Both are bound by memory: single tokens by the weights of the adapters that
-// they name, prompts by x, y and out.  Measured: 48 tokens of 24 adapters of rank
-// 64, 5120 inputs to two linears of 25600, 10 and 32 us for 175 MB (4.2 TB/s; a
-// large copy reaches 5.06); 10313 tokens of 3 prompts, 25600 inputs to 5120 at rank
-// 64, 95 and 55 us for 747 MB (5.0 TB/s); 4260 of 6, 3584 inputs to 3584 + 512 + 512
-// at rank 24, 15 and 24 us for 114 MB (2.9 TB/s: short loops behind each
-// work-group's start); one token, 4096 inputs to 4096 + 1024 + 1024, 4 and 5 us.
+// they name, prompts by x, y and out.  Measured: 48 tokens that name 21 adapters of
+// rank 64, 5120 inputs to two linears of 25600, 10 and 31 us for 28 and 147 MB (2.9
+// and 4.7 TB/s; a large copy reaches 5.06); 10313 tokens of 3 prompts, 25600 inputs
+// to 5120 at rank 64, 95 and 54 us for 747 MB (5.0 TB/s); 4260 of 6, 3584 inputs to
+// 3584 + 512 + 512 at rank 24, 16 and 24 us for 113 MB (2.8 TB/s: short loops behind
+// each work-group's start); one token, 4096 inputs to 4096 + 1024 + 1024, 4 and 6 us.
 //
 // Tokens are taken 64 at a time.  In each 64 those of one adapter form a group
 // (found by ballots: prompts come in runs, single tokens in any order), which
@@ -667,7 +667,7 @@ Plan plan_of(int64_t tokens, int64_t n, int64_t adapters, int count, const int* 
   const int64_t steps = (n + 255) / 256, groups = p.tiles * (p.slots < 8 ? 1 : p.slots / 2);
   // Few tokens need many narrow work-groups, many tokens wide ones that read x
   // once: one token's 48 ranks of 4096 inputs in blocks of 16 take 4.2 us, in one of
-  // 64 5.1; 48 tokens with 24 adapters of 128 ranks in blocks of 32 11.9, of 64 9.8;
+  // 64 5.1; 48 tokens that name 21 adapters of 128 ranks in blocks of 32 11.9, of 64 9.8;
   // 229 tokens with 128 ranks in blocks of 32 6.6, of 64 7.6, of 128 10.4; 848 with
   // 240 ranks 16.2, 13.8 and 16.3; 5641 with 160 ranks of 24296 inputs in blocks of
   // 64 254, of 96 194.
