@@ -360,6 +360,10 @@ class PagedDecoder(StaticDecoder):
         self.which = torch.full((rows,), -1, dtype=torch.int32, device=self.dev)
         self._prompt_which = None  # of a prompt's tokens, while it runs
 
+    def _check_ids(self, ids):
+        if ids.device != self.dev or ids.dtype not in (torch.int64, torch.int32):
+            raise ValueError(f"ids must be int64 or int32 on {self.dev}, got {ids.dtype} on {ids.device}")
+
     def _check_beside(self, tokens):
         """Refuses what the layers would refuse of ``which`` and the adapters: before the cache grows, since it keeps what
         it was given room for."""
@@ -398,6 +402,7 @@ class PagedDecoder(StaticDecoder):
         T = int(sum(counts))
         if ids.shape != (T,) or len(counts) != self.B:
             raise ValueError(f"ids {tuple(ids.shape)} for {T} tokens in {len(counts)} of {self.B} rows")
+        self._check_ids(ids)
         count = torch.tensor(counts, dtype=torch.int32)
         starts = torch.cat([torch.zeros(1, dtype=torch.int32), count.cumsum(0, dtype=torch.int32)]).to(self.dev)
         row = torch.repeat_interleave(torch.arange(self.B), count).to(self.dev)
@@ -455,7 +460,10 @@ class PagedDecoder(StaticDecoder):
         """``prompt`` with scores in place of logits (``logprobs.token_logprobs``): entry t is about the token behind
         ids[t] in its row, of which the row's last has none (log probability 0, rank -1; its entropy and alternatives
         are those of the token to come).  The logits of ``rows`` tokens are there at a time."""
-        from .logprobs import token_logprobs
+        from .logprobs import MAX_TOP, token_logprobs
+        most = min(MAX_TOP, self.model.lm_head.weight.shape[0])
+        if not 0 <= top <= most or rows < 1:
+            raise ValueError(f"{top} alternatives (0 to {most}), the logits of {rows} tokens at a time")
         h, count = self._prompt_hidden(ids, counts)
         behind = torch.full_like(ids, -100)
         behind[:-1] = ids[1:]
@@ -471,6 +479,7 @@ class PagedDecoder(StaticDecoder):
         adapters.  Logits (rows, vocab)."""
         if ids.numel() != self.B:
             raise ValueError(f"ids {tuple(ids.shape)} for {self.B} rows")
+        self._check_ids(ids)
         if self.model.model.embed_tokens.weight.dtype != torch.bfloat16:
             raise TypeError("the decode step runs bf16 models")
         self._check_beside(self.B)

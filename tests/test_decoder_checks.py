@@ -93,6 +93,22 @@ def test_other_ids_are_refused_before_the_cache_grows(decoder):
     assert not decoder.advanced
 
 
+def test_what_a_score_does_not_give_is_refused_before_the_cache_grows(decoder):
+    ids = torch.arange(4)
+    for more in (dict(top=65), dict(top=-1), dict(rows=0), dict(rows=-5)):
+        with pytest.raises(ValueError, match="alternatives"):
+            decoder.score(ids, [3, 1], **more)
+    for bad in (ids.float(), ids.to("meta"), ids.short()):
+        for call in (lambda: decoder.prompt(bad, [3, 1]), lambda: decoder.score(bad, [3, 1]), lambda: decoder.step(bad[:2])):
+            with pytest.raises(ValueError, match="ids must be"):
+                call()
+    assert not decoder.advanced
+    decoder.model.lm_head = torch.nn.Linear(256, 40, dtype=BF)
+    with pytest.raises(ValueError, match="41 alternatives"):
+        decoder.score(ids, [3, 1], top=41)
+    assert not decoder.advanced
+
+
 # ---------------------------------------------------------------------------
 # models
 # ---------------------------------------------------------------------------
