@@ -510,6 +510,16 @@ class PagedDecoder(StaticDecoder):
         c.attend_token(i, q, scale=self.scale, out=out.view(heads), **self.spans)
 
 
+def _each_prompts(which, prompts):
+    """The adapters of every prompt, int32 on the host; None: none."""
+    if which is None:
+        return torch.full((prompts,), -1, dtype=torch.int32)
+    which = torch.as_tensor(which)
+    if which.shape != (prompts,) or which.is_floating_point() or which.dtype == torch.bool:
+        raise ValueError(f"which must be a whole number for each of {prompts} prompts, got {tuple(which.shape)} x {which.dtype}")
+    return which.to("cpu", torch.int64).clamp(-1, 2 ** 31 - 1).int()  # numbers beyond name none either way
+
+
 @torch.no_grad()
 def greedy_decode_paged(model, prompts, new_tokens, which=None, top=0, use_graph=True, page=64):
     """Greedy decode of prompts of any lengths (a list of 1-D id tensors), each with the adapters that ``which`` (a
@@ -520,9 +530,9 @@ def greedy_decode_paged(model, prompts, new_tokens, which=None, top=0, use_graph
     if not prompts or any(len(p) < 1 for p in prompts) or new_tokens < 1:
         raise ValueError(f"{new_tokens} new tokens behind prompts of {[len(p) for p in prompts]}: every prompt has a token or more")
     R, dev = len(prompts), prompts[0].device
+    which = _each_prompts(which, R)
     dec = PagedDecoder(model, R, max(len(p) for p in prompts) + new_tokens, page)
-    if which is not None:
-        dec.which.copy_(torch.as_tensor(which, dtype=torch.int32))
+    dec.which.copy_(which)
     logits = dec.prompt(torch.cat(list(prompts)), [len(p) for p in prompts])
     shapes = (((), torch.int32), ((), torch.float32), ((), torch.float32), ((top,), torch.float32), ((top,), torch.int32))
     out = [torch.zeros(R, new_tokens, *more, dtype=kind, device=dev) for more, kind in shapes]
@@ -586,13 +596,13 @@ def beam_decode(model, prompts, beams, new_tokens, eos=-1, use_graph=True, page=
     descending order of scores (prompts, beams), prompt s, decode s)."""
     from .beam import beam_select, reorder_states
     R, dev = len(prompts), prompts[0].device
+    which = _each_prompts(which, R)
     longest = max(len(p) for p in prompts)
     columns = -(-(longest + new_tokens) // page)
     # every beam may come to hold all its pages after the prompt's last full one, and a copy of what it goes on from
     pages = sum(len(p) // page + 1 for p in prompts) + R * beams * (-(-new_tokens // page) + 2)
     dec = PagedDecoder(model, R * beams, columns * page, page, pages)
-    if which is not None:
-        dec.which.copy_(torch.as_tensor(which, dtype=torch.int32).repeat_interleave(beams))
+    dec.which.copy_(which.repeat_interleave(beams))
     counts = [0] * (R * beams)
     counts[::beams] = [len(p) for p in prompts]
     torch.cuda.synchronize()

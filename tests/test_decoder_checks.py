@@ -109,6 +109,18 @@ def test_what_a_score_does_not_give_is_refused_before_the_cache_grows(decoder):
     assert not decoder.advanced
 
 
+@pytest.mark.parametrize("which", [[1], [0, 1, 2], [[0, 1]], 1, [0.5, 1.0], [True, False]])
+def test_adapters_of_each_prompt(which):
+    """One number for every prompt: one alone is not taken for all of them."""
+    from quipsharp_amd.decode import beam_decode, greedy_decode_paged
+    prompts = [torch.arange(3), torch.arange(5)]
+    for call in (lambda: greedy_decode_paged(None, prompts, 2, which=which), lambda: beam_decode(None, prompts, 1, 2, which=which)):
+        with pytest.raises(ValueError, match="for each of 2 prompts"):
+            call()
+    from quipsharp_amd.decode import _each_prompts
+    assert _each_prompts(None, 2).tolist() == [-1, -1] and _each_prompts(torch.tensor([3, 1 << 40]), 2).tolist() == [3, 2 ** 31 - 1]
+
+
 # ---------------------------------------------------------------------------
 # models
 # ---------------------------------------------------------------------------
