@@ -14,6 +14,7 @@ from .pages import _HALF, _int32, _room, _workspace
 
 MAX_RANK = 128
 MAX_TOKENS = 1 << 19
+MAX_APART = 1 << 24  # rows, in elements
 NAMES = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
 
 
@@ -190,8 +191,8 @@ def check_beside(linears, which: Tensor, rows: int, tokens: int, dtype, device):
         _refuse(g, y, y, down, up, scale, 0, n, count, dtype, device)
         ds, us = down.stride(), up.stride()
         apart = ds[1] | (us[1] if m > 1 else 0) | (ds[0] | us[0] if count > 1 else 0)
-        if not (count and 8 <= rank <= MAX_RANK and not (rank | n | apart) % 8 and ds[1] >= n and (us[1] >= rank or m == 1)
-                and not (down.data_ptr() | up.data_ptr()) & 15):
+        if not (count and 8 <= rank <= MAX_RANK and not (rank | n | apart) % 8 and n <= ds[1] <= MAX_APART
+                and (rank <= us[1] <= MAX_APART or m == 1) and not (down.data_ptr() | up.data_ptr()) & 15):
             raise ValueError(f"adapters {g}: {tuple(shape)} and {tuple(up.shape)}: the rank must be a multiple of 8 up to "
                              f"{MAX_RANK}, rows 16-byte aligned and apart")
 

@@ -71,10 +71,11 @@ def test_adapters_are_refused_before_the_cache_grows(decoder, spoil, error, mess
 def test_ranks_and_alignment_are_refused_before_the_cache_grows(decoder):
     bank = last_bank(decoder)
     down, up = bank.down, bank.up
-    n = down.shape[2]
+    n, far = down.shape[2], (1 << 24) + 8
     for bank.down, bank.up in ((down[:, :4].contiguous(), up[:, :, :4].contiguous()),
                                (torch.zeros(3 * 8 * n + 4, dtype=BF)[4:].view(3, 8, n), up),
-                               (down[:, :1].expand(3, 8, n), up)):
+                               (down[:, :1].expand(3, 8, n), up),
+                               (torch.empty(7 * far + n, dtype=BF).as_strided((3, 8, n), (0, far, 1)), up)):
         with pytest.raises(ValueError, match="multiple of 8"):
             decoder.step(torch.arange(2))
     bank.down, bank.up = torch.zeros(3, 8, n + 8, dtype=BF)[:, :, :n], up  # rows of a wider tensor are fine
